@@ -455,6 +455,105 @@ LLMIK_API llmik_status llmik_add_rmsnorm(const void* x, const void* residual, co
 LLMIK_API llmik_status llmik_silu_mul_halves(const void* gate_up, void* out, long rows, int cols,
                                              void* stream);
 
+/* ------------------------------------------------------------ paged KV cache
+ * A cache of pages for sequences of different lengths, the append that writes
+ * it and the attention that reads it. No counterpart in the reference, whose
+ * caches hold one live length for the whole batch
+ * (integration/prealloc_cache.py:42-110).
+ *
+ * Token t of sequence b lies in page page_table[b][t / page_size], slot
+ * t % page_size. seq_lens[b] counts the tokens that are live at the call, with
+ * those that it brings: an append's rows are the last seq_lens[b] - n .. - 1,
+ * the query of a decode step is the token at seq_lens[b] - 1. The tables live
+ * in device memory and are not read on the host, so a captured graph can be
+ * replayed while they change.
+ *
+ * What the device finds is never an error: a page_table entry outside
+ * [0, n_pages) is an unmapped page (its tokens are not written, and are no keys);
+ * tokens at or behind max_pages * page_size do not exist; a length <= 0 is an
+ * empty sequence; a row that has no key, or belongs to no sequence, gives zeros.
+ * Slots that hold no live token are never used, whatever they contain.
+ */
+#define LLMIK_F16 0
+#define LLMIK_BF16 1
+
+typedef struct llmik_paged_cache {
+    void* k;                /* [n_pages, n_kv_heads, page_size, head_dim] */
+    void* v;                /* the same shape and stride */
+    const int* page_table;  /* [batch, max_pages] */
+    const int* seq_lens;    /* [batch] */
+    int64_t page_stride;    /* elements from one page to the next: >= n_kv_heads * page_size *
+                               head_dim (0: exactly that), a multiple of 8 */
+    int n_pages, page_size; /* page_size: a positive multiple of 8 */
+    int max_pages, batch;
+    int n_kv_heads, head_dim;   /* head_dim 64 or 128 */
+    int dtype;              /* LLMIK_F16 or LLMIK_BF16: cache, q, qkv and outputs */
+} llmik_paged_cache;
+
+/*
+ * score(i, j) = softmax_scale * q_i . k_j; with softcap > 0 softcap *
+ * tanh(score / softcap); with slopes [n_heads] minus slopes[h] * (pos_i -
+ * pos_j); keys pos_j <= pos_i, with window > 0 only the newest `window` of
+ * them (pos_i - pos_j < window).
+ */
+typedef struct llmik_score_options {
+    float softmax_scale;
+    float softcap;          /* 0: none */
+    const float* slopes;    /* NULL: none */
+    int window;             /* 0: none */
+} llmik_score_options;
+
+/*
+ * qkv [rows, (n_heads + 2 n_kv_heads) * head_dim]: q_out [rows, n_heads,
+ * head_dim] = rope(q), the row's slot of the cache = rope(k), v.
+ *   cu_tokens [batch + 1], from 0, non-decreasing: sequence b's new tokens are
+ *     rows cu_tokens[b] .. cu_tokens[b + 1] - 1, its last ones in order; NULL:
+ *     one row per sequence (rows == batch). Rows from cu_tokens[batch] on belong
+ *     to no sequence.
+ *   cos, sin [table_rows, head_dim], of the cache's type or (table_f32) fp32,
+ *     as llmik_rope applies them, indexed by position; a position without a
+ *     table row is written nowhere. Both NULL: no rotation.
+ * Two rows that name the same slot (a page mapped twice) write it in no
+ * particular order.
+ */
+LLMIK_API llmik_status llmik_rope_paged_append(const llmik_paged_cache* cache, const void* qkv, const void* cos,
+                                               const void* sin, int table_rows, int table_f32, const int* cu_tokens,
+                                               void* q_out, int rows, int n_heads, void* stream);
+
+/* Workspace bytes (see the workspace contract above) of the decode and, with
+ * prefix_len > 0, the shared-prefix attention: they depend on the shapes, not
+ * on the lengths. 0 for arguments that the calls refuse. */
+LLMIK_API size_t llmik_paged_workspace_size(const llmik_paged_cache* cache, int n_heads, int prefix_len);
+
+/*
+ * q, out [batch, n_heads, head_dim]: each sequence's newest token over its live
+ * keys. n_heads must be a multiple of n_kv_heads.
+ */
+LLMIK_API llmik_status llmik_paged_decode_attention(const llmik_paged_cache* cache, const void* q, void* out,
+                                                    int n_heads, const llmik_score_options* options,
+                                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * q, out [rows, n_heads, head_dim]: the new tokens of every sequence (rows as
+ * llmik_rope_paged_append's, cu_tokens required), each over the keys of its own
+ * sequence up to its position. No workspace.
+ */
+LLMIK_API llmik_status llmik_paged_prefill_attention(const llmik_paged_cache* cache, const void* q,
+                                                     const int* cu_tokens, void* out, int rows, int n_heads,
+                                                     const llmik_score_options* options, void* stream);
+
+/*
+ * llmik_paged_decode_attention for sequences that share their first prefix_len
+ * tokens: those keys are read from prefix_pages [n_prefix_pages] (n_prefix_pages
+ * * page_size >= prefix_len), once for the whole batch, and page_table rows are
+ * used from position prefix_len on. seq_lens counts the prefix too (a sequence
+ * may be shorter than it).
+ */
+LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cache* cache, const void* q, void* out,
+                                                           int n_heads, const int* prefix_pages, int n_prefix_pages,
+                                                           int prefix_len, const llmik_score_options* options,
+                                                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,54 @@ int launch_quantize_weights_int4(const void* W, bool w_fp16, int K, int N, int g
                                  void* packed, void* scale, void* scale_f16, hipStream_t stream);
 int launch_pack_int4_along_k(const void* q, int K, int N, void* packed, hipStream_t stream);
 
+// ---- paged KV cache --------------------------------------------------------
+struct PagedLaunch {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int* table;
+    const int* lens;
+    const int* cu;          // ragged rows' offsets (prefill), or null
+    const int* prefix_pages;
+    const float* slopes;
+    long page_stride;
+    int n_pages, page_size, max_pages, batch, n_heads, n_kv_heads, head_dim;
+    int rows, prefix_len, window;
+    float softmax_scale, softcap;
+    bool bf16;
+    void* workspace;
+    size_t workspace_bytes;
+};
+// Un-normalised results of a shared prefix that the decode kernel joins:
+// o [n_kv_heads, batch * n_heads / n_kv_heads, splits, head_dim], ml [..., 2].
+struct PagedPrefixParts {
+    const float* o;
+    const float* ml;
+    int splits, len;
+};
+struct PagedAppend {
+    const void* qkv;
+    const void* cos;   // null: no rotation
+    const void* sin;
+    void* q_out;
+    void* k;
+    void* v;
+    const int* table;
+    const int* lens;
+    const int* cu;     // null: row b is the newest token of sequence b
+    long page_stride;
+    int n_pages, page_size, max_pages, batch, n_heads, n_kv_heads, head_dim;
+    int rows, table_rows;
+    bool bf16, table_f32;
+};
+size_t paged_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity);
+size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len);
+int launch_paged_append(const PagedAppend& a, hipStream_t stream);
+int launch_paged_decode(const PagedLaunch& a, const PagedPrefixParts& pre, hipStream_t stream);
+int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream);
+int launch_paged_shared_prefix(const PagedLaunch& a, hipStream_t stream);
+
 // ---- fused elementwise -----------------------------------------------------
 int launch_rmsnorm(const void* x, const void* w, void* out, int rows, int hidden, float eps,
                    hipStream_t stream);

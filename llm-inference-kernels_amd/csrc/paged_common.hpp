@@ -1,0 +1,196 @@
+// Shared by the kernels of the paged KV cache (paged_decode.hip, paged_flash.hip):
+// the two 16-bit types, the cache's addressing and the score options.
+//
+// The cache is k, v [n_pages, n_kv_heads, page_size, D]; token t of sequence b
+// lies in page page_table[b][t / page_size] at slot t % page_size. page_size is
+// a multiple of 8, so eight consecutive tokens starting at a multiple of 8 (an
+// octet) always lie in one page, one row behind the other: kernels look pages
+// up once per octet. Entries outside [0, n_pages) are unmapped pages: no load
+// goes there and their tokens are masked.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+#include <climits>
+
+#include "device_common.hpp"
+#include "llmik_internal.hpp"
+
+namespace llmik {
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Positions stay below this, so that a tile's end is still an int.
+constexpr long kMaxPagedTokens = (long)INT_MAX - 128;
+constexpr float kLog2eF = 1.4426950408889634f;
+
+// fp16 or bf16 values as 16-bit words, with the products and the (round to
+// nearest even) conversions of each.
+template <bool BF>
+struct Half16;
+template <>
+struct Half16<false> {
+    static __device__ __forceinline__ float to_f32(uint16_t b) { return (float)__builtin_bit_cast(f16, b); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+};
+template <>
+struct Half16<true> {
+    static __device__ __forceinline__ float to_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const bf16x2 h = __builtin_convertvector(f32x2{a, b}, bf16x2);
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+
+// Division of 0 <= n < 2^31 by a fixed divisor d >= 1: n / d = (n * mul) >> (32
+// + shift) with shift = ceil(log2 d) - 1 and mul = floor(2^(32 + shift) / d) + 1
+// <= 2^32 - 1 for d that is no power of two (n e < 2^(32 + shift) for the
+// rounding error e = mul d - 2^(32 + shift) <= d <= 2^(shift + 1), as n < 2^31);
+// a power of two is a shift (mul = 0).
+struct FastDiv {
+    uint32_t d, mul, shift;
+    static FastDiv of(uint32_t d) {
+        FastDiv f{d, 0, 0};
+        while ((1ull << f.shift) < d) ++f.shift;
+        if ((d & (d - 1)) != 0) {
+            --f.shift;
+            f.mul = (uint32_t)((1ull << (32 + f.shift)) / d + 1);
+        }
+        return f;
+    }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return mul ? (uint32_t)(((uint64_t)n * mul) >> 32) >> shift : n >> shift;
+    }
+};
+
+// The cache as the kernels see it. Strides in elements of 16 bits.
+struct PagedView {
+    const uint16_t* k;
+    const uint16_t* v;
+    const int* table;     // [batch, max_pages]
+    const int* lens;      // [batch]
+    long page_stride;
+    int n_pages, max_pages, batch, n_kv_heads, capacity;   // capacity: max_pages * page_size tokens
+    FastDiv page;
+};
+
+// Element offset of the row of token t (an octet's first) of sequence b, KV
+// head kvh; -1 where the token lies behind `end` or its page is unmapped.
+template <int D>
+__device__ __forceinline__ long octet_offset(const PagedView& c, const int* table_row, int kvh, int t, int end) {
+    if (t >= end) return -1;
+    const uint32_t pi = c.page.div((uint32_t)t);
+    const int page = table_row[pi];
+    const int slot = t - (int)(pi * c.page.d);
+    if ((uint32_t)page >= (uint32_t)c.n_pages) return -1;
+    return (long)page * c.page_stride + ((long)kvh * c.page.d + slot) * D;
+}
+
+// Scores in the log2 domain. cap > 0: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
+// (e^2x + 1), as exp2 and one reciprocal (absolute error about 2^-23 cap).
+struct ScoreOpts {
+    float scale_log2;   // softmax_scale * log2(e)
+    float cap_in;       // 2 log2(e) * softmax_scale / softcap, or 0
+    float cap_log2;     // softcap * log2(e)
+    const float* slopes;
+    int window;         // keys per query, INT_MAX where unlimited
+};
+__device__ __forceinline__ float capped(float s, float cap_in, float cap_log2) {
+    const float e = __builtin_amdgcn_exp2f(s * cap_in);
+    return fmaf(-2.0f * cap_log2, __builtin_amdgcn_rcpf(e + 1.0f), cap_log2);
+}
+
+// The kernels' views of a call.
+inline PagedView paged_view(const PagedLaunch& a) {
+    PagedView c{};
+    c.k = static_cast<const uint16_t*>(a.k);
+    c.v = static_cast<const uint16_t*>(a.v);
+    c.table = a.table;
+    c.lens = a.lens;
+    c.page_stride = a.page_stride;
+    c.n_pages = a.n_pages;
+    c.max_pages = a.max_pages;
+    c.batch = a.batch;
+    c.n_kv_heads = a.n_kv_heads;
+    c.capacity = (int)std::min((long)a.max_pages * a.page_size, kMaxPagedTokens);
+    c.page = FastDiv::of((uint32_t)a.page_size);
+    return c;
+}
+inline ScoreOpts score_opts(const PagedLaunch& a) {
+    ScoreOpts s{};
+    s.scale_log2 = a.softmax_scale * kLog2eF;
+    if (a.softcap > 0.0f) {
+        s.cap_in = 2.0f * kLog2eF * (a.softmax_scale / a.softcap);
+        s.cap_log2 = a.softcap * kLog2eF;
+    }
+    s.slopes = a.slopes;
+    s.window = a.window > 0 ? a.window : INT_MAX;
+    return s;
+}
+
+// max / sum over lanes l and l ^ 32, or l and l ^ 16.
+__device__ __forceinline__ float xor32_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float xor16_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Running totals of `mine` over the 256 threads of a workgroup: s_pre[i] is the
+// sum of the threads before i (s_pre[256] the total, which is returned).
+__device__ __forceinline__ uint32_t block_totals(uint32_t mine, uint32_t* s_pre) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t up = __shfl_up(incl, d);
+        if (lane >= d) incl += up;
+    }
+    if (lane == 63) s_pre[wave] = incl;
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += s_pre[w];
+        total += s_pre[w];
+    }
+    __syncthreads();
+    s_pre[tid + 1] = before + incl;
+    if (tid == 0) s_pre[0] = 0;
+    __syncthreads();
+    return total;
+}
+
+}  // namespace llmik

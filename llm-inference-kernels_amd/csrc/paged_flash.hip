@@ -1,0 +1,432 @@
+// Attention of many query rows over a paged cache: prompts (ragged chunks of new
+// tokens, causal by position) and the shared prefix of a decoding batch.
+//
+// Rows. All query rows that read one KV head's keys form one list: row r of a
+// sequence is query token r / G, head r % G of the KV head's G query heads (for
+// the prefix: sequence r / G of the batch). A workgroup takes 128 consecutive
+// rows, 32 per wave, so that short chunks of several heads fill a tile as long
+// prompts do, and walks the keys in 64-token tiles.
+//
+// Products on 32x32x16 matrix instructions, transposed so that a lane keeps one
+// row's softmax:
+//   S^T = K Q^T: A = 32 keys from LDS, B = the wave's 32 rows (registers): lane
+//     (h, n) gets row n's scores of tokens 8 i + 4 h + 0..3, i < 4;
+//   O^T = V^T P^T: the scores are the B operand as they lie (k-slots 8h .. 8h + 7
+//     of a 16-token step are its tokens 4h .. + 3 and 8 + 4h .. + 3); A is V read
+//     from LDS by the transposing 64-bit read (16 lanes give four tokens' 16
+//     channels and get one channel's four tokens each).
+// P is rounded once to 16 bits, as 2^8 p (fp16 keeps its full precision down to
+// 2^-22); sums and statistics are fp32.
+//
+// K and V tiles are copied to LDS asynchronously, one tile ahead. The 16-byte
+// chunks of a row are permuted (xor with the row number) so that the operand
+// reads of eight rows fall into different banks; the copies place them so.
+#include "paged_common.hpp"
+
+namespace llmik {
+
+namespace {
+
+constexpr int kPfThreads = 256;
+constexpr int kPfRows = 128;    // query rows of a workgroup
+constexpr int kPfTile = 64;     // tokens of a tile
+constexpr float kPShift = 8.0f;
+
+struct PagedFlashParams {
+    const uint16_t* q;
+    uint16_t* out;
+    PagedView c;
+    ScoreOpts s;
+    const int* cu;            // [batch + 1]
+    int rows;                 // rows of q
+    int n_heads;
+    FastDiv gqa;
+    const int* prefix_pages;  // the prefix form
+    int prefix_len, splits, chunk;
+    float* part_o;
+    float* part_ml;
+};
+
+struct FlashTile {   // of the ragged form
+    int b, tile, row0, rows, pos0;   // sequence, its tile, first row of q, its query tokens, the first one's position
+};
+
+}  // namespace
+
+template <bool BF, int D, bool PREFIX>
+__global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashParams p) {
+    using Hf = Half16<BF>;
+    constexpr int KS = D / 16, CB = D / 32;
+    constexpr int CPR = D / 8;                    // 16-byte chunks of a row
+    constexpr int kRowBytes = D * 2;
+    constexpr int kCopies = 16 * CPR / 64;        // copy instructions for a wave's 16 rows
+    constexpr int kRowsPerCopy = 64 / CPR;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, h = lane >> 5, n = lane & 31;
+
+    __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPfTile * kRowBytes], s_k1[kPfTile * kRowBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t s_v0[kPfTile * kRowBytes], s_v1[kPfTile * kRowBytes];
+    __shared__ uint32_t s_pre[kPfThreads + 1];
+    __shared__ FlashTile s_tile;
+    __shared__ int s_lo[4], s_hi[4];
+    __shared__ uint32_t s_gone[2][4];
+
+    const int kvh = (int)blockIdx.x % p.c.n_kv_heads;
+    const uint32_t item = blockIdx.x / (uint32_t)p.c.n_kv_heads;
+    const int G = (int)p.gqa.d;
+
+    // ---- the workgroup's rows ----
+    FlashTile ft{};
+    int split = 0;
+    if constexpr (PREFIX) {
+        split = (int)(item % (uint32_t)p.splits);
+        ft.tile = (int)(item / (uint32_t)p.splits);
+        ft.rows = p.c.batch;
+    } else {
+        // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
+        const long chunks = (long)p.n_heads * CPR;
+        const long at0 = (long)blockIdx.x * kPfThreads + tid, step = (long)gridDim.x * kPfThreads;
+        for (long i = min(max(p.cu[p.c.batch], 0), p.rows) * chunks + at0; i < p.rows * chunks; i += step)
+            *reinterpret_cast<u32x4*>(p.out + 8 * i) = u32x4{0u, 0u, 0u, 0u};
+        const int per_thread = (p.c.batch + kPfThreads - 1) / kPfThreads;
+        const int b0 = min(tid * per_thread, p.c.batch), b1 = min(b0 + per_thread, p.c.batch);
+        auto tokens_of = [&](int b, int& row0) {   // query tokens of sequence b, kept inside q
+            row0 = max(p.cu[b], 0);
+            return max(min(p.cu[b + 1], p.rows) - row0, 0);
+        };
+        uint32_t mine = 0;
+        int row0;
+        for (int b = b0; b < b1; ++b) mine += (uint32_t)(tokens_of(b, row0) * G + kPfRows - 1) / kPfRows;
+        const uint32_t total = block_totals(mine, s_pre);
+        if (item >= total) return;   // the grid is an upper bound
+        const uint32_t x = total - 1 - item;   // a prompt's last tiles, which see the most keys, first
+        if (s_pre[tid] <= x && x < s_pre[tid + 1]) {
+            uint32_t at = s_pre[tid];
+            for (int b = b0; b < b1; ++b) {
+                FlashTile f;
+                f.rows = tokens_of(b, f.row0);
+                const uint32_t t = (uint32_t)(f.rows * G + kPfRows - 1) / kPfRows;
+                if (x < at + t) {
+                    f.b = b;
+                    f.tile = (int)(x - at);
+                    f.pos0 = p.c.lens[b] - (p.cu[b + 1] - f.row0);
+                    s_tile = f;
+                    break;
+                }
+                at += t;
+            }
+        }
+        __syncthreads();
+        ft = s_tile;
+    }
+    const int n_rows = ft.rows * G;
+    const int r_wave = ft.tile * kPfRows + 32 * wave;   // the wave's first row
+    const bool live = r_wave < n_rows;                  // wave-uniform
+    const int r = min(r_wave + n, n_rows - 1);          // rows past the end repeat the last
+    const int qi = (int)p.gqa.div((uint32_t)r);
+    const int head = kvh * G + (r - qi * G);
+    const long q_row = (PREFIX ? (long)qi : (long)ft.row0 + qi) * p.n_heads + head;
+    const int pos = PREFIX ? p.c.lens[qi] - 1 : ft.pos0 + qi;
+    int pos_lo = pos, pos_hi = pos;                     // of the wave's rows
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
+        pos_hi = max(pos_hi, __shfl_xor(pos_hi, d));
+    }
+    pos_lo = __builtin_amdgcn_readfirstlane(pos_lo);
+    pos_hi = __builtin_amdgcn_readfirstlane(pos_hi);
+    if (lane == 0) {
+        s_lo[wave] = live ? pos_lo : INT_MAX;
+        s_hi[wave] = live ? pos_hi : -1;
+    }
+    __syncthreads();
+    const int wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+    const int wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+
+    // ---- the keys any of them sees, [begin, end), in 64-token tiles ----
+    auto oldest = [&](int at) { return at >= p.s.window ? at - p.s.window + 1 : 0; };
+    int begin = PREFIX ? split * p.chunk : 0;
+    int end = PREFIX ? min(begin + p.chunk, p.prefix_len) : p.c.capacity;
+    begin = max(begin, oldest(wg_lo)) / kPfTile * kPfTile;
+    end = min(end, wg_hi + 1);
+    const int tiles = __builtin_amdgcn_readfirstlane(end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+
+    u32x4 qb[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qb[ks] = load16(p.q + q_row * D + 16 * ks + 8 * h);
+    const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
+
+    // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
+    const int* table_row = PREFIX ? p.prefix_pages : p.c.table + (long)ft.b * p.c.max_pages;
+    const int key_end = PREFIX ? p.prefix_len : p.c.capacity;   // keys with a table entry
+    auto look_up = [&](int i0) {   // lane l: octet 2 w + l % 2 of tile i0 + l / 2
+        const int i = i0 + (lane >> 1);
+        return i < tiles ? octet_offset<D>(p.c, table_row, kvh, begin + kPfTile * i + 16 * wave + 8 * (lane & 1),
+                                           min(end, key_end))
+                         : -1L;
+    };
+    long off = look_up(0), off_next = look_up(32);
+    // Copy instruction i fills rows kRowsPerCopy i .. of the wave's 16: lane l
+    // writes chunk slot l % CPR of row l / CPR, i.e. the chunk that the permutation puts there.
+    const int crow = lane / CPR, cslot = lane % CPR;
+    auto issue = [&](uint8_t* sk, uint8_t* sv, int i) {
+        if ((i & 31) == 0 && i) {
+            off = off_next;
+            off_next = look_up(i + 32);
+        }
+        const int hi = (int)(off >> 32), lo = (int)(uint32_t)off;
+        uint32_t gone = 0;
+#pragma unroll
+        for (int cp = 0; cp < kCopies; ++cp) {
+            const int row = kRowsPerCopy * cp + crow;                // of the wave's 16
+            const int octet = (kRowsPerCopy * cp) / 8;
+            const int l0 = 2 * (i & 31) + octet;
+            const long at = ((long)__builtin_amdgcn_readlane(hi, l0) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, l0);
+            const int trow = 16 * wave + row;                        // of the tile
+            const uint32_t kc = (uint32_t)(cslot ^ (D == 128 ? trow & 15 : trow & 7));
+            const uint32_t vc = (uint32_t)(cslot ^ (D == 128 ? (trow & 3) << 2 : ((trow >> 1) & 1) << 2));
+            uint8_t* lk = sk + (16 * wave + kRowsPerCopy * cp) * kRowBytes;
+            uint8_t* lv = sv + (16 * wave + kRowsPerCopy * cp) * kRowBytes;
+            if (at < 0) gone |= 1u << octet;
+            // Rows behind the end, or without a page, are zeroed: their scores are
+            // masked, and their values must not turn 0 * v into NaN.
+            if (at >= 0 && begin + kPfTile * i + trow < end) {
+                const uint32_t ro = (uint32_t)((row & 7) * kRowBytes);
+                const __amdgpu_buffer_rsrc_t rk = make_buffer_rsrc(p.c.k + at, 8 * kRowBytes);
+                const __amdgpu_buffer_rsrc_t rv = make_buffer_rsrc(p.c.v + at, 8 * kRowBytes);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)lk, 16,
+                                                         (int)(ro + 16 * kc), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)lv, 16,
+                                                         (int)(ro + 16 * vc), 0, 0, 0);
+            } else {
+                *reinterpret_cast<u32x4*>(lk + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4*>(lv + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+        if (lane == 0) s_gone[i & 1][wave] = gone;
+    };
+
+    f32x16 o[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[cb][e] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    // LDS offsets of this lane's operand reads.
+    const uint32_t k_row = (uint32_t)(n * kRowBytes);
+    const uint32_t k_sw = (uint32_t)((h ^ (D == 128 ? n & 15 : n & 7)) * 16);
+    const int vr = (lane & 15) >> 2;                        // token of the group's four
+    const uint32_t v_chunk = (uint32_t)(2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
+    const uint32_t v_sw = (uint32_t)(D == 128 ? vr << 2 : (vr >> 1) << 2);
+    const uint32_t v_at = (uint32_t)((4 * h + vr) * kRowBytes) + 8 * (lane & 1);
+
+    auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i) {
+        const int t0 = begin + kPfTile * i;
+        if (!live || t0 > pos_hi || t0 + kPfTile <= oldest(pos_lo)) return;   // no row sees a key of it
+        float sc[32];
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                acc = Hf::mfma32(*reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks))),
+                                 qb[ks], acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[16 * blk + e] = acc[e];
+        }
+        if (p.s.cap_in != 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e] *= p.s.scale_log2;
+        }
+        // value e belongs to token t0 + 4 h + 8 (e / 4) + e % 4
+        const int tk = t0 + 4 * h;
+        if (p.s.slopes) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
+        }
+        uint32_t gone = 0;   // bit o: octet o of the tile has no page
+#pragma unroll
+        for (int w = 0; w < 4; ++w) gone |= s_gone[i & 1][w] << (2 * w);
+        gone = __builtin_amdgcn_readfirstlane(gone);
+        if (gone || t0 + kPfTile > end || t0 + kPfTile - 1 > pos_lo || t0 < oldest(pos_hi)) {   // wave-uniform
+            const int old = oldest(pos), lim = min(pos + 1, end);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const int tok = tk + 8 * (e >> 2) + (e & 3);
+                if (tok < old || tok >= lim || ((gone >> (e >> 2)) & 1u)) sc[e] = -INFINITY;
+            }
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e]);
+        if (__any(mx > m_run)) {
+            mx = fmaxf(xor32_max(mx), m_run);
+            const float a = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - mx);
+            m_run = mx;
+            l_run *= a;
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[cb][e] *= a;
+        }
+        const float sub = (m_run == -INFINITY) ? 0.0f : m_run - kPShift;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(sc[e] - sub);
+            l_run += sc[e];
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            u32x4 pb;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pb[e] = Hf::pack(sc[8 * kk + 2 * e], sc[8 * kk + 2 * e + 1]);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                const uint8_t* a = sv + v_at + 16 * kk * kRowBytes + 16 * ((v_chunk + 4 * cb) ^ v_sw);
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 8 * kRowBytes));
+                const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+                o[cb] = Hf::mfma32(make_u32x4(l2[0], l2[1], h2[0], h2[1]), pb, o[cb]);
+            }
+        }
+    };
+
+    // One tile ahead: a tile's copies are complete for the whole workgroup, and the
+    // other buffer is read, once every wave has waited for its own copies and
+    // passed the barrier.
+    auto turn = [&](uint8_t* k_cur, uint8_t* v_cur, uint8_t* k_far, uint8_t* v_far, int i) {
+        __builtin_amdgcn_s_waitcnt(0);
+        asm volatile("s_barrier" ::: "memory");
+        if (i + 1 < tiles) issue(k_far, v_far, i + 1);
+        compute(k_cur, v_cur, i);
+    };
+    if (tiles > 0) issue(s_k0, s_v0, 0);
+    for (int i = 0; i < tiles; i += 2) {
+        turn(s_k0, s_v0, s_k1, s_v1, i);
+        if (i + 1 < tiles) turn(s_k1, s_v1, s_k0, s_v0, i + 1);
+    }
+
+    l_run = xor32_sum(l_run);
+    if (!live || r_wave + n >= n_rows) return;
+    if constexpr (PREFIX) {
+        const long at = ((long)kvh * n_rows + r) * p.splits + split;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * cb + 2 * e + 4 * h) =
+                    f32x4{o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]};
+        if (h == 0) {
+            p.part_ml[2 * at] = m_run;
+            p.part_ml[2 * at + 1] = l_run;
+        }
+    } else {
+        const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;   // a row without keys is zero
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<u32x2*>(p.out + q_row * D + 32 * cb + 2 * e + 4 * h) =
+                    u32x2{Hf::pack(o[cb][e] * inv, o[cb][e + 1] * inv), Hf::pack(o[cb][e + 2] * inv, o[cb][e + 3] * inv)};
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+namespace {
+
+struct PagedPrefixPlan {
+    int row_tiles, splits, chunk;
+    size_t off_o, off_ml, bytes;
+};
+
+// The prefix's parts lie behind the decode kernel's workspace.
+PagedPrefixPlan plan_prefix(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len,
+                            int cus) {
+    PagedPrefixPlan pl{};
+    const long rows = (long)batch * (n_heads / n_kv_heads);
+    pl.row_tiles = (int)((rows + kPfRows - 1) / kPfRows);
+    const long base = (long)pl.row_tiles * n_kv_heads;
+    const long most = (prefix_len + 2 * kPfTile - 1) / (2 * kPfTile);   // two tiles a split at least
+    long splits = std::max(1L, std::min({2L * cus / std::max(base, 1L), most, 64L}));
+    const long tiles = (prefix_len + kPfTile - 1) / kPfTile;
+    pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;
+    pl.splits = (prefix_len + pl.chunk - 1) / pl.chunk;
+    pl.off_ml = align_up(paged_decode_workspace(batch, n_heads, n_kv_heads, head_dim, capacity), 256);
+    const size_t parts = (size_t)rows * n_kv_heads * pl.splits;
+    pl.off_o = pl.off_ml + align_up(parts * 2 * sizeof(float), 256);
+    pl.bytes = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
+    return pl;
+}
+
+PagedFlashParams flash_params(const PagedLaunch& a) {
+    PagedFlashParams p{};
+    p.q = static_cast<const uint16_t*>(a.q);
+    p.out = static_cast<uint16_t*>(a.out);
+    p.c = paged_view(a);
+    p.s = score_opts(a);
+    p.cu = a.cu;
+    p.rows = a.rows;
+    p.n_heads = a.n_heads;
+    p.gqa = FastDiv::of((uint32_t)(a.n_heads / a.n_kv_heads));
+    return p;
+}
+
+template <bool PREFIX>
+void launch_flash(const PagedLaunch& a, const PagedFlashParams& p, long workgroups, hipStream_t stream) {
+    const dim3 grid((unsigned)workgroups);
+    if (a.bf16)
+        a.head_dim == 128 ? paged_flash_kernel<true, 128, PREFIX><<<grid, kPfThreads, 0, stream>>>(p)
+                          : paged_flash_kernel<true, 64, PREFIX><<<grid, kPfThreads, 0, stream>>>(p);
+    else
+        a.head_dim == 128 ? paged_flash_kernel<false, 128, PREFIX><<<grid, kPfThreads, 0, stream>>>(p)
+                          : paged_flash_kernel<false, 64, PREFIX><<<grid, kPfThreads, 0, stream>>>(p);
+}
+
+}  // namespace
+
+size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len) {
+    return plan_prefix(batch, n_heads, n_kv_heads, head_dim, capacity, prefix_len, device_cu_count()).bytes;
+}
+
+int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream) {
+    const PagedFlashParams p = flash_params(a);
+    const long G = a.n_heads / a.n_kv_heads;
+    // Tiles of all sequences at most: whole ones, and a part of one for each.
+    const long tiles = (long)a.rows * G / kPfRows + std::min((long)a.batch, (long)a.rows);
+    launch_flash<false>(a, p, tiles * a.n_kv_heads, stream);
+    return check_launch();
+}
+
+int launch_paged_shared_prefix(const PagedLaunch& a, hipStream_t stream) {
+    const long capacity = std::min((long)a.max_pages * a.page_size, kMaxPagedTokens);
+    const PagedPrefixPlan pl = plan_prefix(a.batch, a.n_heads, a.n_kv_heads, a.head_dim, capacity, a.prefix_len,
+                                           device_cu_count());
+    if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
+        return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_workspace_size)");
+    PagedFlashParams p = flash_params(a);
+    char* ws = static_cast<char*>(a.workspace);
+    p.prefix_pages = a.prefix_pages;
+    p.prefix_len = a.prefix_len;
+    p.splits = pl.splits;
+    p.chunk = pl.chunk;
+    p.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
+    p.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+    launch_flash<true>(a, p, (long)pl.row_tiles * pl.splits * a.n_kv_heads, stream);
+    const int st = check_launch();
+    if (st != LLMIK_OK) return st;
+    return launch_paged_decode(a, PagedPrefixParts{p.part_o, p.part_ml, pl.splits, a.prefix_len}, stream);
+}
+
+}  // namespace llmik

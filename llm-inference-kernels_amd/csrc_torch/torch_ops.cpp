@@ -17,9 +17,11 @@
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <optional>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -80,6 +82,28 @@ std::pair<void*, size_t> workspace(const Tensor& like, hipStream_t s, size_t nby
         return {ws.data_ptr(), size};
     }
     return {it->second.data_ptr(), (size_t)it->second.numel()};
+}
+
+// A workspace for the paged attention. Under capture every call has its own,
+// from the graph's memory, with the counters zeroed inside the graph: replays of
+// two graphs that were captured on one stream then share nothing.
+struct CallWorkspace {
+    Tensor own;
+    void* ptr = nullptr;
+    size_t bytes = 0;
+};
+
+CallWorkspace call_workspace(const Tensor& like, hipStream_t s, size_t nbytes) {
+    CallWorkspace w;
+    if (!stream_is_capturing(s)) {
+        std::tie(w.ptr, w.bytes) = workspace(like, s, nbytes);
+        return w;
+    }
+    w.own = at::empty({(int64_t)nbytes}, like.options().dtype(at::kByte));
+    w.own.narrow(0, 0, LLMIK_WORKSPACE_COUNTER_BYTES).zero_();
+    w.ptr = w.own.data_ptr();
+    w.bytes = nbytes;
+    return w;
 }
 
 py::dict workspaces() {
@@ -633,6 +657,181 @@ Tensor silu_mul_halves(const Tensor& gate_up) {
     return out;
 }
 
+// ------------------------------------------------------------ paged KV cache
+
+// The cache's description and the checks that every paged op makes; `like`
+// gives the element type and the device.
+llmik_paged_cache paged_cache(const Tensor& like, const char* name, const Tensor& k_cache, const Tensor& v_cache,
+                              const Tensor& page_table, const Tensor& seq_lens) {
+    TORCH_CHECK(like.scalar_type() == at::kHalf || like.scalar_type() == at::kBFloat16, name,
+                " must be fp16 or bf16");
+    TORCH_CHECK(k_cache.scalar_type() == like.scalar_type() && v_cache.scalar_type() == like.scalar_type(),
+                "k_cache and v_cache must have ", name, "'s dtype");
+    TORCH_CHECK(page_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt,
+                "page_table and seq_lens must be int32");
+    TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(),
+                "k_cache and v_cache must be [n_pages, n_kv_heads, page_size, head_dim] of one shape");
+    TORCH_CHECK(page_table.dim() == 2 && seq_lens.dim() == 1 && page_table.size(0) == seq_lens.size(0),
+                "page_table must be [batch, max_pages] and seq_lens [batch]");
+    TORCH_CHECK(page_table.is_contiguous() && seq_lens.is_contiguous(), "page_table and seq_lens must be contiguous");
+    const int64_t n_pages = k_cache.size(0), hkv = k_cache.size(1), ps = k_cache.size(2), d = k_cache.size(3);
+    TORCH_CHECK(n_pages > 0, "the cache has no pages");
+    TORCH_CHECK(hkv > 0 && ps > 0 && ps % 8 == 0, "page_size must be a positive multiple of 8");
+    TORCH_CHECK(d == 64 || d == 128, "only head_dim=64 and 128 supported");
+    TORCH_CHECK(n_pages <= INT_MAX && hkv <= (1 << 16) && ps <= (1 << 24) && page_table.size(0) <= INT_MAX &&
+                    page_table.size(1) <= INT_MAX, "cache or page_table too large");
+    const int64_t stride = n_pages > 1 ? k_cache.stride(0) : hkv * ps * d;
+    for (const Tensor* t : {&k_cache, &v_cache})
+        TORCH_CHECK(t->stride(3) == 1 && t->stride(2) == d && (hkv == 1 || t->stride(1) == ps * d) &&
+                        (n_pages == 1 || t->stride(0) == stride),
+                    "pages must be contiguous [n_kv_heads, page_size, head_dim] blocks, with one stride in k_cache "
+                    "and v_cache");
+    TORCH_CHECK(stride >= hkv * ps * d && stride % 8 == 0,
+                "the page stride must hold a page and be a multiple of 8 elements");
+    TORCH_CHECK(page_table.size(1) > 0, "page_table must have at least one column");
+    for (const Tensor* t : {&like, &k_cache, &v_cache, &page_table, &seq_lens})
+        TORCH_CHECK(t->is_cuda() && t->device() == like.device(), "all inputs must be CUDA tensors of one device");
+    llmik_paged_cache c{};
+    c.k = ptr(k_cache);
+    c.v = ptr(v_cache);
+    c.page_table = static_cast<const int*>(ptr(page_table));
+    c.seq_lens = static_cast<const int*>(ptr(seq_lens));
+    c.page_stride = stride;
+    c.n_pages = (int)n_pages;
+    c.page_size = (int)ps;
+    c.max_pages = (int)page_table.size(1);
+    c.batch = (int)seq_lens.size(0);
+    c.n_kv_heads = (int)hkv;
+    c.head_dim = (int)d;
+    c.dtype = like.scalar_type() == at::kBFloat16 ? LLMIK_BF16 : LLMIK_F16;
+    return c;
+}
+
+const int* paged_offsets(const Tensor& cu_tokens, const llmik_paged_cache& c, const Tensor& like) {
+    TORCH_CHECK(cu_tokens.scalar_type() == at::kInt && cu_tokens.dim() == 1 && cu_tokens.is_contiguous() &&
+                    cu_tokens.size(0) == (int64_t)c.batch + 1, "cu_tokens must be a contiguous int32 [batch + 1]");
+    TORCH_CHECK(cu_tokens.is_cuda() && cu_tokens.device() == like.device(),
+                "all inputs must be CUDA tensors of one device");
+    return static_cast<const int*>(ptr(cu_tokens));
+}
+
+int paged_heads(const Tensor& q, const llmik_paged_cache& c) {
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim, "q must be [rows, n_heads, head_dim]");
+    TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.n_kv_heads == 0, "n_heads must be a positive multiple of n_kv_heads");
+    TORCH_CHECK(q.size(0) <= INT_MAX && q.size(1) <= (1 << 16), "q has too many rows or heads");
+    return (int)q.size(1);
+}
+
+llmik_score_options paged_options(const Tensor& q, double softmax_scale, double softcap,
+                                  const std::optional<Tensor>& slopes, int64_t window) {
+    TORCH_CHECK(std::isfinite((float)softmax_scale), "softmax_scale must be finite");
+    TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), "softcap must be >= 0 and finite");
+    TORCH_CHECK(window >= 0 && window <= INT_MAX, "window must be >= 0");
+    llmik_score_options o{(float)softmax_scale, (float)softcap, nullptr, (int)window};
+    if (slopes.has_value()) {
+        TORCH_CHECK(slopes->scalar_type() == at::kFloat && slopes->dim() == 1 && slopes->is_contiguous() &&
+                        slopes->size(0) == q.size(1), "slopes must be a contiguous fp32 [n_heads]");
+        TORCH_CHECK(slopes->is_cuda() && slopes->device() == q.device(),
+                    "all inputs must be CUDA tensors of one device");
+        o.slopes = static_cast<const float*>(ptr(*slopes));
+    }
+    return o;
+}
+
+Tensor rope_paged_append(const Tensor& qkv, const std::optional<Tensor>& cos, const std::optional<Tensor>& sin,
+                         const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                         const Tensor& seq_lens, const std::optional<Tensor>& cu_tokens) {
+    const llmik_paged_cache c = paged_cache(qkv, "qkv", k_cache, v_cache, page_table, seq_lens);
+    TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) % c.head_dim == 0, "qkv must be [rows, heads * head_dim]");
+    TORCH_CHECK(qkv.size(0) <= INT_MAX && qkv.size(1) <= INT_MAX, "qkv is too large");
+    const int64_t rows = qkv.size(0), H = qkv.size(1) / c.head_dim - 2L * c.n_kv_heads;
+    TORCH_CHECK(H > 0, "qkv holds fewer than 2 n_kv_heads + 1 heads");
+    TORCH_CHECK(H % c.n_kv_heads == 0, "n_heads must be a positive multiple of n_kv_heads");
+    TORCH_CHECK(cos.has_value() == sin.has_value(), "cos and sin come together");
+    int table_f32 = 0, table_rows = 0;
+    Tensor cc, sc;
+    if (cos.has_value()) {
+        for (const Tensor* t : {&*cos, &*sin}) {
+            TORCH_CHECK(t->dim() == 2 && t->size(1) == c.head_dim && t->sizes() == cos->sizes(),
+                        "cos and sin must be [positions, head_dim]");
+            TORCH_CHECK((t->scalar_type() == at::kFloat || t->scalar_type() == qkv.scalar_type()) &&
+                            t->scalar_type() == cos->scalar_type(), "cos and sin must be fp32 or of qkv's dtype");
+            TORCH_CHECK(t->is_cuda() && t->device() == qkv.device(), "all inputs must be CUDA tensors of one device");
+        }
+        table_f32 = cos->scalar_type() == at::kFloat;
+        table_rows = (int)std::min<int64_t>(cos->size(0), INT_MAX);
+        cc = cos->contiguous();
+        sc = sin->contiguous();
+    }
+    const int* cu = cu_tokens.has_value() ? paged_offsets(*cu_tokens, c, qkv) : nullptr;
+    TORCH_CHECK(cu != nullptr || rows == c.batch, "without cu_tokens qkv must have one row per sequence");
+    const c10::DeviceGuard guard(qkv.device());
+    Tensor x = qkv.contiguous();
+    Tensor q = at::empty({rows, H, c.head_dim}, qkv.options());
+    if (rows == 0) return q;
+    if (c.batch == 0) return q.zero_();
+    check(llmik_rope_paged_append(&c, ptr(x), cc.defined() ? ptr(cc) : nullptr, sc.defined() ? ptr(sc) : nullptr,
+                                  table_rows, table_f32, cu, ptr(q), (int)rows, (int)H, stream_of(qkv)));
+    return q;
+}
+
+Tensor paged_decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                              const Tensor& seq_lens, double softmax_scale, double softcap,
+                              const std::optional<Tensor>& slopes, int64_t window) {
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    TORCH_CHECK(q.size(0) == c.batch, "q must have one row per sequence");
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    if (c.batch == 0) return out;
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_workspace_size(&c, H, 0));
+    check(llmik_paged_decode_attention(&c, ptr(q), ptr(out), H, &o, ws.ptr, ws.bytes, st));
+    return out;
+}
+
+Tensor paged_prefill_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                               const Tensor& seq_lens, const Tensor& cu_tokens, double softmax_scale, double softcap,
+                               const std::optional<Tensor>& slopes, int64_t window) {
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    const int* cu = paged_offsets(cu_tokens, c, q);
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    if (q.size(0) == 0) return out;
+    if (c.batch == 0) return out.zero_();
+    check(llmik_paged_prefill_attention(&c, ptr(q), cu, ptr(out), (int)q.size(0), H, &o, stream_of(q)));
+    return out;
+}
+
+Tensor paged_shared_prefix_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                     const Tensor& page_table, const Tensor& seq_lens, const Tensor& prefix_pages,
+                                     int64_t prefix_len, double softmax_scale, double softcap,
+                                     const std::optional<Tensor>& slopes, int64_t window) {
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    TORCH_CHECK(q.size(0) == c.batch, "q must have one row per sequence");
+    TORCH_CHECK(prefix_pages.scalar_type() == at::kInt && prefix_pages.dim() == 1 && prefix_pages.is_contiguous(),
+                "prefix_pages must be a contiguous int32 vector");
+    TORCH_CHECK(prefix_pages.is_cuda() && prefix_pages.device() == q.device(),
+                "all inputs must be CUDA tensors of one device");
+    TORCH_CHECK(prefix_len >= 0 && prefix_len <= INT_MAX - 256 && prefix_pages.size(0) <= INT_MAX,
+                "prefix_len must be >= 0 and fit the cache");
+    TORCH_CHECK(prefix_pages.size(0) * c.page_size >= prefix_len, "prefix_pages hold fewer than prefix_len tokens");
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    if (c.batch == 0) return out;
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_workspace_size(&c, H, (int)prefix_len));
+    check(llmik_paged_shared_prefix_attention(&c, ptr(q), ptr(out), H, static_cast<const int*>(ptr(prefix_pages)),
+                                              (int)prefix_pages.size(0), (int)prefix_len, &o, ws.ptr, ws.bytes, st));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
@@ -659,6 +858,10 @@ PYBIND11_MODULE(_C, m) {
     m.def("rope_qkv_append", &rope_qkv_append);
     m.def("add_rmsnorm", &add_rmsnorm);
     m.def("silu_mul_halves", &silu_mul_halves);
+    m.def("rope_paged_append", &rope_paged_append);
+    m.def("paged_decode_attention", &paged_decode_attention);
+    m.def("paged_prefill_attention", &paged_prefill_attention);
+    m.def("paged_shared_prefix_attention", &paged_shared_prefix_attention);
     m.def("workspaces", &workspaces);
     m.def("token_rows", &token_rows);
 }

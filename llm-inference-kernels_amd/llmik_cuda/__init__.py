@@ -24,12 +24,15 @@ the reference):
     (reference/quant_matmul_ref.py:39-88, 140-165), same arguments and
     results bit for bit, and `quantize_pack_weights_int4`, the two fused
     into the buffers QuantizedLinear registers
-    (integration/w4a16_patch.py:78-84).
+    (integration/w4a16_patch.py:78-84);
+  * `rope_paged_append`, `paged_decode_attention`, `paged_prefill_attention`,
+    `paged_shared_prefix_attention`: a cache of pages for sequences of
+    different lengths (`llmik_cuda.kv_cache.PagedKVCache` manages one).
 """
 from __future__ import annotations
 
 from collections.abc import Mapping
-from typing import Iterator, Tuple
+from typing import Iterator, Optional, Tuple
 
 import torch
 
@@ -48,7 +51,9 @@ __all__ = [
     "w4a16_gemm_f32out", "quantize_per_token_into", "quantize_v_per_token_int4_into",
     "quantize_k_per_channel_groupwise_int4_into", "quantize_weights_int4_groupwise",
     "pack_int4_along_k", "quantize_pack_weights_int4", "kivi_append_token_int4", "rope_qkv_append", "add_rmsnorm", "silu_mul_halves",
-    "w4a16_gemm_swiglu", "interleave_gate_up", "w4a16_gemm_qkv_rope", "interleave_head_halves", "LIB_PATH",
+    "w4a16_gemm_swiglu", "interleave_gate_up", "w4a16_gemm_qkv_rope", "interleave_head_halves",
+    "rope_paged_append", "paged_decode_attention", "paged_prefill_attention", "paged_shared_prefix_attention",
+    "LIB_PATH",
 ]
 
 
@@ -434,3 +439,78 @@ def silu_mul_halves(gate_up: torch.Tensor) -> torch.Tensor:
     (gate = the first half of the last dim): silu_mul of the two halves."""
     _require(_is_device(gate_up), "inputs must be CUDA")
     return _C.silu_mul_halves(gate_up)
+
+
+# ------------------------------------------------------------ paged KV cache
+# Sequences of different lengths over one pool of pages. k_cache, v_cache
+# [n_pages, n_kv_heads, page_size, head_dim], fp16 or bf16, head_dim 64 or 128,
+# page_size a multiple of 8 (pages contiguous, any page stride); page_table
+# [batch, max_pages] and seq_lens [batch] int32 on the device: token t of
+# sequence b is slot t % page_size of page page_table[b, t // page_size], and
+# seq_lens counts the tokens that the call brings. Entries outside [0, n_pages)
+# are unmapped pages: nothing is written there and their tokens are no keys.
+# Nothing is read back to the host. Inference only: no gradients are recorded.
+
+def rope_paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                      seq_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens' fused q|k|v rows [rows, (n_heads + 2 n_kv_heads) * head_dim]
+    into the cache: returns rope(q) [rows, n_heads, head_dim] and writes
+    rope(k) and v into the tokens' slots, in one launch. cu_tokens [batch + 1]
+    int32 (from 0, non-decreasing): rows cu_tokens[b] .. cu_tokens[b + 1] - 1
+    are the last tokens of sequence b, in order; without it row b is the newest
+    token of sequence b. cos, sin [positions, head_dim], fp32 or of qkv's
+    dtype, are indexed by position; None, None: no rotation. Rows from
+    cu_tokens[-1] on, and rows of empty sequences, give a zero q and are
+    written nowhere; so are positions past the tables. Two rows that name one
+    slot (a page mapped twice) write it in no particular order."""
+    _require(all(_is_device(t) for t in (qkv, k_cache, v_cache, page_table, seq_lens)),
+             "all inputs must be CUDA tensors")
+    return _C.rope_paged_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_tokens)
+
+
+def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           page_table: torch.Tensor, seq_lens: torch.Tensor, softmax_scale: float,
+                           softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                           window: int = 0) -> torch.Tensor:
+    """Decode attention of each sequence's newest token: q, out [batch,
+    n_heads, head_dim] over the seq_lens[b] live tokens of its pages. Scores
+    softmax_scale * q . k, with softcap > 0 softcap * tanh(score / softcap),
+    with slopes [n_heads] fp32 minus slopes[h] * (distance in tokens); with
+    window > 0 only the newest `window` keys. A sequence without a key gives
+    zeros. Deterministic; the bits depend on the lengths of the whole batch."""
+    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens)),
+             "all inputs must be CUDA tensors")
+    return _C.paged_decode_attention(q, k_cache, v_cache, page_table, seq_lens, float(softmax_scale),
+                                     float(softcap), slopes, int(window))
+
+
+def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            page_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: torch.Tensor,
+                            softmax_scale: float, softcap: float = 0.0,
+                            slopes: Optional[torch.Tensor] = None, window: int = 0) -> torch.Tensor:
+    """Attention of ragged chunks of new tokens: q, out [rows, n_heads,
+    head_dim], rows as in rope_paged_append, each row over the keys of its own
+    sequence up to its own position (the chunk's earlier tokens and what the
+    cache held before). Score options as in paged_decode_attention. Rows that
+    belong to no sequence give zeros."""
+    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens, cu_tokens)),
+             "all inputs must be CUDA tensors")
+    return _C.paged_prefill_attention(q, k_cache, v_cache, page_table, seq_lens, cu_tokens,
+                                      float(softmax_scale), float(softcap), slopes, int(window))
+
+
+def paged_shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                  page_table: torch.Tensor, seq_lens: torch.Tensor,
+                                  prefix_pages: torch.Tensor, prefix_len: int, softmax_scale: float,
+                                  softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                                  window: int = 0) -> torch.Tensor:
+    """paged_decode_attention for a batch whose sequences share their first
+    prefix_len tokens: those are read from prefix_pages [n] int32 once for all
+    sequences, page_table from position prefix_len on. seq_lens counts the
+    prefix too; a sequence may be shorter than it."""
+    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens, prefix_pages)),
+             "all inputs must be CUDA tensors")
+    return _C.paged_shared_prefix_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_pages,
+                                            int(prefix_len), float(softmax_scale), float(softcap), slopes,
+                                            int(window))

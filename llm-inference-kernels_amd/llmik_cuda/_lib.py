@@ -30,6 +30,19 @@ _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _l = ctypes.c_long
 
+
+class PagedCache(ctypes.Structure):
+    """llmik_paged_cache."""
+    _fields_ = [("k", _p), ("v", _p), ("page_table", _p), ("seq_lens", _p), ("page_stride", ctypes.c_int64),
+                ("n_pages", _i), ("page_size", _i), ("max_pages", _i), ("batch", _i), ("n_kv_heads", _i),
+                ("head_dim", _i), ("dtype", _i)]
+
+
+class ScoreOptions(ctypes.Structure):
+    """llmik_score_options."""
+    _fields_ = [("softmax_scale", _f), ("softcap", _f), ("slopes", _p), ("window", _i)]
+
+
 _SIGNATURES = {
     "llmik_last_error": (ctypes.c_char_p, []),
     "llmik_abi_version": (_i, []),
@@ -70,6 +83,11 @@ _SIGNATURES = {
     "llmik_rope_qkv_append_f16": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
     "llmik_add_rmsnorm": (_i, [_p, _p, _p, _p, _p, _i, _i, _f, _p]),
     "llmik_silu_mul_halves": (_i, [_p, _p, _l, _i, _p]),
+    "llmik_rope_paged_append": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _i, _i, _p]),
+    "llmik_paged_workspace_size": (_sz, [_p, _i, _i]),
+    "llmik_paged_decode_attention": (_i, [_p, _p, _p, _i, _p, _p, _sz, _p]),
+    "llmik_paged_prefill_attention": (_i, [_p, _p, _p, _p, _i, _i, _p, _p]),
+    "llmik_paged_shared_prefix_attention": (_i, [_p, _p, _p, _i, _p, _i, _i, _p, _p, _sz, _p]),
 }
 
 for _name, (_res, _args) in _SIGNATURES.items():
