@@ -470,7 +470,7 @@ LLMIK_API llmik_status llmik_silu_mul_halves(const void* gate_up, void* out, lon
  *
  * What the device finds is never an error: a page_table entry outside
  * [0, n_pages) is an unmapped page (its tokens are not written, and are no keys);
- * tokens at or behind max_pages * page_size do not exist; a length <= 0 is an
+ * tokens at or behind max_pages * page_size (or 2^30) do not exist; a length <= 0 is an
  * empty sequence; a row that has no key, or belongs to no sequence, gives zeros.
  * Slots that hold no live token are never used, whatever they contain.
  */
@@ -484,7 +484,7 @@ typedef struct llmik_paged_cache {
     const int* seq_lens;    /* [batch] */
     int64_t page_stride;    /* elements from one page to the next: >= n_kv_heads * page_size *
                                head_dim (0: exactly that), a multiple of 8 */
-    int n_pages, page_size; /* page_size: a positive multiple of 8 */
+    int n_pages, page_size; /* page_size: a multiple of 8, 8 .. 2^20 */
     int max_pages, batch;
     int n_kv_heads, head_dim;   /* head_dim 64 or 128 */
     int dtype;              /* LLMIK_F16 or LLMIK_BF16: cache, q, qkv and outputs */

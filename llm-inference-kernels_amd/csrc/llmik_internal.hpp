@@ -136,6 +136,8 @@ int launch_quantize_weights_int4(const void* W, bool w_fp16, int K, int N, int g
 int launch_pack_int4_along_k(const void* q, int K, int N, void* packed, hipStream_t stream);
 
 // ---- paged KV cache --------------------------------------------------------
+// Tokens of a sequence at most: positions a few tiles past the end are still ints.
+constexpr long kMaxPagedTokens = 1L << 30;
 struct PagedLaunch {
     const void* q;
     const void* k;

@@ -28,18 +28,18 @@ int check_shapes(const llmik_paged_cache* c, int n_heads) {
     if (n_heads <= 0 || c->n_kv_heads <= 0) return invalid("head counts must be positive");
     if (n_heads % c->n_kv_heads != 0) return invalid("n_heads must be a multiple of n_kv_heads");
     if (c->page_size <= 0 || c->page_size % 8 != 0) return invalid("page_size must be a positive multiple of 8");
-    if (c->page_size > (1 << 24) || c->n_kv_heads > (1 << 16) || n_heads > (1 << 16))
-        return unsupported("page_size above 2^24 or more than 2^16 heads");
+    if (c->page_size > (1 << 20) || c->n_kv_heads > (1 << 16) || n_heads > (1 << 16))
+        return unsupported("page_size above 2^20 or more than 2^16 heads");
     if (c->n_pages <= 0) return invalid("the cache has no pages");
     if (c->batch < 0) return invalid("batch must be >= 0");
     if (c->max_pages <= 0) return invalid("page_table must have at least one column");
     if (page_stride(*c) < row_elements(*c) || page_stride(*c) % 8 != 0)
         return invalid("page_stride must hold a page and be a multiple of 8");
-    // the 32-token tiles of all sequences are counted in 32 bits
-    const long capacity = std::min((long)c->max_pages * c->page_size, (long)INT_MAX);
+    // the work of all sequences is counted in 32 bits (tiles of 32 tokens and an overhead for each)
+    const long capacity = std::min((long)c->max_pages * c->page_size, kMaxPagedTokens);
     const long chunks = (n_heads / c->n_kv_heads + 15) / 16;
     const long slabs = (long)c->batch * c->n_kv_heads * chunks;
-    if (slabs >= INT_MAX || slabs * (capacity / 32 + 1) >= INT_MAX)
+    if (slabs >= INT_MAX || slabs * (capacity / 32 + 4) >= INT_MAX)
         return unsupported("batch * n_kv_heads * page table capacity too large");
     return LLMIK_OK;
 }
@@ -95,7 +95,7 @@ PagedLaunch launch_of(const llmik_paged_cache& c, const void* q, void* out, int 
 }
 
 long capacity_of(const llmik_paged_cache& c) {
-    return std::min((long)c.max_pages * c.page_size, (long)INT_MAX - 128);
+    return std::min((long)c.max_pages * c.page_size, kMaxPagedTokens);
 }
 
 hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
@@ -202,7 +202,7 @@ LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cac
     if ((st = check_q(q, out)) != LLMIK_OK) return st;
     if ((long)n_prefix_pages * cache->page_size < prefix_len)
         return invalid("prefix_pages hold fewer than prefix_len tokens");
-    if (prefix_len > INT_MAX - 256) return unsupported("prefix_len too large");
+    if (prefix_len > kMaxPagedTokens) return unsupported("prefix_len too large");
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;

@@ -23,8 +23,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// Positions stay below this, so that a tile's end is still an int.
-constexpr long kMaxPagedTokens = (long)INT_MAX - 128;
 constexpr float kLog2eF = 1.4426950408889634f;
 
 // fp16 or bf16 values as 16-bit words, with the products and the (round to
@@ -96,17 +94,23 @@ struct PagedView {
     FastDiv page;
 };
 
-// Element offset of the row of token t (an octet's first) of sequence b, KV
-// head kvh; -1 where the token lies behind `end` or its page is unmapped.
+// Element offset of the row of token t (an octet's first), KV head kvh, of the
+// sequence with this table row; -1 where the token lies at or behind `end` or
+// its page is unmapped. Without branches: every lane loads a table entry (the
+// first one instead of those behind the end).
 template <int D>
 __device__ __forceinline__ long octet_offset(const PagedView& c, const int* table_row, int kvh, int t, int end) {
-    if (t >= end) return -1;
-    const uint32_t pi = c.page.div((uint32_t)t);
+    const bool in = t < end;
+    const uint32_t pi = in ? c.page.div((uint32_t)t) : 0u;
     const int page = table_row[pi];
     const int slot = t - (int)(pi * c.page.d);
-    if ((uint32_t)page >= (uint32_t)c.n_pages) return -1;
-    return (long)page * c.page_stride + ((long)kvh * c.page.d + slot) * D;
+    const long at = (long)page * c.page_stride + (long)kvh * (long)(c.page.d * D) + slot * D;
+    return in && (uint32_t)page < (uint32_t)c.n_pages ? at : -1L;
 }
+
+// A running maximum starts here rather than at -inf: differences of two such are
+// then numbers, and states without a key join like all others (their sums are 0).
+constexpr float kNoMax = -1e30f;
 
 // Scores in the log2 domain. cap > 0: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
 // (e^2x + 1), as exp2 and one reciprocal (absolute error about 2^-23 cap).

@@ -162,11 +162,10 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
     const int* table_row = PREFIX ? p.prefix_pages : p.c.table + (long)ft.b * p.c.max_pages;
     const int key_end = PREFIX ? p.prefix_len : p.c.capacity;   // keys with a table entry
+    const int keys = __builtin_amdgcn_readfirstlane(min(end, key_end));
     auto look_up = [&](int i0) {   // lane l: octet 2 w + l % 2 of tile i0 + l / 2
         const int i = i0 + (lane >> 1);
-        return i < tiles ? octet_offset<D>(p.c, table_row, kvh, begin + kPfTile * i + 16 * wave + 8 * (lane & 1),
-                                           min(end, key_end))
-                         : -1L;
+        return octet_offset<D>(p.c, table_row, kvh, begin + kPfTile * i + 16 * wave + 8 * (lane & 1), keys);
     };
     long off = look_up(0), off_next = look_up(32);
     // Copy instruction i fills rows kRowsPerCopy i .. of the wave's 16: lane l
@@ -214,7 +213,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[cb][e] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = kNoMax, l_run = 0.0f;
 
     // LDS offsets of this lane's operand reads.
     const uint32_t k_row = (uint32_t)(n * kRowBytes);
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
         for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e]);
         if (__any(mx > m_run)) {
             mx = fmaxf(xor32_max(mx), m_run);
-            const float a = (m_run == -INFINITY) ? 0.0f : __builtin_amdgcn_exp2f(m_run - mx);
+            const float a = __builtin_amdgcn_exp2f(m_run - mx);
             m_run = mx;
             l_run *= a;
 #pragma unroll
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[cb][e] *= a;
         }
-        const float sub = (m_run == -INFINITY) ? 0.0f : m_run - kPShift;
+        const float sub = m_run - kPShift;
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
             sc[e] = __builtin_amdgcn_exp2f(sc[e] - sub);

@@ -678,7 +678,7 @@ llmik_paged_cache paged_cache(const Tensor& like, const char* name, const Tensor
     TORCH_CHECK(n_pages > 0, "the cache has no pages");
     TORCH_CHECK(hkv > 0 && ps > 0 && ps % 8 == 0, "page_size must be a positive multiple of 8");
     TORCH_CHECK(d == 64 || d == 128, "only head_dim=64 and 128 supported");
-    TORCH_CHECK(n_pages <= INT_MAX && hkv <= (1 << 16) && ps <= (1 << 24) && page_table.size(0) <= INT_MAX &&
+    TORCH_CHECK(n_pages <= INT_MAX && hkv <= (1 << 16) && ps <= (1 << 20) && page_table.size(0) <= INT_MAX &&
                     page_table.size(1) <= INT_MAX, "cache or page_table too large");
     const int64_t stride = n_pages > 1 ? k_cache.stride(0) : hkv * ps * d;
     for (const Tensor* t : {&k_cache, &v_cache})
@@ -818,7 +818,7 @@ Tensor paged_shared_prefix_attention(const Tensor& q, const Tensor& k_cache, con
                 "prefix_pages must be a contiguous int32 vector");
     TORCH_CHECK(prefix_pages.is_cuda() && prefix_pages.device() == q.device(),
                 "all inputs must be CUDA tensors of one device");
-    TORCH_CHECK(prefix_len >= 0 && prefix_len <= INT_MAX - 256 && prefix_pages.size(0) <= INT_MAX,
+    TORCH_CHECK(prefix_len >= 0 && prefix_len <= (1 << 30) && prefix_pages.size(0) <= INT_MAX,
                 "prefix_len must be >= 0 and fit the cache");
     TORCH_CHECK(prefix_pages.size(0) * c.page_size >= prefix_len, "prefix_pages hold fewer than prefix_len tokens");
     const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);

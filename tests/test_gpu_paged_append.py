@@ -61,7 +61,7 @@ def _run(llmik, dev, ctx, new, H, Hkv, D, page, dtype, tdtype, pad, seed=3, gap=
     return qkv, cos, sin, q, k, v, wq, wk, wv, written, k0, v0, lens, counts
 
 
-@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "B%d-%s" % (len(c[0]), "-".join(str(x) for x in c[2:]).replace("torch.", "")))
 def test_append(llmik, cuda, case):
     dtype = case[6]
     qkv, cos, sin, q, k, v, wq, wk, wv, written, k0, v0, _, _ = _run(llmik, cuda, *case)

@@ -43,6 +43,12 @@ DECODE = [
     ([100, 2000, 31], 32, 8, 128, 64, F16, {"window": 100}),
     ([100, 2000, 31], 32, 8, 128, 24, F16, {"window": 1}),
     ([5000, 2000, 4096], 12, 4, 64, 32, BF16, {"window": 777, "slopes": True, "softcap": 30.0}),
+    ([20000, 20011] * 4, 8, 8, 64, 64, F16, {}),                      # many tiles a wave
+    ([20000, 20011] * 4, 8, 8, 128, 16, BF16, {"window": 19000}),
+    (ref.ragged(1, 70, 0, 900), 16, 8, 128, 64, F16, {}),             # more slabs than workgroups; two lengths a lane
+    (ref.ragged(2, 130, 0, 700), 28, 4, 64, 16, BF16, {"softcap": 30.0, "slopes": True}),
+    (ref.ragged(3, 300, 1, 60), 8, 2, 128, 8, F16, {}),
+    (ref.ragged(4, 64, 300, 1500), 10, 10, 64, 32, BF16, {"window": 500}),
 ]
 
 
@@ -58,7 +64,11 @@ def _decode(llmik, dev, lens, H, Hkv, D, page, dtype, opts, seed=0, **cache):
     return got, want, bound
 
 
-@pytest.mark.parametrize("case", DECODE, ids=str)
+def _id(case):
+    return "-".join(str(x) if not isinstance(x, list) else "B%d_%d" % (len(x), max(x)) for x in case).replace("torch.", "")
+
+
+@pytest.mark.parametrize("case", DECODE, ids=_id)
 def test_decode(llmik, cuda, case):
     got, want, bound = _decode(llmik, cuda, *case)
     ref.check(got, want, bound)
@@ -97,7 +107,7 @@ def _prefill(llmik, dev, ctx, new, H, Hkv, D, page, dtype, opts, seed=0, pad=0, 
     return got, want, bound
 
 
-@pytest.mark.parametrize("case", PREFILL, ids=str)
+@pytest.mark.parametrize("case", PREFILL, ids=_id)
 def test_prefill(llmik, cuda, case):
     got, want, bound = _prefill(llmik, cuda, *case)
     ref.check(got, want, bound)
@@ -120,6 +130,8 @@ PREFIX = [
     (1000, [5, 100, 33], 32, 8, 128, 32, BF16, {"slopes": True}),
     (1000, [5, 100, 33], 32, 8, 128, 32, F16, {"window": 64}),
     (1000, [5, 100, 700], 16, 8, 64, 40, BF16, {"window": 600, "slopes": True, "softcap": 50.0}),
+    (700, ref.ragged(5, 70, 1, 300), 16, 8, 128, 64, F16, {}),
+    (700, ref.ragged(6, 130, 1, 100), 32, 4, 64, 16, BF16, {"slopes": True}),
 ]
 
 
@@ -140,7 +152,7 @@ def _prefix(llmik, dev, P, own, H, Hkv, D, page, dtype, opts, seed=0, lens=None)
     return got, want, bound
 
 
-@pytest.mark.parametrize("case", PREFIX, ids=str)
+@pytest.mark.parametrize("case", PREFIX, ids=_id)
 def test_shared_prefix(llmik, cuda, case):
     got, want, bound = _prefix(llmik, cuda, *case)
     ref.check(got, want, bound)
