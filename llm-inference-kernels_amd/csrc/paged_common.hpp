@@ -36,6 +36,10 @@ struct Half16<false> {
         const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
         return __builtin_bit_cast(uint32_t, h);
     }
+    static __device__ __forceinline__ float add_pair(uint32_t p, float acc) {   // acc + both values
+        const f16x2 one = {(f16)1.0f, (f16)1.0f};
+        return __builtin_amdgcn_fdot2(as_f16x2(p), one, acc, false);
+    }
     static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
@@ -51,6 +55,10 @@ struct Half16<true> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const bf16x2 h = __builtin_convertvector(f32x2{a, b}, bf16x2);
         return __builtin_bit_cast(uint32_t, h);
+    }
+    static __device__ __forceinline__ float add_pair(uint32_t p, float acc) {
+        const bf16x2 one = {(bf16)1.0f, (bf16)1.0f};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), one, acc, false);
     }
     static __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
@@ -172,29 +180,18 @@ __device__ __forceinline__ float xor16_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Running totals of `mine` over the 256 threads of a workgroup: s_pre[i] is the
-// sum of the threads before i (s_pre[256] the total, which is returned).
-__device__ __forceinline__ uint32_t block_totals(uint32_t mine, uint32_t* s_pre) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t up = __shfl_up(incl, d);
-        if (lane >= d) incl += up;
-    }
-    if (lane == 63) s_pre[wave] = incl;
-    __syncthreads();
-    uint32_t before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += s_pre[w];
-        total += s_pre[w];
-    }
-    __syncthreads();
-    s_pre[tid + 1] = before + incl;
-    if (tid == 0) s_pre[0] = 0;
-    __syncthreads();
-    return total;
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 }  // namespace llmik

@@ -31,6 +31,7 @@ constexpr int kPfThreads = 256;
 constexpr int kPfRows = 128;    // query rows of a workgroup
 constexpr int kPfTile = 64;     // tokens of a tile
 constexpr float kPShift = 8.0f;
+constexpr float kPLag = 6.0f;
 
 struct PagedFlashParams {
     const uint16_t* q;
@@ -39,6 +40,7 @@ struct PagedFlashParams {
     ScoreOpts s;
     const int* cu;            // [batch + 1]
     int rows;                 // rows of q
+    uint32_t per_round;       // workgroups of one per CU
     int n_heads;
     FastDiv gqa;
     const int* prefix_pages;  // the prefix form
@@ -67,8 +69,6 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPfTile * kRowBytes], s_k1[kPfTile * kRowBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_v0[kPfTile * kRowBytes], s_v1[kPfTile * kRowBytes];
-    __shared__ uint32_t s_pre[kPfThreads + 1];
-    __shared__ FlashTile s_tile;
     __shared__ int s_lo[4], s_hi[4];
     __shared__ uint32_t s_gone[2][4];
 
@@ -89,36 +89,52 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
         const long at0 = (long)blockIdx.x * kPfThreads + tid, step = (long)gridDim.x * kPfThreads;
         for (long i = min(max(p.cu[p.c.batch], 0), p.rows) * chunks + at0; i < p.rows * chunks; i += step)
             *reinterpret_cast<u32x4*>(p.out + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-        const int per_thread = (p.c.batch + kPfThreads - 1) / kPfThreads;
-        const int b0 = min(tid * per_thread, p.c.batch), b1 = min(b0 + per_thread, p.c.batch);
+        // The tiles of all sequences, counted in every wave for itself: lane l holds
+        // sequences per * l .. + per - 1.
+        const int per = (p.c.batch + 63) / 64;
+        const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
         auto tokens_of = [&](int b, int& row0) {   // query tokens of sequence b, kept inside q
             row0 = max(p.cu[b], 0);
             return max(min(p.cu[b + 1], p.rows) - row0, 0);
         };
+        auto tiles_of = [&](int b) {
+            int row0;
+            return (uint32_t)(tokens_of(b, row0) * G + kPfRows - 1) / kPfRows;
+        };
         uint32_t mine = 0;
-        int row0;
-        for (int b = b0; b < b1; ++b) mine += (uint32_t)(tokens_of(b, row0) * G + kPfRows - 1) / kPfRows;
-        const uint32_t total = block_totals(mine, s_pre);
+        for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+        const uint32_t incl = wave_scan(mine);
+        const uint32_t total = lane_u32(incl, 63);
         if (item >= total) return;   // the grid is an upper bound
-        const uint32_t x = total - 1 - item;   // a prompt's last tiles, which see the most keys, first
-        if (s_pre[tid] <= x && x < s_pre[tid + 1]) {
-            uint32_t at = s_pre[tid];
-            for (int b = b0; b < b1; ++b) {
-                FlashTile f;
-                f.rows = tokens_of(b, f.row0);
-                const uint32_t t = (uint32_t)(f.rows * G + kPfRows - 1) / kPfRows;
-                if (x < at + t) {
-                    f.b = b;
-                    f.tile = (int)(x - at);
-                    f.pos0 = p.c.lens[b] - (p.cu[b + 1] - f.row0);
-                    s_tile = f;
+        // A prompt's last tiles see the most keys and come first. Where all workgroups
+        // run at once, two per CU, the second half goes the other way, so that a CU's two
+        // have about the same work together as another's.
+        const uint32_t half = p.per_round / (uint32_t)p.c.n_kv_heads;   // tiles of one workgroup per CU
+        uint32_t x = total - 1 - item;
+        if (item >= half && total <= 2 * half) x = item - half;
+        const int at_lane = __ffsll((unsigned long long)__ballot(incl > x)) - 1;
+        uint32_t first = lane_u32(incl - mine, at_lane);   // the sequence's first tile
+        int b = at_lane;
+        if (per > 1) {
+            b = at_lane * per;
+            const int last_b = min(b + per, p.c.batch);
+            for (;; b += 64) {   // ends: the lane's sequences hold tile x
+                const uint32_t n = b + lane < last_b ? tiles_of(b + lane) : 0u;
+                const uint32_t upto = wave_scan(n);
+                const uint64_t found = __ballot(first + upto > x);
+                if (found != 0 || b + 64 >= last_b) {
+                    const int l = found != 0 ? __ffsll((unsigned long long)found) - 1 : 0;
+                    first += lane_u32(upto - n, l);
+                    b += l;
                     break;
                 }
-                at += t;
+                first += lane_u32(upto, 63);
             }
         }
-        __syncthreads();
-        ft = s_tile;
+        ft.b = __builtin_amdgcn_readfirstlane(b);
+        ft.rows = tokens_of(ft.b, ft.row0);
+        ft.tile = (int)(x - first);
+        ft.pos0 = p.c.lens[ft.b] - (p.cu[ft.b + 1] - ft.row0);
     }
     const int n_rows = ft.rows * G;
     const int r_wave = ft.tile * kPfRows + 32 * wave;   // the wave's first row
@@ -161,51 +177,46 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
     const int* table_row = PREFIX ? p.prefix_pages : p.c.table + (long)ft.b * p.c.max_pages;
-    const int key_end = PREFIX ? p.prefix_len : p.c.capacity;   // keys with a table entry
-    const int keys = __builtin_amdgcn_readfirstlane(min(end, key_end));
     auto look_up = [&](int i0) {   // lane l: octet 2 w + l % 2 of tile i0 + l / 2
-        const int i = i0 + (lane >> 1);
-        return octet_offset<D>(p.c, table_row, kvh, begin + kPfTile * i + 16 * wave + 8 * (lane & 1), keys);
+        return octet_offset<D>(p.c, table_row, kvh,
+                               begin + kPfTile * (i0 + (lane >> 1)) + 16 * wave + 8 * (lane & 1), end);
     };
-    long off = look_up(0), off_next = look_up(32);
-    // Copy instruction i fills rows kRowsPerCopy i .. of the wave's 16: lane l
-    // writes chunk slot l % CPR of row l / CPR, i.e. the chunk that the permutation puts there.
+    long off = look_up(0), off_next = tiles > 32 ? look_up(32) : -1L;
+    // Copy instruction c fills rows kRowsPerCopy c .. of the wave's 16: lane l writes
+    // chunk slot l % CPR of row l / CPR, i.e. the chunk that the permutation puts there.
     const int crow = lane / CPR, cslot = lane % CPR;
-    auto issue = [&](uint8_t* sk, uint8_t* sv, int i) {
+    __amdgpu_buffer_rsrc_t rk[2], rv[2];   // of the wave's two octets of the tile being copied
+    // Rows behind the end, or without a page, lie outside the buffer's range: the copy
+    // writes zeros for them. Their scores are masked, and their values must not turn
+    // 0 * v into NaN. Where there is no tile i nothing is read.
+    auto prepare = [&](int i) {
         if ((i & 31) == 0 && i) {
             off = off_next;
-            off_next = look_up(i + 32);
+            if (i + 32 < tiles) off_next = look_up(i + 32);
         }
-        const int hi = (int)(off >> 32), lo = (int)(uint32_t)off;
+        const int l0 = 2 * (i & 31), hi = (int)(off >> 32), lo = (int)(uint32_t)off;
         uint32_t gone = 0;
 #pragma unroll
-        for (int cp = 0; cp < kCopies; ++cp) {
-            const int row = kRowsPerCopy * cp + crow;                // of the wave's 16
-            const int octet = (kRowsPerCopy * cp) / 8;
-            const int l0 = 2 * (i & 31) + octet;
-            const long at = ((long)__builtin_amdgcn_readlane(hi, l0) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, l0);
-            const int trow = 16 * wave + row;                        // of the tile
-            const uint32_t kc = (uint32_t)(cslot ^ (D == 128 ? trow & 15 : trow & 7));
-            const uint32_t vc = (uint32_t)(cslot ^ (D == 128 ? (trow & 3) << 2 : ((trow >> 1) & 1) << 2));
-            uint8_t* lk = sk + (16 * wave + kRowsPerCopy * cp) * kRowBytes;
-            uint8_t* lv = sv + (16 * wave + kRowsPerCopy * cp) * kRowBytes;
-            if (at < 0) gone |= 1u << octet;
-            // Rows behind the end, or without a page, are zeroed: their scores are
-            // masked, and their values must not turn 0 * v into NaN.
-            if (at >= 0 && begin + kPfTile * i + trow < end) {
-                const uint32_t ro = (uint32_t)((row & 7) * kRowBytes);
-                const __amdgpu_buffer_rsrc_t rk = make_buffer_rsrc(p.c.k + at, 8 * kRowBytes);
-                const __amdgpu_buffer_rsrc_t rv = make_buffer_rsrc(p.c.v + at, 8 * kRowBytes);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)lk, 16,
-                                                         (int)(ro + 16 * kc), 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)lv, 16,
-                                                         (int)(ro + 16 * vc), 0, 0, 0);
-            } else {
-                *reinterpret_cast<u32x4*>(lk + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-                *reinterpret_cast<u32x4*>(lv + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
-            }
+        for (int o8 = 0; o8 < 2; ++o8) {
+            const int h32 = __builtin_amdgcn_readlane(hi, l0 + o8);
+            const long at = h32 < 0 ? 0L : ((long)h32 << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, l0 + o8);
+            const int rows = __builtin_amdgcn_readfirstlane(
+                h32 < 0 ? 0 : min(max(end - (begin + kPfTile * i + 16 * wave + 8 * o8), 0), 8));
+            rk[o8] = make_buffer_rsrc(p.c.k + at, (uint32_t)(rows * kRowBytes));
+            rv[o8] = make_buffer_rsrc(p.c.v + at, (uint32_t)(rows * kRowBytes));
+            gone |= h32 < 0 ? 1u << o8 : 0u;
         }
         if (lane == 0) s_gone[i & 1][wave] = gone;
+    };
+    auto copy = [&](uint8_t* dst, bool is_v, int c) {
+        const int row = kRowsPerCopy * c + crow, trow = 16 * wave + row;   // of the wave's 16, of the tile
+        const int chunk = cslot ^ (is_v ? (D == 128 ? (trow & 3) << 2 : ((trow >> 1) & 1) << 2)
+                                        : (D == 128 ? trow & 15 : trow & 7));
+        const int octet = (kRowsPerCopy * c) / 8;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            is_v ? rv[octet] : rk[octet],
+            (__attribute__((address_space(3))) void*)(dst + (16 * wave + kRowsPerCopy * c) * kRowBytes), 16,
+            (row & 7) * kRowBytes + 16 * chunk, 0, 0, 0);
     };
 
     f32x16 o[CB];
@@ -213,7 +224,12 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[cb][e] = 0.0f;
-    float m_run = kNoMax, l_run = 0.0f;
+    float m_run = kNoMax, l_run = 0.0f;   // of row n; l_run: this lane's tokens only
+    // Scores as they come from the products, times mult, are in the log2 domain. A
+    // negative scale is multiplied in beforehand, like a cap or a bias: the masked
+    // value must stay the smallest.
+    const bool modified = p.s.cap_in != 0.0f || p.s.slopes != nullptr || p.s.scale_log2 <= 0.0f;
+    const float mult = modified ? 1.0f : p.s.scale_log2;
 
     // LDS offsets of this lane's operand reads.
     const uint32_t k_row = (uint32_t)(n * kRowBytes);
@@ -223,9 +239,13 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     const uint32_t v_sw = (uint32_t)(D == 128 ? vr << 2 : (vr >> 1) << 2);
     const uint32_t v_at = (uint32_t)((4 * h + vr) * kRowBytes) + 8 * (lane & 1);
 
-    auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i) {
+    // copies(0), copies(1): the next tile's copies of K and of V are issued behind the
+    // products of the two blocks' scores, whose time hides them: before all work they
+    // waited for the CU's one vector memory path, 1000 of a tile's 3900 cycles (us, a
+    // prompt of 8192 tokens 562 -> 550, 2048 tokens 58.2 -> 54.5, chunks 198 -> 189;
+    // spread further down to the products with V they come too late: 542, 56.9, 210).
+    auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i, auto copies) {
         const int t0 = begin + kPfTile * i;
-        if (!live || t0 > pos_hi || t0 + kPfTile <= oldest(pos_lo)) return;   // no row sees a key of it
         float sc[32];
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
@@ -238,19 +258,22 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
                                  qb[ks], acc);
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[16 * blk + e] = acc[e];
-        }
-        if (p.s.cap_in != 0.0f) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) sc[e] *= p.s.scale_log2;
+            copies(blk);
         }
         // value e belongs to token t0 + 4 h + 8 (e / 4) + e % 4
         const int tk = t0 + 4 * h;
-        if (p.s.slopes) {
+        if (modified) {   // the cap and the bias, in the log2 domain: `mult` is 1 then
+            if (p.s.cap_in != 0.0f) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
+                for (int e = 0; e < 32; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] *= p.s.scale_log2;
+            }
+            if (p.s.slopes) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
+            }
         }
         uint32_t gone = 0;   // bit o: octet o of the tile has no page
 #pragma unroll
@@ -264,30 +287,46 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
                 if (tok < old || tok >= lim || ((gone >> (e >> 2)) & 1u)) sc[e] = -INFINITY;
             }
         }
-        float mx = sc[0];
+        // Exponents (of 2^kPShift p) against the reference m_run, which is moved only
+        // when a score passes it by kPLag: 2^kPShift p stays below 2^(kPShift + kPLag),
+        // and most tiles rescale nothing.
+        float t[32], mx = -INFINITY;
+        const float sub = m_run - kPShift;
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e]);
-        if (__any(mx > m_run)) {
-            mx = fmaxf(xor32_max(mx), m_run);
-            const float a = __builtin_amdgcn_exp2f(m_run - mx);
-            m_run = mx;
+        for (int e = 0; e < 32; ++e) {
+            t[e] = fmaf(sc[e], mult, -sub);
+            mx = fmaxf(mx, t[e]);
+        }
+        if (__any(mx > kPShift + kPLag)) {
+            mx = fmaxf(xor32_max(mx), kPShift);
+            float m_new = sub + mx;
+            if (m_run == kNoMax) {   // the first keys: the scores themselves (m_run + mx has none of their bits)
+                m_new = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) m_new = fmaxf(m_new, sc[e] * mult);
+                m_new = fmaxf(xor32_max(m_new), kNoMax);
+            }
+            const float a = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
             l_run *= a;
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[cb][e] *= a;
-        }
-        const float sub = m_run - kPShift;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            sc[e] = __builtin_amdgcn_exp2f(sc[e] - sub);
-            l_run += sc[e];
+            for (int e = 0; e < 32; ++e) t[e] = fmaf(sc[e], mult, kPShift - m_run);
         }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) t[e] = __builtin_amdgcn_exp2f(t[e]);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
             u32x4 pb;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pb[e] = Hf::pack(sc[8 * kk + 2 * e], sc[8 * kk + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t p2 = Hf::pack(t[8 * kk + 2 * e], t[8 * kk + 2 * e + 1]);
+                pb[e] = p2;
+                l_run = Hf::add_pair(p2, l_run);   // the sum of what the products use
+            }
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 const uint8_t* a = sv + v_at + 16 * kk * kRowBytes + 16 * ((v_chunk + 4 * cb) ^ v_sw);
@@ -307,14 +346,32 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     auto turn = [&](uint8_t* k_cur, uint8_t* v_cur, uint8_t* k_far, uint8_t* v_far, int i) {
         __builtin_amdgcn_s_waitcnt(0);
         asm volatile("s_barrier" ::: "memory");
-        if (i + 1 < tiles) issue(k_far, v_far, i + 1);
-        compute(k_cur, v_cur, i);
+        prepare(i + 1);
+        auto copies = [&](int v) {
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) copy(v ? v_far : k_far, v, c);
+        };
+        const int t0 = begin + kPfTile * i;
+        if (live && t0 <= pos_hi && t0 + kPfTile > oldest(pos_lo)) {
+            compute(k_cur, v_cur, i, copies);
+        } else {   // no row of this wave sees a key of it
+            copies(0);
+            copies(1);
+        }
     };
-    if (tiles > 0) issue(s_k0, s_v0, 0);
+    if (tiles > 0) {
+        prepare(0);
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            copy(s_k0, false, c);
+            copy(s_v0, true, c);
+        }
+    }
     for (int i = 0; i < tiles; i += 2) {
         turn(s_k0, s_v0, s_k1, s_v1, i);
         if (i + 1 < tiles) turn(s_k1, s_v1, s_k0, s_v0, i + 1);
     }
+    __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup
 
     l_run = xor32_sum(l_run);
     if (!live || r_wave + n >= n_rows) return;
@@ -345,6 +402,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 
 namespace {
 
+#ifndef LLMIK_PX_WGS
+#define LLMIK_PX_WGS 2L
+#endif
 struct PagedPrefixPlan {
     int row_tiles, splits, chunk;
     size_t off_o, off_ml, bytes;
@@ -358,7 +418,7 @@ PagedPrefixPlan plan_prefix(int batch, int n_heads, int n_kv_heads, int head_dim
     pl.row_tiles = (int)((rows + kPfRows - 1) / kPfRows);
     const long base = (long)pl.row_tiles * n_kv_heads;
     const long most = (prefix_len + 2 * kPfTile - 1) / (2 * kPfTile);   // two tiles a split at least
-    long splits = std::max(1L, std::min({2L * cus / std::max(base, 1L), most, 64L}));
+    long splits = std::max(1L, std::min({(LLMIK_PX_WGS * cus) / std::max(base, 1L), most, 64L}));
     const long tiles = (prefix_len + kPfTile - 1) / kPfTile;
     pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;
     pl.splits = (prefix_len + pl.chunk - 1) / pl.chunk;
@@ -377,6 +437,7 @@ PagedFlashParams flash_params(const PagedLaunch& a) {
     p.s = score_opts(a);
     p.cu = a.cu;
     p.rows = a.rows;
+    p.per_round = (uint32_t)device_cu_count();
     p.n_heads = a.n_heads;
     p.gqa = FastDiv::of((uint32_t)(a.n_heads / a.n_kv_heads));
     return p;
