@@ -536,11 +536,14 @@ LLMIK_API llmik_status llmik_paged_decode_attention(const llmik_paged_cache* cac
 /*
  * q, out [rows, n_heads, head_dim]: the new tokens of every sequence (rows as
  * llmik_rope_paged_append's, cu_tokens required), each over the keys of its own
- * sequence up to its position. No workspace.
+ * sequence up to its position. The workspace (0 bytes for many rows) depends on the
+ * shapes, not on the lengths.
  */
+LLMIK_API size_t llmik_paged_prefill_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows);
 LLMIK_API llmik_status llmik_paged_prefill_attention(const llmik_paged_cache* cache, const void* q,
                                                      const int* cu_tokens, void* out, int rows, int n_heads,
-                                                     const llmik_score_options* options, void* stream);
+                                                     const llmik_score_options* options, void* workspace,
+                                                     size_t workspace_bytes, void* stream);
 
 /*
  * llmik_paged_decode_attention for sequences that share their first prefix_len

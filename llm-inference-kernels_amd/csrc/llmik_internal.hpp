@@ -179,6 +179,7 @@ struct PagedAppend {
     bool bf16, table_f32;
 };
 size_t paged_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity);
+size_t paged_prefill_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
 size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len);
 int launch_paged_append(const PagedAppend& a, hipStream_t stream);
 int launch_paged_decode(const PagedLaunch& a, const PagedPrefixParts& pre, hipStream_t stream);

@@ -63,6 +63,17 @@ int check_options(const llmik_score_options* o) {
     return LLMIK_OK;
 }
 
+// A ragged call's rows: its row tiles (of 128 rows per KV head) are counted in 32 bits.
+int check_rows(const llmik_paged_cache* c, int n_heads, int rows) {
+    const int st = check_shapes(c, n_heads);
+    if (st != LLMIK_OK) return st;
+    if (rows < 0) return invalid("rows must be >= 0");
+    const long per_kv = (long)rows * (n_heads / c->n_kv_heads);
+    if (per_kv >= INT_MAX - 256 || (per_kv / 128 + c->batch + 1) * c->n_kv_heads * 256 * 4 > kMaxThreads)
+        return unsupported("too many rows");
+    return LLMIK_OK;
+}
+
 int check_q(const void* q, const void* out) {
     if (!q || !out) return invalid("null q/out pointer");
     if (!aligned(q, 16) || !aligned(out, 16)) return misaligned("q/out must be 16-byte aligned");
@@ -168,25 +179,30 @@ LLMIK_API llmik_status llmik_paged_decode_attention(const llmik_paged_cache* cac
     return launch_paged_decode(a, PagedPrefixParts{}, as_stream(stream));
 }
 
+LLMIK_API size_t llmik_paged_prefill_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows) {
+    if (check_rows(cache, n_heads, rows) != LLMIK_OK || cache->batch == 0 || rows == 0) return 0;
+    return paged_prefill_workspace(cache->batch, rows, n_heads, cache->n_kv_heads, cache->head_dim,
+                                   capacity_of(*cache));
+}
+
 LLMIK_API llmik_status llmik_paged_prefill_attention(const llmik_paged_cache* cache, const void* q,
                                                      const int* cu_tokens, void* out, int rows, int n_heads,
-                                                     const llmik_score_options* options, void* stream) {
+                                                     const llmik_score_options* options, void* workspace,
+                                                     size_t workspace_bytes, void* stream) {
     int st = check_cache(cache, n_heads);
     if (st == LLMIK_OK) st = check_options(options);
+    if (st == LLMIK_OK) st = check_rows(cache, n_heads, rows);
     if (st != LLMIK_OK) return st;
-    if (rows < 0) return invalid("rows must be >= 0");
     if (rows == 0) return LLMIK_OK;
     if (cache->batch == 0) return invalid("rows without a sequence");
     if (cu_tokens == nullptr) return invalid("null cu_tokens pointer");
     if (!aligned(cu_tokens, 4)) return misaligned("cu_tokens must be 4-byte aligned");
     if ((st = check_q(q, out)) != LLMIK_OK) return st;
-    const long per_kv = (long)rows * (n_heads / cache->n_kv_heads);
-    if (per_kv >= INT_MAX - 256 ||
-        (per_kv / 128 + cache->batch + 1) * cache->n_kv_heads * 256 > kMaxThreads)
-        return unsupported("too many rows");
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.cu = cu_tokens;
     a.rows = rows;
+    a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
     return launch_paged_prefill(a, as_stream(stream));
 }
 

@@ -54,8 +54,9 @@ struct PagedDecodeParams {
     int few_steps;        // workgroups that few tiles are spread over, one tile per wave
 };
 
-constexpr int kPieceUnits = 4;
+constexpr int kPieceUnits = 6;
 constexpr int kUncutTiles = 12;
+constexpr int kEachTiles = 24;
 
 // A sequence's length, its live keys [begin, end) and their 32-token tiles.
 // Every sequence has one tile at least, so that its rows are written.
@@ -90,23 +91,37 @@ __global__ __launch_bounds__(kPdThreads, kPdPerCu) void paged_decode_kernel(Page
     const int per = (p.c.batch + 63) / 64;
     const uint32_t slabs = (uint32_t)(p.c.n_kv_heads * p.n_chunks);   // of one sequence
     const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
-    uint32_t steps = 0, mine = 0;
+    uint32_t steps = 0, mine = 0, longest = 0;
     int len0 = 0;   // the lane's last length (its only one where per is 1)
     for (int b = b0; b < b1; ++b) {
         len0 = p.c.lens[b];
         const uint32_t tiles = (uint32_t)keys_of(p, len0).tiles;
+        longest = max(longest, tiles);
         steps += (tiles + kPdWaves - 1) / kPdWaves * slabs;
         mine += (tiles + kPieceUnits) * slabs;
     }
-    // The work in units of a tile's time. Where one workgroup per CU can do with one
-    // tile per wave, every slab is cut into such steps. Otherwise the units are cut
-    // evenly, and a slab counts kPieceUnits more than its tiles, the time of its
-    // look-ups and its join. us, 0, 2 -> 4 units: 32 ragged sequences 45.9, 33.4 ->
-    // 33.2, 256 of 10 .. 1000 tokens 130, 62.7 -> 55.7.
+    // The work in units of a tile's time, cut into equal shares. Three ways, by the
+    // longest slab and the number of tiles:
+    //   each: there are no more slabs than workgroups, and not many fewer, and none is
+    //         long: one slab each;
+    //   few:  one workgroup per CU can do with one tile per wave: slabs are cut into
+    //         such steps;
+    //   else: the units are cut evenly, where a slab counts kPieceUnits more than its
+    //         tiles, the time of its look-ups and its join.
+    // GPU us: 64 sequences of 10 .. 300 tokens 11.9 cut evenly, 10.8 each; 32 ragged
+    // ones 45.9, 33.4, 33.2 with 0, 2, 4 units; 256 of 10 .. 1000 tokens 130, 62.7, 55.7
+    // (6: the same; 4 sequences of 500 .. 2000 tokens, 64 heads 12.5, 11.6 with 4, 6).
     uint32_t incl = wave_scan(steps);
     uint32_t total = lane_u32(incl, 63), share = kPdWaves, piece = 0;
-    const bool few = total <= (uint32_t)p.few_steps;
-    if (few) {
+    const uint32_t all_slabs = (uint32_t)p.c.batch * slabs;
+    const bool each = all_slabs <= gridDim.x && all_slabs >= gridDim.x / 4 && !__any(longest > (uint32_t)kEachTiles);
+    const bool few = !each && total <= (uint32_t)p.few_steps;
+    if (each) {
+        mine = (uint32_t)(b1 - b0) * slabs;
+        incl = (uint32_t)b1 * slabs;
+        total = all_slabs;
+        share = 1;
+    } else if (few) {
         mine = steps * kPdWaves;
         incl *= kPdWaves;
         total *= kPdWaves;
@@ -117,7 +132,7 @@ __global__ __launch_bounds__(kPdThreads, kPdPerCu) void paged_decode_kernel(Page
         share = max((total + gridDim.x - 1) / gridDim.x, 2u * kPdWaves);
     }
     auto cost_of = [&](int tiles) {
-        return few ? (uint32_t)(tiles + kPdWaves - 1) / kPdWaves * kPdWaves : (uint32_t)tiles + kPieceUnits;
+        return each ? 1u : few ? (uint32_t)(tiles + kPdWaves - 1) / kPdWaves * kPdWaves : (uint32_t)tiles + kPieceUnits;
     };
     uint32_t x = blockIdx.x * share;
     const uint32_t x_end = min(x + share, total);
@@ -154,7 +169,7 @@ __global__ __launch_bounds__(kPdThreads, kPdPerCu) void paged_decode_kernel(Page
         const uint32_t unit0 = seq0 + slab * cost;   // its first unit
         // The piece: tiles [first, last) of the slab, whose tile t is its unit piece + t.
         // A slab of few tiles is not cut: it is its first unit's workgroup's.
-        const bool uncut = tiles <= kUncutTiles;
+        const bool uncut = each || tiles <= kUncutTiles;
         const int first = uncut ? 0 : max((int)(x - unit0) - (int)piece, 0);
         const int last = uncut ? tiles : min(max((int)(min(unit0 + cost, x_end) - unit0) - (int)piece, 0), tiles);
         const bool skip = uncut ? x != unit0 : first >= last;

@@ -43,15 +43,97 @@ struct PagedFlashParams {
     uint32_t per_round;       // workgroups of one per CU
     int n_heads;
     FastDiv gqa;
+    int splits;               // parts of a tile's keys at most (the prefix form: exactly)
+    float* part_o;            // ragged: [tiles * n_kv_heads, splits, kPfRows, D] and (m, l); prefix: [n_kv_heads,
+    float* part_ml;           //   rows, splits, D] and (m, l)
     const int* prefix_pages;  // the prefix form
-    int prefix_len, splits, chunk;
-    float* part_o;
-    float* part_ml;
+    int prefix_len, chunk;
 };
 
-struct FlashTile {   // of the ragged form
-    int b, tile, row0, rows, pos0;   // sequence, its tile, first row of q, its query tokens, the first one's position
+// A workgroup's 128 rows: row tile `tile` of sequence b, whose `rows` query tokens
+// begin at row row0 of q and at position pos0. (The prefix form: row i is sequence i.)
+struct RowTile {
+    int b, tile, row0, rows, pos0;
 };
+
+__device__ __forceinline__ int oldest_key(const ScoreOpts& s, int pos) {   // of those that a query at pos sees
+    return pos >= s.window ? pos - s.window + 1 : 0;
+}
+
+// Row tile number `item` of the call, false past the last (the grid is an upper
+// bound). Every wave counts the sequences' tiles for itself: lane l holds sequences
+// per * l .. + per - 1.
+__device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t item, RowTile& t) {
+    const int lane = threadIdx.x & 63;
+    const int per = (p.c.batch + 63) / 64;
+    const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+    auto tokens_of = [&](int b, int& row0) {   // query tokens of sequence b, kept inside q
+        row0 = max(p.cu[b], 0);
+        return max(min(p.cu[b + 1], p.rows) - row0, 0);
+    };
+    auto tiles_of = [&](int b) {
+        int row0;
+        return (uint32_t)(tokens_of(b, row0) * (int)p.gqa.d + kPfRows - 1) / kPfRows;
+    };
+    uint32_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    const uint32_t incl = wave_scan(mine);
+    const uint32_t total = lane_u32(incl, 63);
+    if (item >= total) return false;
+    // A prompt's last tiles see the most keys and come first. Where all workgroups
+    // run at once, two per CU, the second half goes the other way, so that a CU's two
+    // have about the same work together as another's.
+    const uint32_t half = p.per_round / (uint32_t)(p.c.n_kv_heads * p.splits);   // tiles of one workgroup per CU
+    uint32_t x = total - 1 - item;
+    if (item >= half && total <= 2 * half) x = item - half;
+    const int at_lane = __ffsll((unsigned long long)__ballot(incl > x)) - 1;
+    uint32_t first = lane_u32(incl - mine, at_lane);   // the sequence's first tile
+    int b = at_lane;
+    if (per > 1) {
+        b = at_lane * per;
+        const int last_b = min(b + per, p.c.batch);
+        for (;; b += 64) {   // ends: the lane's sequences hold tile x
+            const uint32_t n = b + lane < last_b ? tiles_of(b + lane) : 0u;
+            const uint32_t upto = wave_scan(n);
+            const uint64_t found = __ballot(first + upto > x);
+            if (found != 0 || b + 64 >= last_b) {
+                const int l = found != 0 ? __ffsll((unsigned long long)found) - 1 : 0;
+                first += lane_u32(upto - n, l);
+                b += l;
+                break;
+            }
+            first += lane_u32(upto, 63);
+        }
+    }
+    t.b = __builtin_amdgcn_readfirstlane(b);
+    t.rows = __builtin_amdgcn_readfirstlane(tokens_of(t.b, t.row0));
+    t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
+    t.tile = __builtin_amdgcn_readfirstlane((int)(x - first));
+    t.pos0 = __builtin_amdgcn_readfirstlane(p.c.lens[t.b] - (p.cu[t.b + 1] - t.row0));
+    return true;
+}
+
+// The keys [begin, end) that a row tile's rows see, in `tiles` tiles of 64 tokens, and
+// the parts (of part_tiles tiles) that they are cut into: p.splits, but each of
+// kMinPart tiles at least.
+constexpr int kMinPart = 8;
+constexpr int kMaxParts = 8;
+struct TileKeys {
+    int begin, end, tiles, parts, part_tiles;
+};
+__device__ __forceinline__ TileKeys keys_of_tile(const PagedFlashParams& p, const RowTile& t) {
+    const int n_rows = t.rows * (int)p.gqa.d, r0 = t.tile * kPfRows;
+    const int lo = t.pos0 + (int)p.gqa.div((uint32_t)r0);
+    const int hi = t.pos0 + (int)p.gqa.div((uint32_t)min(r0 + kPfRows, n_rows) - 1u);
+    TileKeys k;
+    k.begin = oldest_key(p.s, lo) / kPfTile * kPfTile;
+    k.end = min(p.c.capacity, hi + 1);
+    k.tiles = k.end > k.begin ? (k.end - k.begin + kPfTile - 1) / kPfTile : 0;
+    k.parts = max(min(p.splits, k.tiles / kMinPart), 1);
+    k.part_tiles = (k.tiles + k.parts - 1) / k.parts;
+    if (k.parts > 1) k.parts = (k.tiles + k.part_tiles - 1) / k.part_tiles;
+    return k;
+}
 
 }  // namespace
 
@@ -73,15 +155,14 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     __shared__ uint32_t s_gone[2][4];
 
     const int kvh = (int)blockIdx.x % p.c.n_kv_heads;
-    const uint32_t item = blockIdx.x / (uint32_t)p.c.n_kv_heads;
+    const uint32_t item = blockIdx.x / (uint32_t)(p.c.n_kv_heads * p.splits);
+    const int split = (int)(blockIdx.x / (uint32_t)p.c.n_kv_heads % (uint32_t)p.splits);
     const int G = (int)p.gqa.d;
 
     // ---- the workgroup's rows ----
-    FlashTile ft{};
-    int split = 0;
+    RowTile ft{};
     if constexpr (PREFIX) {
-        split = (int)(item % (uint32_t)p.splits);
-        ft.tile = (int)(item / (uint32_t)p.splits);
+        ft.tile = (int)item;
         ft.rows = p.c.batch;
     } else {
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
@@ -89,52 +170,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
         const long at0 = (long)blockIdx.x * kPfThreads + tid, step = (long)gridDim.x * kPfThreads;
         for (long i = min(max(p.cu[p.c.batch], 0), p.rows) * chunks + at0; i < p.rows * chunks; i += step)
             *reinterpret_cast<u32x4*>(p.out + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-        // The tiles of all sequences, counted in every wave for itself: lane l holds
-        // sequences per * l .. + per - 1.
-        const int per = (p.c.batch + 63) / 64;
-        const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
-        auto tokens_of = [&](int b, int& row0) {   // query tokens of sequence b, kept inside q
-            row0 = max(p.cu[b], 0);
-            return max(min(p.cu[b + 1], p.rows) - row0, 0);
-        };
-        auto tiles_of = [&](int b) {
-            int row0;
-            return (uint32_t)(tokens_of(b, row0) * G + kPfRows - 1) / kPfRows;
-        };
-        uint32_t mine = 0;
-        for (int b = b0; b < b1; ++b) mine += tiles_of(b);
-        const uint32_t incl = wave_scan(mine);
-        const uint32_t total = lane_u32(incl, 63);
-        if (item >= total) return;   // the grid is an upper bound
-        // A prompt's last tiles see the most keys and come first. Where all workgroups
-        // run at once, two per CU, the second half goes the other way, so that a CU's two
-        // have about the same work together as another's.
-        const uint32_t half = p.per_round / (uint32_t)p.c.n_kv_heads;   // tiles of one workgroup per CU
-        uint32_t x = total - 1 - item;
-        if (item >= half && total <= 2 * half) x = item - half;
-        const int at_lane = __ffsll((unsigned long long)__ballot(incl > x)) - 1;
-        uint32_t first = lane_u32(incl - mine, at_lane);   // the sequence's first tile
-        int b = at_lane;
-        if (per > 1) {
-            b = at_lane * per;
-            const int last_b = min(b + per, p.c.batch);
-            for (;; b += 64) {   // ends: the lane's sequences hold tile x
-                const uint32_t n = b + lane < last_b ? tiles_of(b + lane) : 0u;
-                const uint32_t upto = wave_scan(n);
-                const uint64_t found = __ballot(first + upto > x);
-                if (found != 0 || b + 64 >= last_b) {
-                    const int l = found != 0 ? __ffsll((unsigned long long)found) - 1 : 0;
-                    first += lane_u32(upto - n, l);
-                    b += l;
-                    break;
-                }
-                first += lane_u32(upto, 63);
-            }
-        }
-        ft.b = __builtin_amdgcn_readfirstlane(b);
-        ft.rows = tokens_of(ft.b, ft.row0);
-        ft.tile = (int)(x - first);
-        ft.pos0 = p.c.lens[ft.b] - (p.cu[ft.b + 1] - ft.row0);
+        if (!find_tile(p, item, ft)) return;
     }
     const int n_rows = ft.rows * G;
     const int r_wave = ft.tile * kPfRows + 32 * wave;   // the wave's first row
@@ -144,36 +180,46 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     const int head = kvh * G + (r - qi * G);
     const long q_row = (PREFIX ? (long)qi : (long)ft.row0 + qi) * p.n_heads + head;
     const int pos = PREFIX ? p.c.lens[qi] - 1 : ft.pos0 + qi;
-    int pos_lo = pos, pos_hi = pos;                     // of the wave's rows
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
-        pos_hi = max(pos_hi, __shfl_xor(pos_hi, d));
-    }
-    pos_lo = __builtin_amdgcn_readfirstlane(pos_lo);
-    pos_hi = __builtin_amdgcn_readfirstlane(pos_hi);
-    if (lane == 0) {
-        s_lo[wave] = live ? pos_lo : INT_MAX;
-        s_hi[wave] = live ? pos_hi : -1;
-    }
-    __syncthreads();
-    const int wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-    const int wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-
-    // ---- the keys any of them sees, [begin, end), in 64-token tiles ----
-    auto oldest = [&](int at) { return at >= p.s.window ? at - p.s.window + 1 : 0; };
-    int begin = PREFIX ? split * p.chunk : 0;
-    int end = PREFIX ? min(begin + p.chunk, p.prefix_len) : p.c.capacity;
-    begin = max(begin, oldest(wg_lo)) / kPfTile * kPfTile;
-    end = min(end, wg_hi + 1);
-    const int tiles = __builtin_amdgcn_readfirstlane(end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-
     u32x4 qb[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qb[ks] = load16(p.q + q_row * D + 16 * ks + 8 * h);
     const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
+
+    // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
+    auto oldest = [&](int at) { return oldest_key(p.s, at); };
+    int begin, end, tiles, parts = 1, pos_lo, pos_hi;   // pos_lo, pos_hi: of the wave's rows
+    if constexpr (PREFIX) {
+        pos_lo = pos_hi = pos;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
+            pos_hi = max(pos_hi, __shfl_xor(pos_hi, d));
+        }
+        if (lane == 0) {
+            s_lo[wave] = live ? pos_lo : INT_MAX;
+            s_hi[wave] = live ? pos_hi : -1;
+        }
+        __syncthreads();
+        const int lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+        const int hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+        begin = max(split * p.chunk, oldest(lo)) / kPfTile * kPfTile;
+        end = min(min(split * p.chunk + p.chunk, p.prefix_len), hi + 1);
+        tiles = end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0;
+    } else {
+        pos_lo = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave, n_rows - 1));
+        pos_hi = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave + 31, n_rows - 1));
+        const TileKeys k = keys_of_tile(p, ft);
+        parts = k.parts;
+        if (split >= parts) return;
+        begin = k.begin + split * k.part_tiles * kPfTile;
+        end = min(k.end, begin + k.part_tiles * kPfTile);
+        tiles = min(k.part_tiles, k.tiles - split * k.part_tiles);
+    }
+    pos_lo = __builtin_amdgcn_readfirstlane(pos_lo);
+    pos_hi = __builtin_amdgcn_readfirstlane(pos_hi);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
 
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
     const int* table_row = PREFIX ? p.prefix_pages : p.c.table + (long)ft.b * p.c.max_pages;
@@ -375,8 +421,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 
     l_run = xor32_sum(l_run);
     if (!live || r_wave + n >= n_rows) return;
-    if constexpr (PREFIX) {
-        const long at = ((long)kvh * n_rows + r) * p.splits + split;
+    if (PREFIX || parts > 1) {
+        const long at = PREFIX ? ((long)kvh * n_rows + r) * p.splits + split
+                               : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + 32 * wave + n;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
@@ -398,13 +445,58 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     }
 }
 
+// The parts of the ragged form's row tiles joined: a workgroup takes 32 rows of a
+// tile, a thread four channels of every 256 * 4 / D-th row.
+template <bool BF, int D>
+__global__ __launch_bounds__(256) void paged_flash_join_kernel(PagedFlashParams p) {
+    using Hf = Half16<BF>;
+    const int kvh = (int)blockIdx.x % p.c.n_kv_heads;
+    const uint32_t item = blockIdx.x / (uint32_t)p.c.n_kv_heads;
+    RowTile ft;
+    if (!find_tile(p, item, ft)) return;
+    const int parts = __builtin_amdgcn_readfirstlane(keys_of_tile(p, ft).parts);
+    const int n_rows = ft.rows * (int)p.gqa.d;
+    if (parts == 1) return;
+    constexpr int kStep = 256 * 4 / D;
+    const int c4 = 4 * ((int)threadIdx.x % (D / 4));
+    const long at0 = ((long)item * p.c.n_kv_heads + kvh) * p.splits * kPfRows;
+#pragma unroll 2
+    for (int i = 0; i < 32; i += kStep) {
+        const int row = 32 * (int)blockIdx.y + i + (int)threadIdx.x / (D / 4);   // of the tile
+        const int r = ft.tile * kPfRows + row;
+        if (r >= n_rows) continue;
+        float m[kMaxParts], l[kMaxParts], top = kNoMax;
+        f32x4 v[kMaxParts];
+#pragma unroll
+        for (int u = 0; u < kMaxParts; ++u) {
+            const long at = at0 + (long)min(u, parts - 1) * kPfRows + row;
+            m[u] = p.part_ml[2 * at];
+            l[u] = p.part_ml[2 * at + 1];
+            v[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + c4);
+        }
+#pragma unroll
+        for (int u = 0; u < kMaxParts; ++u) top = fmaxf(top, m[u]);
+        float sum = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < kMaxParts; ++u) {
+            const float w = u < parts ? __builtin_amdgcn_exp2f(m[u] - top) : 0.0f;
+            sum = u < parts ? fmaf(l[u], w, sum) : sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = u < parts ? fmaf(v[u][e], w, o[e]) : o[e];
+        }
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        const int qi = (int)p.gqa.div((uint32_t)r);
+        const long q_row = ((long)ft.row0 + qi) * p.n_heads + kvh * (int)p.gqa.d + (r - qi * (int)p.gqa.d);
+        *reinterpret_cast<u32x2*>(p.out + q_row * D + c4) =
+            u32x2{Hf::pack(o[0] * inv, o[1] * inv), Hf::pack(o[2] * inv, o[3] * inv)};
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 namespace {
 
-#ifndef LLMIK_PX_WGS
-#define LLMIK_PX_WGS 2L
-#endif
 struct PagedPrefixPlan {
     int row_tiles, splits, chunk;
     size_t off_o, off_ml, bytes;
@@ -416,10 +508,13 @@ PagedPrefixPlan plan_prefix(int batch, int n_heads, int n_kv_heads, int head_dim
     PagedPrefixPlan pl{};
     const long rows = (long)batch * (n_heads / n_kv_heads);
     pl.row_tiles = (int)((rows + kPfRows - 1) / kPfRows);
-    const long base = (long)pl.row_tiles * n_kv_heads;
-    const long most = (prefix_len + 2 * kPfTile - 1) / (2 * kPfTile);   // two tiles a split at least
-    long splits = std::max(1L, std::min({(LLMIK_PX_WGS * cus) / std::max(base, 1L), most, 64L}));
+    const long base = std::max((long)pl.row_tiles * n_kv_heads, 1L);
+    // Splits of the prefix: two workgroups per CU, but beyond one per CU only in parts
+    // of eight tiles, as every part's results are written and read again, and never in
+    // less than two tiles. us, 64 sequences behind 8192 tokens, 16 and 32 splits 36.7,
+    // 38.7; 96 sequences of 64 heads behind 8000, 5 and 10 splits 63.1, 58.5.
     const long tiles = (prefix_len + kPfTile - 1) / kPfTile;
+    const long splits = std::max(1L, std::min({2L * cus / base, std::max(cus / base, tiles / 8), (tiles + 1) / 2, 64L}));
     pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;
     pl.splits = (prefix_len + pl.chunk - 1) / pl.chunk;
     pl.off_ml = align_up(paged_decode_workspace(batch, n_heads, n_kv_heads, head_dim, capacity), 256);
@@ -456,16 +551,62 @@ void launch_flash(const PagedLaunch& a, const PagedFlashParams& p, long workgrou
 
 }  // namespace
 
+// Row tiles of a ragged call at most, and the parts that their keys are cut into where
+// there are fewer than two workgroups per CU: at most as many as fill those.
+struct PagedPrefillPlan {
+    long tiles;
+    int splits;
+    size_t off_o, bytes;
+};
+
+namespace {
+PagedPrefillPlan plan_prefill(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity, int cus) {
+    PagedPrefillPlan pl{};
+    const long all = (long)rows * (n_heads / n_kv_heads);
+    pl.tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min(batch, rows));
+    const long base = std::max(pl.tiles * n_kv_heads, 1L);
+    pl.splits = (int)std::max(1L, std::min({2L * cus / base, (long)kMaxParts, capacity / (kPfTile * kMinPart)}));
+    if (pl.splits > 1) {
+        const size_t parts = (size_t)base * pl.splits * kPfRows;
+        pl.off_o = align_up(parts * 2 * sizeof(float), 256);
+        pl.bytes = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
+    }
+    return pl;
+}
+}  // namespace
+
+size_t paged_prefill_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity) {
+    const PagedPrefillPlan pl =
+        plan_prefill(batch, rows, n_heads, n_kv_heads, head_dim, capacity, device_cu_count());
+    return pl.splits > 1 ? kCounterBytes + pl.bytes : 0;
+}
+
 size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len) {
     return plan_prefix(batch, n_heads, n_kv_heads, head_dim, capacity, prefix_len, device_cu_count()).bytes;
 }
 
 int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream) {
-    const PagedFlashParams p = flash_params(a);
-    const long G = a.n_heads / a.n_kv_heads;
-    // Tiles of all sequences at most: whole ones, and a part of one for each.
-    const long tiles = (long)a.rows * G / kPfRows + std::min((long)a.batch, (long)a.rows);
-    launch_flash<false>(a, p, tiles * a.n_kv_heads, stream);
+    PagedFlashParams p = flash_params(a);
+    const PagedPrefillPlan pl =
+        plan_prefill(a.batch, a.rows, a.n_heads, a.n_kv_heads, a.head_dim, p.c.capacity, device_cu_count());
+    p.splits = pl.splits;
+    if (pl.splits > 1) {
+        if (a.workspace == nullptr || a.workspace_bytes < kCounterBytes + pl.bytes)
+            return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_prefill_workspace_size)");
+        char* ws = static_cast<char*>(a.workspace) + kCounterBytes;
+        p.part_ml = reinterpret_cast<float*>(ws);
+        p.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+    }
+    launch_flash<false>(a, p, pl.tiles * a.n_kv_heads * pl.splits, stream);
+    if (pl.splits > 1) {
+        const dim3 grid((unsigned)(pl.tiles * a.n_kv_heads), kPfRows / 32);
+        if (a.bf16)
+            a.head_dim == 128 ? paged_flash_join_kernel<true, 128><<<grid, 256, 0, stream>>>(p)
+                              : paged_flash_join_kernel<true, 64><<<grid, 256, 0, stream>>>(p);
+        else
+            a.head_dim == 128 ? paged_flash_join_kernel<false, 128><<<grid, 256, 0, stream>>>(p)
+                              : paged_flash_join_kernel<false, 64><<<grid, 256, 0, stream>>>(p);
+    }
     return check_launch();
 }
 

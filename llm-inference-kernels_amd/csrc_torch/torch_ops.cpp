@@ -95,6 +95,7 @@ struct CallWorkspace {
 
 CallWorkspace call_workspace(const Tensor& like, hipStream_t s, size_t nbytes) {
     CallWorkspace w;
+    if (nbytes == 0) return w;
     if (!stream_is_capturing(s)) {
         std::tie(w.ptr, w.bytes) = workspace(like, s, nbytes);
         return w;
@@ -803,7 +804,9 @@ Tensor paged_prefill_attention(const Tensor& q, const Tensor& k_cache, const Ten
     Tensor out = at::empty_like(q);
     if (q.size(0) == 0) return out;
     if (c.batch == 0) return out.zero_();
-    check(llmik_paged_prefill_attention(&c, ptr(q), cu, ptr(out), (int)q.size(0), H, &o, stream_of(q)));
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_prefill_workspace_size(&c, H, (int)q.size(0)));
+    check(llmik_paged_prefill_attention(&c, ptr(q), cu, ptr(out), (int)q.size(0), H, &o, ws.ptr, ws.bytes, st));
     return out;
 }
 

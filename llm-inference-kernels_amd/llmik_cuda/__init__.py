@@ -464,8 +464,8 @@ def rope_paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optio
     cu_tokens[-1] on, and rows of empty sequences, give a zero q and are
     written nowhere; so are positions past the tables. Two rows that name one
     slot (a page mapped twice) write it in no particular order."""
-    _require(all(_is_device(t) for t in (qkv, k_cache, v_cache, page_table, seq_lens)),
-             "all inputs must be CUDA tensors")
+    _require(_is_device(qkv) and _is_device(k_cache) and _is_device(v_cache) and
+             _is_device(page_table) and _is_device(seq_lens), "all inputs must be CUDA tensors")
     return _C.rope_paged_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_tokens)
 
 
@@ -479,8 +479,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     with slopes [n_heads] fp32 minus slopes[h] * (distance in tokens); with
     window > 0 only the newest `window` keys. A sequence without a key gives
     zeros. Deterministic; the bits depend on the lengths of the whole batch."""
-    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens)),
-             "all inputs must be CUDA tensors")
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
+             _is_device(page_table) and _is_device(seq_lens), "all inputs must be CUDA tensors")
     return _C.paged_decode_attention(q, k_cache, v_cache, page_table, seq_lens, float(softmax_scale),
                                      float(softcap), slopes, int(window))
 
@@ -494,8 +494,8 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     sequence up to its own position (the chunk's earlier tokens and what the
     cache held before). Score options as in paged_decode_attention. Rows that
     belong to no sequence give zeros."""
-    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens, cu_tokens)),
-             "all inputs must be CUDA tensors")
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
+             _is_device(page_table) and _is_device(seq_lens) and _is_device(cu_tokens), "all inputs must be CUDA tensors")
     return _C.paged_prefill_attention(q, k_cache, v_cache, page_table, seq_lens, cu_tokens,
                                       float(softmax_scale), float(softcap), slopes, int(window))
 
@@ -509,8 +509,8 @@ def paged_shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     prefix_len tokens: those are read from prefix_pages [n] int32 once for all
     sequences, page_table from position prefix_len on. seq_lens counts the
     prefix too; a sequence may be shorter than it."""
-    _require(all(_is_device(t) for t in (q, k_cache, v_cache, page_table, seq_lens, prefix_pages)),
-             "all inputs must be CUDA tensors")
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
+             _is_device(page_table) and _is_device(seq_lens) and _is_device(prefix_pages), "all inputs must be CUDA tensors")
     return _C.paged_shared_prefix_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_pages,
                                             int(prefix_len), float(softmax_scale), float(softcap), slopes,
                                             int(window))

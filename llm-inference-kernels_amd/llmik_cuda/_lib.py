@@ -86,7 +86,8 @@ _SIGNATURES = {
     "llmik_rope_paged_append": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _i, _i, _p]),
     "llmik_paged_workspace_size": (_sz, [_p, _i, _i]),
     "llmik_paged_decode_attention": (_i, [_p, _p, _p, _i, _p, _p, _sz, _p]),
-    "llmik_paged_prefill_attention": (_i, [_p, _p, _p, _p, _i, _i, _p, _p]),
+    "llmik_paged_prefill_workspace_size": (_sz, [_p, _i, _i]),
+    "llmik_paged_prefill_attention": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _sz, _p]),
     "llmik_paged_shared_prefix_attention": (_i, [_p, _p, _p, _i, _p, _i, _i, _p, _p, _sz, _p]),
 }
 
