@@ -67,7 +67,7 @@ __device__ __forceinline__ Keys keys_of(const PagedDecodeParams& p, int len) {
     Keys k;
     k.len = max(len, 0);
     k.end = min(k.len, p.c.capacity);
-    k.begin = max(max(k.len - p.s.window, 0), p.first);
+    k.begin = min(max(max(k.len - p.s.window, 0), p.first), k.end);
     k.tiles = max((k.end + 31) / 32 - k.begin / 32, 1);
     return k;
 }

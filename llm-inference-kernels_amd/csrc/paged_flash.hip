@@ -119,15 +119,16 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
 constexpr int kMinPart = 8;
 constexpr int kMaxParts = 8;
 struct TileKeys {
+    int lo, hi;   // positions of the first and the last row
     int begin, end, tiles, parts, part_tiles;
 };
 __device__ __forceinline__ TileKeys keys_of_tile(const PagedFlashParams& p, const RowTile& t) {
     const int n_rows = t.rows * (int)p.gqa.d, r0 = t.tile * kPfRows;
-    const int lo = t.pos0 + (int)p.gqa.div((uint32_t)r0);
-    const int hi = t.pos0 + (int)p.gqa.div((uint32_t)min(r0 + kPfRows, n_rows) - 1u);
     TileKeys k;
-    k.begin = oldest_key(p.s, lo) / kPfTile * kPfTile;
-    k.end = min(p.c.capacity, hi + 1);
+    k.lo = t.pos0 + (int)p.gqa.div((uint32_t)r0);
+    k.hi = t.pos0 + (int)p.gqa.div((uint32_t)min(r0 + kPfRows, n_rows) - 1u);
+    k.begin = oldest_key(p.s, k.lo) / kPfTile * kPfTile;
+    k.end = min(p.c.capacity, k.hi + 1);
     k.tiles = k.end > k.begin ? (k.end - k.begin + kPfTile - 1) / kPfTile : 0;
     k.parts = max(min(p.splits, k.tiles / kMinPart), 1);
     k.part_tiles = (k.tiles + k.parts - 1) / k.parts;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPfTile * kRowBytes], s_k1[kPfTile * kRowBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_v0[kPfTile * kRowBytes], s_v1[kPfTile * kRowBytes];
     __shared__ int s_lo[4], s_hi[4];
-    __shared__ uint32_t s_gone[2][4];
+    __shared__ uint32_t s_gone[2][4], s_bad;   // s_bad: see row_by_row
 
     const int kvh = (int)blockIdx.x % p.c.n_kv_heads;
     const uint32_t item = blockIdx.x / (uint32_t)(p.c.n_kv_heads * p.splits);
@@ -187,7 +188,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
 
     // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
     auto oldest = [&](int at) { return oldest_key(p.s, at); };
-    int begin, end, tiles, parts = 1, pos_lo, pos_hi;   // pos_lo, pos_hi: of the wave's rows
+    int begin, end, tiles, parts = 1;
+    int pos_lo, pos_hi, wg_lo, wg_hi;   // positions of the wave's rows, of the workgroup's
     if constexpr (PREFIX) {
         pos_lo = pos_hi = pos;
 #pragma unroll
@@ -200,23 +202,28 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
             s_hi[wave] = live ? pos_hi : -1;
         }
         __syncthreads();
-        const int lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
-        const int hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
-        begin = max(split * p.chunk, oldest(lo)) / kPfTile * kPfTile;
-        end = min(min(split * p.chunk + p.chunk, p.prefix_len), hi + 1);
+        wg_lo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3]));
+        wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+        begin = max(split * p.chunk, oldest(wg_lo)) / kPfTile * kPfTile;
+        end = min(min(split * p.chunk + p.chunk, p.prefix_len), wg_hi + 1);
         tiles = end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0;
     } else {
         pos_lo = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave, n_rows - 1));
         pos_hi = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave + 31, n_rows - 1));
         const TileKeys k = keys_of_tile(p, ft);
+        wg_lo = k.lo;
+        wg_hi = k.hi;
         parts = k.parts;
         if (split >= parts) return;
         begin = k.begin + split * k.part_tiles * kPfTile;
         end = min(k.end, begin + k.part_tiles * kPfTile);
         tiles = min(k.part_tiles, k.tiles - split * k.part_tiles);
     }
+    if (tiles <= 0) tiles = begin = end = 0;
     pos_lo = __builtin_amdgcn_readfirstlane(pos_lo);
     pos_hi = __builtin_amdgcn_readfirstlane(pos_hi);
+    wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
+    wg_hi = __builtin_amdgcn_readfirstlane(wg_hi);
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
     tiles = __builtin_amdgcn_readfirstlane(tiles);
@@ -398,6 +405,23 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
             for (int c = 0; c < kCopies; ++c) copy(v ? v_far : k_far, v, c);
         };
         const int t0 = begin + kPfTile * i;
+        // Where some row does not see some token, every wave looks through its 16 rows of V
+        // for infinities and NaN (bits of |x| from the type's infinity on): a probability
+        // of 0 would make NaN of them. Such a tile's rows are done again, below.
+        if (t0 + kPfTile - 1 > wg_lo || t0 < oldest(wg_hi)) {   // workgroup-uniform
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(v_cur + 16 * wave * kRowBytes + 1024 * c + 16 * lane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = w[e];
+                    top = max_abs2(top, x);
+                }
+            }
+            const uint32_t inf = BF ? 0x7F80u : 0x7C00u;
+            if ((top & 0xFFFFu) >= inf || (top >> 16) >= inf) s_bad = 1u;
+        }
         if (live && t0 <= pos_hi && t0 + kPfTile > oldest(pos_lo)) {
             compute(k_cur, v_cur, i, copies);
         } else {   // no row of this wave sees a key of it
@@ -405,6 +429,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
             copies(1);
         }
     };
+    if (tid == 0) s_bad = 0u;   // (the first turn's barrier follows)
     if (tiles > 0) {
         prepare(0);
 #pragma unroll
@@ -420,28 +445,107 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup
 
     l_run = xor32_sum(l_run);
-    if (!live || r_wave + n >= n_rows) return;
-    if (PREFIX || parts > 1) {
-        const long at = PREFIX ? ((long)kvh * n_rows + r) * p.splits + split
-                               : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + 32 * wave + n;
+    // The row's place among the parts.
+    auto part_at = [&](int row) {
+        return PREFIX ? ((long)kvh * n_rows + ft.tile * kPfRows + row) * p.splits + split
+                      : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + row;
+    };
+    const bool as_part = PREFIX || parts > 1;
+    if (live && r_wave + n < n_rows) {
+        if (as_part) {
+            const long at = part_at(32 * wave + n);
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+            for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * cb + 2 * e + 4 * h) =
-                    f32x4{o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]};
-        if (h == 0) {
-            p.part_ml[2 * at] = m_run;
-            p.part_ml[2 * at + 1] = l_run;
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * cb + 2 * e + 4 * h) =
+                        f32x4{o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]};
+            if (h == 0) {
+                p.part_ml[2 * at] = m_run;
+                p.part_ml[2 * at + 1] = l_run;
+            }
+        } else {
+            const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;   // a row without keys is zero
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<u32x2*>(p.out + q_row * D + 32 * cb + 2 * e + 4 * h) = u32x2{
+                        Hf::pack(o[cb][e] * inv, o[cb][e + 1] * inv), Hf::pack(o[cb][e + 2] * inv, o[cb][e + 3] * inv)};
         }
-    } else {
-        const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;   // a row without keys is zero
+    }
+    __syncthreads();
+    if (tiles == 0 || __builtin_amdgcn_readfirstlane((int)s_bad) == 0) return;
+
+    // ---- some V is no number, and not all rows see it: the wave's rows one by one,
+    // 64 keys at a time (a lane its key's score, then two channels of every key's
+    // value that has a probability) ----
+    __builtin_amdgcn_s_waitcnt(0);   // the stores above come first
+    constexpr int kCh = D / 64;      // channels of a lane
+    for (int rr = 0; rr < 32 && r_wave + rr < n_rows; ++rr) {
+        const int r1 = r_wave + rr, qi1 = (int)p.gqa.div((uint32_t)r1);
+        const int head1 = kvh * G + (r1 - qi1 * G);
+        const long q_row1 = (PREFIX ? (long)qi1 : (long)ft.row0 + qi1) * p.n_heads + head1;
+        const int pos1 = PREFIX ? p.c.lens[qi1] - 1 : ft.pos0 + qi1;
+        const int old = oldest(pos1), lim = min(pos1 + 1, end);
+        const float slope1 = p.s.slopes ? p.s.slopes[head1] * kLog2eF : 0.0f;
+        float m = kNoMax, l = 0.0f, acc[kCh];
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+        for (int e = 0; e < kCh; ++e) acc[e] = 0.0f;
+        for (int k0 = begin; k0 < lim; k0 += 64) {
+            const int t = k0 + lane;
+            long at = octet_offset<D>(p.c, table_row, kvh, t & ~7, end);
+            const bool ok = t >= old && t < lim && at >= 0;
+            at = ok ? at + (t & 7) * D : 0L;
+            float dot = 0.0f;
+            for (int d8 = 0; d8 < D; d8 += 8) {
+                const u32x4 a = load16(p.q + q_row1 * D + d8), b = load16(p.c.k + at + d8);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<u32x2*>(p.out + q_row * D + 32 * cb + 2 * e + 4 * h) =
-                    u32x2{Hf::pack(o[cb][e] * inv, o[cb][e + 1] * inv), Hf::pack(o[cb][e + 2] * inv, o[cb][e + 3] * inv)};
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = a[e], y = b[e];
+                    dot = fmaf(Hf::to_f32((uint16_t)x), Hf::to_f32((uint16_t)y), dot);
+                    dot = fmaf(Hf::to_f32((uint16_t)(x >> 16)), Hf::to_f32((uint16_t)(y >> 16)), dot);
+                }
+            }
+            float s1 = p.s.cap_in != 0.0f ? capped(dot, p.s.cap_in, p.s.cap_log2) : dot * p.s.scale_log2;
+            if (p.s.slopes) s1 = fmaf(-slope1, (float)(pos1 - t), s1);
+            s1 = ok ? s1 : -INFINITY;
+            float top = s1;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+            top = fmaxf(top, m);
+            const float a = __builtin_amdgcn_exp2f(m - top), pt = ok ? __builtin_amdgcn_exp2f(s1 - top + kPShift) : 0.0f;
+            float sum = pt;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+            m = top;
+            l = l * a + sum;
+#pragma unroll
+            for (int e = 0; e < kCh; ++e) acc[e] *= a;
+            for (int j = 0; j < 64; ++j) {
+                const float pj = __shfl(pt, j);
+                const long vj = ((long)__shfl((int)(at >> 32), j) << 32) | (uint32_t)__shfl((int)(uint32_t)at, j);
+                if (pj != 0.0f) {   // wave-uniform
+#pragma unroll
+                    for (int e = 0; e < kCh; ++e)
+                        acc[e] = fmaf(pj, Hf::to_f32(p.c.v[vj + kCh * lane + e]), acc[e]);
+                }
+            }
+        }
+        if (as_part) {
+            const long at = part_at(32 * wave + rr);
+#pragma unroll
+            for (int e = 0; e < kCh; ++e) p.part_o[at * D + kCh * lane + e] = acc[e];
+            if (lane == 0) {
+                p.part_ml[2 * at] = m;
+                p.part_ml[2 * at + 1] = l;
+            }
+        } else {
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int e = 0; e < kCh; ++e)
+                p.out[q_row1 * D + kCh * lane + e] = (uint16_t)Hf::pack(acc[e] * inv, 0.0f);
+        }
     }
 }
 
