@@ -18,15 +18,19 @@ bit-identical to the reference cache's view after the same appends:
 * Int8KVCache: K and V per token (the INT8 path of the reference has no
   cache class; this is its prealloc_cache.PreallocCache layout,
   integration/prealloc_cache.py:42-79, in INT8).
+
+PagedKVCache keeps fp16 or bf16 tokens of many sequences, each of its own
+length, in one pool of pages (the reference has no counterpart).
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
-from . import (_C, quantize_k_per_channel_groupwise_int4_into, quantize_per_token_into,
-               quantize_v_per_token_int4_into)
+from . import (_C, paged_decode_attention, paged_prefill_attention, paged_shared_prefix_attention,
+               quantize_k_per_channel_groupwise_int4_into, quantize_per_token_into, quantize_v_per_token_int4_into,
+               rope_paged_append)
 # One-token steps at small batch are bound by the host: these three come from the
 # extension, which checks types, shapes, strides and devices itself, rather
 # than through the module's Python wrappers (a KIVI step of one token and
@@ -199,3 +203,174 @@ class Int4KIVICache:
 
     def reset(self) -> None:
         self.length = 0
+
+
+class PagedBatch(NamedTuple):
+    """The sequences of one call and their new tokens, as the paged ops take
+    them (PagedKVCache.batch)."""
+    page_table: torch.Tensor            # [batch, max_pages] int32
+    seq_lens: torch.Tensor              # [batch] int32, with the new tokens
+    cu_tokens: Optional[torch.Tensor]   # [batch + 1] int32; None: one new token each
+    rows: int                           # new tokens of all sequences
+    prefix_pages: Optional[torch.Tensor]   # pages that all sequences share from the start on
+    prefix_len: int
+
+
+class PagedKVCache:
+    """Sequences of different lengths over one pool of `n_pages` pages of
+    `page_size` tokens: k, v [n_pages, n_kv_heads, page_size, head_dim].
+
+    The host keeps each sequence's length and pages; `batch` reserves pages for
+    a call's new tokens and hands the tables to the device, `append` rotates
+    and writes the tokens, `attention` reads them:
+
+        a = cache.add(); b = cache.add()
+        step = cache.batch([a, b], [len(prompt_a), len(prompt_b)])
+        q = cache.append(step, qkv, cos, sin)         # rows: a's tokens, then b's
+        out = cache.attention(step, q, scale)
+        step = cache.batch([a, b])                    # one more token each
+        ...
+        c = cache.add(share=a, tokens=1000)           # behind the first 1000 tokens of a
+        cache.remove(b)
+
+    One `batch` serves the layers of a model if each layer has its own pool of
+    the same shape: `append` and `attention` take the pool's k and v. Not safe
+    for calls from several threads."""
+
+    # A batch's shared prefix is read once for all sequences from this many shared
+    # tokens of all sequences but one on (_shared_prefix).
+    SHARED_TOKENS = 4096
+
+    def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, head_dim: int = 128,
+                 dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None) -> None:
+        _require(n_pages > 0 and n_kv_heads > 0, "n_pages and n_kv_heads must be positive")
+        _require(page_size > 0 and page_size % 8 == 0, "page_size must be a positive multiple of 8")
+        _require(head_dim in (64, 128), "only head_dim=64 and 128 supported")
+        _require(dtype in (torch.float16, torch.bfloat16), "dtype must be fp16 or bf16")
+        self.device = torch.device("cuda") if device is None else torch.device(device)
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, n_kv_heads, page_size, head_dim
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        self.k = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.v = torch.zeros(shape, dtype=dtype, device=self.device)
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._users = [0] * n_pages             # sequences that hold the page
+        self._pages: dict[int, List[int]] = {}  # sequence -> its pages
+        self._length: dict[int, int] = {}
+        self._next = 0
+
+    # ---- sequences ----
+
+    def add(self, share: Optional[int] = None, tokens: int = 0) -> int:
+        """A new sequence, empty or behind the first `tokens` tokens of the
+        sequence `share`: whole pages are shared, the rest of the last one is
+        copied. Returns its number."""
+        pages: List[int] = []
+        if share is not None:
+            _require(share in self._pages, "no such sequence")
+            _require(0 <= tokens <= self._length[share], "the shared sequence has fewer tokens")
+            whole, rest = divmod(tokens, self.page_size)
+            pages = self._pages[share][:whole]
+            if rest:
+                _require(len(self._free) > 0, "the cache has no free page")
+                page, src = self._free.pop(), self._pages[share][whole]
+                self._users[page] = 1
+                self.k[page, :, :rest] = self.k[src, :, :rest]
+                self.v[page, :, :rest] = self.v[src, :, :rest]
+            for p in pages:
+                self._users[p] += 1
+            if rest:
+                pages = pages + [page]
+        else:
+            _require(tokens == 0, "tokens are shared with a sequence")
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq], self._length[seq] = list(pages), tokens
+        return seq
+
+    def remove(self, seq: int) -> None:
+        """Ends a sequence; pages that no other one shares become free."""
+        _require(seq in self._pages, "no such sequence")
+        for p in self._pages.pop(seq):
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                self._free.append(p)
+        del self._length[seq]
+
+    def length(self, seq: int) -> int:
+        return self._length[seq]
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    # ---- calls ----
+
+    def batch(self, seqs: Sequence[int], new: Optional[Sequence[int]] = None) -> PagedBatch:
+        """Reserves pages for new[i] (default 1) more tokens of seqs[i] and returns
+        the call's tables. The tokens count as live from here on: `append` them
+        before anything reads them. Nothing is reserved if the pages do not
+        suffice."""
+        counts = [1] * len(seqs) if new is None else [int(n) for n in new]
+        _require(len(counts) == len(seqs), "one count per sequence")
+        _require(len(set(seqs)) == len(seqs), "a sequence occurs twice in the batch")
+        _require(all(s in self._pages for s in seqs), "no such sequence")
+        _require(all(n >= 0 for n in counts), "counts must be >= 0")
+        need = [-(-(self._length[s] + n) // self.page_size) - len(self._pages[s]) for s, n in zip(seqs, counts)]
+        _require(sum(need) <= len(self._free), "the cache has no free page")
+        for s, n, m in zip(seqs, counts, need):
+            for _ in range(m):
+                page = self._free.pop()
+                self._users[page] = 1
+                self._pages[s].append(page)
+            self._length[s] += n
+        pages = [self._pages[s] for s in seqs]
+        lens = [self._length[s] for s in seqs]
+        ragged = any(n != 1 for n in counts)
+        cu = [0]
+        for n in counts:
+            cu.append(cu[-1] + n)
+        shared = 0 if ragged else self._shared_prefix(pages, lens)
+        width = max([len(p) for p in pages] + [1])
+        # One copy to the device: lengths, row offsets, then the table.
+        flat = lens + cu + [p for row in pages for p in row + [-1] * (width - len(row))]
+        host = torch.tensor(flat, dtype=torch.int32)
+        if self.device.type == "cuda":
+            dev = host.pin_memory().to(self.device, non_blocking=True)
+        else:
+            dev = host
+        b = len(seqs)
+        table = dev[2 * b + 1:].view(b, width) if b else torch.zeros((0, width), dtype=torch.int32, device=self.device)
+        return PagedBatch(table, dev[:b], dev[b:2 * b + 1] if ragged else None, cu[-1],
+                          table[0, :shared] if shared else None, shared * self.page_size)
+
+    def _shared_prefix(self, pages: List[List[int]], lens: List[int]) -> int:
+        """Whole pages that all sequences share from the start on, or 0 where reading
+        them once for all does not pay: two launches instead of one, and partial
+        results, against the pages' tokens read by all sequences but one again."""
+        if len(pages) < 2:
+            return 0
+        n = min(min(len(p) for p in pages), (min(lens) - 1) // self.page_size)
+        first = pages[0]
+        same = 0
+        while same < n and all(p[same] == first[same] for p in pages):
+            same += 1
+        return same if same * self.page_size * (len(pages) - 1) >= self.SHARED_TOKENS else 0
+
+    def append(self, step: PagedBatch, qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+               k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """rope_paged_append of the batch's new tokens; returns the rotated q
+        [rows, n_heads, head_dim]. k, v: another layer's pool."""
+        return rope_paged_append(qkv, cos, sin, self.k if k is None else k, self.v if v is None else v,
+                                 step.page_table, step.seq_lens, step.cu_tokens)
+
+    def attention(self, step: PagedBatch, q: torch.Tensor, softmax_scale: float, softcap: float = 0.0,
+                  slopes: Optional[torch.Tensor] = None, window: int = 0, k: Optional[torch.Tensor] = None,
+                  v: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the batch's new tokens: decode, decode behind a shared
+        prefix, or prompts, by the batch."""
+        k, v = self.k if k is None else k, self.v if v is None else v
+        if step.cu_tokens is not None:
+            return paged_prefill_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, softmax_scale,
+                                           softcap, slopes, window)
+        if step.prefix_pages is not None:
+            return paged_shared_prefix_attention(q, k, v, step.page_table, step.seq_lens, step.prefix_pages,
+                                                 step.prefix_len, softmax_scale, softcap, slopes, window)
+        return paged_decode_attention(q, k, v, step.page_table, step.seq_lens, softmax_scale, softcap, slopes, window)
