@@ -158,11 +158,6 @@ struct PagedLaunch {
 };
 // Un-normalised results of a shared prefix that the decode kernel joins:
 // o [n_kv_heads, batch * n_heads / n_kv_heads, splits, head_dim], ml [..., 2].
-struct PagedPrefixParts {
-    const float* o;
-    const float* ml;
-    int splits, len;
-};
 struct PagedAppend {
     const void* qkv;
     const void* cos;   // null: no rotation
@@ -182,7 +177,7 @@ size_t paged_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_d
 size_t paged_prefill_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
 size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len);
 int launch_paged_append(const PagedAppend& a, hipStream_t stream);
-int launch_paged_decode(const PagedLaunch& a, const PagedPrefixParts& pre, hipStream_t stream);
+int launch_paged_decode(const PagedLaunch& a, hipStream_t stream);
 int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream);
 int launch_paged_shared_prefix(const PagedLaunch& a, hipStream_t stream);
 

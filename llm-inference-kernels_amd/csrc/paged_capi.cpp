@@ -176,7 +176,7 @@ LLMIK_API llmik_status llmik_paged_decode_attention(const llmik_paged_cache* cac
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;
-    return launch_paged_decode(a, PagedPrefixParts{}, as_stream(stream));
+    return launch_paged_decode(a, as_stream(stream));
 }
 
 LLMIK_API size_t llmik_paged_prefill_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows) {
@@ -222,7 +222,7 @@ LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cac
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;
-    if (prefix_len == 0) return launch_paged_decode(a, PagedPrefixParts{}, as_stream(stream));
+    if (prefix_len == 0) return launch_paged_decode(a, as_stream(stream));
     if (prefix_pages == nullptr) return invalid("null prefix_pages pointer");
     if (!aligned(prefix_pages, 4)) return misaligned("prefix_pages must be 4-byte aligned");
     const long per_kv = (long)cache->batch * (n_heads / cache->n_kv_heads);

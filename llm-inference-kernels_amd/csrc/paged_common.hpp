@@ -119,6 +119,7 @@ __device__ __forceinline__ long octet_offset(const PagedView& c, const int* tabl
 // A running maximum starts here rather than at -inf: differences of two such are
 // then numbers, and states without a key join like all others (their sums are 0).
 constexpr float kNoMax = -1e30f;
+constexpr float kPShift = 8.0f;   // p is held as 2^8 p: fp16 keeps its full precision down to 2^-22
 
 // Scores in the log2 domain. cap > 0: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
 // (e^2x + 1), as exp2 and one reciprocal (absolute error about 2^-23 cap).

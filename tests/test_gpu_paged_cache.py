@@ -31,7 +31,7 @@ def test_a_serving_loop(llmik, cuda, dtype, D, page, opts):
     rng = random.Random(11)
     gen = torch.Generator(device=cuda).manual_seed(12)
     cache = PagedKVCache(200, Hkv, page_size=page, head_dim=D, dtype=dtype)
-    cache.SHARED_TOKENS = 200
+    cache.SHARED_TOKENS, cache.SHARED_ROWS = 16, 400
     cos, sin = _tables(2000, D, cuda)
     kept = {}            # sequence -> (k, v) rows [n, Hkv, D] as the cache stores them
     shared_steps = 0

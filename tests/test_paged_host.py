@@ -258,7 +258,7 @@ def test_sharing_and_removal(cache):
 
 
 def test_a_batch_knows_its_shared_prefix(cache):
-    cache.SHARED_TOKENS = 16
+    cache.SHARED_TOKENS, cache.SHARED_ROWS = 24, 2 * 24 * 2
     a = cache.add()
     cache.batch([a], [24])
     seqs = [a] + [cache.add(share=a, tokens=24) for _ in range(2)]
@@ -269,8 +269,12 @@ def test_a_batch_knows_its_shared_prefix(cache):
     other = cache.add()
     cache.batch([other], [5])
     assert cache.batch(seqs + [other]).prefix_len == 0                 # nothing in common
-    cache.SHARED_TOKENS = 1000
-    assert cache.batch(seqs).prefix_pages is None                      # too little to pay
+    cache.SHARED_ROWS += 1
+    assert cache.batch(seqs).prefix_pages is None                      # too few rows to pay
+    cache.SHARED_TOKENS, cache.SHARED_ROWS = 25, 2 * 24 * 2 // 16
+    assert cache.batch(seqs).prefix_len == 24                          # few tokens, many rows
+    cache.SHARED_ROWS += 1
+    assert cache.batch(seqs).prefix_pages is None
 
 
 def test_pages_are_never_lost_or_given_twice():
