@@ -130,9 +130,11 @@ struct ScoreOpts {
     const float* slopes;
     int window;         // keys per query, INT_MAX where unlimited
 };
+__device__ __forceinline__ float capped_part(float s, float cap_in) {   // (tanh(x) - 1) / 2
+    return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * cap_in));
+}
 __device__ __forceinline__ float capped(float s, float cap_in, float cap_log2) {
-    const float e = __builtin_amdgcn_exp2f(s * cap_in);
-    return fmaf(-2.0f * cap_log2, __builtin_amdgcn_rcpf(e + 1.0f), cap_log2);
+    return fmaf(2.0f * cap_log2, capped_part(s, cap_in), cap_log2);
 }
 
 // The kernels' views of a call.

@@ -288,11 +288,13 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[cb][e] = 0.0f;
     float m_run = kNoMax, l_run = 0.0f;   // of row n; l_run: this lane's tokens only
-    // Scores as they come from the products, times mult, are in the log2 domain. A
-    // negative scale is multiplied in beforehand, like a cap or a bias: the masked
-    // value must stay the smallest.
-    const bool modified = p.s.cap_in != 0.0f || p.s.slopes != nullptr || p.s.scale_log2 <= 0.0f;
-    const float mult = modified ? 1.0f : p.s.scale_log2;
+    // sc * mult + add are the scores in the log2 domain: sc as it comes from the products,
+    // or -1 / (e^2x + 1) where there is a cap (the rest of cap * tanh x is mult and add),
+    // or, with a bias or a negative scale, the score itself (mult must be positive: the
+    // masked value, -inf, must stay the smallest).
+    const bool cap = p.s.cap_in != 0.0f, modified = p.s.slopes != nullptr || (!cap && p.s.scale_log2 <= 0.0f);
+    const float mult = modified ? 1.0f : cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2;
+    const float add = cap && !modified ? p.s.cap_log2 : 0.0f;
 
     // LDS offsets of this lane's operand reads.
     const uint32_t k_row = (uint32_t)(n * kRowBytes);
@@ -302,37 +304,49 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const uint32_t v_sw = (uint32_t)(D == 128 ? vr << 2 : (vr >> 1) << 2);
     const uint32_t v_at = (uint32_t)((4 * h + vr) * kRowBytes) + 8 * (lane & 1);
 
-    // copies(0), copies(1): the next tile's copies of K and of V are issued behind the
-    // products of the two blocks' scores, whose time hides them: before all work they
+    // copies(0, c), copies(1, c): copy c of the next tile's K and of its V, issued among
+    // the products of the two blocks' scores, whose time hides them: before all work they
     // waited for the CU's one vector memory path, 1000 of a tile's 3900 cycles (us, a
     // prompt of 8192 tokens 562 -> 550, 2048 tokens 58.2 -> 54.5, chunks 198 -> 189;
     // spread further down to the products with V they come too late: 542, 56.9, 210).
     auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i, auto copies) {
         const int t0 = begin + kPfTile * i;
         float sc[32];
+        // K's operands are requested eight products ahead, in this order: left to itself the
+        // compiler saves the registers and waits for each (us, 8192 tokens 562 -> 536,
+        // 2048 tokens 56.9 -> 52.5, chunks 195 -> 180).
+        u32x4 ka[2][KS];
+        auto load_k = [&](int blk, int ks) {
+            ka[blk][ks] = *reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks)));
+        };
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) load_k(0, ks);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             f32x16 acc;
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                acc = Hf::mfma32(*reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks))),
-                                 qb[ks], acc);
+            for (int ks = 0; ks < KS; ++ks) {
+                acc = Hf::mfma32(ka[blk][ks], qb[ks], acc);
+                if (blk == 0) load_k(1, ks);
+                if (ks % 2 == 1) copies(blk, ks / 2);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[16 * blk + e] = acc[e];
-            copies(blk);
         }
         // value e belongs to token t0 + 4 h + 8 (e / 4) + e % 4
         const int tk = t0 + 4 * h;
-        if (modified) {   // the cap and the bias, in the log2 domain: `mult` is 1 then
-            if (p.s.cap_in != 0.0f) {
+        if (cap) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
-            } else {
+            for (int e = 0; e < 32; ++e) sc[e] = capped_part(sc[e], p.s.cap_in);
+        }
+        if (modified) {
+            const float by = cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2, plus = cap ? p.s.cap_log2 : 0.0f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) sc[e] *= p.s.scale_log2;
-            }
+            for (int e = 0; e < 32; ++e) sc[e] = fmaf(sc[e], by, plus);
             if (p.s.slopes) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
@@ -357,7 +371,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         const float sub = m_run - kPShift;
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-            t[e] = fmaf(sc[e], mult, -sub);
+            t[e] = fmaf(sc[e], mult, add - sub);
             mx = fmaxf(mx, t[e]);
         }
         if (__any(mx > kPShift + kPLag)) {
@@ -366,7 +380,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             if (m_run == kNoMax) {   // the first keys: the scores themselves (m_run + mx has none of their bits)
                 m_new = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) m_new = fmaxf(m_new, sc[e] * mult);
+                for (int e = 0; e < 32; ++e) m_new = fmaxf(m_new, fmaf(sc[e], mult, add));
                 m_new = fmaxf(xor32_max(m_new), kNoMax);
             }
             const float a = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -377,7 +391,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[cb][e] *= a;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) t[e] = fmaf(sc[e], mult, kPShift - m_run);
+            for (int e = 0; e < 32; ++e) t[e] = fmaf(sc[e], mult, add + (kPShift - m_run));
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) t[e] = __builtin_amdgcn_exp2f(t[e]);
@@ -410,10 +424,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         __builtin_amdgcn_s_waitcnt(0);
         asm volatile("s_barrier" ::: "memory");
         prepare(i + 1);
-        auto copies = [&](int v) {
-#pragma unroll
-            for (int c = 0; c < kCopies; ++c) copy(v ? v_far : k_far, v, c);
-        };
+        auto copies = [&](int v, int c) { copy(v ? v_far : k_far, v, c); };
         const int t0 = begin + kPfTile * i;
         // Where some row does not see some token, every wave looks through its 16 rows of V
         // for infinities and NaN (bits of |x| from the type's infinity on): a probability
@@ -435,8 +446,8 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         if (live && t0 <= pos_hi && t0 + kPfTile > oldest(pos_lo)) {
             compute(k_cur, v_cur, i, copies);
         } else {   // no row of this wave sees a key of it
-            copies(0);
-            copies(1);
+#pragma unroll
+            for (int c = 0; c < 2 * kCopies; ++c) copies(c / kCopies, c % kCopies);
         }
     };
     if (tid == 0) s_bad = 0u;   // (the first turn's barrier follows)
