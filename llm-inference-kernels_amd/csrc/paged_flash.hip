@@ -10,8 +10,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kTileBytes], s_k1[kTileBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_v0[kTileBytes], s_v1[kTileBytes];
     __shared__ int s_lo[4], s_hi[4];
-    __shared__ uint32_t s_gone[2][4], s_bad;
-    paged_flash<BF, D, false>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, s_gone, &s_bad});
+    __shared__ uint32_t s_bad;
+    paged_flash<BF, D, false>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_bad});
 }
 
 constexpr int kJoinRows = 8;

@@ -29,7 +29,8 @@ namespace llmik {
 
 constexpr int kPfThreads = 256;
 constexpr int kPfRows = 128;    // query rows of a workgroup
-constexpr int kPfTile = 64;     // tokens of a tile
+constexpr int kPfTileLog = 6;   // tokens of a tile
+constexpr int kPfTile = 1 << kPfTileLog;
 constexpr float kPLag = 6.0f;
 
 struct PagedFlashParams {
@@ -142,7 +143,6 @@ struct FlashLds {
     static constexpr int kTileBytes = kPfTile * D * 2;
     uint8_t *k0, *k1, *v0, *v1;
     int *lo, *hi;              // [4]
-    uint32_t (*gone)[4];       // [2][4]
     uint32_t* bad;             // see row_by_row
 };
 
@@ -162,7 +162,6 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 
     uint8_t *const s_k0 = lds.k0, *const s_k1 = lds.k1, *const s_v0 = lds.v0, *const s_v1 = lds.v1;
     int *const s_lo = lds.lo, *const s_hi = lds.hi;
-    uint32_t(*const s_gone)[4] = lds.gone;
     uint32_t& s_bad = *lds.bad;
 
     const int kvh = (int)(wg % (uint32_t)p.c.n_kv_heads);
@@ -238,38 +237,57 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     end = __builtin_amdgcn_readfirstlane(end);
     tiles = __builtin_amdgcn_readfirstlane(tiles);
 
+    // Tiles that all of the wave's rows see wholly, that some row sees, and that all rows
+    // of the workgroup see wholly: [lo, hi).
+    const int full_lo = (oldest(pos_hi) - begin + kPfTile - 1) >> kPfTileLog;
+    const int full_hi = (min(end, pos_lo + 1) - begin) >> kPfTileLog;
+    const int seen_lo = (oldest(pos_lo) - begin) >> kPfTileLog;
+    const int seen_hi = live ? ((pos_hi - begin) >> kPfTileLog) + 1 : INT_MIN;
+    const int wg_full_lo = (oldest(wg_hi) - begin + kPfTile - 1) >> kPfTileLog;
+    const int wg_full_hi = (wg_lo + 1 - begin) >> kPfTileLog;
+
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
+    // Every wave looks up all octets, eight tiles at a time: lane l octet l % 8 of tile
+    // i0 + l / 8. A copy is a load from a buffer of the octet's rows in front of the end;
+    // rows behind it, or without a page, lie outside the buffer's range and come as
+    // zeros (their scores are masked, and their values must not turn 0 * v into NaN).
     const int* table_row = PREFIX ? p.prefix_pages : p.c.table + (long)ft.b * p.c.max_pages;
-    auto look_up = [&](int i0) {   // lane l: octet 2 w + l % 2 of tile i0 + l / 2
-        return octet_offset<D>(p.c, table_row, kvh,
-                               begin + kPfTile * (i0 + (lane >> 1)) + 16 * wave + 8 * (lane & 1), end);
+    auto token_of = [&](int i0) { return begin + kPfTile * (i0 + (lane >> 3)) + 8 * (lane & 7); };
+    auto look_up = [&](int i0) { return octet_offset<D>(p.c, table_row, kvh, token_of(i0), end); };
+    int at_lo, at_hi, at_bytes;   // the lane's octet of the batch: its place in bytes, its rows' bytes
+    uint64_t batch_gone;          // lanes whose octet has no page (or lies behind the end)
+    auto adopt = [&](long off, int i0) {
+        const bool gone = off < 0;
+        const long at = gone ? 0L : 2 * off;
+        at_lo = (int)(uint32_t)at;
+        at_hi = (int)(at >> 32);
+        at_bytes = gone ? 0 : min(max(end - token_of(i0), 0), 8) * kRowBytes;
+        batch_gone = __ballot(gone);
     };
-    long off = look_up(0), off_next = tiles > 32 ? look_up(32) : -1L;
+    adopt(look_up(0), 0);
+    long off_next = tiles > 8 ? look_up(8) : -1L;
     // Copy instruction c fills rows kRowsPerCopy c .. of the wave's 16: lane l writes
     // chunk slot l % CPR of row l / CPR, i.e. the chunk that the permutation puts there.
     const int crow = lane / CPR, cslot = lane % CPR;
     __amdgpu_buffer_rsrc_t rk[2], rv[2];   // of the wave's two octets of the tile being copied
-    // Rows behind the end, or without a page, lie outside the buffer's range: the copy
-    // writes zeros for them. Their scores are masked, and their values must not turn
-    // 0 * v into NaN. Where there is no tile i nothing is read.
+    uint32_t gone_next = 0;                // bit o: octet o of that tile has no page
+    // (Where there is no tile i nothing is read.)
     auto prepare = [&](int i) {
-        if ((i & 31) == 0 && i) {
-            off = off_next;
-            if (i + 32 < tiles) off_next = look_up(i + 32);
+        if ((i & 7) == 0 && i) {
+            adopt(off_next, i);
+            off_next = i + 8 < tiles ? look_up(i + 8) : -1L;
         }
-        const int l0 = 2 * (i & 31), hi = (int)(off >> 32), lo = (int)(uint32_t)off;
-        uint32_t gone = 0;
+        const int l0 = 8 * (i & 7);
+        gone_next = (uint32_t)(batch_gone >> l0) & 255u;
 #pragma unroll
         for (int o8 = 0; o8 < 2; ++o8) {
-            const int h32 = __builtin_amdgcn_readlane(hi, l0 + o8);
-            const long at = h32 < 0 ? 0L : ((long)h32 << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, l0 + o8);
-            const int rows = __builtin_amdgcn_readfirstlane(
-                h32 < 0 ? 0 : min(max(end - (begin + kPfTile * i + 16 * wave + 8 * o8), 0), 8));
-            rk[o8] = make_buffer_rsrc(p.c.k + at, (uint32_t)(rows * kRowBytes));
-            rv[o8] = make_buffer_rsrc(p.c.v + at, (uint32_t)(rows * kRowBytes));
-            gone |= h32 < 0 ? 1u << o8 : 0u;
+            const int l = l0 + 2 * wave + o8;
+            const long at = ((long)__builtin_amdgcn_readlane(at_hi, l) << 32) |
+                            (uint32_t)__builtin_amdgcn_readlane(at_lo, l);
+            const uint32_t bytes = (uint32_t)__builtin_amdgcn_readlane(at_bytes, l);
+            rk[o8] = make_buffer_rsrc(reinterpret_cast<const uint8_t*>(p.c.k) + at, bytes);
+            rv[o8] = make_buffer_rsrc(reinterpret_cast<const uint8_t*>(p.c.v) + at, bytes);
         }
-        if (lane == 0) s_gone[i & 1][wave] = gone;
     };
     auto copy = [&](uint8_t* dst, bool is_v, int c) {
         const int row = kRowsPerCopy * c + crow, trow = 16 * wave + row;   // of the wave's 16, of the tile
@@ -309,7 +327,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     // waited for the CU's one vector memory path, 1000 of a tile's 3900 cycles (us, a
     // prompt of 8192 tokens 562 -> 550, 2048 tokens 58.2 -> 54.5, chunks 198 -> 189;
     // spread further down to the products with V they come too late: 542, 56.9, 210).
-    auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i, auto copies) {
+    auto compute = [&](const uint8_t* sk, const uint8_t* sv, int i, uint32_t gone, auto copies) {
         const int t0 = begin + kPfTile * i;
         float sc[32];
         // K's operands are requested eight products ahead, in this order: left to itself the
@@ -352,11 +370,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                 for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
             }
         }
-        uint32_t gone = 0;   // bit o: octet o of the tile has no page
-#pragma unroll
-        for (int w = 0; w < 4; ++w) gone |= s_gone[i & 1][w] << (2 * w);
-        gone = __builtin_amdgcn_readfirstlane(gone);
-        if (gone || t0 + kPfTile > end || t0 + kPfTile - 1 > pos_lo || t0 < oldest(pos_hi)) {   // wave-uniform
+        if (gone || i < full_lo || i >= full_hi) {   // wave-uniform
             const int old = oldest(pos), lim = min(pos + 1, end);
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
@@ -423,13 +437,13 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     auto turn = [&](uint8_t* k_cur, uint8_t* v_cur, uint8_t* k_far, uint8_t* v_far, int i) {
         __builtin_amdgcn_s_waitcnt(0);
         asm volatile("s_barrier" ::: "memory");
+        const uint32_t gone = gone_next;
         prepare(i + 1);
         auto copies = [&](int v, int c) { copy(v ? v_far : k_far, v, c); };
-        const int t0 = begin + kPfTile * i;
         // Where some row does not see some token, every wave looks through its 16 rows of V
         // for infinities and NaN (bits of |x| from the type's infinity on): a probability
         // of 0 would make NaN of them. Such a tile's rows are done again, below.
-        if (t0 + kPfTile - 1 > wg_lo || t0 < oldest(wg_hi)) {   // workgroup-uniform
+        if (i < wg_full_lo || i >= wg_full_hi) {   // workgroup-uniform
             uint32_t top = 0;
 #pragma unroll
             for (int c = 0; c < kCopies; ++c) {
@@ -443,8 +457,8 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             const uint32_t inf = BF ? 0x7F80u : 0x7C00u;
             if ((top & 0xFFFFu) >= inf || (top >> 16) >= inf) s_bad = 1u;
         }
-        if (live && t0 <= pos_hi && t0 + kPfTile > oldest(pos_lo)) {
-            compute(k_cur, v_cur, i, copies);
+        if (i >= seen_lo && i < seen_hi) {
+            compute(k_cur, v_cur, i, gone, copies);
         } else {   // no row of this wave sees a key of it
 #pragma unroll
             for (int c = 0; c < 2 * kCopies; ++c) copies(c / kCopies, c % kCopies);

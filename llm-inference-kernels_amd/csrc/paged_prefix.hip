@@ -19,10 +19,10 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_prefix_kernel(PagedFlashP
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kTileBytes], s_k1[kTileBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_v0[kTileBytes], s_v1[kTileBytes];
     __shared__ int s_lo[4], s_hi[4];
-    __shared__ uint32_t s_gone[2][4], s_flag;
+    __shared__ uint32_t s_flag;
     __shared__ float s_m[kPdWaves][16], s_l[kPdWaves][16];
     if (blockIdx.x < flash_wgs)
-        paged_flash<BF, D, true>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, s_gone, &s_flag});
+        paged_flash<BF, D, true>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_flag});
     else
         paged_decode<BF, D, UNI>(d, blockIdx.x - flash_wgs, gridDim.x - flash_wgs,
                                  {reinterpret_cast<float*>(s_k0), reinterpret_cast<float*>(s_k1),
