@@ -498,7 +498,7 @@ typedef struct llmik_paged_cache {
  */
 typedef struct llmik_score_options {
     float softmax_scale;
-    float softcap;          /* 0: none */
+    float softcap;          /* 0: none; at most 4096 */
     const float* slopes;    /* NULL: none */
     int window;             /* 0: none */
 } llmik_score_options;

@@ -27,6 +27,13 @@
 // P enters as a pair hi + lo of 16-bit values (two products): its rounding then
 // leaves 2^-22 (fp16) or 2^-16 (bf16) of each probability, less than the output's
 // own; the second product is free beside the loads.
+//
+// Registers hold one tile: the next tile's keys are requested when the scores are
+// computed, its values when their products are (two buffers spilled). Measured, GPU
+// us: 64 sequences of 8192 tokens, 8 KV heads of 8 317 (6.8 TB/s); 32 of 30 .. 8000 in
+// bf16 33.4 (5.0 TB/s); one of 50001, heads of 64, 22.4 (4.6 TB/s); 24 of 100 .. 12000
+// in a window of 4096 22.7 (3.9 TB/s: small pages, a look-up per octet); one of 700 8.2,
+// a chain of dependent reads (lengths, pages, keys, hand-off) behind the launch.
 #pragma once
 
 #include "paged_common.hpp"
@@ -35,7 +42,7 @@ namespace llmik {
 
 constexpr int kPdWaves = 4;
 constexpr int kPdThreads = kPdWaves * kWave;
-constexpr int kPdPerCu = 2;       // workgroups per CU
+constexpr int kPdPerCu = 2;       // workgroups per CU (3 spill: 32 ragged sequences 81 us instead of 33)
 
 struct PagedDecodeParams {
     const uint16_t* q;
@@ -53,9 +60,9 @@ struct PagedDecodeParams {
     int few_steps;        // workgroups that few tiles are spread over, one tile per wave
 };
 
-constexpr int kPieceUnits = 6;
-constexpr int kUncutTiles = 12;
-constexpr int kEachTiles = 24;
+constexpr int kPieceUnits = 6;    // a piece's overhead in units of a tile's time (see the shares)
+constexpr int kUncutTiles = 12;   // a slab of so few tiles is not cut: three per wave cost less than a hand-off
+constexpr int kEachTiles = 24;    // the longest slab where every workgroup takes one
 
 // A sequence's length, its live keys [begin, end) and their 32-token tiles.
 // Every sequence has one tile at least, so that its rows are written.

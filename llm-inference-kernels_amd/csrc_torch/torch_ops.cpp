@@ -727,7 +727,7 @@ int paged_heads(const Tensor& q, const llmik_paged_cache& c) {
 llmik_score_options paged_options(const Tensor& q, double softmax_scale, double softcap,
                                   const std::optional<Tensor>& slopes, int64_t window) {
     TORCH_CHECK(std::isfinite((float)softmax_scale), "softmax_scale must be finite");
-    TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), "softcap must be >= 0 and finite");
+    TORCH_CHECK(softcap >= 0 && softcap <= 4096, "softcap must be >= 0 and at most 4096");
     TORCH_CHECK(window >= 0 && window <= INT_MAX, "window must be >= 0");
     llmik_score_options o{(float)softmax_scale, (float)softcap, nullptr, (int)window};
     if (slopes.has_value()) {

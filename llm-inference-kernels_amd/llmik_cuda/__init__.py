@@ -475,8 +475,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            window: int = 0) -> torch.Tensor:
     """Decode attention of each sequence's newest token: q, out [batch,
     n_heads, head_dim] over the seq_lens[b] live tokens of its pages. Scores
-    softmax_scale * q . k, with softcap > 0 softcap * tanh(score / softcap),
-    with slopes [n_heads] fp32 minus slopes[h] * (distance in tokens); with
+    softmax_scale * q . k, with softcap > 0 (at most 4096) softcap *
+    tanh(score / softcap), with slopes [n_heads] fp32 minus slopes[h] * (distance in tokens); with
     window > 0 only the newest `window` keys. A sequence without a key gives
     zeros. Deterministic; the bits depend on the lengths of the whole batch."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and

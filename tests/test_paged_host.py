@@ -100,7 +100,8 @@ def test_c_layer_refuses_arguments(lib):
                          (dict(rows=1 << 30), UNSUPPORTED, "too many rows")]:
         assert append(**a) == code and msg in err(), a
     for more, msg in [(dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
-                      (dict(softcap=float("inf")), "softcap"), (dict(softmax_scale=float("nan")), "softmax_scale"),
+                      (dict(softcap=float("inf")), "softcap"), (dict(softcap=4097.0), "softcap"),
+                      (dict(softcap=1e-38, softmax_scale=100.0), "softcap too small"), (dict(softmax_scale=float("nan")), "softmax_scale"),
                       (dict(softmax_scale=float("inf")), "softmax_scale"), (dict(window=-1), "window")]:
         bad = _options(**more)
         assert lib.llmik_paged_decode_attention(_at(c), 16, 16, 4, _at(bad), 16, 0, None) == INVALID and msg in err()
