@@ -217,8 +217,9 @@ class PagedBatch(NamedTuple):
 
 
 class PagedKVCache:
-    """Sequences of different lengths over one pool of `n_pages` pages of
-    `page_size` tokens: k, v [n_pages, n_kv_heads, page_size, head_dim].
+    """Sequences of different lengths over a pool of `n_pages` pages of `page_size`
+    tokens per layer: k, v [n_layers, n_pages, n_kv_heads, page_size, head_dim]. A
+    page number means the same tokens in every layer.
 
     The host keeps each sequence's length and pages; `batch` reserves pages for
     a call's new tokens and hands the tables to the device, `append` rotates
@@ -233,9 +234,8 @@ class PagedKVCache:
         c = cache.add(share=a, tokens=1000)           # behind the first 1000 tokens of a
         cache.remove(b)
 
-    One `batch` serves the layers of a model if each layer has its own pool of
-    the same shape: `append` and `attention` take the pool's k and v. Not safe
-    for calls from several threads."""
+    One `batch` serves all layers: `append` and `attention` take the layer's
+    number. All calls belong on one stream; not safe for several threads."""
 
     # A batch's shared prefix is read once for all sequences where that saves so many
     # token rows (of one KV head) and has so many tokens; a shorter one where it saves
@@ -244,14 +244,15 @@ class PagedKVCache:
     SHARED_TOKENS = 512
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, head_dim: int = 128,
-                 dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None) -> None:
-        _require(n_pages > 0 and n_kv_heads > 0, "n_pages and n_kv_heads must be positive")
+                 dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None,
+                 n_layers: int = 1) -> None:
+        _require(n_pages > 0 and n_kv_heads > 0 and n_layers > 0, "n_pages, n_kv_heads and n_layers must be positive")
         _require(page_size > 0 and page_size % 8 == 0, "page_size must be a positive multiple of 8")
         _require(head_dim in (64, 128), "only head_dim=64 and 128 supported")
         _require(dtype in (torch.float16, torch.bfloat16), "dtype must be fp16 or bf16")
         self.device = torch.device("cuda") if device is None else torch.device(device)
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, n_kv_heads, page_size, head_dim
-        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v = torch.zeros(shape, dtype=dtype, device=self.device)
         self._free = list(range(n_pages - 1, -1, -1))
@@ -276,8 +277,8 @@ class PagedKVCache:
                 _require(len(self._free) > 0, "the cache has no free page")
                 page, src = self._free.pop(), self._pages[share][whole]
                 self._users[page] = 1
-                self.k[page, :, :rest] = self.k[src, :, :rest]
-                self.v[page, :, :rest] = self.v[src, :, :rest]
+                self.k[:, page, :, :rest] = self.k[:, src, :, :rest]
+                self.v[:, page, :, :rest] = self.v[:, src, :, :rest]
             for p in pages:
                 self._users[p] += 1
             if rest:
@@ -364,18 +365,17 @@ class PagedKVCache:
         return same if tokens > 0 and saved >= least else 0
 
     def append(self, step: PagedBatch, qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
-               k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """rope_paged_append of the batch's new tokens; returns the rotated q
-        [rows, n_heads, head_dim]. k, v: another layer's pool."""
-        return rope_paged_append(qkv, cos, sin, self.k if k is None else k, self.v if v is None else v,
-                                 step.page_table, step.seq_lens, step.cu_tokens)
+               layer: int = 0) -> torch.Tensor:
+        """rope_paged_append of the batch's new tokens to a layer; returns the
+        rotated q [rows, n_heads, head_dim]."""
+        return rope_paged_append(qkv, cos, sin, self.k[layer], self.v[layer], step.page_table, step.seq_lens,
+                                 step.cu_tokens)
 
     def attention(self, step: PagedBatch, q: torch.Tensor, softmax_scale: float, softcap: float = 0.0,
-                  slopes: Optional[torch.Tensor] = None, window: int = 0, k: Optional[torch.Tensor] = None,
-                  v: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Attention of the batch's new tokens: decode, decode behind a shared
-        prefix, or prompts, by the batch."""
-        k, v = self.k if k is None else k, self.v if v is None else v
+                  slopes: Optional[torch.Tensor] = None, window: int = 0, layer: int = 0) -> torch.Tensor:
+        """Attention of the batch's new tokens in a layer: decode, decode behind a
+        shared prefix, or prompts, by the batch."""
+        k, v = self.k[layer], self.v[layer]
         if step.cu_tokens is not None:
             return paged_prefill_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, softmax_scale,
                                            softcap, slopes, window)

@@ -54,8 +54,8 @@ def test_a_serving_loop(llmik, cuda, dtype, D, page, opts):
             assert bool(((q[at:at + n].double() - turned[:, :H]).abs() <= 2 * ref.U[dtype] * turned[:, :H].abs()
                          + 2.0 ** -20).all())
             row = batch.page_table[seqs.index(s)]
-            k, ok = ref.tokens_of(cache.k, row, h + n, page)
-            v, _ = ref.tokens_of(cache.v, row, h + n, page)
+            k, ok = ref.tokens_of(cache.k[0], row, h + n, page)
+            v, _ = ref.tokens_of(cache.v[0], row, h + n, page)
             assert bool(ok.all())
             k, v = k.transpose(0, 1), v.transpose(0, 1)
             old_k, old_v = kept[s]
@@ -98,15 +98,20 @@ def test_a_serving_loop(llmik, cuda, dtype, D, page, opts):
 
 
 def test_layers_share_a_batch(llmik, cuda):
-    """One batch description serves a second layer's pool."""
+    """One batch serves two layers, and a fork's tokens are there in both."""
     from llmik_cuda.kv_cache import PagedKVCache
     H, Hkv, D = 8, 2, 128
-    cache = PagedKVCache(20, Hkv, page_size=16)
-    k2, v2 = torch.zeros_like(cache.k), torch.zeros_like(cache.v)
+    cache = PagedKVCache(20, Hkv, page_size=16, n_layers=2)
     a, b = cache.add(), cache.add()
     batch = cache.batch([a, b], [33, 5])
     x = torch.randn(38, (H + 2 * Hkv) * D, device=cuda).half()
     q1 = cache.append(batch, x, None, None)
-    q2 = cache.append(batch, x, None, None, k=k2, v=v2)
-    assert torch.equal(q1, q2) and torch.equal(cache.k, k2) and torch.equal(cache.v, v2)
-    assert torch.equal(cache.attention(batch, q1, 0.1), cache.attention(batch, q2, 0.1, k=k2, v=v2))
+    q2 = cache.append(batch, x, None, None, layer=1)
+    assert torch.equal(q1, q2) and torch.equal(cache.k[0], cache.k[1]) and torch.equal(cache.v[0], cache.v[1])
+    assert torch.equal(cache.attention(batch, q1, 0.1), cache.attention(batch, q2, 0.1, layer=1))
+    batch = cache.batch([a, cache.add(share=a, tokens=33)])
+    x = torch.randn(1, (H + 2 * Hkv) * D, device=cuda).half().expand(2, -1)
+    for layer in range(2):
+        q = cache.append(batch, x, None, None, layer=layer)
+        out = cache.attention(batch, q, 0.1, layer=layer)
+        assert torch.equal(out[0], out[1])      # the same tokens, the same query

@@ -238,13 +238,13 @@ def test_a_batch_that_does_not_fit_changes_nothing(cache):
 def test_sharing_and_removal(cache):
     a = cache.add()
     first = cache.batch([a], [20]).page_table[0].tolist()
-    cache.k[first[2], :, :4] = 3.0
+    cache.k[0, first[2], :, :4] = 3.0
     b = cache.add(share=a, tokens=18)
     assert cache.length(b) == 18 and cache.free_pages() == 6
     step = cache.batch([a, b])
     rows = step.page_table.tolist()
     assert rows[0][:2] == rows[1][:2] and rows[0][2] != rows[1][2]
-    assert bool((cache.k[rows[1][2], :, :2] == 3.0).all()) and bool((cache.k[rows[1][2], :, 2:] == 0.0).all())
+    assert bool((cache.k[0, rows[1][2], :, :2] == 3.0).all()) and bool((cache.k[0, rows[1][2], :, 2:] == 0.0).all())
     cache.remove(a)
     assert cache.free_pages() == 7        # the two shared pages are still b's
     cache.remove(b)
@@ -256,6 +256,20 @@ def test_sharing_and_removal(cache):
     c = cache.add()
     with pytest.raises(RuntimeError, match="fewer tokens"):
         cache.add(share=c, tokens=1)
+
+
+def test_a_fork_copies_the_last_page_in_every_layer():
+    from llmik_cuda.kv_cache import PagedKVCache
+    cache = PagedKVCache(6, 2, page_size=8, head_dim=64, device="cpu", n_layers=3)
+    a = cache.add()
+    src = cache.batch([a], [12]).page_table[0, 1]
+    cache.k.normal_()
+    cache.v.normal_()
+    b = cache.add(share=a, tokens=11)
+    dst = cache.batch([b]).page_table[0, 1]
+    assert dst != src
+    assert torch.equal(cache.k[:, dst, :, :3], cache.k[:, src, :, :3])
+    assert torch.equal(cache.v[:, dst, :, :3], cache.v[:, src, :, :3])
 
 
 def test_a_batch_knows_its_shared_prefix(cache):
