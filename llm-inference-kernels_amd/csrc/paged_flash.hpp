@@ -86,7 +86,15 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
         return (uint32_t)(tokens_of(b, row0) * (int)p.gqa.d + kPfRows - 1) / kPfRows;
     };
     uint32_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    int row0 = 0, rows = 0, pos0 = 0;   // the lane's only sequence, where per is 1: one round trip less
+    if (per == 1 && b0 < b1) {
+        const int len = p.c.lens[b0], stop = p.cu[b0 + 1];
+        rows = tokens_of(b0, row0);
+        mine = (uint32_t)(rows * (int)p.gqa.d + kPfRows - 1) / kPfRows;
+        pos0 = len - (stop - row0);
+    } else {
+        for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    }
     const uint32_t incl = wave_scan(mine);
     const uint32_t total = lane_u32(incl, 63);
     if (item >= total) return false;
@@ -116,10 +124,16 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
         }
     }
     t.b = __builtin_amdgcn_readfirstlane(b);
-    t.rows = __builtin_amdgcn_readfirstlane(tokens_of(t.b, t.row0));
-    t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
     t.tile = __builtin_amdgcn_readfirstlane((int)(x - first));
-    t.pos0 = __builtin_amdgcn_readfirstlane(p.c.lens[t.b] - (p.cu[t.b + 1] - t.row0));
+    if (per == 1) {
+        t.rows = __builtin_amdgcn_readlane(rows, t.b);
+        t.row0 = __builtin_amdgcn_readlane(row0, t.b);
+        t.pos0 = __builtin_amdgcn_readlane(pos0, t.b);
+    } else {
+        t.rows = __builtin_amdgcn_readfirstlane(tokens_of(t.b, t.row0));
+        t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
+        t.pos0 = __builtin_amdgcn_readfirstlane(p.c.lens[t.b] - (p.cu[t.b + 1] - t.row0));
+    }
     return true;
 }
 
@@ -185,12 +199,14 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         ft.tile = (int)item;
         ft.rows = p.c.batch;
     } else {
+        const int used = p.cu[p.c.batch];
+        const bool found = find_tile(p, item, ft);
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
         const long chunks = (long)p.n_heads * CPR;
         const long at0 = (long)wg * kPfThreads + tid, step = (long)n_wg * kPfThreads;
-        for (long i = min(max(p.cu[p.c.batch], 0), p.rows) * chunks + at0; i < p.rows * chunks; i += step)
+        for (long i = min(max(used, 0), p.rows) * chunks + at0; i < p.rows * chunks; i += step)
             *reinterpret_cast<u32x4*>(p.out + 8 * i) = u32x4{0u, 0u, 0u, 0u};
-        if (!find_tile(p, item, ft)) return;
+        if (!found) return;
     }
     const int n_rows = ft.rows * G;
     const int r_wave = ft.tile * kPfRows + 32 * wave;   // the wave's first row
@@ -200,11 +216,6 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const int head = kvh * G + (r - qi * G);
     const long q_row = (PREFIX ? (long)qi : (long)ft.row0 + qi) * p.n_heads + head;
     const int pos = PREFIX ? p.c.lens[qi] - 1 : ft.pos0 + qi;
-    u32x4 qb[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qb[ks] = load16(p.q + q_row * D + 16 * ks + 8 * h);
-    const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
-
     // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
     auto oldest = [&](int at) { return oldest_key(p.s, at); };
     int begin, end, tiles, parts = 1;
@@ -274,7 +285,12 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         at_bytes = gone ? 0 : min(max(end - token_of(i0), 0), 8) * kRowBytes;
         batch_gone = __ballot(gone);
     };
-    adopt(look_up(0), 0);
+    const long off_first = look_up(0);
+    u32x4 qb[KS];   // (requested behind the look-up, which is waited for first)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qb[ks] = load16(p.q + q_row * D + 16 * ks + 8 * h);
+    const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
+    adopt(off_first, 0);
     long off_next = tiles > 8 ? look_up(8) : -1L;
     // Copy instruction c fills rows kRowsPerCopy c .. of the wave's 16: lane l writes
     // chunk slot l % CPR of row l / CPR, i.e. the chunk that the permutation puts there.
@@ -496,30 +512,59 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                       : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + row;
     };
     const bool as_part = PREFIX || parts > 1;
-    if (live && r_wave + n < n_rows) {
-        if (as_part) {
-            const long at = part_at(32 * wave + n);
+    // The wave's rows go through LDS, so that whole rows are stored, 16 bytes a lane: from
+    // the registers a store of outputs has 64 pieces of 8 bytes, a row apart (us, three
+    // short prompts 8.96, 8.15 through LDS), one of parts pieces of 16, which wins where
+    // few rows are there (64 sequences behind 8192 tokens 31.1, 29.7 through LDS, 6 behind
+    // 1500 10.3, 10.9). Chunks of 16 bytes are permuted like the tiles'.
+    const bool direct = as_part && ft.tile * kPfRows + kPfRows > n_rows;
+    const int n_live = min(n_rows - r_wave, 32);   // rows of the wave; none: <= 0
+    uint8_t* const rows_at = wave == 0 ? s_k0 : wave == 1 ? s_k1 : wave == 2 ? s_v0 : s_v1;
+    auto place = [&](int row, int chunk, int chunks) {
+        return rows_at + 16 * (row * chunks + (chunk ^ (row & (chunks - 1))));
+    };
+    auto quad = [&](int cb, int e) { return f32x4{o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]}; };
+    __syncthreads();   // the tiles are read
+    if (live && as_part) {
+        constexpr int kChunks = D / 4;
+        const long at = part_at(32 * wave + n);
+        if (h == 0 && n < n_live) *reinterpret_cast<f32x2*>(p.part_ml + 2 * at) = f32x2{m_run, l_run};
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
+        for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * cb + 2 * e + 4 * h) =
-                        f32x4{o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]};
-            if (h == 0) {
-                p.part_ml[2 * at] = m_run;
-                p.part_ml[2 * at + 1] = l_run;
+            for (int e = 0; e < 16; e += 4) {
+                const int c = 8 * cb + e / 2 + h;
+                if (!direct) *reinterpret_cast<f32x4*>(place(n, c, kChunks)) = quad(cb, e);
+                else if (n < n_live) *reinterpret_cast<f32x4*>(p.part_o + at * D + 4 * c) = quad(cb, e);
             }
-        } else {
-            const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;   // a row without keys is zero
+        if (!direct) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
+            for (int j = 0; j < kChunks / 2; ++j) {
+                const int row = (64 * j + lane) / kChunks, c = lane % kChunks;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(place(row, c, kChunks));
+                *reinterpret_cast<u32x4*>(p.part_o + part_at(32 * wave + row) * D + 4 * c) = v;   // (all rows live)
+            }
+        }
+    } else if (live) {
+        constexpr int kChunks = D / 8;
+        const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;   // a row without keys is zero
 #pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<u32x2*>(p.out + q_row * D + 32 * cb + 2 * e + 4 * h) = u32x2{
-                        Hf::pack(o[cb][e] * inv, o[cb][e + 1] * inv), Hf::pack(o[cb][e + 2] * inv, o[cb][e + 3] * inv)};
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 v = quad(cb, e);
+                *reinterpret_cast<u32x2*>(place(n, 4 * cb + e / 4, kChunks) + 8 * h) =
+                    u32x2{Hf::pack(v[0] * inv, v[1] * inv), Hf::pack(v[2] * inv, v[3] * inv)};
+            }
+#pragma unroll
+        for (int j = 0; j < kChunks / 2; ++j) {
+            const int row = (64 * j + lane) / kChunks, c = lane % kChunks, rw = r_wave + row;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(place(row, c, kChunks));
+            const int qr = (int)p.gqa.div((uint32_t)rw);
+            const long to = ((long)ft.row0 + qr) * p.n_heads + kvh * G + (rw - qr * G);
+            if (row < n_live) *reinterpret_cast<u32x4*>(p.out + to * D + 8 * c) = v;
         }
     }
-    __syncthreads();
     if (tiles == 0 || __builtin_amdgcn_readfirstlane((int)s_bad) == 0) return;
 
     // ---- some V is no number, and not all rows see it: the wave's rows one by one,
