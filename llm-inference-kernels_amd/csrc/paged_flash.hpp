@@ -470,16 +470,19 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         // for infinities and NaN (bits of |x| from the type's infinity on): a probability
         // of 0 would make NaN of them. Such a tile's rows are done again, below.
         if (i < wg_full_lo || i >= wg_full_hi) {   // workgroup-uniform
+            u32x4 w[kCopies];
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c)
+                w[c] = *reinterpret_cast<const u32x4*>(v_cur + 16 * wave * kRowBytes + 1024 * c + 16 * lane);
+            __builtin_amdgcn_sched_barrier(0);   // (one wait for all)
             uint32_t top = 0;
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(v_cur + 16 * wave * kRowBytes + 1024 * c + 16 * lane);
+            for (int c = 0; c < kCopies; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t x = w[e];
+                    const uint32_t x = w[c][e];
                     top = max_abs2(top, x);
                 }
-            }
             const uint32_t inf = BF ? 0x7F80u : 0x7C00u;
             if ((top & 0xFFFFu) >= inf || (top >> 16) >= inf) s_bad = 1u;
         }
