@@ -116,6 +116,11 @@ __device__ __forceinline__ long octet_offset(const PagedView& c, const int* tabl
     return in && (uint32_t)page < (uint32_t)c.n_pages ? at : -1L;
 }
 
+// publish_load16's 8-byte form.
+__device__ __forceinline__ u32x2 publish_load8(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
+    return __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, kPublishAux);
+}
+
 // A running maximum starts here rather than at -inf: differences of two such are
 // then numbers, and states without a key join like all others (their sums are 0).
 constexpr float kNoMax = -1e30f;

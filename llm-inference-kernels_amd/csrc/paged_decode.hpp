@@ -466,35 +466,41 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
             const int groups = 16 / span;
             const int h = (tid >> 4) & (span - 1);
             const int grp = __builtin_amdgcn_readfirstlane(tid / (16 * span));
-            constexpr int kBatch = 8;
-            const std::integral_constant<int, kBatch> batch{};
             if (!whole) {
                 const int parts = (int)(wg1 - wg0 + 1);
+                const __amdgpu_buffer_rsrc_t rml =
+                    make_buffer_rsrc(p.part_ml, (uint32_t)(2u * n_wg * p.chunk_heads * 2 * 4));
                 wm = kNoMax;
                 wl = 0.0f;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) wo[e] = 0.0f;
-                if (h < nh) {
-                    for (int i0 = grp; i0 < parts; i0 += kBatch * groups) {
-                        float m[kBatch], l[kBatch], v[kBatch][VEC];
+                auto fetch = [&](auto batch, int i0) {   // parts i0, i0 + groups, ...
+                    constexpr int N = decltype(batch)::value;
+                    float m[N], l[N], v[N][VEC];
 #pragma unroll
-                        for (int u = 0; u < kBatch; ++u) {
-                            const int i = min(i0 + u * groups, parts - 1);
-                            const uint32_t row = (2 * (wg0 + (uint32_t)i) + (i == 0 ? 1u : 0u)) * p.chunk_heads + h;
-                            m[u] = publish_load(&p.part_ml[2 * row]);
-                            l[u] = publish_load(&p.part_ml[2 * row + 1]);
+                    for (int u = 0; u < N; ++u) {
+                        const int i = min(i0 + u * groups, parts - 1);
+                        const uint32_t row = (2 * (wg0 + (uint32_t)i) + (i == 0 ? 1u : 0u)) * p.chunk_heads + h;
+                        const u32x2 ml = publish_load8(rml, row * 8u);
+                        const uint32_t mb = ml[0], lb = ml[1];
+                        m[u] = __uint_as_float(mb);
+                        l[u] = __uint_as_float(lb);
 #pragma unroll
-                            for (int e = 0; e < VEC; e += 4) {
-                                const u32x4 r = publish_load16(ro, (row * D + ch + e) * 4u);
+                        for (int e = 0; e < VEC; e += 4) {
+                            const u32x4 r = publish_load16(ro, (row * D + ch + e) * 4u);
 #pragma unroll
-                                for (int e2 = 0; e2 < 4; ++e2) {
-                                    const uint32_t bits = r[e2];
-                                    v[u][e + e2] = __uint_as_float(bits);
-                                }
+                            for (int e2 = 0; e2 < 4; ++e2) {
+                                const uint32_t bits = r[e2];
+                                v[u][e + e2] = __uint_as_float(bits);
                             }
                         }
-                        join(batch, (parts - i0 + groups - 1) / groups, m, l, v);
                     }
+                    join(batch, (parts - i0 + groups - 1) / groups, m, l, v);
+                };
+                if (h < nh) {
+                    int i0 = grp;
+                    for (; parts - i0 > 2 * groups; i0 += 8 * groups) fetch(std::integral_constant<int, 8>{}, i0);
+                    if (i0 < parts) fetch(std::integral_constant<int, 2>{}, i0);
                 }
             }
             if (groups > 1 && !whole) {   // workgroup-uniform
