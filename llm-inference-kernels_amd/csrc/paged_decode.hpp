@@ -31,8 +31,8 @@
 // Registers hold one tile: the next tile's keys are requested when the scores are
 // computed, its values when their products are (two buffers spilled). Measured, GPU
 // us: 64 sequences of 8192 tokens, 8 KV heads of 8 317 (6.8 TB/s); 32 of 30 .. 8000 in
-// bf16 33.4 (5.0 TB/s); one of 50001, heads of 64, 22.4 (4.6 TB/s); 24 of 100 .. 12000
-// in a window of 4096 22.7 (3.9 TB/s: small pages, a look-up per octet); one of 700 8.2,
+// bf16 33.2 (5.1 TB/s); one of 50001, heads of 64, 22.6 (4.5 TB/s); 24 of 100 .. 12000
+// in a window of 4096 23.0 (3.9 TB/s: small pages, a look-up per octet); one of 700 8.1,
 // a chain of dependent reads (lengths, pages, keys, hand-off) behind the launch.
 #pragma once
 
@@ -461,7 +461,8 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
         if (finish) {
             // The parts of the slab's workgroups. All threads fetch: groups of 16 threads per
             // head (rounded up to 4, 8 or 16 heads) take every groups-th part, eight of them
-            // requested at a time, and are joined through LDS.
+            // requested at a time (two where there are no more: each bypasses the L2, us,
+            // one sequence of 700 tokens 8.7, 8.05), and are joined through LDS.
             const int span = nh <= 4 ? 4 : nh <= 8 ? 8 : 16;
             const int groups = 16 / span;
             const int h = (tid >> 4) & (span - 1);

@@ -25,11 +25,11 @@
 // Where there are fewer row tiles than two workgroups per CU, their keys are cut into
 // parts, whose sums a second kernel joins (paged_flash.hip, paged_prefix.hip).
 //
-// Measured: a prompt of 8192 tokens, 32 heads over 8 KV heads of 128, bf16: 528 us,
-// 1.04 PFLOP/s (a large matrix product reaches 1.42): the matrix units work 57 % of
+// Measured: a prompt of 8192 tokens, 32 heads over 8 KV heads of 128, bf16: 520 .. 535
+// us, 1.03 .. 1.06 PFLOP/s (a large matrix product reaches 1.42): the matrix units work 57 % of
 // the cycles, beside 3 vector instructions per score, and the clock falls to 1.8 GHz.
-// Chunks of four prompts over up to 6000 cached tokens, capped scores: 168 us, 0.69
-// PFLOP/s, bound by the cap's two transcendentals per score. Three short prompts 9.1 us:
+// Chunks of four prompts over up to 6000 cached tokens, capped scores: 165 us, 0.70
+// PFLOP/s, bound by the cap's two transcendentals per score. Three short prompts 8.2 us:
 // launch, look-ups, two or three tiles.
 #pragma once
 
