@@ -14,12 +14,12 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashPa
     paged_flash<BF, D, false>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_bad});
 }
 
-constexpr int kJoinRows = 8;
+// Rows of a workgroup of the join: a thread has four channels of one.
+constexpr int join_rows(int head_dim) { return 256 * 4 / head_dim; }
 
-// The parts of the row tiles joined: a workgroup takes kJoinRows rows of a tile, a
-// thread four channels of every 256 * 4 / D-th row. The time is a chain of loads, so
-// each is requested once (us, 512 rows of a prompt over 16000 tokens with 32 rows and
-// 8: 57.6, 56.3; 8 x 8 rows over 8000: 41.1, 39.0).
+// The parts of the row tiles joined. The time is a chain of loads, so every thread has
+// one (us, 512 rows of a prompt over 16000 tokens with 32 rows a workgroup and 8: 57.6,
+// 56.3; 8 x 8 rows over 8000: 41.1, 39.0).
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void paged_flash_join_kernel(PagedFlashParams p) {
     using Hf = Half16<BF>;
@@ -30,40 +30,37 @@ __global__ __launch_bounds__(256) void paged_flash_join_kernel(PagedFlashParams 
     const int parts = __builtin_amdgcn_readfirstlane(keys_of_tile(p, ft).parts);
     const int n_rows = ft.rows * (int)p.gqa.d;
     if (parts == 1) return;
-    constexpr int kStep = 256 * 4 / D;
+    static_assert(kPfRows % join_rows(D) == 0, "a workgroup's rows belong to one tile");
     const int c4 = 4 * ((int)threadIdx.x % (D / 4));
     const long at0 = ((long)item * p.c.n_kv_heads + kvh) * p.splits * kPfRows;
+    const int row = join_rows(D) * (int)blockIdx.y + (int)threadIdx.x / (D / 4);   // of the tile
+    const int r = ft.tile * kPfRows + row;
+    if (r >= n_rows) return;
+    float m[kMaxParts], l[kMaxParts], top = kNoMax;
+    f32x4 v[kMaxParts];
 #pragma unroll
-    for (int i = 0; i < kJoinRows; i += kStep) {
-        const int row = kJoinRows * (int)blockIdx.y + i + (int)threadIdx.x / (D / 4);   // of the tile
-        const int r = ft.tile * kPfRows + row;
-        if (r >= n_rows) continue;
-        float m[kMaxParts], l[kMaxParts], top = kNoMax;
-        f32x4 v[kMaxParts];
-#pragma unroll
-        for (int u = 0; u < kMaxParts; ++u) {
-            const long at = at0 + (long)min(u, parts - 1) * kPfRows + row;
-            m[u] = p.part_ml[2 * at];
-            l[u] = p.part_ml[2 * at + 1];
-            v[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + c4);
-        }
-#pragma unroll
-        for (int u = 0; u < kMaxParts; ++u) top = fmaxf(top, m[u]);
-        float sum = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int u = 0; u < kMaxParts; ++u) {
-            const float w = u < parts ? __builtin_amdgcn_exp2f(m[u] - top) : 0.0f;
-            sum = u < parts ? fmaf(l[u], w, sum) : sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = u < parts ? fmaf(v[u][e], w, o[e]) : o[e];
-        }
-        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-        const int qi = (int)p.gqa.div((uint32_t)r);
-        const long q_row = ((long)ft.row0 + qi) * p.n_heads + kvh * (int)p.gqa.d + (r - qi * (int)p.gqa.d);
-        *reinterpret_cast<u32x2*>(p.out + q_row * D + c4) =
-            u32x2{Hf::pack(o[0] * inv, o[1] * inv), Hf::pack(o[2] * inv, o[3] * inv)};
+    for (int u = 0; u < kMaxParts; ++u) {
+        const long at = at0 + (long)min(u, parts - 1) * kPfRows + row;
+        m[u] = p.part_ml[2 * at];
+        l[u] = p.part_ml[2 * at + 1];
+        v[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + c4);
     }
+#pragma unroll
+    for (int u = 0; u < kMaxParts; ++u) top = fmaxf(top, m[u]);
+    float sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kMaxParts; ++u) {
+        const float w = u < parts ? __builtin_amdgcn_exp2f(m[u] - top) : 0.0f;
+        sum = u < parts ? fmaf(l[u], w, sum) : sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = u < parts ? fmaf(v[u][e], w, o[e]) : o[e];
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int qi = (int)p.gqa.div((uint32_t)r);
+    const long q_row = ((long)ft.row0 + qi) * p.n_heads + kvh * (int)p.gqa.d + (r - qi * (int)p.gqa.d);
+    *reinterpret_cast<u32x2*>(p.out + q_row * D + c4) =
+        u32x2{Hf::pack(o[0] * inv, o[1] * inv), Hf::pack(o[2] * inv, o[3] * inv)};
 }
 
 // ---------------------------------------------------------------- host
@@ -126,7 +123,7 @@ int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream) {
     }
     launch_flash(a, p, pl.tiles * a.n_kv_heads * pl.splits, stream);
     if (pl.splits > 1) {
-        const dim3 grid((unsigned)(pl.tiles * a.n_kv_heads), kPfRows / kJoinRows);
+        const dim3 grid((unsigned)(pl.tiles * a.n_kv_heads), (unsigned)(kPfRows / join_rows(a.head_dim)));
         if (a.bf16)
             a.head_dim == 128 ? paged_flash_join_kernel<true, 128><<<grid, 256, 0, stream>>>(p)
                               : paged_flash_join_kernel<true, 64><<<grid, 256, 0, stream>>>(p);

@@ -91,6 +91,10 @@ PREFILL = [
     ([10, 300], [200, 577], 32, 8, 128, 32, F16, {"window": 50}),
     ([10, 300], [20, 77], 8, 1, 128, 40, F16, {"window": 1}),
     ([1010, 300], [200, 577], 12, 4, 128, 32, BF16, {"window": 333, "slopes": True, "softcap": 30.0}),
+    # keys in parts, several row tiles each
+    ([715, 1136, 360], [106, 114, 87], 16, 8, 64, 16, F16, {"slopes": True}),
+    ([3000, 0, 1500], [333, 65, 1], 8, 2, 64, 64, BF16, {}),
+    ([3000, 0, 1500], [333, 65, 1], 8, 2, 128, 64, BF16, {"softcap": 40.0}),
 ]
 
 
