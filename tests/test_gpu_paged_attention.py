@@ -3,6 +3,7 @@ the float64 definition (tests/paged_ref.py, where the tolerances are derived).""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -484,4 +485,65 @@ def test_a_long_table_of_many_sequences(llmik, cuda):
     new = [min(n, 1 + i % 7) for i, n in enumerate(lens)]
     got, want, bound = _prefill(llmik, cuda, [n - m for n, m in zip(lens, new)], new, 4, 2, 64, 8, F16, {},
                                 extra_columns=50)
+    ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_scales_of_zero_and_below(llmik, cuda, scale, softcap):
+    lens, H, Hkv, D, page = [300, 65], 8, 2, 128, 16
+    k, v, table, seq = ref.make_cache(lens, Hkv, D, page, F16, cuda, 3)
+    for new in ([1, 1], [130, 65]):
+        q = _q(sum(new), H, D, F16, cuda, 4)
+        if new == [1, 1]:
+            got = llmik.paged_decode_attention(q, k, v, table, seq, scale, softcap)
+        else:
+            got = llmik.paged_prefill_attention(q, k, v, table, seq, ref.offsets(new, cuda), scale, softcap)
+        want, bound = ref.attention(q, k, v, table, lens, new, scale, page, new == [1, 1], softcap=softcap)
+        ref.check(got, want, bound)
+
+
+# ----------------------------------------------------------------- drawn shapes
+
+def _drawn(seed):
+    rng = random.Random(seed)
+    log = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))   # noqa: E731
+    Hkv = rng.choice([1, 2, 3, 4, 8])
+    shape = (Hkv * rng.choice([1, 2, 3, 4, 5, 7, 8, 12, 17]), Hkv, rng.choice([64, 128]),
+             8 * rng.choice([1, 2, 3, 4, 5, 8, 16]), rng.choice([F16, BF16]))
+    opts = {}
+    if rng.random() < 0.3:
+        opts["softcap"] = rng.choice([5.0, 30.0])
+    if rng.random() < 0.3:
+        opts["slopes"] = True
+    if rng.random() < 0.3:
+        opts["window"] = log(1, 3000)
+    return rng, log, shape, opts
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_drawn_decodes(llmik, cuda, seed):
+    rng, log, shape, opts = _drawn(100 + seed)
+    hi = log(1, 6000)
+    lens = [rng.randint(0, hi) for _ in range(log(1, 90))]
+    got, want, bound = _decode(llmik, cuda, lens, *shape, opts, seed=seed)
+    ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_prompts(llmik, cuda, seed):
+    rng, log, shape, opts = _drawn(200 + seed)
+    B = rng.randint(1, 6)
+    ctx = [rng.choice([0, log(1, 4000)]) for _ in range(B)]
+    new = [rng.choice([0, log(1, 400)]) for _ in range(B)]
+    got, want, bound = _prefill(llmik, cuda, ctx, new, *shape, opts, seed=seed, pad=rng.randint(0, 3))
+    ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_drawn_prefixes(llmik, cuda, seed):
+    rng, log, shape, opts = _drawn(300 + seed)
+    P = log(1, 5000)
+    own = [rng.randint(1, 300) for _ in range(log(1, 60))]
+    got, want, bound = _prefix(llmik, cuda, P, own, *shape, opts, seed=seed)
     ref.check(got, want, bound)
