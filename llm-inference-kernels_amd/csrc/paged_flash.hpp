@@ -88,7 +88,7 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
     uint32_t mine = 0;
     int row0 = 0, rows = 0, pos0 = 0;   // the lane's only sequence, where per is 1: one round trip less
     if (per == 1 && b0 < b1) {
-        const int len = p.c.lens[b0], stop = p.cu[b0 + 1];
+        const int len = max(p.c.lens[b0], 0), stop = p.cu[b0 + 1];
         rows = tokens_of(b0, row0);
         mine = (uint32_t)(rows * (int)p.gqa.d + kPfRows - 1) / kPfRows;
         pos0 = len - (stop - row0);
@@ -132,7 +132,7 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
     } else {
         t.rows = __builtin_amdgcn_readfirstlane(tokens_of(t.b, t.row0));
         t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
-        t.pos0 = __builtin_amdgcn_readfirstlane(p.c.lens[t.b] - (p.cu[t.b + 1] - t.row0));
+        t.pos0 = __builtin_amdgcn_readfirstlane(max(p.c.lens[t.b], 0) - (p.cu[t.b + 1] - t.row0));
     }
     return true;
 }
@@ -215,7 +215,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const int qi = (int)p.gqa.div((uint32_t)r);
     const int head = kvh * G + (r - qi * G);
     const long q_row = (PREFIX ? (long)qi : (long)ft.row0 + qi) * p.n_heads + head;
-    const int pos = PREFIX ? p.c.lens[qi] - 1 : ft.pos0 + qi;
+    const int pos = PREFIX ? max(p.c.lens[qi], 0) - 1 : ft.pos0 + qi;
     // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
     auto oldest = [&](int at) { return oldest_key(p.s, at); };
     int begin, end, tiles, parts = 1;
@@ -579,7 +579,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         const int r1 = r_wave + rr, qi1 = (int)p.gqa.div((uint32_t)r1);
         const int head1 = kvh * G + (r1 - qi1 * G);
         const long q_row1 = (PREFIX ? (long)qi1 : (long)ft.row0 + qi1) * p.n_heads + head1;
-        const int pos1 = PREFIX ? p.c.lens[qi1] - 1 : ft.pos0 + qi1;
+        const int pos1 = PREFIX ? max(p.c.lens[qi1], 0) - 1 : ft.pos0 + qi1;
         const int old = oldest(pos1), lim = min(pos1 + 1, end);
         const float slope1 = p.s.slopes ? p.s.slopes[head1] * kLog2eF : 0.0f;
         float m = kNoMax, l = 0.0f, acc[kCh];

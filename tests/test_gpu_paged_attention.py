@@ -305,6 +305,20 @@ def test_lengths_past_the_table_and_below_zero(llmik, cuda):
     assert int(got[12:].count_nonzero()) == 0
 
 
+@pytest.mark.parametrize("length", [-1, -2 ** 31])
+def test_negative_lengths_are_empty(llmik, cuda, length):
+    H, Hkv, D, page = 4, 2, 64, 16
+    k, v, table, _ = ref.make_cache([200, 200], Hkv, D, page, F16, cuda, 13)
+    seq = torch.full((2,), length, dtype=torch.int32, device=cuda)
+    q = _q(2, H, D, F16, cuda, 14)
+    for window in (0, 5):
+        assert int(llmik.paged_decode_attention(q, k, v, table, seq, 0.1, window=window).count_nonzero()) == 0
+        assert int(llmik.paged_prefill_attention(q, k, v, table, seq, ref.offsets([1, 1], cuda), 0.1,
+                                                 window=window).count_nonzero()) == 0
+        assert int(llmik.paged_shared_prefix_attention(q, k, v, table, seq, table[0].contiguous(), 150, 0.1,
+                                                       window=window).count_nonzero()) == 0
+
+
 def test_nan_queries_stay_nan(llmik, cuda):
     k, v, table, seq = ref.make_cache([50, 60], 2, 64, 16, F16, cuda, 16)
     q = _q(2, 4, 64, F16, cuda, 17)
