@@ -41,12 +41,14 @@ constexpr int kJoinBatch = 10;   // parts that a lane requests at a time
 // up to twenty parts in one round trip (all by one thread, eight at a time: 8.0 us
 // instead of 5.0 for 64 sequences behind 8192 tokens).
 template <bool BF, int D>
-__global__ __launch_bounds__(256) void paged_prefix_join_kernel(const float* part_o, const float* part_ml, uint16_t* out,
-                                                                int parts, int rows, FastDiv per_kv, FastDiv gqa) {
+__global__ __launch_bounds__(256) void paged_prefix_join_kernel(const float* part_o, const float* part_ml,
+                                                                uint16_t* out, int parts, int rows, FastDiv per_kv,
+                                                                FastDiv gqa) {
     using Hf = Half16<BF>;
     constexpr int kRows = 128 / D;   // of a wave
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int row = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows + (lane & 31) / (D / 4);   // [n_kv_heads, batch, gqa]
+    // Rows as the parts': [n_kv_heads, batch, gqa].
+    const int row = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows + (lane & 31) / (D / 4);
     const int c4 = 4 * (lane % (D / 4));
     if (row >= rows) return;   // (both halves)
     const long at0 = (long)row * parts;
@@ -112,7 +114,8 @@ PagedPrefixPlan plan_prefix(int batch, int n_heads, int n_kv_heads, int head_dim
     // less than two tiles. us, 64 sequences behind 8192 tokens, 16 and 32 splits 29.4,
     // 39.7; 2 sequences behind 4096, 16 and 32 splits 13.2, 12.4.
     const long tiles = (prefix_len + kPfTile - 1) / kPfTile;
-    const long splits = std::max(1L, std::min({2L * cus / base, std::max(cus / base, tiles / 8), (tiles + 1) / 2, 64L}));
+    const long splits =
+        std::max(1L, std::min({2L * cus / base, std::max(cus / base, tiles / 8), (tiles + 1) / 2, 64L}));
     pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;
     pl.splits = (prefix_len + pl.chunk - 1) / pl.chunk;
     pl.off_ml = align_up(paged_decode_workspace(batch, n_heads, n_kv_heads, head_dim, capacity), 256);
