@@ -82,7 +82,7 @@ void launch_flash(const PagedLaunch& a, const PagedFlashParams& p, long workgrou
 // Row tiles of a ragged call at most, and the parts that their keys are cut into where
 // there are fewer than two workgroups per CU: at most as many as fill those.
 struct PagedPrefillPlan {
-    long tiles;
+    long tiles, base;
     int splits;
     size_t off_o, bytes;
 };
@@ -92,10 +92,14 @@ PagedPrefillPlan plan_prefill(int batch, int rows, int n_heads, int n_kv_heads, 
     PagedPrefillPlan pl{};
     const long all = (long)rows * (n_heads / n_kv_heads);
     pl.tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min(batch, rows));
-    const long base = std::max(pl.tiles * n_kv_heads, 1L);
-    pl.splits = (int)std::max(1L, std::min({2L * cus / base, (long)kMaxParts, capacity / (kPfTile * kMinPart)}));
+    pl.base = std::max(pl.tiles * n_kv_heads, 1L);
+    // As for the longest sequence that the table holds; the join's launch must pay too.
+    const long longest = std::min((capacity + kPfTile - 1) / kPfTile, 1L << 20);
+    const long most = 2L * cus / pl.base;
+    const long n = most > 1 ? std::min(most, (long)parts_of((uint32_t)longest, (uint32_t)pl.base)) : 1;
+    pl.splits = n > 1 && 1300 * longest * (n - 1) / n > 3000 + 26 * pl.base * n ? (int)n : 1;
     if (pl.splits > 1) {
-        const size_t parts = (size_t)base * pl.splits * kPfRows;
+        const size_t parts = (size_t)pl.base * pl.splits * kPfRows;
         pl.off_o = align_up(parts * 2 * sizeof(float), 256);
         pl.bytes = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
     }
@@ -114,6 +118,7 @@ int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream) {
     const PagedPrefillPlan pl =
         plan_prefill(a.batch, a.rows, a.n_heads, a.n_kv_heads, a.head_dim, p.c.capacity, device_cu_count());
     p.splits = pl.splits;
+    p.base = (int)std::min(pl.base, (long)INT_MAX);
     if (pl.splits > 1) {
         if (a.workspace == nullptr || a.workspace_bytes < kCounterBytes + pl.bytes)
             return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_prefill_workspace_size)");

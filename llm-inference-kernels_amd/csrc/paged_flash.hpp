@@ -53,6 +53,7 @@ struct PagedFlashParams {
     uint32_t per_round;       // workgroups of one per CU
     int n_heads;
     FastDiv gqa;
+    int base;                 // the ragged form: workgroups without parts
     int splits;               // parts of a tile's keys at most (the prefix form: exactly)
     float* part_o;            // ragged: [tiles * n_kv_heads, splits, kPfRows, D] and (m, l); prefix: [n_kv_heads,
     float* part_ml;           //   rows, splits + 1, D] and (m, l), the last one not this kernel's
@@ -138,10 +139,24 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
 }
 
 // The keys [begin, end) that a row tile's rows see, in `tiles` tiles of 64 tokens, and
-// the parts (of part_tiles tiles) that they are cut into: p.splits, but each of
-// kMinPart tiles at least (a part costs its look-ups and its share of the join).
-constexpr int kMinPart = 8;
+// the parts (of part_tiles tiles) that they are cut into (parts_of, p.splits at most).
 constexpr int kMaxParts = 8;
+constexpr int kMinPart = 4;   // tiles of a part at least
+
+// The number of parts for `tiles` key tiles where the call has `base` workgroups uncut.
+// A tile takes 1.3 us, a part's sums (64 KiB) are written and read again: per workgroup
+// and part 0.026 us of the card's time. tiles * 1.3 / n + base * 0.026 * n is least at
+// n^2 = 50 tiles / base (here the nearest n). Measured with n = 1, 2, 3, 4, 5, 6, 8: two sequences of 100 rows
+// over up to 1214 tokens (base 40) 28.6, 21.9, 17.9, 16.5, 15.7, 15.9, 15.2; three of up
+// to 199 over up to 2271 (base 80) 48.9, 34.0, 28.4, 24.9, 24.2, 27.2, 27.4; 400 over 244
+// (base 104) 18.3, 19.2, 19.8, 20.5, 20.8, 21.1, 21.8 (the join's launch, 3 us, included).
+__host__ __device__ __forceinline__ int parts_of(uint32_t tiles, uint32_t base) {   // tiles <= 2^24, base <= 2^24
+    uint32_t n = 1;
+#pragma unroll
+    for (uint32_t k = 2; k <= kMaxParts; ++k)
+        n = (2 * k - 1) * (2 * k - 1) * base <= 200 * tiles && k * kMinPart <= tiles ? k : n;
+    return (int)n;
+}
 struct TileKeys {
     int lo, hi;   // positions of the first and the last row
     int begin, end, tiles, parts, part_tiles;
@@ -154,7 +169,7 @@ __device__ __forceinline__ TileKeys keys_of_tile(const PagedFlashParams& p, cons
     k.begin = oldest_key(p.s, k.lo) / kPfTile * kPfTile;
     k.end = min(p.c.capacity, k.hi + 1);
     k.tiles = k.end > k.begin ? (k.end - k.begin + kPfTile - 1) / kPfTile : 0;
-    k.parts = max(min(p.splits, k.tiles / kMinPart), 1);
+    k.parts = p.splits > 1 ? min(p.splits, parts_of((uint32_t)k.tiles, (uint32_t)p.base)) : 1;
     k.part_tiles = (k.tiles + k.parts - 1) / k.parts;
     if (k.parts > 1) k.parts = (k.tiles + k.part_tiles - 1) / k.part_tiles;
     return k;
