@@ -473,6 +473,10 @@ LLMIK_API llmik_status llmik_silu_mul_halves(const void* gate_up, void* out, lon
  * tokens at or behind max_pages * page_size (or 2^30) do not exist; a length <= 0 is an
  * empty sequence; a row that has no key, or belongs to no sequence, gives zeros.
  * Slots that hold no live token are never used, whatever they contain.
+ * An infinity or NaN in a live V makes that channel of every row that sees its
+ * token, and of no other, what the sum with positive weights is: inf, -inf or NaN.
+ * (Prompts and a shared prefix round probabilities to 16 bits: where one is 0
+ * then, an infinity becomes NaN.)
  */
 #define LLMIK_F16 0
 #define LLMIK_BF16 1

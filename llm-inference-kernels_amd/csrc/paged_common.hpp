@@ -124,6 +124,10 @@ __device__ __forceinline__ u32x2 publish_load8(__amdgpu_buffer_rsrc_t r, uint32_
 // A running maximum starts here rather than at -inf: differences of two such are
 // then numbers, and states without a key join like all others (their sums are 0).
 constexpr float kNoMax = -1e30f;
+// The least weight of sums that are joined: 0 would make NaN of an infinity in V, which reaches every row
+// that sees it. (Of finite sums it adds less than fp32 keeps.)
+constexpr float kMinWeight = 1.1754944e-38f;
+__device__ __forceinline__ float join_weight(float d) { return fmaxf(__builtin_amdgcn_exp2f(d), kMinWeight); }
 constexpr float kPShift = 8.0f;   // p is held as 2^8 p: fp16 keeps its full precision down to 2^-22
 
 // Scores in the log2 domain. cap > 0: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
@@ -168,6 +172,13 @@ inline ScoreOpts score_opts(const PagedLaunch& a) {
     s.slopes = a.slopes;
     s.window = a.window > 0 ? a.window : INT_MAX;
     return s;
+}
+
+// Those of two 16-bit values that are infinities or NaN; zeros in place of the others.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
+    constexpr uint32_t inf = BF ? 0x7F80u : 0x7C00u;
+    return ((x & inf) == inf ? x & 0xFFFFu : 0u) | ((x & (inf << 16)) == inf << 16 ? x & 0xFFFF0000u : 0u);
 }
 
 // max / sum over lanes l and l ^ 32, or l and l ^ 16.

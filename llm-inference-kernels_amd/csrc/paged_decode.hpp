@@ -212,7 +212,7 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
             const int i = i0 + (lane >> 2);
             return octet_offset<D>(p.c, table_row, kvh, 32 * (base + kPdWaves * i) + 8 * (lane & 3), end);
         };
-        long off = look_up(0), off_next = -1;
+        long off, off_next;
 
         u32x4 qb[KS];
 #pragma unroll
@@ -221,9 +221,7 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
         const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
 
         f32x4 o[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float m_run = kNoMax, l_run = 0.0f;   // of column c; l_run: this lane's tokens only
+        float m_run, l_run;   // of column c
 
         u32x4 kt[2][KS];
         uint32_t vt[8][VW];
@@ -286,96 +284,125 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
             }
         };
 
-        uint64_t unmapped = __ballot(off < 0);
-        if (count > 0) {
-            load_k(0);
-            load_v(0);
-        }
-        if (count > 16) off_next = look_up(16);
-        for (int i = 0; i < count; ++i) {
-            const int t0 = 32 * (base + kPdWaves * i);
-            const uint32_t gone = (uint32_t)(unmapped >> (4 * (i & 15))) & 15u;   // the tile's octets without a page
-            float sc[8];
+        // One pass over the tiles. An infinity in V must reach the rows that see it as one, but the
+        // pair hi + lo makes NaN of it (lo may be zero or negative). So a piece whose sums hold NaN
+        // where its weights do not is done again, with the values that are no numbers in a product
+        // of their own, whose weights are 1. (Looking costs 0.1 .. 0.3 us a call, 1 .. 2 %.)
+        auto pass = [&](auto careful) {
+            constexpr bool kCareful = decltype(careful)::value;
+            off = look_up(0);
+            off_next = -1;
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) acc = Hf::mfma16(kt[blk][ks], qb[ks], acc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sc[4 * blk + r] = acc[r];
+            for (int j = 0; j < VEC; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m_run = kNoMax;
+            l_run = 0.0f;   // (until the end: of this lane's tokens only)
+            uint64_t unmapped = __ballot(off < 0);
+            if (count > 0) {
+                load_k(0);
+                load_v(0);
             }
-            // K's registers are free: the next tile's keys are requested before this
-            // tile's softmax, and its values (below) as soon as V's registers are.
-            const bool more = i + 1 < count;
-            if (more) {
-                if (((i + 1) & 15) == 0) {
-                    off = off_next;
-                    unmapped = __ballot(off < 0);
-                    if (i + 17 < count) off_next = look_up(i + 17);
+            if (count > 16) off_next = look_up(16);
+            for (int i = 0; i < count; ++i) {
+                const int t0 = 32 * (base + kPdWaves * i);
+                const uint32_t gone = (uint32_t)(unmapped >> (4 * (i & 15))) & 15u;   // the tile's octets without a page
+                float sc[8];
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) acc = Hf::mfma16(kt[blk][ks], qb[ks], acc);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[4 * blk + r] = acc[r];
                 }
-                load_k(i + 1);
-            }
-            if (p.s.cap_in != 0.0f) {
+                // K's registers are free: the next tile's keys are requested before this
+                // tile's softmax, and its values (below) as soon as V's registers are.
+                const bool more = i + 1 < count;
+                if (more) {
+                    if (((i + 1) & 15) == 0) {
+                        off = off_next;
+                        unmapped = __ballot(off < 0);
+                        if (i + 17 < count) off_next = look_up(i + 17);
+                    }
+                    load_k(i + 1);
+                }
+                if (p.s.cap_in != 0.0f) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
-            } else {
+                    for (int e = 0; e < 8; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sc[e] *= p.s.scale_log2;
-            }
-            const int tk = t0 + 4 * g;   // token of slot e: tk + 16 (e / 4) + e % 4
-            if (p.s.slopes) {
+                    for (int e = 0; e < 8; ++e) sc[e] *= p.s.scale_log2;
+                }
+                const int tk = t0 + 4 * g;   // token of slot e: tk + 16 (e / 4) + e % 4
+                if (p.s.slopes) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 16 * (e >> 2) + (e & 3))), sc[e]);
-            }
-            if (gone || t0 < begin || t0 + 32 > end) {   // wave-uniform
-                // Masked tokens: no score, and no value either (0 * NaN would stay NaN).
+                    for (int e = 0; e < 8; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 16 * (e >> 2) + (e & 3))), sc[e]);
+                }
+                if (gone || t0 < begin || t0 + 32 > end) {   // wave-uniform
+                    // Masked tokens: no score, and no value either (0 * NaN would stay NaN).
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int tok = tk + 16 * (e >> 2) + (e & 3);
-                    const bool ok = tok >= begin && tok < end && !((gone >> (2 * (e >> 2) + (g >> 1))) & 1u);
-                    if (!ok) {
-                        sc[e] = -INFINITY;
+                    for (int e = 0; e < 8; ++e) {
+                        const int tok = tk + 16 * (e >> 2) + (e & 3);
+                        const bool ok = tok >= begin && tok < end && !((gone >> (2 * (e >> 2) + (g >> 1))) & 1u);
+                        if (!ok) {
+                            sc[e] = -INFINITY;
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) vt[e][w] = 0u;
+                            for (int w = 0; w < VW; ++w) vt[e][w] = 0u;
+                        }
                     }
                 }
+                float mx = sc[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
+                if (__any(mx > m_run)) {
+                    mx = fmaxf(xor32_max(xor16_max(mx)), m_run);
+                    const float a = kCareful ? join_weight(m_run - mx) : __builtin_amdgcn_exp2f(m_run - mx);
+                    m_run = mx;
+                    l_run *= a;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[j][r] *= a;
+                }
+                const float sub = m_run - kPShift;
+                u32x4 hi, lo;
+                [[maybe_unused]] u32x4 seen;   // 1 for a token with a score
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(sc[e] - sub), p1 = __builtin_amdgcn_exp2f(sc[e + 1] - sub);
+                    l_run += p0 + p1;
+                    const uint32_t h2 = Hf::pack(p0, p1);
+                    hi[e >> 1] = h2;
+                    lo[e >> 1] = Hf::pack(p0 - Hf::to_f32((uint16_t)h2), p1 - Hf::to_f32((uint16_t)(h2 >> 16)));
+                    if constexpr (kCareful) seen[e >> 1] = Hf::pack(sc[e] > -INFINITY, sc[e + 1] > -INFINITY);
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+                    u32x4 a;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[e] = perm_b32(vt[2 * e + 1][j >> 1], vt[2 * e][j >> 1], sel);
+                    if constexpr (kCareful) {
+                        u32x4 bad;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bad[e] = not_finite2<BF>(a[e]);
+                            a[e] ^= bad[e];
+                        }
+                        o[j] = Hf::mfma16(bad, seen, o[j]);
+                    }
+                    o[j] = Hf::mfma16(a, hi, o[j]);
+                    o[j] = Hf::mfma16(a, lo, o[j]);
+                }
+                if (more) load_v(i + 1);
             }
-            float mx = sc[0];
+            l_run = xor32_sum(xor16_sum(l_run));
+        };
+        pass(std::false_type{});
+        f32x4 all = o[0];   // NaN if any sum is (or where infinities of both signs are, which does no harm)
 #pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
-            if (__any(mx > m_run)) {
-                mx = fmaxf(xor32_max(xor16_max(mx)), m_run);
-                const float a = __builtin_amdgcn_exp2f(m_run - mx);
-                m_run = mx;
-                l_run *= a;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[j][r] *= a;
-            }
-            const float sub = m_run - kPShift;
-            u32x4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(sc[e] - sub), p1 = __builtin_amdgcn_exp2f(sc[e + 1] - sub);
-                l_run += p0 + p1;
-                const uint32_t h2 = Hf::pack(p0, p1);
-                hi[e >> 1] = h2;
-                lo[e >> 1] = Hf::pack(p0 - Hf::to_f32((uint16_t)h2), p1 - Hf::to_f32((uint16_t)(h2 >> 16)));
-            }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-                u32x4 a;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = perm_b32(vt[2 * e + 1][j >> 1], vt[2 * e][j >> 1], sel);
-                o[j] = Hf::mfma16(a, hi, o[j]);
-                o[j] = Hf::mfma16(a, lo, o[j]);
-            }
-            if (more) load_v(i + 1);
-        }
-
-        l_run = xor32_sum(xor16_sum(l_run));
+        for (int j = 1; j < VEC; ++j) all += o[j];
+        const float any = (all[0] + all[1]) + (all[2] + all[3]);
+        if (__any(any != any && l_run == l_run)) pass(std::true_type{});
         // ---- join the waves; write the output or hand the part over ----
         float* const mine_o = lds.o(wave);
         if (c < nh) {
@@ -405,17 +432,17 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
                 w[u] = u < live ? m[u] : kNoMax;
                 top = fmaxf(top, w[u]);
             }
-            const float a = __builtin_amdgcn_exp2f(wm - top);
+            const float a = join_weight(wm - top);
             wm = top;
             wl *= a;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) wo[e] *= a;
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-                w[u] = u < live ? __builtin_amdgcn_exp2f(w[u] - top) : 0.0f;
-                wl = fmaf(l[u], w[u], wl);
+            for (int u = 0; u < N; ++u) {   // (the others' places hold anything)
+                w[u] = join_weight(w[u] - top);
+                wl = u < live ? fmaf(l[u], w[u], wl) : wl;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) wo[e] = fmaf(v[u][e], w[u], wo[e]);
+                for (int e = 0; e < VEC; ++e) wo[e] = u < live ? fmaf(v[u][e], w[u], wo[e]) : wo[e];
             }
         };
         auto join_lds = [&](int n, int h) {   // the first n <= 4 of the waves' places

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void paged_flash_join_kernel(PagedFlashParams 
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int u = 0; u < kMaxParts; ++u) {
-        const float w = u < parts ? __builtin_amdgcn_exp2f(m[u] - top) : 0.0f;
+        const float w = join_weight(m[u] - top);
         sum = u < parts ? fmaf(l[u], w, sum) : sum;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = u < parts ? fmaf(v[u][e], w, o[e]) : o[e];

@@ -438,7 +438,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                 for (int e = 0; e < 32; ++e) m_new = fmaxf(m_new, fmaf(sc[e], mult, add));
                 m_new = fmaxf(xor32_max(m_new), kNoMax);
             }
-            const float a = __builtin_amdgcn_exp2f(m_run - m_new);
+            const float a = join_weight(m_run - m_new);
             m_run = m_new;
             l_run *= a;
 #pragma unroll
@@ -587,7 +587,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 
     // ---- some V is no number, and not all rows see it: the wave's rows one by one,
     // 64 keys at a time (a lane its key's score, then two channels of every key's
-    // value that has a probability) ----
+    // value that the row sees) ----
     __builtin_amdgcn_s_waitcnt(0);   // the stores above come first
     constexpr int kCh = D / 64;      // channels of a lane
     for (int rr = 0; rr < 32 && r_wave + rr < n_rows; ++rr) {
@@ -622,7 +622,8 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
             top = fmaxf(top, m);
-            const float a = __builtin_amdgcn_exp2f(m - top), pt = ok ? __builtin_amdgcn_exp2f(s1 - top + kPShift) : 0.0f;
+            const float a = join_weight(m - top), p1 = __builtin_amdgcn_exp2f(s1 - top + kPShift);
+            const float pt = ok ? (p1 < kMinWeight ? kMinWeight : p1) : 0.0f;   // (NaN stays)
             float sum = pt;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void paged_prefix_join_kernel(const float* par
         float m = top;
 #pragma unroll
         for (int u = 0; u < kJoinBatch; ++u) m = fmaxf(m, ml[u][0]);
-        const float a = __builtin_amdgcn_exp2f(top - m);
+        const float a = join_weight(top - m);
         top = m;
         sum *= a;
 #pragma unroll
@@ -74,13 +74,13 @@ __global__ __launch_bounds__(256) void paged_prefix_join_kernel(const float* par
 #pragma unroll
         for (int u = 0; u < kJoinBatch; ++u) {
             const bool in = u0 + 2 * u < parts;
-            const float w = __builtin_amdgcn_exp2f(ml[u][0] - m);
+            const float w = join_weight(ml[u][0] - m);
             sum = in ? fmaf(ml[u][1], w, sum) : sum;
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = in ? fmaf(v[u][e], w, o[e]) : o[e];
         }
     }
-    const float m = xor32_max(top), a = __builtin_amdgcn_exp2f(top - m);
+    const float m = xor32_max(top), a = join_weight(top - m);
     sum = xor32_sum(sum * a);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = xor32_sum(o[e] * a);
