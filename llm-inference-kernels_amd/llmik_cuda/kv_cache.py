@@ -214,6 +214,8 @@ class PagedBatch(NamedTuple):
     rows: int                           # new tokens of all sequences
     prefix_pages: Optional[torch.Tensor]   # pages that all sequences share from the start on
     prefix_len: int
+    shortest: int = 0                   # the shortest length, the mean length: how much of the
+    mean: int = 0                       # prefix a window leaves
 
 
 class PagedKVCache:
@@ -342,16 +344,12 @@ class PagedKVCache:
         b = len(seqs)
         table = dev[2 * b + 1:].view(b, width) if b else torch.zeros((0, width), dtype=torch.int32, device=self.device)
         return PagedBatch(table, dev[:b], dev[b:2 * b + 1] if ragged else None, cu[-1],
-                          table[0, :shared] if shared else None, shared * self.page_size)
+                          table[0, :shared] if shared else None, shared * self.page_size,
+                          min(lens, default=0), sum(lens) // max(b, 1))
 
     def _shared_prefix(self, pages: List[List[int]], lens: List[int]) -> int:
         """Whole pages that all sequences share from the start on, or 0 where reading
-        them once for all does not pay: partial results and a second launch against
-        the rows that all sequences but one would read again. us, decode against
-        shared, sequences x shared tokens, heads of 128: 8 KV heads 2 x 1024 10.5,
-        11.1; 2 x 2048 12.3, 11.5; 4 x 512 10.4, 11.2; 4 x 1024 12.8, 11.5; 8 x 512
-        12.4, 11.5; 64 x 256 16.0, 16.8; 64 x 512 27.5, 18.4; 32 KV heads 2 x 256 9.4,
-        10.7; 2 x 512 12.9, 11.2; 16 x 256 13.4, 13.2; 64 x 256 53.6, 38.6."""
+        them once for all does not pay (_pays)."""
         if len(pages) < 2:
             return 0
         n = min(min(len(p) for p in pages), (min(lens) - 1) // self.page_size)
@@ -360,9 +358,27 @@ class PagedKVCache:
         while same < n and all(p[same] == first[same] for p in pages):
             same += 1
         tokens = same * self.page_size
-        saved = tokens * (len(pages) - 1) * self.n_kv_heads
+        return same if self._pays(tokens, tokens * (len(pages) - 1)) else 0
+
+    def _pays(self, tokens: int, again: int) -> bool:
+        """Whether to read `tokens` shared tokens once for all, where the sequences but
+        one would read `again` of them again: partial results and a second launch
+        against those rows. us, decode against shared, sequences x shared tokens, heads
+        of 128: 8 KV heads 2 x 1024 10.5, 11.1; 2 x 2048 12.3, 11.5; 4 x 512 10.4, 11.2;
+        4 x 1024 12.8, 11.5; 8 x 512 12.4, 11.5; 64 x 256 16.0, 16.8; 64 x 512 27.5, 18.4;
+        32 KV heads 2 x 256 9.4, 10.7; 2 x 512 12.9, 11.2; 16 x 256 13.4, 13.2; 64 x 256
+        53.6, 38.6."""
         least = self.SHARED_ROWS * (1 if tokens >= self.SHARED_TOKENS else 16)
-        return same if tokens > 0 and saved >= least else 0
+        return tokens > 0 and again * self.n_kv_heads >= least
+
+    def _window_pays(self, step: PagedBatch, window: int) -> bool:
+        """_pays for what a window leaves of the shared prefix: the shortest sequence
+        sees the most of it, the mean length stands for all. us, decode against shared,
+        64 sequences behind 8192 tokens, windows of 64, 256, 512, 1024, 4096: 8.6, 21.4;
+        13.7, 23.5; 19.1, 29.3; 33.6, 29.5; 91, 29.7; 16 behind 2048, 64, 512, 1024: 7.4,
+        12.8; 11.7, 14.7; 17.4, 14.7. (8 behind 8192 with 1024 go the wrong way: 15.8, 16.6.)"""
+        sees = lambda length: min(max(step.prefix_len - max(length - window, 0), 0), step.prefix_len)  # noqa: E731
+        return self._pays(sees(step.shortest), sees(step.mean) * (step.page_table.shape[0] - 1))
 
     def append(self, step: PagedBatch, qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
                layer: int = 0) -> torch.Tensor:
@@ -374,12 +390,12 @@ class PagedKVCache:
     def attention(self, step: PagedBatch, q: torch.Tensor, softmax_scale: float, softcap: float = 0.0,
                   slopes: Optional[torch.Tensor] = None, window: int = 0, layer: int = 0) -> torch.Tensor:
         """Attention of the batch's new tokens in a layer: decode, decode behind a
-        shared prefix, or prompts, by the batch."""
+        shared prefix, or prompts, by the batch (and what a window leaves of the prefix)."""
         k, v = self.k[layer], self.v[layer]
         if step.cu_tokens is not None:
             return paged_prefill_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, softmax_scale,
                                            softcap, slopes, window)
-        if step.prefix_pages is not None:
+        if step.prefix_pages is not None and (window <= 0 or self._window_pays(step, window)):
             return paged_shared_prefix_attention(q, k, v, step.page_table, step.seq_lens, step.prefix_pages,
                                                  step.prefix_len, softmax_scale, softcap, slopes, window)
         return paged_decode_attention(q, k, v, step.page_table, step.seq_lens, softmax_scale, softcap, slopes, window)

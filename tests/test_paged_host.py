@@ -318,3 +318,36 @@ def test_pages_are_never_lost_or_given_twice():
         assert len(set(held)) + cache.free_pages() == 40 and not set(held) & set(cache._free)
         assert all(held.count(p) == cache._users[p] for p in set(held))
         assert all(len(cache._pages[s]) == -(-cache.length(s) // 8) for s in live)
+
+
+def test_a_window_decides_whether_the_prefix_is_read_once(monkeypatch):
+    """What counts is what the window leaves of the shared prefix."""
+    import llmik_cuda.kv_cache as kv
+    taken = []
+    monkeypatch.setattr(kv, "paged_decode_attention", lambda *a: taken.append(("decode", a[3], a[-1])))
+    monkeypatch.setattr(kv, "paged_shared_prefix_attention", lambda *a: taken.append(("shared", a[3], a[-1])))
+    cache = kv.PagedKVCache(600, 8, page_size=64, head_dim=64, device="cpu")
+    a = cache.add()
+    cache.batch([a], [8192])
+    seqs = [a] + [cache.add(share=a, tokens=8192) for _ in range(63)]
+    step = cache.batch(seqs)
+    assert step.prefix_len == 8192 and step.shortest == 8193 and step.mean == 8193
+
+    def path(step, window):
+        cache.attention(step, None, 0.1, window=window)
+        kind, table, w = taken.pop()
+        assert w == window and table is step.page_table and bool((table[:, :128] >= 0).all())
+        return kind
+
+    assert path(step, 0) == "shared"
+    for window, want in [(1, "decode"), (64, "decode"), (256, "decode"), (512, "decode"), (1024, "shared"),
+                         (8192, "shared"), (10 ** 6, "shared")]:
+        assert path(step, window) == want, window
+    # sequences that have left the prefix behind see none of it; one short one among them changes little
+    long = cache.batch(seqs[1:40], [300] * 39)
+    assert long.prefix_pages is None                                    # prompts
+    mixed = cache.batch(seqs[:40])
+    assert mixed.shortest == 8194 and mixed.mean == 8194 + 39 * 300 // 40
+    assert path(mixed, 280) == "decode" and path(mixed, 1024) == "shared"
+    # a batch without the lengths (made by hand) counts the whole prefix
+    assert path(step._replace(shortest=0, mean=0), 2048) == "shared"
