@@ -477,6 +477,12 @@ LLMIK_API llmik_status llmik_silu_mul_halves(const void* gate_up, void* out, lon
  * token, and of no other, what the sum with positive weights is: inf, -inf or NaN.
  * (Prompts and a shared prefix round probabilities to 16 bits: where one is 0
  * then, an infinity becomes NaN.)
+ *
+ * Scores, sums and softmax statistics are fp32, and outputs are rounded once. A
+ * probability enters the product with V as 22 (fp16) or 16 (bf16) bits in decode
+ * attention and for a sequence's own tokens behind a shared prefix, rounded once to
+ * the type, 11 or 8 bits, in prompts and for the shared prefix: an error of at most
+ * 2^-11 (2^-8) of sum_j p_j |v_j - out|, the size of the output's own rounding.
  */
 #define LLMIK_F16 0
 #define LLMIK_BF16 1

@@ -478,7 +478,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     softmax_scale * q . k, with softcap > 0 (at most 4096) softcap *
     tanh(score / softcap), with slopes [n_heads] fp32 minus slopes[h] * (distance in tokens); with
     window > 0 only the newest `window` keys. A sequence without a key gives
-    zeros. Deterministic; the bits depend on the lengths of the whole batch."""
+    zeros. Deterministic; the bits depend on the lengths of the whole batch.
+    Probabilities keep 22 bits (fp16) or 16 (bf16) before the product with V."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
              _is_device(page_table) and _is_device(seq_lens), "all inputs must be CUDA tensors")
     return _C.paged_decode_attention(q, k_cache, v_cache, page_table, seq_lens, float(softmax_scale),
@@ -493,7 +494,8 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     head_dim], rows as in rope_paged_append, each row over the keys of its own
     sequence up to its own position (the chunk's earlier tokens and what the
     cache held before). Score options as in paged_decode_attention. Rows that
-    belong to no sequence give zeros."""
+    belong to no sequence give zeros. Probabilities are rounded to q's dtype (11
+    or 8 bits) before the product with V; their sums are of what was rounded."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
              _is_device(page_table) and _is_device(seq_lens) and _is_device(cu_tokens), "all inputs must be CUDA tensors")
     return _C.paged_prefill_attention(q, k_cache, v_cache, page_table, seq_lens, cu_tokens,
@@ -508,7 +510,8 @@ def paged_shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     """paged_decode_attention for a batch whose sequences share their first
     prefix_len tokens: those are read from prefix_pages [n] int32 once for all
     sequences, page_table from position prefix_len on. seq_lens counts the
-    prefix too; a sequence may be shorter than it."""
+    prefix too; a sequence may be shorter than it. The prefix's probabilities
+    are rounded as paged_prefill_attention's, the others as decode's."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and
              _is_device(page_table) and _is_device(seq_lens) and _is_device(prefix_pages), "all inputs must be CUDA tensors")
     return _C.paged_shared_prefix_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_pages,

@@ -237,7 +237,14 @@ class PagedKVCache:
         cache.remove(b)
 
     One `batch` serves all layers: `append` and `attention` take the layer's
-    number. All calls belong on one stream; not safe for several threads."""
+    number. All calls belong on one stream; not safe for several threads.
+
+    A batch of single tokens behind whole shared pages may be read through
+    paged_shared_prefix_attention, which rounds the prefix's probabilities to 16
+    bits once where decode attention keeps a second part: a sequence's results
+    then change (within the output type's rounding, fp16 2^-11, bf16 2^-8 of the
+    values' weighted spread) with the sequences beside it. shared_prefix=False
+    keeps decode attention for all batches."""
 
     # A batch's shared prefix is read once for all sequences where that saves so many
     # token rows (of one KV head) and has so many tokens; a shorter one where it saves
@@ -247,12 +254,13 @@ class PagedKVCache:
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, head_dim: int = 128,
                  dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None,
-                 n_layers: int = 1) -> None:
+                 n_layers: int = 1, shared_prefix: bool = True) -> None:
         _require(n_pages > 0 and n_kv_heads > 0 and n_layers > 0, "n_pages, n_kv_heads and n_layers must be positive")
         _require(page_size > 0 and page_size % 8 == 0, "page_size must be a positive multiple of 8")
         _require(head_dim in (64, 128), "only head_dim=64 and 128 supported")
         _require(dtype in (torch.float16, torch.bfloat16), "dtype must be fp16 or bf16")
         self.device = torch.device("cuda") if device is None else torch.device(device)
+        self.shared_prefix = bool(shared_prefix)
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, n_kv_heads, page_size, head_dim
         shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=self.device)
@@ -332,7 +340,7 @@ class PagedKVCache:
         cu = [0]
         for n in counts:
             cu.append(cu[-1] + n)
-        shared = 0 if ragged else self._shared_prefix(pages, lens)
+        shared = 0 if ragged or not self.shared_prefix else self._shared_prefix(pages, lens)
         width = max([len(p) for p in pages] + [1])
         # One copy to the device: lengths, row offsets, then the table.
         flat = lens + cu + [p for row in pages for p in row + [-1] * (width - len(row))]

@@ -351,3 +351,15 @@ def test_a_window_decides_whether_the_prefix_is_read_once(monkeypatch):
     assert path(mixed, 280) == "decode" and path(mixed, 1024) == "shared"
     # a batch without the lengths (made by hand) counts the whole prefix
     assert path(step._replace(shortest=0, mean=0), 2048) == "shared"
+
+
+def test_decode_for_all_batches():
+    """shared_prefix=False: no batch is read through the shared prefix, whose
+    probabilities have fewer bits."""
+    from llmik_cuda.kv_cache import PagedKVCache
+    for share in (True, False):
+        cache = PagedKVCache(300, 8, page_size=64, head_dim=64, device="cpu", shared_prefix=share)
+        a = cache.add()
+        cache.batch([a], [8192])
+        step = cache.batch([a] + [cache.add(share=a, tokens=8192) for _ in range(9)])
+        assert (step.prefix_pages is not None) == share and step.prefix_len == (8192 if share else 0)
