@@ -15,8 +15,8 @@ int invalid(const char* msg) { return set_error(LLMIK_ERR_INVALID, msg); }
 int unsupported(const char* msg) { return set_error(LLMIK_ERR_UNSUPPORTED, msg); }
 int misaligned(const char* msg) { return set_error(LLMIK_ERR_ALIGNMENT, msg); }
 
+constexpr float kMaxSoftcap = 4096.0f;   // (as far as capped scores are tested)
 // HIP launches hold fewer than 2^32 threads.
-constexpr float kMaxSoftcap = 4096.0f;
 constexpr long kMaxThreads = (1L << 32) - 1;
 
 long row_elements(const llmik_paged_cache& c) { return (long)c.page_size * c.head_dim * c.n_kv_heads; }
@@ -58,8 +58,6 @@ int check_cache(const llmik_paged_cache* c, int n_heads) {
 int check_options(const llmik_score_options* o) {
     if (o == nullptr) return invalid("null score options");
     if (!std::isfinite(o->softmax_scale)) return invalid("softmax_scale must be finite");
-    // A capped score is exact to about 2^-23 of the cap: from kMaxSoftcap on that would be
-    // more than an fp16 output's rounding (2^-11).
     if (!(o->softcap >= 0.0f && o->softcap <= kMaxSoftcap)) return invalid("softcap must be >= 0 and at most 4096");
     if (o->softcap > 0.0f && !std::isfinite(4.0f * (o->softmax_scale / o->softcap)))
         return invalid("softcap too small for softmax_scale");

@@ -130,12 +130,18 @@ constexpr float kMinWeight = 1.1754944e-38f;
 __device__ __forceinline__ float join_weight(float d) { return fmaxf(__builtin_amdgcn_exp2f(d), kMinWeight); }
 constexpr float kPShift = 8.0f;   // p is held as 2^8 p: fp16 keeps its full precision down to 2^-22
 
-// Scores in the log2 domain. cap > 0: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
-// (e^2x + 1), as exp2 and one reciprocal (absolute error about 2^-23 cap).
+// Scores in the log2 domain. A cap: cap * tanh(s / cap) with tanh(x) = 1 - 2 /
+// (e^2x + 1), as exp2 and one reciprocal. That is exact to about 2^-22 of the cap, up
+// to a cap of kPlainCap 2^-16, less than the products' own rounding. Above it small scores
+// would lose their bits (of 4096 2^-10), so there |x| < 1/2 goes by tanh's series (to
+// x^15; the next term is below 2^-26 of the sum) and all scores are exact to 2^-21 of
+// themselves.
+constexpr float kPlainCap = 64.0f;
 struct ScoreOpts {
     float scale_log2;   // softmax_scale * log2(e)
     float cap_in;       // 2 log2(e) * softmax_scale / softcap, or 0
     float cap_log2;     // softcap * log2(e)
+    float cap_x;        // softmax_scale / softcap above kPlainCap, or 0
     const float* slopes;
     int window;         // keys per query, INT_MAX where unlimited
 };
@@ -144,6 +150,22 @@ __device__ __forceinline__ float capped_part(float s, float cap_in) {   // (tanh
 }
 __device__ __forceinline__ float capped(float s, float cap_in, float cap_log2) {
     return fmaf(2.0f * cap_log2, capped_part(s, cap_in), cap_log2);
+}
+
+__device__ __forceinline__ float tanh_series(float x) {   // |x| < 1/2
+    const float y = x * x;
+    float p = -929569.0f / 638512875.0f;
+    p = fmaf(p, y, 21844.0f / 6081075.0f);
+    p = fmaf(p, y, -1382.0f / 155925.0f);
+    p = fmaf(p, y, 62.0f / 2835.0f);
+    p = fmaf(p, y, -17.0f / 315.0f);
+    p = fmaf(p, y, 2.0f / 15.0f);
+    p = fmaf(p, y, -1.0f / 3.0f);
+    return fmaf(p * y, x, x);
+}
+__device__ __forceinline__ float capped_tanh(float s, const ScoreOpts& o) {   // the score over the cap
+    const float x = s * o.cap_x;
+    return fabsf(x) < 0.5f ? tanh_series(x) : capped(s, o.cap_in, 1.0f);
 }
 
 // The kernels' views of a call.
@@ -168,6 +190,7 @@ inline ScoreOpts score_opts(const PagedLaunch& a) {
     if (a.softcap > 0.0f) {
         s.cap_in = 2.0f * kLog2eF * (a.softmax_scale / a.softcap);
         s.cap_log2 = a.softcap * kLog2eF;
+        s.cap_x = a.softcap > kPlainCap ? a.softmax_scale / a.softcap : 0.0f;
     }
     s.slopes = a.slopes;
     s.window = a.window > 0 ? a.window : INT_MAX;

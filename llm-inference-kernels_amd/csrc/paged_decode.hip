@@ -3,22 +3,28 @@
 
 namespace llmik {
 
-template <bool BF, int D, bool UNI>
+template <bool BF, int D, bool UNI, bool EXACT>
 __global__ __launch_bounds__(kPdThreads, kPdPerCu) void paged_decode_kernel(PagedDecodeParams p) {
     constexpr int kFloats = DecodeLds<D>::kFloats;
     __shared__ __attribute__((aligned(16))) float s_o[kPdWaves * kFloats];
     __shared__ float s_m[kPdWaves][16], s_l[kPdWaves][16];
     __shared__ uint32_t s_last;
-    paged_decode<BF, D, UNI>(p, blockIdx.x, gridDim.x,
-                             {s_o, s_o + kFloats, s_o + 2 * kFloats, s_o + 3 * kFloats, s_m, s_l, &s_last});
+    paged_decode<BF, D, UNI, EXACT>(p, blockIdx.x, gridDim.x,
+                                    {s_o, s_o + kFloats, s_o + 2 * kFloats, s_o + 3 * kFloats, s_m, s_l, &s_last});
 }
 
 namespace {
 
 template <bool BF, int D>
 void launch_decode(const PagedDecodeParams& p, int workgroups, bool uniform, hipStream_t stream) {
-    if (uniform) paged_decode_kernel<BF, D, true><<<workgroups, kPdThreads, 0, stream>>>(p);
-    else paged_decode_kernel<BF, D, false><<<workgroups, kPdThreads, 0, stream>>>(p);
+    auto go = [&](auto uni, auto exact) {
+        paged_decode_kernel<BF, D, decltype(uni)::value, decltype(exact)::value>
+            <<<workgroups, kPdThreads, 0, stream>>>(p);
+    };
+    using std::false_type;
+    using std::true_type;
+    if (p.s.cap_x != 0.0f) uniform ? go(true_type{}, true_type{}) : go(false_type{}, true_type{});
+    else uniform ? go(true_type{}, false_type{}) : go(false_type{}, false_type{});
 }
 
 }  // namespace

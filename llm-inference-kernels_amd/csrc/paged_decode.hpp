@@ -90,8 +90,8 @@ struct DecodeLds {
     __device__ __forceinline__ float* o(int w) const { return w == 0 ? o0 : w == 1 ? o1 : w == 2 ? o2 : o3; }
 };
 
-// Workgroup wg of n_wg.
-template <bool BF, int D, bool UNI>
+// Workgroup wg of n_wg. EXACT: for a cap above kPlainCap (capped_tanh).
+template <bool BF, int D, bool UNI, bool EXACT>
 __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_t wg, uint32_t n_wg,
                                              const DecodeLds<D>& lds) {
     using Hf = Half16<BF>;
@@ -325,7 +325,10 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
                     }
                     load_k(i + 1);
                 }
-                if (p.s.cap_in != 0.0f) {
+                if constexpr (EXACT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sc[e] = capped_tanh(sc[e], p.s) * p.s.cap_log2;
+                } else if (p.s.cap_in != 0.0f) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sc[e] = capped(sc[e], p.s.cap_in, p.s.cap_log2);
                 } else {

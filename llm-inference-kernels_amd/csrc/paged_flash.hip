@@ -4,14 +4,14 @@
 
 namespace llmik {
 
-template <bool BF, int D>
+template <bool BF, int D, bool EXACT>
 __global__ __launch_bounds__(kPfThreads, 2) void paged_flash_kernel(PagedFlashParams p) {
     constexpr int kTileBytes = FlashLds<D>::kTileBytes;
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kTileBytes], s_k1[kTileBytes];
     __shared__ __attribute__((aligned(16))) uint8_t s_v0[kTileBytes], s_v1[kTileBytes];
     __shared__ int s_lo[4], s_hi[4];
     __shared__ uint32_t s_bad;
-    paged_flash<BF, D, false>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_bad});
+    paged_flash<BF, D, false, EXACT>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_bad});
 }
 
 // Rows of a workgroup of the join: a thread has four channels of one.
@@ -67,14 +67,20 @@ __global__ __launch_bounds__(256) void paged_flash_join_kernel(PagedFlashParams 
 
 namespace {
 
+template <bool BF, int D>
+void launch_flash_kernel(const PagedFlashParams& p, unsigned grid, hipStream_t stream) {
+    if (p.s.cap_x != 0.0f) paged_flash_kernel<BF, D, true><<<grid, kPfThreads, 0, stream>>>(p);
+    else paged_flash_kernel<BF, D, false><<<grid, kPfThreads, 0, stream>>>(p);
+}
+
 void launch_flash(const PagedLaunch& a, const PagedFlashParams& p, long workgroups, hipStream_t stream) {
-    const dim3 grid((unsigned)workgroups);
+    const unsigned grid = (unsigned)workgroups;
     if (a.bf16)
-        a.head_dim == 128 ? paged_flash_kernel<true, 128><<<grid, kPfThreads, 0, stream>>>(p)
-                          : paged_flash_kernel<true, 64><<<grid, kPfThreads, 0, stream>>>(p);
+        a.head_dim == 128 ? launch_flash_kernel<true, 128>(p, grid, stream)
+                          : launch_flash_kernel<true, 64>(p, grid, stream);
     else
-        a.head_dim == 128 ? paged_flash_kernel<false, 128><<<grid, kPfThreads, 0, stream>>>(p)
-                          : paged_flash_kernel<false, 64><<<grid, kPfThreads, 0, stream>>>(p);
+        a.head_dim == 128 ? launch_flash_kernel<false, 128>(p, grid, stream)
+                          : launch_flash_kernel<false, 64>(p, grid, stream);
 }
 
 }  // namespace

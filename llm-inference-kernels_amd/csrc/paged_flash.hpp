@@ -185,8 +185,11 @@ struct FlashLds {
     uint32_t* bad;             // some V is no number (see the end of paged_flash)
 };
 
-// Workgroup wg of n_wg.
-template <bool BF, int D, bool PREFIX>
+// Workgroup wg of n_wg. EXACT: for a cap above kPlainCap (capped_tanh; a kernel of its
+// own, as its instructions beside the others cost all calls: us, 8192 tokens 565, 583
+// with it, 2048 tokens 52.9, 55.5. Four chunks over up to 6000 tokens with a cap of 50
+// 167, of 1000 202).
+template <bool BF, int D, bool PREFIX, bool EXACT>
 __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t wg, uint32_t n_wg,
                                             const FlashLds<D>& lds) {
     using Hf = Half16<BF>;
@@ -348,12 +351,12 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         for (int e = 0; e < 16; ++e) o[cb][e] = 0.0f;
     float m_run = kNoMax, l_run = 0.0f;   // of row n; l_run: this lane's tokens only
     // sc * mult + add are the scores in the log2 domain: sc as it comes from the products,
-    // or -1 / (e^2x + 1) where there is a cap (the rest of cap * tanh x is mult and add),
-    // or, with a bias or a negative scale, the score itself (mult must be positive: the
-    // masked value, -inf, must stay the smallest).
+    // or -1 / (e^2x + 1) where there is a cap (the rest of cap * tanh x is mult and add; with
+    // EXACT tanh x), or, with a bias or a negative scale, the score itself (mult must be
+    // positive: the masked value, -inf, must stay the smallest).
     const bool cap = p.s.cap_in != 0.0f, modified = p.s.slopes != nullptr || (!cap && p.s.scale_log2 <= 0.0f);
-    const float mult = modified ? 1.0f : cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2;
-    const float add = cap && !modified ? p.s.cap_log2 : 0.0f;
+    const float mult = modified ? 1.0f : EXACT ? p.s.cap_log2 : cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2;
+    const float add = cap && !modified && !EXACT ? p.s.cap_log2 : 0.0f;
 
     // LDS offsets of this lane's operand reads.
     const uint32_t k_row = (uint32_t)(n * kRowBytes);
@@ -398,12 +401,24 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         }
         // value e belongs to token t0 + 4 h + 8 (e / 4) + e % 4
         const int tk = t0 + 4 * h;
-        if (cap) {
+        if constexpr (EXACT) {
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(sc[e]));
+            if (__any(top * fabsf(p.s.cap_x) >= 0.5f)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] = capped_tanh(sc[e], p.s);
+            } else {   // what scores are below a cap that is far from most
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] = tanh_series(sc[e] * p.s.cap_x);
+            }
+        } else if (cap) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) sc[e] = capped_part(sc[e], p.s.cap_in);
         }
         if (modified) {
-            const float by = cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2, plus = cap ? p.s.cap_log2 : 0.0f;
+            const float by = EXACT ? p.s.cap_log2 : cap ? 2.0f * p.s.cap_log2 : p.s.scale_log2;
+            const float plus = cap && !EXACT ? p.s.cap_log2 : 0.0f;
 #pragma unroll
             for (int e = 0; e < 32; ++e) sc[e] = fmaf(sc[e], by, plus);
             if (p.s.slopes) {
@@ -615,7 +630,8 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                     dot = fmaf(Hf::to_f32((uint16_t)(x >> 16)), Hf::to_f32((uint16_t)(y >> 16)), dot);
                 }
             }
-            float s1 = p.s.cap_in != 0.0f ? capped(dot, p.s.cap_in, p.s.cap_log2) : dot * p.s.scale_log2;
+            float s1 = EXACT ? capped_tanh(dot, p.s) * p.s.cap_log2
+                             : p.s.cap_in != 0.0f ? capped(dot, p.s.cap_in, p.s.cap_log2) : dot * p.s.scale_log2;
             if (p.s.slopes) s1 = fmaf(-slope1, (float)(pos1 - t), s1);
             s1 = ok ? s1 : -INFINITY;
             float top = s1;

@@ -14,7 +14,7 @@
 
 namespace llmik {
 
-template <bool BF, int D, bool UNI>
+template <bool BF, int D, bool UNI, bool EXACT>
 __global__ __launch_bounds__(kPfThreads, 2) void paged_prefix_kernel(PagedFlashParams f, PagedDecodeParams d,
                                                                      uint32_t flash_wgs) {
     static_assert(kPfThreads == kPdThreads, "one workgroup size for both");
@@ -26,9 +26,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_prefix_kernel(PagedFlashP
     __shared__ uint32_t s_flag;
     __shared__ float s_m[kPdWaves][16], s_l[kPdWaves][16];
     if (blockIdx.x < flash_wgs)
-        paged_flash<BF, D, true>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_flag});
+        paged_flash<BF, D, true, EXACT>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_flag});
     else
-        paged_decode<BF, D, UNI>(d, blockIdx.x - flash_wgs, gridDim.x - flash_wgs,
+        paged_decode<BF, D, UNI, EXACT>(d, blockIdx.x - flash_wgs, gridDim.x - flash_wgs,
                                  {reinterpret_cast<float*>(s_k0), reinterpret_cast<float*>(s_k1),
                                   reinterpret_cast<float*>(s_v0), reinterpret_cast<float*>(s_v1), s_m, s_l, &s_flag});
 }
@@ -129,8 +129,14 @@ template <bool BF, int D>
 void launch_prefix(const PagedFlashParams& f, const PagedDecodeParams& d, int flash_wgs, int decode_wgs, bool uniform,
                    hipStream_t stream) {
     const unsigned grid = (unsigned)(flash_wgs + decode_wgs);
-    if (uniform) paged_prefix_kernel<BF, D, true><<<grid, kPfThreads, 0, stream>>>(f, d, (uint32_t)flash_wgs);
-    else paged_prefix_kernel<BF, D, false><<<grid, kPfThreads, 0, stream>>>(f, d, (uint32_t)flash_wgs);
+    auto go = [&](auto uni, auto exact) {
+        paged_prefix_kernel<BF, D, decltype(uni)::value, decltype(exact)::value>
+            <<<grid, kPfThreads, 0, stream>>>(f, d, (uint32_t)flash_wgs);
+    };
+    using std::false_type;
+    using std::true_type;
+    if (f.s.cap_x != 0.0f) uniform ? go(true_type{}, true_type{}) : go(false_type{}, true_type{});
+    else uniform ? go(true_type{}, false_type{}) : go(false_type{}, false_type{});
     const int rows = f.c.batch * f.n_heads, per_wg = 4 * 128 / D;
     paged_prefix_join_kernel<BF, D><<<(unsigned)((rows + per_wg - 1) / per_wg), 256, 0, stream>>>(
         f.part_o, f.part_ml, f.out, f.splits + 1, rows, FastDiv::of((uint32_t)(f.c.batch * d.gqa)), f.gqa);
