@@ -93,7 +93,7 @@ __global__ __launch_bounds__(1024) void paged_append_kernel(PagedAppendParams p)
         }
         if (b < p.batch) ahead = p.cu[b + 1] - t;
     }
-    const int pos = b < p.batch ? p.lens[b] - ahead : -1;
+    const int pos = b < p.batch ? max(p.lens[b], 0) - ahead : -1;   // (the lowest length: no overflow)
     const bool rotate = p.cos != nullptr;
     const bool live = pos >= 0 && pos < (rotate ? p.table_rows : INT_MAX);
     if (!work) return;
