@@ -724,11 +724,15 @@ int paged_heads(const Tensor& q, const llmik_paged_cache& c) {
     return (int)q.size(1);
 }
 
-llmik_score_options paged_options(const Tensor& q, double softmax_scale, double softcap,
-                                  const std::optional<Tensor>& slopes, int64_t window) {
+void paged_numbers(double softmax_scale, double softcap, int64_t window) {
     TORCH_CHECK(std::isfinite((float)softmax_scale), "softmax_scale must be finite");
     TORCH_CHECK(softcap >= 0 && softcap <= 4096, "softcap must be >= 0 and at most 4096");
+    TORCH_CHECK(softcap == 0 || (float)softcap > 0.0f, "softcap too small: 0 in fp32, which is no cap");
     TORCH_CHECK(window >= 0 && window <= INT_MAX, "window must be >= 0");
+}
+
+llmik_score_options paged_options(const Tensor& q, double softmax_scale, double softcap,
+                                  const std::optional<Tensor>& slopes, int64_t window) {
     llmik_score_options o{(float)softmax_scale, (float)softcap, nullptr, (int)window};
     if (slopes.has_value()) {
         TORCH_CHECK(slopes->scalar_type() == at::kFloat && slopes->dim() == 1 && slopes->is_contiguous() &&
@@ -780,6 +784,7 @@ Tensor rope_paged_append(const Tensor& qkv, const std::optional<Tensor>& cos, co
 Tensor paged_decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                               const Tensor& seq_lens, double softmax_scale, double softcap,
                               const std::optional<Tensor>& slopes, int64_t window) {
+    paged_numbers(softmax_scale, softcap, window);
     const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
     const int H = paged_heads(q, c);
     TORCH_CHECK(q.size(0) == c.batch, "q must have one row per sequence");
@@ -796,6 +801,7 @@ Tensor paged_decode_attention(const Tensor& q, const Tensor& k_cache, const Tens
 Tensor paged_prefill_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                                const Tensor& seq_lens, const Tensor& cu_tokens, double softmax_scale, double softcap,
                                const std::optional<Tensor>& slopes, int64_t window) {
+    paged_numbers(softmax_scale, softcap, window);
     const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
     const int H = paged_heads(q, c);
     const int* cu = paged_offsets(cu_tokens, c, q);
@@ -814,6 +820,7 @@ Tensor paged_shared_prefix_attention(const Tensor& q, const Tensor& k_cache, con
                                      const Tensor& page_table, const Tensor& seq_lens, const Tensor& prefix_pages,
                                      int64_t prefix_len, double softmax_scale, double softcap,
                                      const std::optional<Tensor>& slopes, int64_t window) {
+    paged_numbers(softmax_scale, softcap, window);
     const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
     const int H = paged_heads(q, c);
     TORCH_CHECK(q.size(0) == c.batch, "q must have one row per sequence");

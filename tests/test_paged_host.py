@@ -363,3 +363,17 @@ def test_decode_for_all_batches():
         cache.batch([a], [8192])
         step = cache.batch([a] + [cache.add(share=a, tokens=8192) for _ in range(9)])
         assert (step.prefix_pages is not None) == share and step.prefix_len == (8192 if share else 0)
+
+
+@pytest.mark.parametrize("more,msg", [
+    (dict(softcap=1e-50), "softcap too small"), (dict(softcap=5e-46), "softcap too small"),
+    (dict(softcap=-1e-50), "softcap must be"), (dict(softcap=float("nan")), "softcap must be"),
+    (dict(softcap=4096.5), "softcap must be"), (dict(scale=1e39), "softmax_scale"),
+    (dict(scale=float("nan")), "softmax_scale"), (dict(window=-1), "window"), (dict(window=1 << 31), "window"),
+], ids=str)
+def test_python_refuses_numbers(as_device, more, msg):
+    """Before anything of the tensors is looked at; a cap that fp32 cannot hold is refused,
+    not taken for none."""
+    for call in _calls(as_device, _args(**more)):
+        with pytest.raises(RuntimeError, match=msg):
+            call()
