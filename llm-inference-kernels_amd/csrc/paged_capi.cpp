@@ -77,6 +77,17 @@ int check_rows(const llmik_paged_cache* c, int n_heads, int rows) {
     return LLMIK_OK;
 }
 
+// A shared-prefix call's sizes (those of a cache that check_shapes accepts).
+int check_prefix(const llmik_paged_cache* c, int n_heads, int prefix_len) {
+    if (prefix_len < 0) return invalid("prefix_len must be >= 0");
+    if (prefix_len > kMaxPagedTokens) return unsupported("prefix_len too large");
+    const long per_kv = (long)c->batch * (n_heads / c->n_kv_heads);
+    if (prefix_len > 0 &&
+        (per_kv >= INT_MAX - 256 || (per_kv / 128 + 1) * 64 * c->n_kv_heads * 256 > kMaxThreads))
+        return unsupported("too many rows");
+    return LLMIK_OK;
+}
+
 int check_q(const void* q, const void* out) {
     if (!q || !out) return invalid("null q/out pointer");
     if (!aligned(q, 16) || !aligned(out, 16)) return misaligned("q/out must be 16-byte aligned");
@@ -163,6 +174,7 @@ LLMIK_API llmik_status llmik_rope_paged_append(const llmik_paged_cache* cache, c
 
 LLMIK_API size_t llmik_paged_workspace_size(const llmik_paged_cache* cache, int n_heads, int prefix_len) {
     if (check_shapes(cache, n_heads) != LLMIK_OK || cache->batch == 0) return 0;
+    if (check_prefix(cache, n_heads, prefix_len) != LLMIK_OK) return 0;
     if (prefix_len > 0)
         return paged_prefix_workspace(cache->batch, n_heads, cache->n_kv_heads, cache->head_dim, capacity_of(*cache),
                                       prefix_len);
@@ -215,22 +227,17 @@ LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cac
                                                            void* workspace, size_t workspace_bytes, void* stream) {
     int st = check_cache(cache, n_heads);
     if (st == LLMIK_OK) st = check_options(options);
-    if (st != LLMIK_OK) return st;
-    if (prefix_len < 0) return invalid("prefix_len must be >= 0");
-    if (cache->batch == 0) return LLMIK_OK;
+    if (st == LLMIK_OK) st = check_prefix(cache, n_heads, prefix_len);
+    if (st != LLMIK_OK || cache->batch == 0) return st;
     if ((st = check_q(q, out)) != LLMIK_OK) return st;
     if ((long)n_prefix_pages * cache->page_size < prefix_len)
         return invalid("prefix_pages hold fewer than prefix_len tokens");
-    if (prefix_len > kMaxPagedTokens) return unsupported("prefix_len too large");
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;
     if (prefix_len == 0) return launch_paged_decode(a, as_stream(stream));
     if (prefix_pages == nullptr) return invalid("null prefix_pages pointer");
     if (!aligned(prefix_pages, 4)) return misaligned("prefix_pages must be 4-byte aligned");
-    const long per_kv = (long)cache->batch * (n_heads / cache->n_kv_heads);
-    if (per_kv >= INT_MAX - 256 || (per_kv / 128 + 1) * 64 * cache->n_kv_heads * 256 > kMaxThreads)
-        return unsupported("too many rows");
     a.prefix_pages = prefix_pages;
     a.prefix_len = prefix_len;
     a.rows = cache->batch;

@@ -113,11 +113,11 @@ PagedPrefixPlan plan_prefix(int batch, int n_heads, int n_kv_heads, int head_dim
     // of eight tiles, as every part's results are written and read again, and never in
     // less than two tiles. us, 64 sequences behind 8192 tokens, 16 and 32 splits 29.4,
     // 39.7; 2 sequences behind 4096, 16 and 32 splits 13.2, 12.4.
-    const long tiles = (prefix_len + kPfTile - 1) / kPfTile;
+    const long tiles = ((long)prefix_len + kPfTile - 1) / kPfTile;
     const long splits =
         std::max(1L, std::min({2L * cus / base, std::max(cus / base, tiles / 8), (tiles + 1) / 2, 64L}));
-    pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;
-    pl.splits = (prefix_len + pl.chunk - 1) / pl.chunk;
+    pl.chunk = (int)((tiles + splits - 1) / splits) * kPfTile;   // (prefix_len <= kMaxPagedTokens)
+    pl.splits = (int)(((long)prefix_len + pl.chunk - 1) / pl.chunk);
     pl.off_ml = align_up(paged_decode_workspace(batch, n_heads, n_kv_heads, head_dim, capacity), 256);
     const size_t parts = (size_t)rows * n_kv_heads * (pl.splits + 1);
     pl.off_o = pl.off_ml + align_up(parts * 2 * sizeof(float), 256);

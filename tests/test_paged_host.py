@@ -377,3 +377,26 @@ def test_python_refuses_numbers(as_device, more, msg):
     for call in _calls(as_device, _args(**more)):
         with pytest.raises(RuntimeError, match=msg):
             call()
+
+
+def test_workspace_sizes_are_0_for_what_the_calls_refuse(lib):
+    c, o = _cache(), _options()
+    for prefix, code in [(-1, INVALID), (-2 ** 31, INVALID), ((1 << 30) + 1, UNSUPPORTED), (2 ** 31 - 64, UNSUPPORTED),
+                         (2 ** 31 - 1, UNSUPPORTED)]:
+        assert lib.llmik_paged_workspace_size(_at(c), 4, prefix) == 0, prefix
+        assert lib.llmik_paged_shared_prefix_attention(_at(c), 16, 16, 4, 16, 2 ** 31 - 1, prefix, _at(o), 16, 1 << 60,
+                                                       None) == code, prefix
+    # rows that no launch holds: with a prefix only
+    many = _cache(batch=1 << 20, max_pages=1, n_kv_heads=1)
+    assert lib.llmik_paged_workspace_size(_at(many), 512, 16) == 0
+    assert lib.llmik_paged_shared_prefix_attention(_at(many), 16, 16, 512, 16, 1, 16, _at(o), 16, 1 << 60,
+                                                   None) == UNSUPPORTED
+    assert lib.llmik_paged_workspace_size(_at(many), 512, 0) > 0
+    # what is accepted: sizes that hold a part of every row, and for the longest prefix
+    sizes = [lib.llmik_paged_workspace_size(_at(c), 4, n) for n in (0, 1, 64, 8192, 1 << 30)]
+    assert 0 < sizes[0] < sizes[1] <= sizes[2] <= sizes[3] <= sizes[4] < 1 << 24
+    for bad in (dict(head_dim=96), dict(page_size=12), dict(batch=-1)):
+        assert lib.llmik_paged_workspace_size(_at(_cache(**bad)), 4, 16) == 0
+        assert lib.llmik_paged_prefill_workspace_size(_at(_cache(**bad)), 4, 16) == 0
+    assert lib.llmik_paged_prefill_workspace_size(_at(c), 4, -1) == 0
+    assert lib.llmik_paged_prefill_workspace_size(_at(c), 4, 2 ** 31 - 1) == 0
