@@ -138,6 +138,9 @@ int launch_pack_int4_along_k(const void* q, int K, int N, void* packed, hipStrea
 // ---- paged KV cache --------------------------------------------------------
 // Tokens of a sequence at most: positions a few tiles past the end are still ints.
 constexpr long kMaxPagedTokens = 1L << 30;
+// Decode attention counts its work in 32 bits: 32-token tiles, of every (sequence, KV head,
+// head chunk) slab one at least, and kPieceUnits more for each slab.
+constexpr int kPieceUnits = 6;
 struct PagedLaunch {
     const void* q;
     const void* k;

@@ -36,11 +36,11 @@ int check_shapes(const llmik_paged_cache* c, int n_heads) {
     if (c->max_pages <= 0) return invalid("page_table must have at least one column");
     if (page_stride(*c) < row_elements(*c) || page_stride(*c) % 8 != 0)
         return invalid("page_stride must hold a page and be a multiple of 8");
-    // the work of all sequences is counted in 32 bits (tiles of 32 tokens and an overhead for each)
+    // the work of all sequences is counted in 32 bits
     const long capacity = std::min((long)c->max_pages * c->page_size, kMaxPagedTokens);
     const long chunks = (n_heads / c->n_kv_heads + 15) / 16;
     const long slabs = (long)c->batch * c->n_kv_heads * chunks;
-    if (slabs >= INT_MAX || slabs * (capacity / 32 + 4) >= INT_MAX)
+    if (slabs >= INT_MAX || slabs * ((capacity + 31) / 32 + kPieceUnits) >= INT_MAX)
         return unsupported("batch * n_kv_heads * page table capacity too large");
     return LLMIK_OK;
 }

@@ -60,7 +60,7 @@ struct PagedDecodeParams {
     int few_steps;        // workgroups that few tiles are spread over, one tile per wave
 };
 
-constexpr int kPieceUnits = 6;    // a piece's overhead in units of a tile's time (see the shares)
+// kPieceUnits (llmik_internal.hpp) is a piece's overhead in units of a tile's time: see the shares.
 constexpr int kUncutTiles = 12;   // a slab of so few tiles is not cut: three per wave cost less than a hand-off
 constexpr int kEachTiles = 24;    // the longest slab where every workgroup takes one
 

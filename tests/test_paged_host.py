@@ -400,3 +400,15 @@ def test_workspace_sizes_are_0_for_what_the_calls_refuse(lib):
         assert lib.llmik_paged_prefill_workspace_size(_at(_cache(**bad)), 4, 16) == 0
     assert lib.llmik_paged_prefill_workspace_size(_at(c), 4, -1) == 0
     assert lib.llmik_paged_prefill_workspace_size(_at(c), 4, 2 ** 31 - 1) == 0
+
+
+@pytest.mark.parametrize("page,tiles", [(8, 1), (32, 1), (40, 2), (64, 2)])
+def test_the_work_of_all_sequences_fits_32_bits(lib, page, tiles):
+    """A slab counts its 32-token tiles, the last one begun too, and six more."""
+    most = (2 ** 31 - 2) // (tiles + 6)
+    fits = _cache(batch=most, max_pages=1, page_size=page, n_kv_heads=1)
+    over = _cache(batch=most + 1, max_pages=1, page_size=page, n_kv_heads=1)
+    o = _options()
+    assert lib.llmik_paged_workspace_size(_at(fits), 1, 0) > 0
+    assert lib.llmik_paged_workspace_size(_at(over), 1, 0) == 0
+    assert lib.llmik_paged_decode_attention(_at(over), 16, 16, 1, _at(o), 16, 1 << 60, None) == UNSUPPORTED
