@@ -265,6 +265,7 @@ class PagedKVCache:
         shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.device = self.k.device   # with its index: batch() is not the current device's
         self._free = list(range(n_pages - 1, -1, -1))
         self._users = [0] * n_pages             # sequences that hold the page
         self._pages: dict[int, List[int]] = {}  # sequence -> its pages

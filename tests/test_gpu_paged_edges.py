@@ -35,3 +35,12 @@ def test_appends_to_empty_sequences(llmik, cuda, length, tables, rows):
                                 None if rows is None else ref.offsets(rows, cuda))
     assert int(q.count_nonzero()) == 0
     assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+def test_a_cache_stays_on_its_device(llmik, cuda):
+    """Made on the current device, its batches go there whatever device is current later."""
+    from llmik_cuda.kv_cache import PagedKVCache
+    cache = PagedKVCache(4, 2, page_size=16, head_dim=64)
+    assert cache.device == cache.k.device and cache.device.index is not None
+    step = cache.batch([cache.add()], [3])
+    assert step.page_table.device == step.seq_lens.device == cache.k.device
