@@ -159,8 +159,6 @@ struct PagedLaunch {
     void* workspace;
     size_t workspace_bytes;
 };
-// Un-normalised results of a shared prefix that the decode kernel joins:
-// o [n_kv_heads, batch * n_heads / n_kv_heads, splits, head_dim], ml [..., 2].
 struct PagedAppend {
     const void* qkv;
     const void* cos;   // null: no rotation

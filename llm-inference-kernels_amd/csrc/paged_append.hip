@@ -33,7 +33,7 @@ struct PagedAppendParams {
     const int* lens;
     const int* cu;
     long page_stride;
-    int n_pages, max_pages, batch, n_heads, n_kv_heads, capacity, rows, table_rows;
+    int n_pages, max_pages, batch, n_heads, n_kv_heads, capacity, table_rows;
     FastDiv page;
 };
 
@@ -169,7 +169,6 @@ int launch_paged_append(const PagedAppend& a, hipStream_t stream) {
     p.n_heads = a.n_heads;
     p.n_kv_heads = a.n_kv_heads;
     p.capacity = (int)std::min((long)a.max_pages * a.page_size, kMaxPagedTokens);
-    p.rows = a.rows;
     p.table_rows = a.table_rows;
     p.page = FastDiv::of((uint32_t)a.page_size);
     // One workgroup per row up to 512 threads, in whole waves.

@@ -31,8 +31,8 @@
 // Registers hold one tile: the next tile's keys are requested when the scores are
 // computed, its values when their products are (two buffers spilled). Measured, GPU
 // us: 64 sequences of 8192 tokens, 8 KV heads of 8 317 (6.8 TB/s); 32 of 30 .. 8000 in
-// bf16 33.2 (5.1 TB/s); one of 50001, heads of 64, 22.6 (4.5 TB/s); 24 of 100 .. 12000
-// in a window of 4096 23.0 (3.9 TB/s: small pages, a look-up per octet); one of 700 8.1,
+// bf16 33.6 (5.0 TB/s); one of 50001, heads of 64, 23.4 (4.4 TB/s); 24 of 100 .. 12000
+// in a window of 4096 23.1 (3.9 TB/s: small pages, a look-up per octet); one of 700 8.3,
 // a chain of dependent reads (lengths, pages, keys, hand-off) behind the launch.
 #pragma once
 

@@ -25,12 +25,16 @@
 // Where there are fewer row tiles than two workgroups per CU, their keys are cut into
 // parts, whose sums a second kernel joins (paged_flash.hip, paged_prefix.hip).
 //
-// Measured: a prompt of 8192 tokens, 32 heads over 8 KV heads of 128, bf16: 520 .. 535
-// us, 1.03 .. 1.06 PFLOP/s (a large matrix product reaches 1.42): the matrix units work 57 % of
-// the cycles, beside 3 vector instructions per score, and the clock falls to 1.8 GHz.
-// Chunks of four prompts over up to 6000 cached tokens, capped scores: 165 us, 0.70
-// PFLOP/s, bound by the cap's two transcendentals per score. Three short prompts 8.2 us:
-// launch, look-ups, two or three tiles.
+// Measured: a prompt of 8192 tokens, 32 heads over 8 KV heads of 128, bf16: 518 .. 570
+// us, 0.96 .. 1.06 PFLOP/s (a large matrix product reaches 1.42): the matrix units work 57 % of
+// the cycles and vector instructions (4.7 a score, the products not counted) about half of
+// them, which overlap little. Of 2048 tokens 50 .. 56 us, twice the products' time: a CU's
+// longer workgroup ends alone, one wave per SIMD. Of 2000 tokens with heads of 64 35 us: the
+// vector work of heads of 128 on half of the products. Chunks of four prompts over up to
+// 6000 cached tokens, capped scores: 161 .. 175 us, 0.67 .. 0.72 PFLOP/s, bound by the cap's
+// two transcendentals per score. Three short prompts 8.2 us: launch, look-ups, two or three
+// tiles (12.8 with a table for 1024 tokens or more, where plan_prefill cuts keys and launches
+// the join).
 #pragma once
 
 #include "paged_common.hpp"
@@ -99,9 +103,11 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
     const uint32_t incl = wave_scan(mine);
     const uint32_t total = lane_u32(incl, 63);
     if (item >= total) return false;
-    // A prompt's last tiles see the most keys and come first. Where all workgroups
-    // run at once, two per CU, the second half goes the other way, so that a CU's two
-    // have about the same work together as another's.
+    // The call's last tiles come first: of one prompt those that see the most keys.
+    // (Between sequences the order is the batch's, whatever their lengths.) Where all
+    // workgroups run at once, two per CU, the second half goes the other way, so that a
+    // CU's two have about the same work together as another's. (Of heads of 64 three fit a
+    // CU; the rule counts two.)
     const uint32_t half = p.per_round / (uint32_t)(p.c.n_kv_heads * p.splits);   // tiles of one workgroup per CU
     uint32_t x = total - 1 - item;
     if (item >= half && total <= 2 * half) x = item - half;
@@ -143,7 +149,8 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
 constexpr int kMaxParts = 8;
 constexpr int kMinPart = 4;   // tiles of a part at least
 
-// The number of parts for `tiles` key tiles where the call has `base` workgroups uncut.
+// The number of parts for `tiles` key tiles where the call has `base` workgroups uncut,
+// from heads of 128 (those of 64 have half the sums and less than half of a tile's time).
 // A tile takes 1.3 us, a part's sums (64 KiB) are written and read again: per workgroup
 // and part 0.026 us of the card's time. tiles * 1.3 / n + base * 0.026 * n is least at
 // n^2 = 50 tiles / base (here the nearest n). Measured with n = 1, 2, 3, 4, 5, 6, 8: two sequences of 100 rows

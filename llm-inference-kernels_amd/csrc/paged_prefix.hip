@@ -4,11 +4,12 @@
 // one joins a row's parts: those of the prefix, then its own.
 //
 // The two kinds of workgroups run beside each other: the prefix's are bound by their
-// chain of products and exponentials, the others by memory. Measured, GPU us: 64
-// sequences behind 8192 tokens 29.3 (in launches of their own 37.1), of which the join
-// is 5.0 (17 parts a row, written and read in fp32); 6 behind 1500 10.6 (16.0), two
-// launches of dependent reads; 64 behind 4096 28, where decode attention, which reads
-// the prefix 64 times, takes 110.
+// chain of products, exponentials and waits (one wave per SIMD: 46 % of its cycles wait,
+// products take 4 us of 25), the others by memory. Measured, GPU us: 64 sequences behind
+// 8192 tokens 30.1 (in launches of their own 37.1), of which the join is 4.9 (17 parts a
+// row, written and read in fp32); 6 behind 1500 10.9 (16.0), two launches of dependent
+// reads; 64 behind 4096 28, where decode attention, which reads the prefix 64 times,
+// takes 110.
 #include "paged_decode.hpp"
 #include "paged_flash.hpp"
 
