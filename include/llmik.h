@@ -567,6 +567,105 @@ LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cac
                                                            int prefix_len, const llmik_score_options* options,
                                                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------ drafted trees, bounded caches
+ * Attention of drafted token trees, and a cache whose sequences keep the tokens
+ * that attention uses most. No counterpart in the reference.
+ */
+
+/*
+ * llmik_rope_paged_append with the rows' positions given: positions [rows] are
+ * what cos and sin are indexed by; the slots stay those of the rows' order. (A
+ * drafted token's depth; a sequence that is shorter than its text.) A position
+ * outside [0, table_rows) is written nowhere. NULL: llmik_rope_paged_append.
+ */
+LLMIK_API llmik_status llmik_rope_paged_append_at(const llmik_paged_cache* cache, const void* qkv, const void* cos,
+                                                  const void* sin, int table_rows, int table_f32,
+                                                  const int* cu_tokens, const int* positions, void* q_out, int rows,
+                                                  int n_heads, void* stream);
+
+/*
+ * q, out [rows, n_heads, head_dim]: the drafted tokens of every sequence, its last
+ * cu_tokens[b + 1] - cu_tokens[b] slots (rows as llmik_rope_paged_append's). Each
+ * sees all tokens that were cached before, and the drafted token j of its own
+ * sequence where bit j % 64 of tree_mask [rows, words], word j / 64, is set
+ * (unsigned 64-bit words; drafted tokens from 64 words on are seen by none).
+ *   positions [rows]: of the drafted tokens, for slopes and window; one below the
+ *     sequence's cached tokens counts as their number, one above 2^30 as that. NULL:
+ *     their slots. A cached token's position is its slot.
+ * Probabilities are rounded as llmik_paged_prefill_attention's. A row that sees no
+ * token gives zeros.
+ */
+LLMIK_API size_t llmik_paged_tree_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows);
+LLMIK_API llmik_status llmik_paged_tree_attention(const llmik_paged_cache* cache, const void* q,
+                                                  const int* cu_tokens, const uint64_t* tree_mask, int words,
+                                                  const int* positions, void* out, int rows, int n_heads,
+                                                  const llmik_score_options* options, void* workspace,
+                                                  size_t workspace_bytes, void* stream);
+
+/*
+ * The attention weight that each token has had: weights [n_rows, n_kv_heads,
+ * max_len] fp32, of sequence b in row rows[b] (NULL: row b; n_rows >= batch then),
+ * by the token's slot. A sequence whose row is outside [0, n_rows) is not recorded,
+ * nor are tokens at or behind max_len. Two sequences with one row give it no
+ * particular sum.
+ */
+typedef struct llmik_token_weights {
+    float* weights;
+    const int* rows;
+    int n_rows, max_len;
+} llmik_token_weights;
+
+/*
+ * llmik_paged_decode_attention that also adds, for every live key t, the sum of its
+ * probabilities over the KV head's query heads to weights[row][kv_head][t]. out has
+ * the same bits as llmik_paged_decode_attention's.
+ */
+LLMIK_API size_t llmik_paged_decode_weights_workspace_size(const llmik_paged_cache* cache, int n_heads,
+                                                           const llmik_token_weights* weights);
+LLMIK_API llmik_status llmik_paged_decode_attention_weights(const llmik_paged_cache* cache, const void* q, void* out,
+                                                            int n_heads, const llmik_score_options* options,
+                                                            const llmik_token_weights* weights, void* workspace,
+                                                            size_t workspace_bytes, void* stream);
+
+/*
+ * The same sums for the rows of a prompt (q and cu_tokens as
+ * llmik_paged_prefill_attention's): of each sequence's last `observe` new rows (0: of
+ * all). Only the cache's k is read.
+ */
+LLMIK_API size_t llmik_paged_prefill_weights_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows,
+                                                            int observe);
+LLMIK_API llmik_status llmik_paged_prefill_weights(const llmik_paged_cache* cache, const void* q,
+                                                   const int* cu_tokens, int rows, int n_heads,
+                                                   const llmik_score_options* options, int observe,
+                                                   const llmik_token_weights* weights, void* workspace,
+                                                   size_t workspace_bytes, void* stream);
+
+/*
+ * The slots that each (sequence, KV head) keeps: the first `first`, the last `recent`,
+ * and of the others those of the largest weight (NaN above all; ties to the lowest
+ * slot), `keep` in all, in order, -1 behind; all of a sequence of at most `keep`
+ * tokens. Tokens at or behind weights->max_len do not exist; a sequence without a row
+ * has weights 0. kept [batch, n_kv_heads, keep]; new_lens [batch]: the tokens kept.
+ */
+LLMIK_API llmik_status llmik_paged_select_tokens(const llmik_token_weights* weights, const int* seq_lens, int batch,
+                                                 int n_kv_heads, int keep, int first, int recent, int* kept,
+                                                 int* new_lens, void* stream);
+
+/*
+ * Moves tokens together, in place: the token in slot kept[b][h][i] goes to slot
+ * starts[b] + i (NULL: i), for i < n.
+ *   kept [batch, kept_heads, n]: kept_heads n_kv_heads, or 1 for one list for all heads.
+ *     An entry that is negative, at or behind the sequence's length, or in front of its
+ *     new slot moves nothing, nor do unmapped pages. The entries may have any order.
+ *   weights (NULL: none) are moved alike, and those from the first negative entry's new
+ *     slot on become 0.
+ * Slots behind the moved tokens keep what they hold. seq_lens are the lengths before;
+ * they are not changed. Sequences that share a page that is written, or that map one
+ * twice, get no particular order.
+ */
+LLMIK_API llmik_status llmik_paged_compact(const llmik_paged_cache* cache, const int* kept, int kept_heads, int n,
+                                           const int* starts, const llmik_token_weights* weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -159,6 +159,13 @@ struct PagedLaunch {
     void* workspace;
     size_t workspace_bytes;
 };
+// Each token's accumulated attention weight: fp32 [n_rows, n_kv_heads, max_len], of
+// sequence b in row rows[b] (rows null: b). weights null: none.
+struct PagedWeights {
+    void* weights;
+    const int* rows;
+    int n_rows, max_len;
+};
 struct PagedAppend {
     const void* qkv;
     const void* cos;   // null: no rotation
@@ -169,6 +176,7 @@ struct PagedAppend {
     const int* table;
     const int* lens;
     const int* cu;     // null: row b is the newest token of sequence b
+    const int* positions;   // [rows], or null: a row's position is its slot
     long page_stride;
     int n_pages, page_size, max_pages, batch, n_heads, n_kv_heads, head_dim;
     int rows, table_rows;
@@ -177,7 +185,19 @@ struct PagedAppend {
 size_t paged_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity);
 size_t paged_prefill_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
 size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len);
+size_t paged_tree_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
+size_t paged_decode_weights_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity,
+                                      int max_len);
+size_t paged_prefill_weights_workspace(int batch, int rows, int n_heads, int n_kv_heads, int observe);
 int launch_paged_append(const PagedAppend& a, hipStream_t stream);
+int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, const int* positions,
+                      hipStream_t stream);
+int launch_paged_prefill_weights(const PagedLaunch& a, const PagedWeights& w, int observe, hipStream_t stream);
+int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, hipStream_t stream);
+int launch_paged_select(const PagedWeights& w, const int* lens, int batch, int n_kv_heads, int keep, int first,
+                        int recent, int* kept, int* new_lens, hipStream_t stream);
+int launch_paged_compact(const PagedLaunch& a, const PagedWeights& w, const int* kept, int kept_heads, int n,
+                         const int* starts, hipStream_t stream);
 int launch_paged_decode(const PagedLaunch& a, hipStream_t stream);
 int launch_paged_prefill(const PagedLaunch& a, hipStream_t stream);
 int launch_paged_shared_prefix(const PagedLaunch& a, hipStream_t stream);

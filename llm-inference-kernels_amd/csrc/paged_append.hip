@@ -4,7 +4,8 @@
 // Row t of qkv is a token of sequence b (the one whose range of cu_tokens holds
 // t; without cu_tokens row b is sequence b's newest token) at position
 //   pos = seq_lens[b] - (cu_tokens[b + 1] - t)      (seq_lens[b] - 1),
-// and for d < D/2 with the position's rows of the cos and sin tables
+// unless the caller gives its position (a drafted tree's depths; a sequence that lost
+// tokens): pos is then its slot only. For d < D/2 with the position's rows of the cos and sin tables
 //   x'[d] = x[d] cos[d] - x[d + D/2] sin[d],
 //   x'[d + D/2] = x[d + D/2] cos[d + D/2] + x[d] sin[d + D/2]
 // in fp32, rounded once (the arithmetic of rope). The bytes bound it: each row
@@ -32,6 +33,7 @@ struct PagedAppendParams {
     const int* table;
     const int* lens;
     const int* cu;
+    const int* positions;
     long page_stride;
     int n_pages, max_pages, batch, n_heads, n_kv_heads, capacity, table_rows;
     FastDiv page;
@@ -95,14 +97,15 @@ __global__ __launch_bounds__(1024) void paged_append_kernel(PagedAppendParams p)
     }
     const int pos = b < p.batch ? max(p.lens[b], 0) - ahead : -1;   // (the lowest length: no overflow)
     const bool rotate = p.cos != nullptr;
-    const bool live = pos >= 0 && pos < (rotate ? p.table_rows : INT_MAX);
+    const int at = p.positions ? p.positions[t] : pos;   // of the tables; pos: the slot
+    const bool live = pos >= 0 && (!rotate || (uint32_t)at < (uint32_t)p.table_rows);
     if (!work) return;
 
     const bool is_q = head < p.n_heads;
     u32x4 y1 = x1, y2 = x2;
     if (rotate && live && head < p.n_heads + p.n_kv_heads) {
         float c1[8], s1[8], c2[8], s2[8];
-        const long row = (long)pos * D + d;
+        const long row = (long)at * D + d;
         table8<BF, F32>(p.cos, row, c1);
         table8<BF, F32>(p.sin, row, s1);
         table8<BF, F32>(p.cos, row + D / 2, c2);
@@ -162,6 +165,7 @@ int launch_paged_append(const PagedAppend& a, hipStream_t stream) {
     p.table = a.table;
     p.lens = a.lens;
     p.cu = a.cu;
+    p.positions = a.positions;
     p.page_stride = a.page_stride;
     p.n_pages = a.n_pages;
     p.max_pages = a.max_pages;

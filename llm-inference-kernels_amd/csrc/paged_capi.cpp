@@ -45,11 +45,11 @@ int check_shapes(const llmik_paged_cache* c, int n_heads) {
     return LLMIK_OK;
 }
 
-int check_cache(const llmik_paged_cache* c, int n_heads) {
+int check_cache(const llmik_paged_cache* c, int n_heads, bool with_v = true) {
     const int st = check_shapes(c, n_heads);
     if (st != LLMIK_OK || c->batch == 0) return st;
-    if (!c->k || !c->v || !c->page_table || !c->seq_lens) return invalid("null cache pointer");
-    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return misaligned("k and v must be 16-byte aligned");
+    if (!c->k || (with_v && !c->v) || !c->page_table || !c->seq_lens) return invalid("null cache pointer");
+    if (!aligned(c->k, 16) || (with_v && !aligned(c->v, 16))) return misaligned("k and v must be 16-byte aligned");
     if (!aligned(c->page_table, 4) || !aligned(c->seq_lens, 4))
         return misaligned("page_table and seq_lens must be 4-byte aligned");
     return LLMIK_OK;
@@ -76,6 +76,29 @@ int check_rows(const llmik_paged_cache* c, int n_heads, int rows) {
         return unsupported("too many rows");
     return LLMIK_OK;
 }
+
+// A call whose row tiles' keys are cut by length counts pairs of both kinds of tiles in 32 bits.
+int check_cut(const llmik_paged_cache* c, int n_heads, int rows) {
+    const int st = check_rows(c, n_heads, rows);
+    if (st != LLMIK_OK) return st;
+    const long capacity = std::min((long)c->max_pages * c->page_size, kMaxPagedTokens);
+    const long per_kv = (long)rows * (n_heads / c->n_kv_heads);
+    if ((per_kv / 64 + c->batch + 1) * (capacity / 64 + 2) >= INT_MAX)
+        return unsupported("rows * page table capacity too large");
+    return LLMIK_OK;
+}
+
+int check_weights(const llmik_token_weights* w, int batch) {
+    if (w == nullptr) return invalid("null token weights");
+    if (w->n_rows < 0) return invalid("n_rows must be >= 0");
+    if (w->max_len <= 0 || w->max_len > kMaxPagedTokens) return invalid("max_len must be positive and at most 2^30");
+    if (w->rows == nullptr && w->n_rows < batch) return invalid("without rows there is one row per sequence");
+    if (w->weights == nullptr && w->n_rows > 0) return invalid("null weights pointer");
+    if (!aligned(w->weights, 4) || !aligned(w->rows, 4)) return misaligned("weights and rows must be 4-byte aligned");
+    return LLMIK_OK;
+}
+
+PagedWeights weights_of(const llmik_token_weights& w) { return {w.weights, w.rows, w.n_rows, w.max_len}; }
 
 // A shared-prefix call's sizes (those of a cache that check_shapes accepts).
 int check_prefix(const llmik_paged_cache* c, int n_heads, int prefix_len) {
@@ -132,6 +155,14 @@ extern "C" {
 LLMIK_API llmik_status llmik_rope_paged_append(const llmik_paged_cache* cache, const void* qkv, const void* cos,
                                                const void* sin, int table_rows, int table_f32, const int* cu_tokens,
                                                void* q_out, int rows, int n_heads, void* stream) {
+    return llmik_rope_paged_append_at(cache, qkv, cos, sin, table_rows, table_f32, cu_tokens, nullptr, q_out, rows,
+                                      n_heads, stream);
+}
+
+LLMIK_API llmik_status llmik_rope_paged_append_at(const llmik_paged_cache* cache, const void* qkv, const void* cos,
+                                                  const void* sin, int table_rows, int table_f32,
+                                                  const int* cu_tokens, const int* positions, void* q_out, int rows,
+                                                  int n_heads, void* stream) {
     const int st = check_cache(cache, n_heads);
     if (st != LLMIK_OK) return st;
     if (rows < 0) return invalid("rows must be >= 0");
@@ -145,6 +176,7 @@ LLMIK_API llmik_status llmik_rope_paged_append(const llmik_paged_cache* cache, c
     if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(cos, 16) || !aligned(sin, 16))
         return misaligned("qkv, q_out, cos and sin must be 16-byte aligned");
     if (!aligned(cu_tokens, 4)) return misaligned("cu_tokens must be 4-byte aligned");
+    if (!aligned(positions, 4)) return misaligned("positions must be 4-byte aligned");
     const long threads = ((long)n_heads + 2L * cache->n_kv_heads) * (cache->head_dim / 16) + 1024;
     if (threads > 65535L * 64 || (long)rows * threads > kMaxThreads) return unsupported("too many rows or heads");
     PagedAppend a{};
@@ -157,6 +189,7 @@ LLMIK_API llmik_status llmik_rope_paged_append(const llmik_paged_cache* cache, c
     a.table = cache->page_table;
     a.lens = cache->seq_lens;
     a.cu = cu_tokens;
+    a.positions = positions;
     a.page_stride = page_stride(*cache);
     a.n_pages = cache->n_pages;
     a.page_size = cache->page_size;
@@ -242,6 +275,129 @@ LLMIK_API llmik_status llmik_paged_shared_prefix_attention(const llmik_paged_cac
     a.prefix_len = prefix_len;
     a.rows = cache->batch;
     return launch_paged_shared_prefix(a, as_stream(stream));
+}
+
+LLMIK_API size_t llmik_paged_tree_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows) {
+    if (check_cut(cache, n_heads, rows) != LLMIK_OK || cache->batch == 0 || rows == 0) return 0;
+    return paged_tree_workspace(cache->batch, rows, n_heads, cache->n_kv_heads, cache->head_dim,
+                                capacity_of(*cache));
+}
+
+LLMIK_API llmik_status llmik_paged_tree_attention(const llmik_paged_cache* cache, const void* q,
+                                                  const int* cu_tokens, const uint64_t* tree_mask, int words,
+                                                  const int* positions, void* out, int rows, int n_heads,
+                                                  const llmik_score_options* options, void* workspace,
+                                                  size_t workspace_bytes, void* stream) {
+    int st = check_cache(cache, n_heads);
+    if (st == LLMIK_OK) st = check_options(options);
+    if (st == LLMIK_OK) st = check_cut(cache, n_heads, rows);
+    if (st != LLMIK_OK) return st;
+    if (words <= 0) return invalid("tree_mask must have at least one word per row");
+    if (words > (1 << 24)) return unsupported("tree_mask has more than 2^24 words per row");
+    if (rows == 0) return LLMIK_OK;
+    if (cache->batch == 0) return invalid("rows without a sequence");
+    if (cu_tokens == nullptr || tree_mask == nullptr) return invalid("null cu_tokens/tree_mask pointer");
+    if (!aligned(cu_tokens, 4) || !aligned(positions, 4))
+        return misaligned("cu_tokens and positions must be 4-byte aligned");
+    if (!aligned(tree_mask, 8)) return misaligned("tree_mask must be 8-byte aligned");
+    if ((st = check_q(q, out)) != LLMIK_OK) return st;
+    PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
+    a.cu = cu_tokens;
+    a.rows = rows;
+    a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
+    return launch_paged_tree(a, tree_mask, words, positions, as_stream(stream));
+}
+
+LLMIK_API size_t llmik_paged_decode_weights_workspace_size(const llmik_paged_cache* cache, int n_heads,
+                                                           const llmik_token_weights* weights) {
+    if (check_shapes(cache, n_heads) != LLMIK_OK || cache->batch == 0) return 0;
+    if (check_weights(weights, cache->batch) != LLMIK_OK) return 0;
+    return paged_decode_weights_workspace(cache->batch, n_heads, cache->n_kv_heads, cache->head_dim,
+                                          capacity_of(*cache), weights->max_len);
+}
+
+LLMIK_API llmik_status llmik_paged_decode_attention_weights(const llmik_paged_cache* cache, const void* q, void* out,
+                                                            int n_heads, const llmik_score_options* options,
+                                                            const llmik_token_weights* weights, void* workspace,
+                                                            size_t workspace_bytes, void* stream) {
+    int st = check_cache(cache, n_heads);
+    if (st == LLMIK_OK) st = check_options(options);
+    if (st == LLMIK_OK) st = check_weights(weights, cache->batch);
+    if (st != LLMIK_OK || cache->batch == 0) return st;
+    if ((st = check_q(q, out)) != LLMIK_OK) return st;
+    PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
+    a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
+    return launch_paged_decode_weights(a, weights_of(*weights), as_stream(stream));
+}
+
+LLMIK_API size_t llmik_paged_prefill_weights_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows,
+                                                            int observe) {
+    if (check_cut(cache, n_heads, rows) != LLMIK_OK || cache->batch == 0 || rows == 0 || observe < 0) return 0;
+    return paged_prefill_weights_workspace(cache->batch, rows, n_heads, cache->n_kv_heads, observe);
+}
+
+LLMIK_API llmik_status llmik_paged_prefill_weights(const llmik_paged_cache* cache, const void* q,
+                                                   const int* cu_tokens, int rows, int n_heads,
+                                                   const llmik_score_options* options, int observe,
+                                                   const llmik_token_weights* weights, void* workspace,
+                                                   size_t workspace_bytes, void* stream) {
+    int st = check_cache(cache, n_heads, false);
+    if (st == LLMIK_OK) st = check_options(options);
+    if (st == LLMIK_OK) st = check_cut(cache, n_heads, rows);
+    if (st == LLMIK_OK) st = check_weights(weights, cache->batch);
+    if (st != LLMIK_OK) return st;
+    if (observe < 0) return invalid("observe must be >= 0");
+    if (rows == 0) return LLMIK_OK;
+    if (cache->batch == 0) return invalid("rows without a sequence");
+    if (cu_tokens == nullptr) return invalid("null cu_tokens pointer");
+    if (!aligned(cu_tokens, 4)) return misaligned("cu_tokens must be 4-byte aligned");
+    if (q == nullptr) return invalid("null q pointer");
+    if (!aligned(q, 16)) return misaligned("q must be 16-byte aligned");
+    PagedLaunch a = launch_of(*cache, q, nullptr, n_heads, *options);
+    a.cu = cu_tokens;
+    a.rows = rows;
+    a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
+    return launch_paged_prefill_weights(a, weights_of(*weights), observe, as_stream(stream));
+}
+
+LLMIK_API llmik_status llmik_paged_select_tokens(const llmik_token_weights* weights, const int* seq_lens, int batch,
+                                                 int n_kv_heads, int keep, int first, int recent, int* kept,
+                                                 int* new_lens, void* stream) {
+    if (batch < 0) return invalid("batch must be >= 0");
+    if (n_kv_heads <= 0) return invalid("head counts must be positive");
+    const int st = check_weights(weights, batch);
+    if (st != LLMIK_OK) return st;
+    if (keep <= 0) return invalid("keep must be positive");
+    if (first < 0 || recent < 0 || (long)first + recent > keep)
+        return invalid("first and recent must be >= 0, together at most keep");
+    if (batch == 0) return LLMIK_OK;
+    if (!seq_lens || !kept || !new_lens) return invalid("null seq_lens/kept/new_lens pointer");
+    if (!aligned(seq_lens, 4) || !aligned(kept, 4) || !aligned(new_lens, 4))
+        return misaligned("seq_lens, kept and new_lens must be 4-byte aligned");
+    if ((long)batch * n_kv_heads * 1024 > kMaxThreads) return unsupported("batch * n_kv_heads too large");
+    return launch_paged_select(weights_of(*weights), seq_lens, batch, n_kv_heads, keep, first, recent, kept, new_lens,
+                               as_stream(stream));
+}
+
+LLMIK_API llmik_status llmik_paged_compact(const llmik_paged_cache* cache, const int* kept, int kept_heads, int n,
+                                           const int* starts, const llmik_token_weights* weights, void* stream) {
+    int st = check_cache(cache, cache != nullptr ? cache->n_kv_heads : 1);
+    if (st == LLMIK_OK && weights != nullptr) st = check_weights(weights, cache->batch);
+    if (st != LLMIK_OK) return st;
+    if (kept_heads != 1 && kept_heads != cache->n_kv_heads) return invalid("kept_heads must be 1 or n_kv_heads");
+    if (n < 0) return invalid("n must be >= 0");
+    if (n > kMaxPagedTokens) return unsupported("n too large");
+    if (cache->batch == 0) return LLMIK_OK;
+    if (kept == nullptr && n > 0) return invalid("null kept pointer");
+    if (!aligned(kept, 4) || !aligned(starts, 4)) return misaligned("kept and starts must be 4-byte aligned");
+    if ((long)cache->batch * cache->n_kv_heads * 16 * 1024 > kMaxThreads)
+        return unsupported("batch * n_kv_heads too large");
+    const PagedLaunch a = launch_of(*cache, nullptr, nullptr, cache->n_kv_heads, llmik_score_options{});
+    const PagedWeights w = weights != nullptr ? weights_of(*weights) : PagedWeights{};
+    return launch_paged_compact(a, w, kept, kept_heads, n, starts, as_stream(stream));
 }
 
 }  // extern "C"

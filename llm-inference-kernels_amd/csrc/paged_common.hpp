@@ -197,6 +197,24 @@ inline ScoreOpts score_opts(const PagedLaunch& a) {
     return s;
 }
 
+// Each token's accumulated attention weight, as the kernels see it.
+struct WeightsView {
+    float* w;           // [n_rows, n_kv_heads, max_len], or null
+    const int* rows;    // [batch], or null: row b is sequence b's
+    int n_rows, max_len, n_kv_heads;
+};
+
+inline WeightsView weights_view(const PagedWeights& a, int n_kv_heads) {
+    return {static_cast<float*>(a.weights), a.rows, a.n_rows, a.max_len, n_kv_heads};
+}
+
+// The weights of sequence b, KV head kvh; null where it has no row.
+__device__ __forceinline__ float* weights_of(const WeightsView& v, int b, int kvh) {
+    const int row = v.rows ? v.rows[b] : b;
+    return v.w != nullptr && (uint32_t)row < (uint32_t)v.n_rows
+               ? v.w + ((long)row * v.n_kv_heads + kvh) * v.max_len : nullptr;
+}
+
 // Those of two 16-bit values that are infinities or NaN; zeros in place of the others.
 template <bool BF>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t x) {

@@ -58,6 +58,9 @@ struct PagedDecodeParams {
     float* part_ml;       // [2 * workgroups, chunk_heads, 2]
     uint32_t* counters;   // [workgroups], zero between calls
     int few_steps;        // workgroups that few tiles are spread over, one tile per wave
+    float* scores;        // with SCORES: [batch, n_heads, score_tokens], every key's score (log2), and
+    float* row_ml;        //   [batch, n_heads] (maximum, 1 / sum of 2^(score - maximum))
+    int score_tokens;     // a multiple of 32
 };
 
 // kPieceUnits (llmik_internal.hpp) is a piece's overhead in units of a tile's time: see the shares.
@@ -90,8 +93,9 @@ struct DecodeLds {
     __device__ __forceinline__ float* o(int w) const { return w == 0 ? o0 : w == 1 ? o1 : w == 2 ? o2 : o3; }
 };
 
-// Workgroup wg of n_wg. EXACT: for a cap above kPlainCap (capped_tanh).
-template <bool BF, int D, bool UNI, bool EXACT>
+// Workgroup wg of n_wg. EXACT: for a cap above kPlainCap (capped_tanh). SCORES: the scores
+// and their statistics are stored too (paged_decode_weights.hip).
+template <bool BF, int D, bool UNI, bool EXACT, bool SCORES = false>
 __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_t wg, uint32_t n_wg,
                                              const DecodeLds<D>& lds) {
     using Hf = Half16<BF>;
@@ -353,6 +357,13 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
                         }
                     }
                 }
+                if constexpr (SCORES) {
+                    if (c < nh && t0 < p.score_tokens) {
+                        float* dst = p.scores + ((long)b * p.n_heads + head) * p.score_tokens + tk;
+                        *reinterpret_cast<f32x4*>(dst) = f32x4{sc[0], sc[1], sc[2], sc[3]};
+                        *reinterpret_cast<f32x4*>(dst + 16) = f32x4{sc[4], sc[5], sc[6], sc[7]};
+                    }
+                }
                 float mx = sc[0];
 #pragma unroll
                 for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
@@ -559,6 +570,11 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
                 if (ch == 0) *reinterpret_cast<f32x2*>(p.own_ml + 2 * at) = f32x2{wm, wl};
             } else if (h < nh && grp == 0) {
                 const float inv = wl > 0.0f || wl != wl ? 1.0f / wl : 0.0f;   // a row without keys is zero
+                if constexpr (SCORES) {
+                    if (ch == 0)
+                        *reinterpret_cast<f32x2*>(p.row_ml + 2 * ((long)b * p.n_heads + head0 + h)) =
+                            f32x2{wm, inv * __builtin_amdgcn_exp2f(kPShift)};   // (wl sums 2^kPShift p)
+                }
                 uint16_t* dst = p.out + ((long)b * p.n_heads + head0 + h) * D + ch;
                 uint32_t w2[VW];
 #pragma unroll

@@ -1,5 +1,6 @@
 // Attention of many query rows over a paged cache: prompts (ragged chunks of new
-// tokens, causal by position) and the shared prefix of a decoding batch.
+// tokens, causal by position), the shared prefix of a decoding batch, and drafted trees
+// (ragged rows that see the cached tokens and, of each other, what a mask says).
 //
 // Rows. All query rows that read one KV head's keys form one list: row r of a
 // sequence is query token r / G, head r % G of the KV head's G query heads (for
@@ -63,7 +64,16 @@ struct PagedFlashParams {
     float* part_ml;           //   rows, splits + 1, D] and (m, l), the last one not this kernel's
     const int* prefix_pages;  // the prefix form
     int prefix_len, chunk;
+    // The tree form (paged_tree.hip).
+    const uint64_t* mask;     // [rows, words]: bit j, the sequence's drafted token j is seen
+    int words;
+    const int* positions;     // [rows], or null: a row's slot
+    // Work that is cut by length (find_cut).
+    int observe;              // rows of a sequence that count: its last ones
+    int target, least;
+    uint32_t slots;           // parts that the workspace holds: [slots, n_kv_heads, kPfRows, D] and (m, l)
 };
+enum class Flash { kRagged, kPrefix, kTree };
 
 // A workgroup's 128 rows: row tile `tile` of sequence b, whose `rows` query tokens
 // begin at row row0 of q and at position pos0. (The prefix form: row i is sequence i.)
@@ -182,6 +192,117 @@ __device__ __forceinline__ TileKeys keys_of_tile(const PagedFlashParams& p, cons
     return k;
 }
 
+// A share of a ragged call's work. A sequence has `fixed` tiles of one kind, each with
+// `tiles` of another that are cut into parts: all sequences' into about `target` parts of
+// one length (at least `least` tiles), so that long ones have more parts than short ones.
+// Drafted trees and row statistics: fixed are row tiles, tiles the keys'.
+struct CutItem {
+    int b, row0, rows;    // the sequence, its (recorded) rows in q
+    int ctx;              // position of the first of them: what was cached before
+    int begin, end;       // its keys that some row sees, from a multiple of kPfTile on
+    int fixed, tiles, parts, part_tiles;
+    int tile, part;       // this share: which of the fixed, which part
+    uint32_t slot;        // of the tile's first part among all parts of tiles that are cut; part i: fixed i further
+};
+constexpr int kMaxPosition = 1 << 30;   // positions that are given count as at most this
+
+// The rows and keys of sequence b; row tiles of kPfRows and key tiles of kPfTile.
+__device__ __forceinline__ void cut_sequence(const PagedFlashParams& p, int b, CutItem& s) {
+    const int stop = p.cu[b + 1], len = max(p.c.lens[b], 0);
+    s.b = b;
+    s.row0 = max(p.cu[b], 0);
+    const int all = max(min(stop, p.rows) - s.row0, 0);
+    s.rows = min(all, p.observe);
+    s.row0 += all - s.rows;
+    s.ctx = len - (stop - s.row0);
+    s.end = min(len, p.c.capacity);
+    s.begin = min(oldest_key(p.s, s.ctx), s.end) / kPfTile * kPfTile;   // (no row's position is below ctx)
+    s.tiles = s.rows > 0 ? (s.end - s.begin + kPfTile - 1) / kPfTile : 0;
+    s.fixed = (int)((uint32_t)(s.rows * (int)p.gqa.d + kPfRows - 1) / kPfRows);
+}
+
+// Number `item` of the call's shares, or of the fixed tiles that are cut, false past the
+// last; `total`: how many there are. Every wave counts for itself: lane l holds sequences
+// per * l .. + per - 1.
+enum class Cuts { kParts, kCutTiles };
+template <Cuts OF, typename F>
+__device__ __forceinline__ bool find_cut(const PagedFlashParams& p, uint32_t item, F sequence, CutItem& t,
+                                         uint32_t& total) {
+    const int lane = threadIdx.x & 63;
+    const int per = (p.c.batch + 63) / 64;
+    const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+    uint32_t mine = 0;
+    CutItem own{};   // the lane's last sequence: its only one where per is 1
+    for (int b = b0; b < b1; ++b) {
+        sequence(b, own);
+        mine += (uint32_t)own.tiles * (uint32_t)own.fixed;
+    }
+    const uint32_t units = lane_u32(wave_scan(mine), 63);
+    const int length = max((int)((units + (uint32_t)p.target - 1) / (uint32_t)p.target), p.least);
+    auto cut = [&](CutItem& s) {
+        s.parts = max((s.tiles + length - 1) / length, 1);
+        s.part_tiles = max((s.tiles + s.parts - 1) / s.parts, 1);   // even ones
+        s.parts = max((s.tiles + s.part_tiles - 1) / s.part_tiles, 1);
+    };
+    auto items_of = [](const CutItem& s) {
+        return (uint32_t)s.fixed * (OF == Cuts::kParts ? (uint32_t)s.parts : s.parts > 1 ? 1u : 0u);
+    };
+    uint32_t items = 0, slots = 0;
+    for (int b = b0; b < b1; ++b) {
+        if (per > 1) sequence(b, own);
+        cut(own);
+        items += items_of(own);
+        slots += own.parts > 1 ? (uint32_t)(own.fixed * own.parts) : 0u;
+    }
+    const uint32_t incl = wave_scan(items), upto = wave_scan(slots);
+    total = lane_u32(incl, 63);
+    if (item >= total) return false;
+    const int at = __ffsll((unsigned long long)__ballot(incl > item)) - 1;
+    uint32_t first = lane_u32(incl - items, at), slot = lane_u32(upto - slots, at);
+    if (per == 1) {
+        t = own;
+        t.b = at;
+    } else {
+        for (int b = at * per;; ++b) {   // ends: the lane's sequences hold the item
+            sequence(b, t);
+            cut(t);
+            const uint32_t n = items_of(t);
+            if (item - first < n || b + 1 >= min(at * per + per, p.c.batch)) break;
+            first += n;
+            slot += t.parts > 1 ? (uint32_t)(t.fixed * t.parts) : 0u;
+        }
+    }
+    const int from = per == 1 ? at : 0;   // (every lane has the same where per > 1)
+    t.b = __builtin_amdgcn_readfirstlane(t.b);
+    t.row0 = __builtin_amdgcn_readlane(t.row0, from);
+    t.rows = __builtin_amdgcn_readlane(t.rows, from);
+    t.ctx = __builtin_amdgcn_readlane(t.ctx, from);
+    t.begin = __builtin_amdgcn_readlane(t.begin, from);
+    t.end = __builtin_amdgcn_readlane(t.end, from);
+    t.fixed = __builtin_amdgcn_readlane(t.fixed, from);
+    t.tiles = __builtin_amdgcn_readlane(t.tiles, from);
+    t.parts = __builtin_amdgcn_readlane(t.parts, from);
+    t.part_tiles = __builtin_amdgcn_readlane(t.part_tiles, from);
+    const uint32_t r = item - first;
+    t.part = __builtin_amdgcn_readfirstlane(OF == Cuts::kParts ? (int)(r / (uint32_t)t.fixed) : 0);
+    t.tile = __builtin_amdgcn_readfirstlane((int)r - t.part * t.fixed);
+    t.slot = (uint32_t)__builtin_amdgcn_readfirstlane((int)slot + t.tile);
+    return true;
+}
+template <Cuts OF>
+__device__ __forceinline__ bool find_row_part(const PagedFlashParams& p, uint32_t item, CutItem& t) {
+    uint32_t total;
+    return find_cut<OF>(p, item, [&](int b, CutItem& s) { cut_sequence(p, b, s); }, t, total);
+}
+__device__ __forceinline__ uint32_t part_slot(const CutItem& t, int part) {
+    return t.slot + (uint32_t)(part * t.fixed);
+}
+
+// Where a row of a row tile lies in part `part` of its KV head's sums.
+__device__ __forceinline__ long part_row(const PagedFlashParams& p, const CutItem& t, int part, int kvh, int row) {
+    return ((long)part_slot(t, part) * p.c.n_kv_heads + kvh) * kPfRows + row;
+}
+
 // What a workgroup keeps in LDS: two tiles of K and of V. (Separate arrays: the
 // compiler then knows that a tile's copies and the other's reads are apart.)
 template <int D>
@@ -196,10 +317,11 @@ struct FlashLds {
 // own, as its instructions beside the others cost all calls: us, 8192 tokens 565, 583
 // with it, 2048 tokens 52.9, 55.5. Four chunks over up to 6000 tokens with a cap of 50
 // 167, of 1000 202).
-template <bool BF, int D, bool PREFIX, bool EXACT>
+template <bool BF, int D, Flash MODE, bool EXACT>
 __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t wg, uint32_t n_wg,
                                             const FlashLds<D>& lds) {
     using Hf = Half16<BF>;
+    constexpr bool PREFIX = MODE == Flash::kPrefix, TREE = MODE == Flash::kTree;
     constexpr int KS = D / 16, CB = D / 32;
     constexpr int CPR = D / 8;                    // 16-byte chunks of a row
     constexpr int kRowBytes = D * 2;
@@ -219,13 +341,15 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const int G = (int)p.gqa.d;
 
     // ---- the workgroup's rows ----
-    RowTile ft{};
+    std::conditional_t<TREE, CutItem, RowTile> ft{};
     if constexpr (PREFIX) {
         ft.tile = (int)item;
         ft.rows = p.c.batch;
     } else {
         const int used = p.cu[p.c.batch];
-        const bool found = find_tile(p, item, ft);
+        bool found;
+        if constexpr (TREE) found = find_row_part<Cuts::kParts>(p, item, ft);
+        else found = find_tile(p, item, ft);
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
         const long chunks = (long)p.n_heads * CPR;
         const long at0 = (long)wg * kPfThreads + tid, step = (long)n_wg * kPfThreads;
@@ -240,7 +364,33 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const int qi = (int)p.gqa.div((uint32_t)r);
     const int head = kvh * G + (r - qi * G);
     const long q_row = (PREFIX ? (long)qi : (long)ft.row0 + qi) * p.n_heads + head;
-    const int pos = PREFIX ? max(p.c.lens[qi], 0) - 1 : ft.pos0 + qi;
+    // The tree form: where drafted token j of the sequence stands (row qi is token qi).
+    [[maybe_unused]] auto tree_pos = [&](int j) {
+        if constexpr (TREE) {
+            j = min(j, ft.rows - 1);
+            const int at = p.positions != nullptr ? p.positions[ft.row0 + j] : ft.ctx + j;
+            return min(max(at, max(ft.ctx, 0)), kMaxPosition);
+        }
+        return 0;
+    };
+    // The 64 tokens from t0 on that query token j sees (the window apart): those cached, and by its mask
+    // those drafted. A query token in front of the cache's first slot does not exist and sees none.
+    [[maybe_unused]] auto tree_seen = [&](int j, int t0) -> uint64_t {
+        if constexpr (TREE) {
+            const uint64_t* row = p.mask + ((long)ft.row0 + j) * p.words;
+            auto word = [&](int w) -> uint64_t { return (uint32_t)w < (uint32_t)p.words ? row[w] : 0ull; };
+            const int j0 = t0 - ft.ctx;
+            if (ft.ctx + j < 0) return 0ull;
+            if (j0 <= -64) return ~0ull;
+            if (j0 < 0) return word(0) << -j0 | ((1ull << -j0) - 1ull);
+            const int w = j0 >> 6, s = j0 & 63;
+            return s == 0 ? word(w) : word(w) >> s | word(w + 1) << (64 - s);
+        }
+        return 0ull;
+    };
+    int pos;
+    if constexpr (TREE) pos = tree_pos(qi);
+    else pos = PREFIX ? max(p.c.lens[qi], 0) - 1 : ft.pos0 + qi;
     // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
     auto oldest = [&](int at) { return oldest_key(p.s, at); };
     int begin, end, tiles, parts = 1;
@@ -262,6 +412,23 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         begin = max(split * p.chunk, oldest(wg_lo)) / kPfTile * kPfTile;
         end = min(min(split * p.chunk + p.chunk, p.prefix_len), wg_hi + 1);
         tiles = end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0;
+    } else if constexpr (TREE) {
+        pos_lo = pos_hi = wg_lo = wg_hi = pos;
+        if (p.s.window != INT_MAX) {   // (else positions hide nothing)
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
+                pos_hi = max(pos_hi, __shfl_xor(pos_hi, d));
+            }
+            if (lane == 0) s_hi[wave] = live ? pos_hi : 0;
+            __syncthreads();
+            wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+        }
+        parts = ft.parts;
+        if (parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (offsets that decrease)
+        begin = ft.begin + ft.part * ft.part_tiles * kPfTile;
+        end = min(ft.end, begin + ft.part_tiles * kPfTile);
+        tiles = min(ft.part_tiles, ft.tiles - ft.part * ft.part_tiles);
     } else {
         pos_lo = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave, n_rows - 1));
         pos_hi = ft.pos0 + (int)p.gqa.div((uint32_t)min(r_wave + 31, n_rows - 1));
@@ -286,11 +453,21 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     // Tiles that all of the wave's rows see wholly, that some row sees, and that all rows
     // of the workgroup see wholly: [lo, hi).
     const int full_lo = (oldest(pos_hi) - begin + kPfTile - 1) >> kPfTileLog;
-    const int full_hi = (min(end, pos_lo + 1) - begin) >> kPfTileLog;
-    const int seen_lo = (oldest(pos_lo) - begin) >> kPfTileLog;
-    const int seen_hi = live ? ((pos_hi - begin) >> kPfTileLog) + 1 : INT_MIN;
+    int first_own, last_seen = pos_hi;   // from here on a row of the wave does not see all; the last that one sees
+    int seen_lo = (oldest(pos_lo) - begin) >> kPfTileLog;
+    if constexpr (TREE) {
+        first_own = ft.ctx;
+        last_seen = end - 1;
+        seen_lo = min(seen_lo, (ft.ctx - begin) >> kPfTileLog);
+    } else {
+        first_own = pos_lo + 1;
+    }
+    const int full_hi = (min(end, first_own) - begin) >> kPfTileLog;
+    const int seen_hi = live ? ((last_seen - begin) >> kPfTileLog) + 1 : INT_MIN;
     const int wg_full_lo = (oldest(wg_hi) - begin + kPfTile - 1) >> kPfTileLog;
-    const int wg_full_hi = (wg_lo + 1 - begin) >> kPfTileLog;
+    int wg_full_hi;
+    if constexpr (TREE) wg_full_hi = (ft.ctx - begin) >> kPfTileLog;
+    else wg_full_hi = (wg_lo + 1 - begin) >> kPfTileLog;
 
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
     // Every wave looks up all octets, eight tiles at a time: lane l octet l % 8 of tile
@@ -430,15 +607,33 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             for (int e = 0; e < 32; ++e) sc[e] = fmaf(sc[e], by, plus);
             if (p.s.slopes) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
+                for (int e = 0; e < 32; ++e) {
+                    int at = tk + 8 * (e >> 2) + (e & 3);
+                    if constexpr (TREE)
+                        if (at >= ft.ctx) at = tree_pos(at - ft.ctx);
+                    sc[e] = fmaf(-slope, (float)(pos - at), sc[e]);
+                }
             }
         }
         if (gone || i < full_lo || i >= full_hi) {   // wave-uniform
-            const int old = oldest(pos), lim = min(pos + 1, end);
+            const int old = oldest(pos);
+            if constexpr (TREE) {
+                const uint64_t seen = tree_seen(qi, t0) >> (4 * h);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const int tok = tk + 8 * (e >> 2) + (e & 3);
-                if (tok < old || tok >= lim || ((gone >> (e >> 2)) & 1u)) sc[e] = -INFINITY;
+                for (int e = 0; e < 32; ++e) {
+                    const int tok = tk + 8 * (e >> 2) + (e & 3);
+                    const bool hides = tok < ft.ctx ? tok < old
+                                                    : p.s.window != INT_MAX && pos - tree_pos(tok - ft.ctx) >= p.s.window;
+                    if (hides || tok >= end || !((seen >> (8 * (e >> 2) + (e & 3))) & 1ull) || ((gone >> (e >> 2)) & 1u))
+                        sc[e] = -INFINITY;
+                }
+            } else {
+                const int lim = min(pos + 1, end);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int tok = tk + 8 * (e >> 2) + (e & 3);
+                    if (tok < old || tok >= lim || ((gone >> (e >> 2)) & 1u)) sc[e] = -INFINITY;
+                }
             }
         }
         // Exponents (of 2^kPShift p) against the reference m_run, which is moved only
@@ -548,8 +743,9 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     l_run = xor32_sum(l_run);
     // The row's place among the parts.
     auto part_at = [&](int row) {
-        return PREFIX ? ((long)kvh * n_rows + ft.tile * kPfRows + row) * (p.splits + 1) + split
-                      : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + row;
+        if constexpr (TREE) return part_row(p, ft, ft.part, kvh, row);
+        else return PREFIX ? ((long)kvh * n_rows + ft.tile * kPfRows + row) * (p.splits + 1) + split
+                           : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + row;
     };
     const bool as_part = PREFIX || parts > 1;
     // The wave's rows go through LDS, so that whole rows are stored, 16 bytes a lane: from
@@ -616,8 +812,15 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         const int r1 = r_wave + rr, qi1 = (int)p.gqa.div((uint32_t)r1);
         const int head1 = kvh * G + (r1 - qi1 * G);
         const long q_row1 = (PREFIX ? (long)qi1 : (long)ft.row0 + qi1) * p.n_heads + head1;
-        const int pos1 = PREFIX ? max(p.c.lens[qi1], 0) - 1 : ft.pos0 + qi1;
-        const int old = oldest(pos1), lim = min(pos1 + 1, end);
+        int pos1, lim;
+        if constexpr (TREE) {
+            pos1 = tree_pos(qi1);
+            lim = end;
+        } else {
+            pos1 = PREFIX ? max(p.c.lens[qi1], 0) - 1 : ft.pos0 + qi1;
+            lim = min(pos1 + 1, end);
+        }
+        const int old = oldest(pos1);
         const float slope1 = p.s.slopes ? p.s.slopes[head1] * kLog2eF : 0.0f;
         float m = kNoMax, l = 0.0f, acc[kCh];
 #pragma unroll
@@ -625,7 +828,14 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         for (int k0 = begin; k0 < lim; k0 += 64) {
             const int t = k0 + lane;
             long at = octet_offset<D>(p.c, table_row, kvh, t & ~7, end);
-            const bool ok = t >= old && t < lim && at >= 0;
+            bool ok = t >= old && t < lim && at >= 0;
+            int at_pos = t;
+            if constexpr (TREE) {
+                const bool drafted = t >= ft.ctx;
+                if (drafted) at_pos = tree_pos(t - ft.ctx);
+                ok = t < lim && at >= 0 && (drafted ? pos1 - at_pos < p.s.window : t >= old) &&
+                     ((tree_seen(qi1, k0) >> lane) & 1ull);
+            }
             at = ok ? at + (t & 7) * D : 0L;
             float dot = 0.0f;
             for (int d8 = 0; d8 < D; d8 += 8) {
@@ -639,7 +849,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             }
             float s1 = EXACT ? capped_tanh(dot, p.s) * p.s.cap_log2
                              : p.s.cap_in != 0.0f ? capped(dot, p.s.cap_in, p.s.cap_log2) : dot * p.s.scale_log2;
-            if (p.s.slopes) s1 = fmaf(-slope1, (float)(pos1 - t), s1);
+            if (p.s.slopes) s1 = fmaf(-slope1, (float)(pos1 - at_pos), s1);
             s1 = ok ? s1 : -INFINITY;
             float top = s1;
 #pragma unroll

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_prefix_kernel(PagedFlashP
     __shared__ uint32_t s_flag;
     __shared__ float s_m[kPdWaves][16], s_l[kPdWaves][16];
     if (blockIdx.x < flash_wgs)
-        paged_flash<BF, D, true, EXACT>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_flag});
+        paged_flash<BF, D, Flash::kPrefix, EXACT>(f, blockIdx.x, flash_wgs, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_flag});
     else
         paged_decode<BF, D, UNI, EXACT>(d, blockIdx.x - flash_wgs, gridDim.x - flash_wgs,
                                  {reinterpret_cast<float*>(s_k0), reinterpret_cast<float*>(s_k1),

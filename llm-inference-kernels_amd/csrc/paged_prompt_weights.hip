@@ -1,0 +1,538 @@
+// The attention weight that a prompt's rows give each token:
+//   weights[row(b), kvh, t] += sum over the sequence's last `observe` new rows i and
+//                              the KV head's G query heads of softmax_t(s(i, t)).
+// A softmax's weights are known once its row's maximum and sum are, so the scores are
+// computed twice, by two kernels that keep one operand in registers and stream the
+// other through LDS:
+//   statistics: 128 rows (32 per wave) over the keys in tiles of 64. S^T = K Q^T gives
+//     a lane one row's scores, so its maximum and sum stay in the lane.
+//   sums: 128 keys (32 per wave) over the rows in tiles of 64. S = Q K^T gives a lane
+//     one key's scores, so its sum of 2^(s - m) / l stays in the lane.
+// Both cut their streamed axis where there are few tiles of the other (find_cut). The
+// statistics of a cut row tile are joined by the last of its workgroups to arrive; the
+// sums of a cut key tile are added in order by a third kernel. Nothing depends on timing.
+#include "paged_flash.hpp"
+
+namespace llmik {
+
+constexpr int kPwThreads = 256;
+constexpr int kPwKeys = 128;     // of a workgroup of the sums
+constexpr int kPwTile = 64;      // rows or keys of a streamed tile
+
+struct PromptWeightsParams {
+    PagedFlashParams f;          // target, least and slots: the statistics' cuts
+    f32x2* stats;                // [rows, n_heads]: (maximum, 1 / sum)
+    uint32_t* counters;          // [slots, n_kv_heads], zero between calls
+    WeightsView w;
+    float* part_sum;             // [sum_slots, n_kv_heads, kPwKeys]
+    int sum_target, sum_least;
+    uint32_t sum_slots;
+};
+
+namespace {
+
+// How scores become exponents (see paged_flash): sc * mult + add, after `score`.
+template <bool EXACT>
+struct ScoreForm {
+    bool cap, modified;
+    float mult, add;
+    __device__ __forceinline__ explicit ScoreForm(const ScoreOpts& s) {
+        cap = s.cap_in != 0.0f;
+        modified = s.slopes != nullptr || (!cap && s.scale_log2 <= 0.0f);
+        mult = modified ? 1.0f : EXACT ? s.cap_log2 : cap ? 2.0f * s.cap_log2 : s.scale_log2;
+        add = cap && !modified && !EXACT ? s.cap_log2 : 0.0f;
+    }
+    // N scores as they come from the products; bias(e): the slope times the distance of score e.
+    template <int N, typename B>
+    __device__ __forceinline__ void apply(const ScoreOpts& s, float (&sc)[N], B bias) const {
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sc[e] = capped_tanh(sc[e], s);
+        } else if (cap) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sc[e] = capped_part(sc[e], s.cap_in);
+        }
+        if (modified) {
+            const float by = EXACT ? s.cap_log2 : cap ? 2.0f * s.cap_log2 : s.scale_log2;
+            const float plus = cap && !EXACT ? s.cap_log2 : 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sc[e] = fmaf(sc[e], by, plus);
+            if (s.slopes) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) sc[e] -= bias(e);
+            }
+        }
+    }
+};
+
+// 16-byte chunk slots of a tile's row in LDS are permuted by the row's number.
+template <int D>
+__device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : row & 7; }
+
+}  // namespace
+
+template <bool BF, int D, bool EXACT>
+__device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t* s_k0, uint8_t* s_k1,
+                                          uint32_t& s_last) {
+    using Hf = Half16<BF>;
+    constexpr int KS = D / 16, CPR = D / 8, kRowBytes = 2 * D;
+    constexpr int kCopies = 16 * CPR / 64, kRowsPerCopy = 64 / CPR;
+    const PagedFlashParams& p = pw.f;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, h = lane >> 5, n = lane & 31;
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), G = (int)p.gqa.d;
+    CutItem ft{};
+    if (!find_row_part<Cuts::kParts>(p, blockIdx.x / (uint32_t)p.c.n_kv_heads, ft)) return;
+    if (ft.parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (offsets that decrease)
+
+    const int n_rows = ft.rows * G;
+    const int r0 = ft.tile * kPfRows, r_wave = r0 + 32 * wave;
+    const bool live = r_wave < n_rows;
+    const int r = min(r_wave + n, n_rows - 1);
+    const int qi = (int)p.gqa.div((uint32_t)r);
+    const int head = kvh * G + (r - qi * G);
+    const long q_row = ((long)ft.row0 + qi) * p.n_heads + head;
+    const int pos = ft.ctx + qi;
+    auto pos_of = [&](int row) { return ft.ctx + (int)p.gqa.div((uint32_t)min(row, n_rows - 1)); };
+    const int pos_lo = __builtin_amdgcn_readfirstlane(pos_of(r_wave));
+    const int pos_hi = __builtin_amdgcn_readfirstlane(pos_of(r_wave + 31));
+    const int wg_lo = __builtin_amdgcn_readfirstlane(pos_of(r0));
+    const int wg_hi = __builtin_amdgcn_readfirstlane(pos_of(r0 + kPfRows - 1));
+    auto oldest = [&](int at) { return oldest_key(p.s, at); };
+    // The part's keys that some row sees.
+    const int part0 = ft.begin + ft.part * ft.part_tiles * kPwTile;
+    const int begin = max(part0, oldest(wg_lo) / kPwTile * kPwTile);
+    const int end = min(min(ft.end, wg_hi + 1), part0 + ft.part_tiles * kPwTile);
+    const int tiles = end > begin ? (end - begin + kPwTile - 1) / kPwTile : 0;
+    const int full_lo = (oldest(pos_hi) - begin + kPwTile - 1) >> 6;
+    const int full_hi = (min(end, pos_lo + 1) - begin) >> 6;
+    const int seen_lo = (oldest(pos_lo) - begin) >> 6;
+    const int seen_hi = live ? ((pos_hi - begin) >> 6) + 1 : INT_MIN;
+
+    // ---- copies, as paged_flash's: wave w brings tokens 16 w .. + 15 of every tile ----
+    const int* const table_row = p.c.table + (long)ft.b * p.c.max_pages;
+    auto token_of = [&](int i0) { return begin + kPwTile * (i0 + (lane >> 3)) + 8 * (lane & 7); };
+    auto look_up = [&](int i0) { return octet_offset<D>(p.c, table_row, kvh, token_of(i0), end); };
+    int at_lo = 0, at_hi = 0, at_bytes = 0;
+    uint64_t batch_gone = 0;
+    auto adopt = [&](long off, int i0) {
+        const bool gone = off < 0;
+        const long at = gone ? 0L : 2 * off;
+        at_lo = (int)(uint32_t)at;
+        at_hi = (int)(at >> 32);
+        at_bytes = gone ? 0 : min(max(end - token_of(i0), 0), 8) * kRowBytes;
+        batch_gone = __ballot(gone);
+    };
+    long off_next = -1;
+    u32x4 qb[KS];
+    if (tiles > 0) adopt(look_up(0), 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qb[ks] = load16(p.q + q_row * D + 16 * ks + 8 * h);
+    const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
+    if (tiles > 8) off_next = look_up(8);
+    const int crow = lane / CPR, cslot = lane % CPR;
+    uint32_t gone_next = 0;
+    auto copy_tile = [&](uint8_t* dst, int i) {   // (where there is no tile i nothing is read)
+        if ((i & 7) == 0 && i) {
+            adopt(off_next, i);
+            off_next = i + 8 < tiles ? look_up(i + 8) : -1L;
+        }
+        const int l0 = 8 * (i & 7);
+        gone_next = (uint32_t)(batch_gone >> l0) & 255u;
+        auto octet = [&](int l) {
+            const long at = ((long)__builtin_amdgcn_readlane(at_hi, l) << 32) |
+                            (uint32_t)__builtin_amdgcn_readlane(at_lo, l);
+            return make_buffer_rsrc(reinterpret_cast<const uint8_t*>(p.c.k) + at,
+                                    (uint32_t)__builtin_amdgcn_readlane(at_bytes, l));
+        };
+        const __amdgpu_buffer_rsrc_t rk0 = octet(l0 + 2 * wave), rk1 = octet(l0 + 2 * wave + 1);
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            const int row = kRowsPerCopy * c + crow, trow = 16 * wave + row;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                (kRowsPerCopy * c) / 8 ? rk1 : rk0,
+                (__attribute__((address_space(3))) void*)(dst + (16 * wave + kRowsPerCopy * c) * kRowBytes), 16,
+                (row & 7) * kRowBytes + 16 * (cslot ^ swizzle<D>(trow)), 0, 0, 0);
+        }
+    };
+
+    const ScoreForm<EXACT> form(p.s);
+    float m_run = kNoMax, l_run = 0.0f;   // of row n, this lane's tokens
+    const uint32_t k_row = (uint32_t)(n * kRowBytes);
+    const uint32_t k_sw = (uint32_t)((h ^ swizzle<D>(n)) * 16);
+    auto compute = [&](const uint8_t* sk, int i, uint32_t gone) {
+        const int t0 = begin + kPwTile * i, tk = t0 + 4 * h;
+        float sc[32];
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                acc = Hf::mfma32(*reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks))),
+                                 qb[ks], acc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[16 * blk + e] = acc[e];
+        }
+        form.apply(p.s, sc, [&](int e) { return slope * (float)(pos - (tk + 8 * (e >> 2) + (e & 3))); });
+        if (gone || i < full_lo || i >= full_hi) {   // wave-uniform
+            const int old = oldest(pos), lim = min(pos + 1, end);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const int tok = tk + 8 * (e >> 2) + (e & 3);
+                if (tok < old || tok >= lim || ((gone >> (e >> 2)) & 1u)) sc[e] = -INFINITY;
+            }
+        }
+        float top = sc[0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e]);
+        const float m_new = fmaxf(m_run, fmaf(top, form.mult, form.add));
+        l_run *= __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        const float by = form.add - m_new;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum[e & 3] += __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by));
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    auto turn = [&](uint8_t* cur, uint8_t* far, int i) {
+        __builtin_amdgcn_s_waitcnt(0);
+        asm volatile("s_barrier" ::: "memory");
+        const uint32_t gone = gone_next;
+        copy_tile(far, i + 1);
+        if (i >= seen_lo && i < seen_hi) compute(cur, i, gone);
+    };
+    if (tiles > 0) copy_tile(s_k0, 0);
+    for (int i = 0; i < tiles; i += 2) {
+        turn(s_k0, s_k1, i);
+        if (i + 1 < tiles) turn(s_k1, s_k0, i + 1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup
+
+    const float m_row = xor32_max(m_run);
+    const float l_row = xor32_sum(l_run * __builtin_amdgcn_exp2f(m_run - m_row));
+    auto store = [&](long at, float m, float l) {
+        pw.stats[at] = f32x2{m, l > 0.0f || l != l ? 1.0f / l : 0.0f};
+    };
+    const bool mine = h == 0 && r_wave + n < n_rows;
+    if (ft.parts == 1) {
+        if (mine) store(q_row, m_row, l_row);
+        return;
+    }
+    if (mine) {
+        float* to = p.part_ml + 2 * part_row(p, ft, ft.part, kvh, 32 * wave + n);
+        publish_store(to, m_row);
+        publish_store(to + 1, l_row);
+    }
+    publish_wait();
+    __syncthreads();
+    uint32_t* const counter = pw.counters + (long)ft.slot * p.c.n_kv_heads + kvh;
+    if (tid == 0) s_last = arrive_last(counter, (uint32_t)ft.parts) ? 1u : 0u;
+    __syncthreads();
+    if (s_last == 0) return;
+    if (tid == 0) *counter = 0u;   // for the next call
+    const int rj = r0 + tid;
+    if (tid >= kPfRows || rj >= n_rows) return;
+    float m = kNoMax, l = 0.0f;
+    for (int u = 0; u < ft.parts; ++u) {
+        const float* from = p.part_ml + 2 * part_row(p, ft, u, kvh, tid);
+        const float mu = publish_load(from), lu = publish_load(from + 1);
+        const float top = fmaxf(m, mu);
+        l = l * __builtin_amdgcn_exp2f(m - top) + lu * __builtin_amdgcn_exp2f(mu - top);
+        m = top;
+    }
+    const int qj = (int)p.gqa.div((uint32_t)rj);
+    store(((long)ft.row0 + qj) * p.n_heads + kvh * G + (rj - qj * G), m, l);
+}
+
+template <bool BF, int D, bool EXACT>
+__global__ __launch_bounds__(kPwThreads, 3) void paged_row_stats_kernel(PromptWeightsParams pw) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPwTile * 2 * D], s_k1[kPwTile * 2 * D];
+    __shared__ uint32_t s_last;
+    row_stats<BF, D, EXACT>(pw, s_k0, s_k1, s_last);
+}
+
+namespace {
+
+// The sums' shares: fixed are key tiles of kPwKeys, cut the row tiles of kPwTile.
+template <Cuts OF>
+__device__ __forceinline__ bool find_key_part(const PromptWeightsParams& pw, uint32_t item, CutItem& t,
+                                              uint32_t& total) {
+    PagedFlashParams p = pw.f;
+    p.target = pw.sum_target;
+    p.least = pw.sum_least;
+    return find_cut<OF>(p, item, [&](int b, CutItem& s) {
+        cut_sequence(p, b, s);
+        s.fixed = s.rows > 0 ? (s.end - s.begin + kPwKeys - 1) / kPwKeys : 0;
+        s.tiles = (int)((uint32_t)(s.rows * (int)p.gqa.d + kPwTile - 1) / kPwTile);
+    }, t, total);
+}
+
+}  // namespace
+
+// The shares are taken by the workgroups in turn: the host does not know the lengths.
+template <bool BF, int D, bool EXACT>
+__global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWeightsParams pw) {
+    using Hf = Half16<BF>;
+    constexpr int KS = D / 16, CPR = D / 8, kRowBytes = 2 * D;
+    constexpr int kCopies = 16 * CPR / 64, kRowsPerCopy = 64 / CPR;
+    __shared__ __attribute__((aligned(16))) uint8_t s_q0[kPwTile * kRowBytes], s_q1[kPwTile * kRowBytes];
+    __shared__ __attribute__((aligned(16))) float s_by[2][kPwTile], s_inv[2][kPwTile], s_slope[2][kPwTile];
+    __shared__ __attribute__((aligned(16))) int s_pos[2][kPwTile];
+    const PagedFlashParams& p = pw.f;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, h = lane >> 5, n = lane & 31;
+    const int G = (int)p.gqa.d;
+    const ScoreForm<EXACT> form(p.s);
+    const uint32_t q_at = (uint32_t)(n * kRowBytes);
+    const uint32_t q_sw = (uint32_t)((h ^ swizzle<D>(n)) * 16);
+    uint32_t total = 1;
+    for (uint32_t wg = blockIdx.x;; wg += gridDim.x) {
+        const int kvh = (int)(wg % (uint32_t)p.c.n_kv_heads);
+        CutItem t{};
+        if (!find_key_part<Cuts::kParts>(pw, wg / (uint32_t)p.c.n_kv_heads, t, total)) return;
+        if (t.parts > 1 && part_slot(t, t.part) >= pw.sum_slots) continue;   // (offsets that decrease)
+        const int n_rows = t.rows * G;
+        const int key0 = t.begin + kPwKeys * t.tile, key_end = min(t.end, key0 + kPwKeys);
+        // The part's rows that see one of the keys: positions key0 .. key_end - 1 + window - 1.
+        const int qi_lo = max(key0 - t.ctx, 0);
+        const int qi_hi = (int)min((long)t.rows, (long)key_end - 1 + p.s.window - t.ctx);
+        const int part0 = t.part * t.part_tiles * kPwTile;
+        const int r_lo = max((int)min((long)qi_lo * G, (long)n_rows) / kPwTile * kPwTile, part0);
+        const int r_hi = min(max(qi_hi, 0) * G, part0 + t.part_tiles * kPwTile);
+        const int tiles = r_hi > r_lo ? (r_hi - r_lo + kPwTile - 1) / kPwTile : 0;
+
+        // ---- the wave's keys ----
+        const int key_w = key0 + 32 * wave, key = key_w + n;
+        const int* const table_row = p.c.table + (long)t.b * p.c.max_pages;
+        const long off = octet_offset<D>(p.c, table_row, kvh, key & ~7, key_end);
+        const bool key_ok = off >= 0 && key < key_end;
+        u32x4 kb[KS];
+        {
+            const uint16_t* from = p.c.k + (off < 0 ? 0L : off + (key & 7) * D) + 8 * h;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kb[ks] = load16(from + 16 * ks);
+        }
+
+        // ---- rows of a tile: wave w brings 16 w .. + 15; threads 0 .. 63 their numbers ----
+        const uint16_t* const q_seq = p.q + ((long)t.row0 * p.n_heads + kvh * G) * D;
+        const int crow = lane / CPR, cslot = lane % CPR;
+        auto copy_tile = [&](uint8_t* dst, int i) {
+            if (i >= tiles) return;
+            const int r0 = r_lo + kPwTile * i;
+            const int q0 = __builtin_amdgcn_readfirstlane((int)p.gqa.div((uint32_t)r0));
+            const __amdgpu_buffer_rsrc_t rq = make_buffer_rsrc(q_seq + (long)q0 * p.n_heads * D, 0xFFFFFFFFu);
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+                const int trow = 16 * wave + kRowsPerCopy * c + crow;
+                const int r = min(r0 + trow, n_rows - 1);   // rows past the end repeat the last
+                const int qi = (int)p.gqa.div((uint32_t)r);
+                const uint32_t at = (uint32_t)((qi - q0) * p.n_heads + (r - qi * G)) * kRowBytes;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rq, (__attribute__((address_space(3))) void*)(dst + (16 * wave + kRowsPerCopy * c) * kRowBytes), 16,
+                    (int)(at + 16 * (cslot ^ swizzle<D>(trow))), 0, 0, 0);
+            }
+        };
+        f32x2 st = {0.0f, 0.0f};
+        auto load_stats = [&](int i) {
+            const int r = r_lo + kPwTile * i + tid;
+            if (tid < kPwTile && i < tiles) {
+                const int rc = min(r, n_rows - 1), qi = (int)p.gqa.div((uint32_t)rc);
+                st = pw.stats[((long)t.row0 + qi) * p.n_heads + kvh * G + (rc - qi * G)];
+            }
+        };
+        auto put_stats = [&](int i) {
+            if (tid < kPwTile && i < tiles) {
+                const int r = r_lo + kPwTile * i + tid, rc = min(r, n_rows - 1);
+                const int qi = (int)p.gqa.div((uint32_t)rc), at = i & 1;
+                s_by[at][tid] = form.add - st[0];
+                s_inv[at][tid] = r < r_hi ? st[1] : 0.0f;
+                s_pos[at][tid] = r < r_hi ? t.ctx + qi : INT_MIN;   // (sees no key)
+                if (p.s.slopes) s_slope[at][tid] = p.s.slopes[kvh * G + (rc - qi * G)] * kLog2eF;
+            }
+        };
+
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // of key n, this lane's rows
+        auto compute = [&](const uint8_t* sq, int i) {
+            const int r0 = r_lo + kPwTile * i, at = i & 1;
+            const int pos_lo = t.ctx + (int)p.gqa.div((uint32_t)r0);
+            const int pos_hi = t.ctx + (int)p.gqa.div((uint32_t)min(r0 + kPwTile, r_hi) - 1u);
+            if (pos_hi < key_w || key_w >= key_end) return;   // wave-uniform
+            const bool full = r0 + kPwTile <= r_hi && pos_lo >= key_w + 31 && pos_hi - key_w < p.s.window;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                f32x16 acc;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    acc = Hf::mfma32(
+                        *reinterpret_cast<const u32x4*>(sq + q_at + 32 * blk * kRowBytes + (q_sw ^ (32u * ks))), kb[ks],
+                        acc);
+                float sc[16], by[16], inv[16];
+                auto row_of = [&](int e) { return 32 * blk + 8 * (e >> 2) + 4 * h + (e & 3); };
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f32x4 b4 = *reinterpret_cast<const f32x4*>(&s_by[at][row_of(e)]);
+                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(&s_inv[at][row_of(e)]);
+#pragma unroll
+                    for (int e2 = 0; e2 < 4; ++e2) {
+                        by[e + e2] = b4[e2];
+                        inv[e + e2] = i4[e2];
+                    }
+                }
+                form.apply(p.s, sc, [&](int e) {
+                    return s_slope[at][row_of(e)] * (float)(s_pos[at][row_of(e)] - key);
+                });
+                if (full) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sum[e & 3] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by[e])), inv[e], sum[e & 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int pos = s_pos[at][row_of(e)];
+                        const float x = __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by[e]));
+                        if (pos >= key && pos - key < p.s.window) sum[e & 3] = fmaf(x, inv[e], sum[e & 3]);
+                    }
+                }
+            }
+        };
+        auto turn = [&](uint8_t* cur, uint8_t* far, int i) {
+            __builtin_amdgcn_s_waitcnt(0);
+            asm volatile("s_barrier" ::: "memory");
+            put_stats(i + 1);
+            load_stats(i + 2);
+            copy_tile(far, i + 1);
+            compute(cur, i);
+        };
+        load_stats(0);
+        copy_tile(s_q0, 0);
+        put_stats(0);
+        load_stats(1);
+        for (int i = 0; i < tiles; i += 2) {
+            turn(s_q0, s_q1, i);
+            if (i + 1 < tiles) turn(s_q1, s_q0, i + 1);
+        }
+        const float all = xor32_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        if (h == 0) {
+            if (t.parts > 1) {
+                pw.part_sum[((long)part_slot(t, t.part) * p.c.n_kv_heads + kvh) * kPwKeys + 32 * wave + n] = all;
+            } else if (key_ok && key < pw.w.max_len && tiles > 0) {
+                float* const w = weights_of(pw.w, t.b, kvh);
+                if (w != nullptr) w[key] += all;
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();   // the tiles are read before the next share's are copied
+    }
+}
+
+// The parts of the key tiles whose rows were cut, added in order.
+__global__ __launch_bounds__(kPwKeys) void paged_key_sums_join_kernel(PromptWeightsParams pw) {
+    const PagedFlashParams& p = pw.f;
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads);
+    CutItem t{};
+    uint32_t total;
+    if (!find_key_part<Cuts::kCutTiles>(pw, blockIdx.x / (uint32_t)p.c.n_kv_heads, t, total)) return;
+    if (part_slot(t, t.parts - 1) >= pw.sum_slots) return;
+    const int key = t.begin + kPwKeys * t.tile + (int)threadIdx.x;
+    float* const w = weights_of(pw.w, t.b, kvh);
+    if (w == nullptr || key >= min(t.end, pw.w.max_len)) return;
+    const uint32_t pi = p.c.page.div((uint32_t)key);
+    if ((uint32_t)p.c.table[(long)t.b * p.c.max_pages + pi] >= (uint32_t)p.c.n_pages) return;   // no key
+    float sum = 0.0f;
+    for (int u = 0; u < t.parts; ++u)
+        sum += pw.part_sum[((long)part_slot(t, u) * p.c.n_kv_heads + kvh) * kPwKeys + threadIdx.x];
+    w[key] += sum;
+}
+
+// ---------------------------------------------------------------- host
+
+namespace {
+
+constexpr int kStatsLeast = 4;   // key tiles of a part at least
+constexpr int kSumsLeast = 8;    // row tiles of a part at least
+
+struct PromptWeightsPlan {
+    long row_tiles, sum_grid;
+    int target, sum_target;
+    uint32_t slots, sum_slots;
+    size_t off_ml, off_stats, off_sum, bytes;
+};
+
+PromptWeightsPlan plan_prompt_weights(int batch, int rows, int n_heads, int n_kv_heads, int observe, int cus) {
+    PromptWeightsPlan pl{};
+    const long seen = observe > 0 ? std::min((long)rows, (long)batch * observe) : rows;
+    const long all = seen * (n_heads / n_kv_heads);
+    pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min((long)batch, seen));
+    pl.target = std::max(3 * cus / n_kv_heads, 1);
+    pl.slots = 2u * (uint32_t)pl.target;
+    pl.sum_target = std::max(4 * cus / n_kv_heads, 1);
+    pl.sum_slots = all > (long)kSumsLeast * kPwTile ? 2u * (uint32_t)pl.sum_target : 0u;
+    pl.sum_grid = 2L * cus;
+    pl.off_ml = kCounterBytes;
+    pl.off_stats = pl.off_ml + align_up((size_t)pl.slots * n_kv_heads * kPfRows * 2 * sizeof(float), 256);
+    pl.off_sum = pl.off_stats + align_up((size_t)rows * n_heads * 2 * sizeof(float), 256);
+    pl.bytes = pl.off_sum + (size_t)pl.sum_slots * n_kv_heads * kPwKeys * sizeof(float);
+    return pl;
+}
+
+template <bool BF, int D, bool EXACT>
+void launch_prompt(const PromptWeightsParams& pw, const PromptWeightsPlan& pl, hipStream_t stream) {
+    const int hkv = pw.f.c.n_kv_heads;
+    paged_row_stats_kernel<BF, D, EXACT>
+        <<<(unsigned)((pl.row_tiles + pl.target) * hkv), kPwThreads, 0, stream>>>(pw);
+    paged_key_sums_kernel<BF, D, EXACT><<<(unsigned)pl.sum_grid, kPwThreads, 0, stream>>>(pw);
+    if (pl.sum_slots > 0)   // (a tile that is cut has two parts at least)
+        paged_key_sums_join_kernel<<<(unsigned)(pl.sum_target * hkv), kPwKeys, 0, stream>>>(pw);
+}
+
+}  // namespace
+
+size_t paged_prefill_weights_workspace(int batch, int rows, int n_heads, int n_kv_heads, int observe) {
+    return plan_prompt_weights(batch, rows, n_heads, n_kv_heads, observe, device_cu_count()).bytes;
+}
+
+int launch_paged_prefill_weights(const PagedLaunch& a, const PagedWeights& w, int observe, hipStream_t stream) {
+    const PromptWeightsPlan pl =
+        plan_prompt_weights(a.batch, a.rows, a.n_heads, a.n_kv_heads, observe, device_cu_count());
+    if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
+        return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_prefill_weights_workspace_size)");
+    if ((long)pl.slots * a.n_kv_heads > kMaxCounters)
+        return set_error(LLMIK_ERR_UNSUPPORTED, "too many KV heads or compute units for the workspace's counters");
+    PromptWeightsParams pw{};
+    pw.f = flash_params(a);
+    pw.f.splits = 1;
+    pw.f.observe = observe > 0 ? observe : INT_MAX;
+    pw.f.target = pl.target;
+    pw.f.least = kStatsLeast;
+    pw.f.slots = pl.slots;
+    char* ws = static_cast<char*>(a.workspace);
+    pw.counters = reinterpret_cast<uint32_t*>(ws);
+    pw.f.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
+    pw.stats = reinterpret_cast<f32x2*>(ws + pl.off_stats);
+    pw.part_sum = reinterpret_cast<float*>(ws + pl.off_sum);
+    pw.w = weights_view(w, a.n_kv_heads);
+    pw.sum_target = pl.sum_target;
+    pw.sum_least = pl.sum_slots > 0 ? kSumsLeast : INT_MAX;
+    pw.sum_slots = pl.sum_slots;
+    auto go = [&](auto bf, auto exact) {
+        constexpr bool BF = decltype(bf)::value, EXACT = decltype(exact)::value;
+        if (a.head_dim == 128) launch_prompt<BF, 128, EXACT>(pw, pl, stream);
+        else launch_prompt<BF, 64, EXACT>(pw, pl, stream);
+    };
+    using std::false_type;
+    using std::true_type;
+    const bool exact = pw.f.s.cap_x != 0.0f;
+    if (a.bf16) exact ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
+    else exact ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
+    return check_launch();
+}
+
+}  // namespace llmik

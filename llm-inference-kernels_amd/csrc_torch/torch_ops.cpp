@@ -716,6 +716,15 @@ const int* paged_offsets(const Tensor& cu_tokens, const llmik_paged_cache& c, co
     return static_cast<const int*>(ptr(cu_tokens));
 }
 
+const int* paged_positions(const std::optional<Tensor>& positions, int64_t rows, const Tensor& like) {
+    if (!positions.has_value()) return nullptr;
+    TORCH_CHECK(positions->scalar_type() == at::kInt && positions->dim() == 1 && positions->is_contiguous() &&
+                    positions->size(0) == rows, "positions must be a contiguous int32 [rows]");
+    TORCH_CHECK(positions->is_cuda() && positions->device() == like.device(),
+                "all inputs must be CUDA tensors of one device");
+    return static_cast<const int*>(ptr(*positions));
+}
+
 int paged_heads(const Tensor& q, const llmik_paged_cache& c) {
     TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim, "q must be [rows, n_heads, head_dim]");
     TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
@@ -746,7 +755,8 @@ llmik_score_options paged_options(const Tensor& q, double softmax_scale, double 
 
 Tensor rope_paged_append(const Tensor& qkv, const std::optional<Tensor>& cos, const std::optional<Tensor>& sin,
                          const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
-                         const Tensor& seq_lens, const std::optional<Tensor>& cu_tokens) {
+                         const Tensor& seq_lens, const std::optional<Tensor>& cu_tokens,
+                         const std::optional<Tensor>& positions) {
     const llmik_paged_cache c = paged_cache(qkv, "qkv", k_cache, v_cache, page_table, seq_lens);
     TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) % c.head_dim == 0, "qkv must be [rows, heads * head_dim]");
     TORCH_CHECK(qkv.size(0) <= INT_MAX && qkv.size(1) <= INT_MAX, "qkv is too large");
@@ -771,13 +781,14 @@ Tensor rope_paged_append(const Tensor& qkv, const std::optional<Tensor>& cos, co
     }
     const int* cu = cu_tokens.has_value() ? paged_offsets(*cu_tokens, c, qkv) : nullptr;
     TORCH_CHECK(cu != nullptr || rows == c.batch, "without cu_tokens qkv must have one row per sequence");
+    const int* at = paged_positions(positions, rows, qkv);
     const c10::DeviceGuard guard(qkv.device());
     Tensor x = qkv.contiguous();
     Tensor q = at::empty({rows, H, c.head_dim}, qkv.options());
     if (rows == 0) return q;
     if (c.batch == 0) return q.zero_();
-    check(llmik_rope_paged_append(&c, ptr(x), cc.defined() ? ptr(cc) : nullptr, sc.defined() ? ptr(sc) : nullptr,
-                                  table_rows, table_f32, cu, ptr(q), (int)rows, (int)H, stream_of(qkv)));
+    check(llmik_rope_paged_append_at(&c, ptr(x), cc.defined() ? ptr(cc) : nullptr, sc.defined() ? ptr(sc) : nullptr,
+                                     table_rows, table_f32, cu, at, ptr(q), (int)rows, (int)H, stream_of(qkv)));
     return q;
 }
 
@@ -842,6 +853,146 @@ Tensor paged_shared_prefix_attention(const Tensor& q, const Tensor& k_cache, con
     return out;
 }
 
+// ---------------------------------------------- drafted trees, bounded caches
+
+Tensor paged_tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                            const Tensor& seq_lens, const Tensor& cu_tokens, const Tensor& tree_mask,
+                            double softmax_scale, double softcap, const std::optional<Tensor>& slopes, int64_t window,
+                            const std::optional<Tensor>& positions) {
+    paged_numbers(softmax_scale, softcap, window);
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    const int* cu = paged_offsets(cu_tokens, c, q);
+    TORCH_CHECK(tree_mask.scalar_type() == at::kLong && tree_mask.dim() == 2 && tree_mask.is_contiguous() &&
+                    tree_mask.size(0) == q.size(0) && tree_mask.size(1) > 0,
+                "tree_mask must be a contiguous int64 [rows, words] with at least one word per row");
+    TORCH_CHECK(tree_mask.size(1) <= (1 << 24), "tree_mask has too many words per row");
+    TORCH_CHECK(tree_mask.is_cuda() && tree_mask.device() == q.device(),
+                "all inputs must be CUDA tensors of one device");
+    const int* at = paged_positions(positions, q.size(0), q);
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    if (q.size(0) == 0) return out;
+    if (c.batch == 0) return out.zero_();
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_tree_workspace_size(&c, H, (int)q.size(0)));
+    check(llmik_paged_tree_attention(&c, ptr(q), cu, static_cast<const uint64_t*>(ptr(tree_mask)),
+                                     (int)tree_mask.size(1), at, ptr(out), (int)q.size(0), H, &o, ws.ptr, ws.bytes,
+                                     st));
+    return out;
+}
+
+// The weights of a batch's tokens.
+llmik_token_weights token_weights(const Tensor& weights, const std::optional<Tensor>& weight_rows, int64_t batch,
+                                  int64_t n_kv_heads, const Tensor& like) {
+    TORCH_CHECK(weights.scalar_type() == at::kFloat && weights.dim() == 3 && weights.is_contiguous() &&
+                    weights.size(1) == n_kv_heads,
+                "weights must be a contiguous fp32 [rows, n_kv_heads, max_len]");
+    TORCH_CHECK(weights.size(0) <= INT_MAX && weights.size(2) > 0 && weights.size(2) <= (1 << 30),
+                "weights must have 1 .. 2^30 tokens per row");
+    TORCH_CHECK(weights.is_cuda() && weights.device() == like.device(),
+                "all inputs must be CUDA tensors of one device");
+    llmik_token_weights w{static_cast<float*>(ptr(weights)), nullptr, (int)weights.size(0), (int)weights.size(2)};
+    if (weight_rows.has_value()) {
+        TORCH_CHECK(weight_rows->scalar_type() == at::kInt && weight_rows->dim() == 1 &&
+                        weight_rows->is_contiguous() && weight_rows->size(0) == batch,
+                    "weight_rows must be a contiguous int32 [batch]");
+        TORCH_CHECK(weight_rows->is_cuda() && weight_rows->device() == like.device(),
+                    "all inputs must be CUDA tensors of one device");
+        w.rows = static_cast<const int*>(ptr(*weight_rows));
+    } else {
+        TORCH_CHECK(weights.size(0) >= batch, "without weight_rows weights must have a row per sequence");
+    }
+    return w;
+}
+
+Tensor paged_decode_attention_weights(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                      const Tensor& page_table, const Tensor& seq_lens, const Tensor& weights,
+                                      double softmax_scale, double softcap, const std::optional<Tensor>& slopes,
+                                      int64_t window, const std::optional<Tensor>& weight_rows) {
+    paged_numbers(softmax_scale, softcap, window);
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, v_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    TORCH_CHECK(q.size(0) == c.batch, "q must have one row per sequence");
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const llmik_token_weights w = token_weights(weights, weight_rows, c.batch, c.n_kv_heads, q);
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    if (c.batch == 0) return out;
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_decode_weights_workspace_size(&c, H, &w));
+    check(llmik_paged_decode_attention_weights(&c, ptr(q), ptr(out), H, &o, &w, ws.ptr, ws.bytes, st));
+    return out;
+}
+
+Tensor paged_prefill_weights(const Tensor& q, const Tensor& k_cache, const Tensor& page_table, const Tensor& seq_lens,
+                             const Tensor& cu_tokens, const Tensor& weights, double softmax_scale, double softcap,
+                             const std::optional<Tensor>& slopes, int64_t window, int64_t observe,
+                             const std::optional<Tensor>& weight_rows) {
+    paged_numbers(softmax_scale, softcap, window);
+    TORCH_CHECK(observe >= 0 && observe <= INT_MAX, "observe must be >= 0");
+    const llmik_paged_cache c = paged_cache(q, "q", k_cache, k_cache, page_table, seq_lens);
+    const int H = paged_heads(q, c);
+    const int* cu = paged_offsets(cu_tokens, c, q);
+    const llmik_score_options o = paged_options(q, softmax_scale, softcap, slopes, window);
+    const llmik_token_weights w = token_weights(weights, weight_rows, c.batch, c.n_kv_heads, q);
+    if (q.size(0) == 0 || c.batch == 0) return weights;
+    const c10::DeviceGuard guard(q.device());
+    const hipStream_t st = stream_of(q);
+    const CallWorkspace ws =
+        call_workspace(q, st, llmik_paged_prefill_weights_workspace_size(&c, H, (int)q.size(0), (int)observe));
+    check(llmik_paged_prefill_weights(&c, ptr(q), cu, (int)q.size(0), H, &o, (int)observe, &w, ws.ptr, ws.bytes, st));
+    return weights;
+}
+
+std::tuple<Tensor, Tensor> paged_select_tokens(const Tensor& weights, const Tensor& seq_lens, int64_t keep,
+                                               int64_t first, int64_t recent,
+                                               const std::optional<Tensor>& weight_rows) {
+    TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.is_contiguous() &&
+                    seq_lens.size(0) <= INT_MAX, "seq_lens must be a contiguous int32 [batch]");
+    TORCH_CHECK(seq_lens.is_cuda(), "all inputs must be CUDA tensors of one device");
+    const int64_t batch = seq_lens.size(0), hkv = weights.dim() == 3 ? weights.size(1) : 0;
+    const llmik_token_weights w = token_weights(weights, weight_rows, batch, hkv, seq_lens);
+    TORCH_CHECK(hkv > 0 && hkv <= (1 << 16), "weights must have 1 .. 2^16 KV heads");
+    TORCH_CHECK(keep > 0 && keep <= (1 << 30), "keep must be positive and at most 2^30");
+    TORCH_CHECK(first >= 0 && recent >= 0 && first <= keep && recent <= keep - first,
+                "first and recent must be >= 0, together at most keep");
+    const c10::DeviceGuard guard(seq_lens.device());
+    Tensor kept = at::empty({batch, hkv, keep}, seq_lens.options()), lens = at::empty({batch}, seq_lens.options());
+    if (batch == 0) return {kept, lens};
+    check(llmik_paged_select_tokens(&w, static_cast<const int*>(ptr(seq_lens)), (int)batch, (int)hkv, (int)keep,
+                                    (int)first, (int)recent, static_cast<int*>(ptr(kept)),
+                                    static_cast<int*>(ptr(lens)), stream_of(seq_lens)));
+    return {kept, lens};
+}
+
+void paged_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table, const Tensor& seq_lens,
+                   const Tensor& kept, const std::optional<Tensor>& starts, const std::optional<Tensor>& weights,
+                   const std::optional<Tensor>& weight_rows) {
+    const llmik_paged_cache c = paged_cache(k_cache, "k_cache", k_cache, v_cache, page_table, seq_lens);
+    TORCH_CHECK(kept.scalar_type() == at::kInt && kept.is_contiguous() && (kept.dim() == 2 || kept.dim() == 3) &&
+                    kept.size(0) == c.batch && (kept.dim() == 2 || kept.size(1) == c.n_kv_heads),
+                "kept must be a contiguous int32 [batch, n] or [batch, n_kv_heads, n]");
+    const int64_t n = kept.size(-1);
+    TORCH_CHECK(n <= (1 << 30), "kept has too many entries");
+    TORCH_CHECK(kept.is_cuda() && kept.device() == k_cache.device(), "all inputs must be CUDA tensors of one device");
+    const int* first = nullptr;
+    if (starts.has_value()) {
+        TORCH_CHECK(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->is_contiguous() &&
+                        starts->size(0) == c.batch, "starts must be a contiguous int32 [batch]");
+        TORCH_CHECK(starts->is_cuda() && starts->device() == k_cache.device(),
+                    "all inputs must be CUDA tensors of one device");
+        first = static_cast<const int*>(ptr(*starts));
+    }
+    TORCH_CHECK(weights.has_value() || !weight_rows.has_value(), "weight_rows come with weights");
+    llmik_token_weights w{};
+    if (weights.has_value()) w = token_weights(*weights, weight_rows, c.batch, c.n_kv_heads, k_cache);
+    const c10::DeviceGuard guard(k_cache.device());
+    check(llmik_paged_compact(&c, static_cast<const int*>(ptr(kept)), kept.dim() == 3 ? c.n_kv_heads : 1, (int)n,
+                              first, weights.has_value() ? &w : nullptr, stream_of(k_cache)));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
@@ -872,6 +1023,11 @@ PYBIND11_MODULE(_C, m) {
     m.def("paged_decode_attention", &paged_decode_attention);
     m.def("paged_prefill_attention", &paged_prefill_attention);
     m.def("paged_shared_prefix_attention", &paged_shared_prefix_attention);
+    m.def("paged_tree_attention", &paged_tree_attention);
+    m.def("paged_decode_attention_weights", &paged_decode_attention_weights);
+    m.def("paged_prefill_weights", &paged_prefill_weights);
+    m.def("paged_select_tokens", &paged_select_tokens);
+    m.def("paged_compact", &paged_compact);
     m.def("workspaces", &workspaces);
     m.def("token_rows", &token_rows);
 }

@@ -53,6 +53,8 @@ __all__ = [
     "pack_int4_along_k", "quantize_pack_weights_int4", "kivi_append_token_int4", "rope_qkv_append", "add_rmsnorm", "silu_mul_halves",
     "w4a16_gemm_swiglu", "interleave_gate_up", "w4a16_gemm_qkv_rope", "interleave_head_halves",
     "rope_paged_append", "paged_decode_attention", "paged_prefill_attention", "paged_shared_prefix_attention",
+    "paged_tree_attention", "paged_decode_attention_weights", "paged_prefill_weights", "paged_select_tokens",
+    "paged_compact",
     "LIB_PATH",
 ]
 
@@ -453,20 +455,22 @@ def silu_mul_halves(gate_up: torch.Tensor) -> torch.Tensor:
 
 def rope_paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
                       k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
-                      seq_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      seq_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """New tokens' fused q|k|v rows [rows, (n_heads + 2 n_kv_heads) * head_dim]
     into the cache: returns rope(q) [rows, n_heads, head_dim] and writes
     rope(k) and v into the tokens' slots, in one launch. cu_tokens [batch + 1]
     int32 (from 0, non-decreasing): rows cu_tokens[b] .. cu_tokens[b + 1] - 1
     are the last tokens of sequence b, in order; without it row b is the newest
     token of sequence b. cos, sin [positions, head_dim], fp32 or of qkv's
-    dtype, are indexed by position; None, None: no rotation. Rows from
-    cu_tokens[-1] on, and rows of empty sequences, give a zero q and are
+    dtype, are indexed by position, which is the token's slot or, with positions
+    [rows] int32, what that says (a drafted token's depth, a sequence that has
+    lost tokens); None, None: no rotation. Rows from cu_tokens[-1] on, and rows of empty sequences, give a zero q and are
     written nowhere; so are positions past the tables. Two rows that name one
     slot (a page mapped twice) write it in no particular order."""
     _require(_is_device(qkv) and _is_device(k_cache) and _is_device(v_cache) and
              _is_device(page_table) and _is_device(seq_lens), "all inputs must be CUDA tensors")
-    return _C.rope_paged_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_tokens)
+    return _C.rope_paged_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_tokens, positions)
 
 
 def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -517,3 +521,86 @@ def paged_shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     return _C.paged_shared_prefix_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_pages,
                                             int(prefix_len), float(softmax_scale), float(softcap), slopes,
                                             int(window))
+
+
+# ---------------------------------------------- drafted trees, bounded caches
+# weights [rows, n_kv_heads, max_len] fp32: the attention weight that the tokens of
+# a sequence have had, by slot; sequence b's row is weight_rows[b] (int32 on the
+# device; default: b). Rows outside the tensor are not recorded, nor tokens at or
+# behind max_len. Two sequences with one row give it no particular sum.
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                         seq_lens: torch.Tensor, cu_tokens: torch.Tensor, tree_mask: torch.Tensor,
+                         softmax_scale: float, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                         window: int = 0, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted token trees: q, out [rows, n_heads, head_dim], rows as
+    in rope_paged_append. The drafted tokens of sequence b are its last
+    cu_tokens[b + 1] - cu_tokens[b] slots; each sees all tokens cached before
+    them, and of its own sequence's drafted tokens those j whose bit j % 64 is
+    set in word j // 64 of its tree_mask [rows, words] (int64; its own bit and its
+    ancestors'). Score options as in paged_decode_attention; distances go by
+    positions [rows] int32 (a drafted token's depth; at least the number of cached
+    tokens, the slot by default) and, of cached tokens, by slots. A row that sees
+    no token, and rows of no sequence, give zeros. Probabilities are rounded as
+    paged_prefill_attention's."""
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and
+             _is_device(seq_lens) and _is_device(cu_tokens) and _is_device(tree_mask), "all inputs must be CUDA tensors")
+    return _C.paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, cu_tokens, tree_mask,
+                                   float(softmax_scale), float(softcap), slopes, int(window), positions)
+
+
+def paged_decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   page_table: torch.Tensor, seq_lens: torch.Tensor, weights: torch.Tensor,
+                                   softmax_scale: float, softcap: float = 0.0,
+                                   slopes: Optional[torch.Tensor] = None, window: int = 0,
+                                   weight_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode_attention (the same bits) that adds each live key's
+    probabilities, summed over the query heads of its KV head, to `weights` in
+    place. Deterministic; the weights' last bits depend on the lengths of the
+    whole batch, as the output's do."""
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and
+             _is_device(seq_lens) and _is_device(weights), "all inputs must be CUDA tensors")
+    return _C.paged_decode_attention_weights(q, k_cache, v_cache, page_table, seq_lens, weights,
+                                             float(softmax_scale), float(softcap), slopes, int(window), weight_rows)
+
+
+def paged_prefill_weights(q: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                          cu_tokens: torch.Tensor, weights: torch.Tensor, softmax_scale: float, softcap: float = 0.0,
+                          slopes: Optional[torch.Tensor] = None, window: int = 0, observe: int = 0,
+                          weight_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What paged_prefill_attention's rows (q and cu_tokens as there) give each key:
+    adds the probabilities of the last `observe` new rows of every sequence (0: of
+    all), summed over these rows and the query heads of the key's KV head, to
+    `weights` in place, and returns it. Deterministic."""
+    _require(_is_device(q) and _is_device(k_cache) and _is_device(page_table) and _is_device(seq_lens) and
+             _is_device(cu_tokens) and _is_device(weights), "all inputs must be CUDA tensors")
+    return _C.paged_prefill_weights(q, k_cache, page_table, seq_lens, cu_tokens, weights, float(softmax_scale),
+                                    float(softcap), slopes, int(window), int(observe), weight_rows)
+
+
+def paged_select_tokens(weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, first: int = 0, recent: int = 0,
+                        weight_rows: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The tokens that a cache of at most `keep` per sequence keeps, for every KV
+    head: the first `first` slots, the last `recent`, and of the others those of the
+    largest weight (NaN above all, ties to the lowest slot). Returns (kept [batch,
+    n_kv_heads, keep] int32, slots in order, -1 behind; lengths [batch] int32). A
+    sequence of at most `keep` tokens keeps all. Tokens at or behind max_len do not
+    exist; a sequence without a row has weights 0."""
+    _require(_is_device(weights) and _is_device(seq_lens), "all inputs must be CUDA tensors")
+    return _C.paged_select_tokens(weights, seq_lens, int(keep), int(first), int(recent), weight_rows)
+
+
+def paged_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                  kept: torch.Tensor, starts: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                  weight_rows: Optional[torch.Tensor] = None) -> None:
+    """Moves tokens together in the cache, in place: the token in slot kept[b, h, i]
+    (kept [batch, n_kv_heads, n] or, for all heads alike, [batch, n] int32) goes to
+    slot starts[b] + i (starts [batch] int32; default 0). seq_lens are the lengths
+    before. Entries that are negative, at or behind the length, or in front of their
+    new slot move nothing; otherwise the order is free. With `weights` each token's
+    weight moves along, and the weights from the first negative entry's new slot on
+    become 0. Slots behind the moved tokens keep what they hold. A page that is
+    written must be one sequence's own."""
+    _require(_is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and _is_device(seq_lens) and
+             _is_device(kept), "all inputs must be CUDA tensors")
+    _C.paged_compact(k_cache, v_cache, page_table, seq_lens, kept, starts, weights, weight_rows)

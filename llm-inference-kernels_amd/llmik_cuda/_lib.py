@@ -43,6 +43,11 @@ class ScoreOptions(ctypes.Structure):
     _fields_ = [("softmax_scale", _f), ("softcap", _f), ("slopes", _p), ("window", _i)]
 
 
+class TokenWeights(ctypes.Structure):
+    """llmik_token_weights."""
+    _fields_ = [("weights", _p), ("rows", _p), ("n_rows", _i), ("max_len", _i)]
+
+
 _SIGNATURES = {
     "llmik_last_error": (ctypes.c_char_p, []),
     "llmik_abi_version": (_i, []),
@@ -89,6 +94,15 @@ _SIGNATURES = {
     "llmik_paged_prefill_workspace_size": (_sz, [_p, _i, _i]),
     "llmik_paged_prefill_attention": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _sz, _p]),
     "llmik_paged_shared_prefix_attention": (_i, [_p, _p, _p, _i, _p, _i, _i, _p, _p, _sz, _p]),
+    "llmik_rope_paged_append_at": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _p, _i, _i, _p]),
+    "llmik_paged_tree_workspace_size": (_sz, [_p, _i, _i]),
+    "llmik_paged_tree_attention": (_i, [_p, _p, _p, _p, _i, _p, _p, _i, _i, _p, _p, _sz, _p]),
+    "llmik_paged_decode_weights_workspace_size": (_sz, [_p, _i, _p]),
+    "llmik_paged_decode_attention_weights": (_i, [_p, _p, _p, _i, _p, _p, _p, _sz, _p]),
+    "llmik_paged_prefill_weights_workspace_size": (_sz, [_p, _i, _i, _i]),
+    "llmik_paged_prefill_weights": (_i, [_p, _p, _p, _i, _i, _p, _i, _p, _p, _sz, _p]),
+    "llmik_paged_select_tokens": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p]),
+    "llmik_paged_compact": (_i, [_p, _p, _i, _i, _p, _p, _p]),
 }
 
 for _name, (_res, _args) in _SIGNATURES.items():
