@@ -48,6 +48,7 @@ constexpr int kPfTileLog = 6;   // tokens of a tile
 constexpr int kPfTile = 1 << kPfTileLog;
 constexpr float kPLag = 6.0f;     // by so much (log2) may a score pass the exponents' reference
 
+struct CutRecord;
 struct PagedFlashParams {
     const uint16_t* q;
     uint16_t* out;
@@ -68,10 +69,11 @@ struct PagedFlashParams {
     const uint64_t* mask;     // [rows, words]: bit j, the sequence's drafted token j is seen
     int words;
     const int* positions;     // [rows], or null: a row's slot
-    // Work that is cut by length (find_cut).
+    // Work that is cut by length (Cutter).
     int observe;              // rows of a sequence that count: its last ones
     int target, least;
     uint32_t slots;           // parts that the workspace holds: [slots, n_kv_heads, kPfRows, D] and (m, l)
+    CutRecord* records;       // [slots / 2]
 };
 enum class Flash { kRagged, kPrefix, kTree };
 
@@ -203,7 +205,15 @@ struct CutItem {
     int fixed, tiles, parts, part_tiles;
     int tile, part;       // this share: which of the fixed, which part
     uint32_t slot;        // of the tile's first part among all parts of tiles that are cut; part i: fixed i further
+    uint32_t cut;         // the tile's number among those that are cut
 };
+// What a kernel that joins parts knows of a tile that is cut, and of the call how many there are.
+struct CutRecord {
+    int b, row0, rows, tile, fixed, parts;
+    uint32_t slot;
+    int count;
+};
+constexpr int kUncut = 1 << 29;         // a part's tiles at least, where nothing is to be cut
 constexpr int kMaxPosition = 1 << 30;   // positions that are given count as at most this
 
 // The rows and keys of sequence b; row tiles of kPfRows and key tiles of kPfTile.
@@ -221,86 +231,139 @@ __device__ __forceinline__ void cut_sequence(const PagedFlashParams& p, int b, C
     s.fixed = (int)((uint32_t)(s.rows * (int)p.gqa.d + kPfRows - 1) / kPfRows);
 }
 
-// Number `item` of the call's shares, or of the fixed tiles that are cut, false past the
-// last; `total`: how many there are. Every wave counts for itself: lane l holds sequences
-// per * l .. + per - 1.
-enum class Cuts { kParts, kCutTiles };
-template <Cuts OF, typename F>
-__device__ __forceinline__ bool find_cut(const PagedFlashParams& p, uint32_t item, F sequence, CutItem& t,
-                                         uint32_t& total) {
-    const int lane = threadIdx.x & 63;
-    const int per = (p.c.batch + 63) / 64;
-    const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
-    uint32_t mine = 0;
-    CutItem own{};   // the lane's last sequence: its only one where per is 1
-    for (int b = b0; b < b1; ++b) {
-        sequence(b, own);
-        mine += (uint32_t)own.tiles * (uint32_t)own.fixed;
+// n / d, rounded up, for n + d < 2^31 and d > 0. The quotient of floats is off by at most n 2^-21 / d + 1, so
+// its remainder is below 2^11 + 2 d, and that one's quotient off by one at most.
+__device__ __forceinline__ uint32_t quick_ceil(uint32_t n, uint32_t d) {
+    const uint32_t x = n + d - 1;
+    const float rd = __builtin_amdgcn_rcpf((float)d);
+    uint32_t q = (uint32_t)((float)x * rd);
+    int r = (int)(x - q * d);
+    const int more = (int)floorf((float)r * rd);
+    q += (uint32_t)more;
+    r -= more * (int)d;
+    return q + (r >= (int)d ? 1u : 0u) - (r < 0 ? 1u : 0u);
+}
+
+// The shares of a call. Every wave counts for itself: lane l holds sequences per * l ..
+// per * l + per - 1, counted once for all shares that the wave looks for.
+template <typename F>
+struct Cutter {
+    const PagedFlashParams& p;
+    F sequence;              // (b, CutItem&): its rows, keys, fixed and tiles
+    CutItem own{};           // the lane's last sequence: its only one where per is 1
+    int per;
+    uint32_t length, items = 0, slots = 0, some = 0, incl, upto, numbered;   // of the lane; running totals
+    uint32_t shares, cuts;   // of the call; cuts: fixed tiles that are cut
+
+    __device__ __forceinline__ uint32_t parts_of_length(int tiles) const {
+        return max(quick_ceil((uint32_t)tiles, length), 1u);
     }
-    const uint32_t units = lane_u32(wave_scan(mine), 63);
-    const int length = max((int)((units + (uint32_t)p.target - 1) / (uint32_t)p.target), p.least);
-    auto cut = [&](CutItem& s) {
-        s.parts = max((s.tiles + length - 1) / length, 1);
-        s.part_tiles = max((s.tiles + s.parts - 1) / s.parts, 1);   // even ones
-        s.parts = max((s.tiles + s.part_tiles - 1) / s.part_tiles, 1);
-    };
-    auto items_of = [](const CutItem& s) {
-        return (uint32_t)s.fixed * (OF == Cuts::kParts ? (uint32_t)s.parts : s.parts > 1 ? 1u : 0u);
-    };
-    uint32_t items = 0, slots = 0;
-    for (int b = b0; b < b1; ++b) {
-        if (per > 1) sequence(b, own);
-        cut(own);
-        items += items_of(own);
-        slots += own.parts > 1 ? (uint32_t)(own.fixed * own.parts) : 0u;
+    __device__ __forceinline__ void cut(CutItem& s) const {
+        s.parts = (int)parts_of_length(s.tiles);
+        s.part_tiles = (int)max(quick_ceil((uint32_t)s.tiles, (uint32_t)s.parts), 1u);   // even ones
+        s.parts = (int)max(quick_ceil((uint32_t)s.tiles, (uint32_t)s.part_tiles), 1u);
     }
-    const uint32_t incl = wave_scan(items), upto = wave_scan(slots);
-    total = lane_u32(incl, 63);
-    if (item >= total) return false;
-    const int at = __ffsll((unsigned long long)__ballot(incl > item)) - 1;
-    uint32_t first = lane_u32(incl - items, at), slot = lane_u32(upto - slots, at);
-    if (per == 1) {
+    __device__ __forceinline__ static uint32_t items_of(const CutItem& s) {
+        return (uint32_t)s.fixed * (uint32_t)s.parts;
+    }
+    // About `target` parts, of `least` tiles or more; with `few`, of two or more where they are not more than that.
+    __device__ __forceinline__ Cutter(const PagedFlashParams& p_, int target_, int least, int few, F f)
+        : p(p_), sequence(f) {
+        const int lane = threadIdx.x & 63;
+        per = (p.c.batch + 63) / 64;
+        const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+        const uint32_t target = (uint32_t)target_;
+        uint32_t mine = 0, fixed = 0;
+        for (int b = b0; b < b1; ++b) {
+            sequence(b, own);
+            mine += (uint32_t)own.tiles * (uint32_t)own.fixed;
+            fixed += (uint32_t)own.fixed;
+        }
+        const uint32_t units = lane_u32(wave_scan(mine), 63);
+        length = (uint32_t)least;
+        if (few != 0) length = min(length, max(quick_ceil(units, (uint32_t)few), 2u));
+        length = max(length, quick_ceil(units, target));
+        // Every sequence's last part is short, so there are more than the target: where it can be met, twice
+        // a greater length for as many as there were.
+        if (per == 1 && lane_u32(wave_scan(fixed), 63) <= target) {
+#pragma unroll
+            for (int turn = 0; turn < 2; ++turn) {
+                const uint32_t n = lane_u32(wave_scan((uint32_t)own.fixed * parts_of_length(own.tiles)), 63);
+                if (n > target) length = quick_ceil(length * n, target);
+            }
+        }
+        for (int b = b0; b < b1; ++b) {
+            if (per > 1) sequence(b, own);
+            cut(own);
+            items += items_of(own);
+            slots += own.parts > 1 ? items_of(own) : 0u;
+            some += own.parts > 1 ? (uint32_t)own.fixed : 0u;
+        }
+        incl = wave_scan(items);
+        upto = wave_scan(slots);
+        numbered = wave_scan(some);
+        shares = lane_u32(incl, 63);
+        cuts = lane_u32(numbered, 63);
+    }
+    // Share number `item`, false past the last. The last ones come first: a prompt's last rows see the most keys.
+    __device__ __forceinline__ bool find(uint32_t item, CutItem& t) const {
+        if (item >= shares) return false;
+        item = shares - 1 - item;
+        const int at = __ffsll((unsigned long long)__ballot(incl > item)) - 1;
+        uint32_t first = lane_u32(incl - items, at), slot = lane_u32(upto - slots, at);
+        uint32_t cut_at = lane_u32(numbered - some, at);
         t = own;
         t.b = at;
-    } else {
-        for (int b = at * per;; ++b) {   // ends: the lane's sequences hold the item
-            sequence(b, t);
-            cut(t);
-            const uint32_t n = items_of(t);
-            if (item - first < n || b + 1 >= min(at * per + per, p.c.batch)) break;
-            first += n;
-            slot += t.parts > 1 ? (uint32_t)(t.fixed * t.parts) : 0u;
+        if (per > 1) {
+            for (int b = at * per;; ++b) {   // ends: the lane's sequences hold the item
+                sequence(b, t);
+                cut(t);
+                const uint32_t n = items_of(t);
+                if (item - first < n || b + 1 >= min(at * per + per, p.c.batch)) break;
+                first += n;
+                slot += t.parts > 1 ? n : 0u;
+                cut_at += t.parts > 1 ? (uint32_t)t.fixed : 0u;
+            }
         }
+        const int from = per == 1 ? at : 0;   // (every lane has the same where per > 1)
+        t.b = __builtin_amdgcn_readfirstlane(t.b);
+        t.row0 = __builtin_amdgcn_readlane(t.row0, from);
+        t.rows = __builtin_amdgcn_readlane(t.rows, from);
+        t.ctx = __builtin_amdgcn_readlane(t.ctx, from);
+        t.begin = __builtin_amdgcn_readlane(t.begin, from);
+        t.end = __builtin_amdgcn_readlane(t.end, from);
+        t.fixed = __builtin_amdgcn_readlane(t.fixed, from);
+        t.tiles = __builtin_amdgcn_readlane(t.tiles, from);
+        t.parts = __builtin_amdgcn_readlane(t.parts, from);
+        t.part_tiles = __builtin_amdgcn_readlane(t.part_tiles, from);
+        const uint32_t r = item - first;
+        t.part = __builtin_amdgcn_readfirstlane((int)(quick_ceil(r + 1, (uint32_t)t.fixed) - 1));   // r / fixed
+        t.tile = __builtin_amdgcn_readfirstlane((int)r - t.part * t.fixed);
+        t.slot = (uint32_t)__builtin_amdgcn_readfirstlane((int)slot + t.tile);
+        t.cut = (uint32_t)__builtin_amdgcn_readfirstlane((int)cut_at + t.tile);
+        return true;
     }
-    const int from = per == 1 ? at : 0;   // (every lane has the same where per > 1)
-    t.b = __builtin_amdgcn_readfirstlane(t.b);
-    t.row0 = __builtin_amdgcn_readlane(t.row0, from);
-    t.rows = __builtin_amdgcn_readlane(t.rows, from);
-    t.ctx = __builtin_amdgcn_readlane(t.ctx, from);
-    t.begin = __builtin_amdgcn_readlane(t.begin, from);
-    t.end = __builtin_amdgcn_readlane(t.end, from);
-    t.fixed = __builtin_amdgcn_readlane(t.fixed, from);
-    t.tiles = __builtin_amdgcn_readlane(t.tiles, from);
-    t.parts = __builtin_amdgcn_readlane(t.parts, from);
-    t.part_tiles = __builtin_amdgcn_readlane(t.part_tiles, from);
-    const uint32_t r = item - first;
-    t.part = __builtin_amdgcn_readfirstlane(OF == Cuts::kParts ? (int)(r / (uint32_t)t.fixed) : 0);
-    t.tile = __builtin_amdgcn_readfirstlane((int)r - t.part * t.fixed);
-    t.slot = (uint32_t)__builtin_amdgcn_readfirstlane((int)slot + t.tile);
-    return true;
-}
-template <Cuts OF>
-__device__ __forceinline__ bool find_row_part(const PagedFlashParams& p, uint32_t item, CutItem& t) {
-    uint32_t total;
-    return find_cut<OF>(p, item, [&](int b, CutItem& s) { cut_sequence(p, b, s); }, t, total);
+};
+// Written by the call's first workgroup, and by each cut tile's first part: for the kernel that joins them.
+__device__ __forceinline__ void write_records(CutRecord* to, uint32_t slots, bool first, uint32_t cuts, bool found,
+                                              const CutItem& t) {
+    if (first) to[0].count = (int)min(cuts, slots / 2);   // (a tile that is cut has two parts at least)
+    if (!found || t.parts == 1 || t.part != 0 || t.cut >= slots / 2) return;
+    to[t.cut].b = t.b;
+    to[t.cut].row0 = t.row0;
+    to[t.cut].rows = t.rows;
+    to[t.cut].tile = t.tile;
+    to[t.cut].fixed = t.fixed;
+    to[t.cut].parts = t.slot + (uint32_t)((t.parts - 1) * t.fixed) < slots ? t.parts : 0;   // (0: offsets that decrease)
+    to[t.cut].slot = t.slot;
 }
 __device__ __forceinline__ uint32_t part_slot(const CutItem& t, int part) {
     return t.slot + (uint32_t)(part * t.fixed);
 }
 
 // Where a row of a row tile lies in part `part` of its KV head's sums.
-__device__ __forceinline__ long part_row(const PagedFlashParams& p, const CutItem& t, int part, int kvh, int row) {
-    return ((long)part_slot(t, part) * p.c.n_kv_heads + kvh) * kPfRows + row;
+__device__ __forceinline__ long part_row(const PagedFlashParams& p, uint32_t slot, int kvh, int row) {
+    return ((long)slot * p.c.n_kv_heads + kvh) * kPfRows + row;
 }
 
 // What a workgroup keeps in LDS: two tiles of K and of V. (Separate arrays: the
@@ -348,7 +411,12 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     } else {
         const int used = p.cu[p.c.batch];
         bool found;
-        if constexpr (TREE) found = find_row_part<Cuts::kParts>(p, item, ft);
+        if constexpr (TREE) {
+            auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
+            const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
+            found = cutter.find(item, ft);
+            if (p.slots != 0 && kvh == 0 && tid == 0) write_records(p.records, p.slots, wg == 0, cutter.cuts, found, ft);
+        }
         else found = find_tile(p, item, ft);
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
         const long chunks = (long)p.n_heads * CPR;
@@ -388,9 +456,10 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         }
         return 0ull;
     };
-    int pos;
-    if constexpr (TREE) pos = tree_pos(qi);
-    else pos = PREFIX ? max(p.c.lens[qi], 0) - 1 : ft.pos0 + qi;
+    int pos = 0;
+    if constexpr (TREE) {
+        if (p.s.slopes != nullptr || p.s.window != INT_MAX) pos = tree_pos(qi);   // (a load)
+    } else pos = PREFIX ? max(p.c.lens[qi], 0) - 1 : ft.pos0 + qi;
     // ---- the keys that any of them sees, [begin, end), in 64-token tiles ----
     auto oldest = [&](int at) { return oldest_key(p.s, at); };
     int begin, end, tiles, parts = 1;
@@ -413,8 +482,9 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         end = min(min(split * p.chunk + p.chunk, p.prefix_len), wg_hi + 1);
         tiles = end > begin ? (end - begin + kPfTile - 1) / kPfTile : 0;
     } else if constexpr (TREE) {
-        pos_lo = pos_hi = wg_lo = wg_hi = pos;
+        pos_lo = pos_hi = wg_lo = wg_hi = ft.ctx;
         if (p.s.window != INT_MAX) {   // (else positions hide nothing)
+            pos_lo = pos_hi = pos;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
@@ -585,6 +655,11 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         }
         // value e belongs to token t0 + 4 h + 8 (e / 4) + e % 4
         const int tk = t0 + 4 * h;
+        [[maybe_unused]] int tile_pos = 0;   // the tree form, where distances count: lane l's is token l's position
+        if constexpr (TREE) {
+            if (t0 + kPfTile > ft.ctx && (p.s.slopes != nullptr || p.s.window != INT_MAX))   // wave-uniform
+                tile_pos = t0 + lane < ft.ctx ? t0 + lane : tree_pos(t0 + lane - ft.ctx);
+        }
         if constexpr (EXACT) {
             float top = 0.0f;
 #pragma unroll
@@ -606,29 +681,43 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
 #pragma unroll
             for (int e = 0; e < 32; ++e) sc[e] = fmaf(sc[e], by, plus);
             if (p.s.slopes) {
+                if (TREE && t0 + kPfTile > first_own) {   // wave-uniform
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    int at = tk + 8 * (e >> 2) + (e & 3);
-                    if constexpr (TREE)
-                        if (at >= ft.ctx) at = tree_pos(at - ft.ctx);
-                    sc[e] = fmaf(-slope, (float)(pos - at), sc[e]);
+                    for (int e = 0; e < 32; ++e) {
+                        const int at = 8 * (e >> 2) + (e & 3);
+                        const int a0 = __builtin_amdgcn_readlane(tile_pos, at);
+                        const int a4 = __builtin_amdgcn_readlane(tile_pos, at + 4);
+                        sc[e] = fmaf(-slope, (float)(pos - (h ? a4 : a0)), sc[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        sc[e] = fmaf(-slope, (float)(pos - (tk + 8 * (e >> 2) + (e & 3))), sc[e]);
                 }
             }
         }
         if (gone || i < full_lo || i >= full_hi) {   // wave-uniform
-            const int old = oldest(pos);
             if constexpr (TREE) {
-                const uint64_t seen = tree_seen(qi, t0) >> (4 * h);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int tok = tk + 8 * (e >> 2) + (e & 3);
-                    const bool hides = tok < ft.ctx ? tok < old
-                                                    : p.s.window != INT_MAX && pos - tree_pos(tok - ft.ctx) >= p.s.window;
-                    if (hides || tok >= end || !((seen >> (8 * (e >> 2) + (e & 3))) & 1ull) || ((gone >> (e >> 2)) & 1u))
-                        sc[e] = -INFINITY;
+                // The tile's tokens as bits: those that the row's mask shows, in the window, in front of the
+                // end and of pages that are there.
+                uint64_t seen = tree_seen(qi, t0);
+                if (p.s.window != INT_MAX) {
+                    const int hidden = min(max(min(oldest(pos), ft.ctx) - t0, 0), 64);   // cached ones
+                    seen &= hidden == 64 ? 0ull : ~0ull << hidden;
+#pragma unroll 1
+                    for (int j = max(ft.ctx - t0, 0); j < min(end - t0, kPfTile); ++j)   // drafted ones
+                        if (pos - __builtin_amdgcn_readlane(tile_pos, j) >= p.s.window) seen &= ~(1ull << j);
                 }
+                if (end - t0 < kPfTile) seen &= (1ull << (end - t0)) - 1ull;
+                // (a page's octet as a byte: the bits of `gone` seven places apart, times 255)
+                const uint32_t g_lo = ((gone & 15u) * 0x00204081u & 0x01010101u) * 255u;
+                const uint32_t g_hi = ((gone >> 4) * 0x00204081u & 0x01010101u) * 255u;
+                const uint32_t lo = ((uint32_t)seen & ~g_lo) >> (4 * h), hi = ((uint32_t)(seen >> 32) & ~g_hi) >> (4 * h);
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (!((e < 16 ? lo : hi) & 1u << (8 * (e >> 2 & 3) + (e & 3)))) sc[e] = -INFINITY;
             } else {
-                const int lim = min(pos + 1, end);
+                const int old = oldest(pos), lim = min(pos + 1, end);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     const int tok = tk + 8 * (e >> 2) + (e & 3);
@@ -743,7 +832,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     l_run = xor32_sum(l_run);
     // The row's place among the parts.
     auto part_at = [&](int row) {
-        if constexpr (TREE) return part_row(p, ft, ft.part, kvh, row);
+        if constexpr (TREE) return part_row(p, part_slot(ft, ft.part), kvh, row);
         else return PREFIX ? ((long)kvh * n_rows + ft.tile * kPfRows + row) * (p.splits + 1) + split
                            : (((long)item * p.c.n_kv_heads + kvh) * p.splits + split) * kPfRows + row;
     };

@@ -8,9 +8,9 @@
 //     a lane one row's scores, so its maximum and sum stay in the lane.
 //   sums: 128 keys (32 per wave) over the rows in tiles of 64. S = Q K^T gives a lane
 //     one key's scores, so its sum of 2^(s - m) / l stays in the lane.
-// Both cut their streamed axis where there are few tiles of the other (find_cut). The
-// statistics of a cut row tile are joined by the last of its workgroups to arrive; the
-// sums of a cut key tile are added in order by a third kernel. Nothing depends on timing.
+// Both cut their streamed axis where there are few tiles of the other (Cutter). The parts
+// of a cut row or key tile are joined, in order, by the last of its workgroups to arrive:
+// nothing depends on timing.
 #include "paged_flash.hpp"
 
 namespace llmik {
@@ -22,10 +22,11 @@ constexpr int kPwTile = 64;      // rows or keys of a streamed tile
 struct PromptWeightsParams {
     PagedFlashParams f;          // target, least and slots: the statistics' cuts
     f32x2* stats;                // [rows, n_heads]: (maximum, 1 / sum)
-    uint32_t* counters;          // [slots, n_kv_heads], zero between calls
+    uint32_t* counters;          // of the cut tiles [slots / 2, n_kv_heads], zero between calls
+    uint32_t* sum_counters;      // [sum_slots / 2, n_kv_heads]
     WeightsView w;
     float* part_sum;             // [sum_slots, n_kv_heads, kPwKeys]
-    int sum_target, sum_least;
+    int sum_target, sum_least, sum_few;
     uint32_t sum_slots;
 };
 
@@ -72,7 +73,7 @@ __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : r
 }  // namespace
 
 template <bool BF, int D, bool EXACT>
-__device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t* s_k0, uint8_t* s_k1,
+__device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t* s_k0, uint8_t* s_k1, uint8_t* s_k2,
                                           uint32_t& s_last) {
     using Hf = Half16<BF>;
     constexpr int KS = D / 16, CPR = D / 8, kRowBytes = 2 * D;
@@ -82,9 +83,17 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, h = lane >> 5, n = lane & 31;
     const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), G = (int)p.gqa.d;
+    // Of the workgroups that run at once, one per CU and turn, every other turn's order is reversed: a CU's
+    // then have about the same work together as another's.
+    uint32_t item = blockIdx.x / (uint32_t)p.c.n_kv_heads;
+    const uint32_t turn_items = p.per_round / (uint32_t)p.c.n_kv_heads, turn_no = item / max(turn_items, 1u);
+    if (turn_no & 1u && (turn_no + 1) * turn_items <= gridDim.x / (uint32_t)p.c.n_kv_heads)
+        item = (2 * turn_no + 1) * turn_items - 1 - item;
     CutItem ft{};
-    if (!find_row_part<Cuts::kParts>(p, blockIdx.x / (uint32_t)p.c.n_kv_heads, ft)) return;
-    if (ft.parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (offsets that decrease)
+    auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
+    const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
+    if (!cutter.find(item, ft)) return;
+    if (ft.parts > 1 && (part_slot(ft, ft.parts - 1) >= p.slots || ft.cut >= p.slots / 2)) return;   // (offsets that decrease)
 
     const int n_rows = ft.rows * G;
     const int r0 = ft.tile * kPfRows, r_wave = r0 + 32 * wave;
@@ -132,8 +141,8 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
     const float slope = p.s.slopes ? p.s.slopes[head] * kLog2eF : 0.0f;
     if (tiles > 8) off_next = look_up(8);
     const int crow = lane / CPR, cslot = lane % CPR;
-    uint32_t gone_next = 0;
-    auto copy_tile = [&](uint8_t* dst, int i) {   // (where there is no tile i nothing is read)
+    uint32_t gone_next = 0, gone_now = 0;   // of the last tile requested, of the one before
+    auto copy_tile = [&](uint8_t* dst, int i) {   // (where there is no tile i nothing is read, but counted)
         if ((i & 7) == 0 && i) {
             adopt(off_next, i);
             off_next = i + 8 < tiles ? look_up(i + 8) : -1L;
@@ -197,17 +206,28 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
         for (int e = 0; e < 32; ++e) sum[e & 3] += __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by));
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     };
-    auto turn = [&](uint8_t* cur, uint8_t* far, int i) {
-        __builtin_amdgcn_s_waitcnt(0);
+    // Two tiles ahead: a tile's copies are complete once at most the next one's are outstanding (loads
+    // complete in order), and for the whole workgroup behind the barrier, where the buffer of the tile
+    // before is free.
+    auto turn = [&](uint8_t* cur, uint8_t* free, int i) {
+        if constexpr (kCopies == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
-        const uint32_t gone = gone_next;
-        copy_tile(far, i + 1);
+        const uint32_t gone = gone_now;
+        gone_now = gone_next;
+        copy_tile(free, i + 2);
         if (i >= seen_lo && i < seen_hi) compute(cur, i, gone);
     };
-    if (tiles > 0) copy_tile(s_k0, 0);
-    for (int i = 0; i < tiles; i += 2) {
-        turn(s_k0, s_k1, i);
+    static_assert(kCopies == 4 || kCopies == 2, "the wait counts a tile's copies");
+    if (tiles > 0) {
+        copy_tile(s_k0, 0);
+        gone_now = gone_next;
+        copy_tile(s_k1, 1);
+    }
+    for (int i = 0; i < tiles; i += 3) {
+        turn(s_k0, s_k2, i);
         if (i + 1 < tiles) turn(s_k1, s_k0, i + 1);
+        if (i + 2 < tiles) turn(s_k2, s_k1, i + 2);
     }
     __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup
 
@@ -222,13 +242,13 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
         return;
     }
     if (mine) {
-        float* to = p.part_ml + 2 * part_row(p, ft, ft.part, kvh, 32 * wave + n);
-        publish_store(to, m_row);
-        publish_store(to + 1, l_row);
+        float* to = p.part_ml + 2 * part_row(p, part_slot(ft, ft.part), kvh, 32 * wave + n);
+        const uint64_t ml = (uint64_t)__float_as_uint(l_row) << 32 | __float_as_uint(m_row);
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(to), ml, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     publish_wait();
     __syncthreads();
-    uint32_t* const counter = pw.counters + (long)ft.slot * p.c.n_kv_heads + kvh;
+    uint32_t* const counter = pw.counters + (long)ft.cut * p.c.n_kv_heads + kvh;
     if (tid == 0) s_last = arrive_last(counter, (uint32_t)ft.parts) ? 1u : 0u;
     __syncthreads();
     if (s_last == 0) return;
@@ -236,12 +256,22 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
     const int rj = r0 + tid;
     if (tid >= kPfRows || rj >= n_rows) return;
     float m = kNoMax, l = 0.0f;
-    for (int u = 0; u < ft.parts; ++u) {
-        const float* from = p.part_ml + 2 * part_row(p, ft, u, kvh, tid);
-        const float mu = publish_load(from), lu = publish_load(from + 1);
-        const float top = fmaxf(m, mu);
-        l = l * __builtin_amdgcn_exp2f(m - top) + lu * __builtin_amdgcn_exp2f(mu - top);
-        m = top;
+    constexpr int kBatch = 8;   // requested at a time
+    for (int u0 = 0; u0 < ft.parts; u0 += kBatch) {
+        uint64_t ml[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const uint32_t slot = part_slot(ft, min(u0 + u, ft.parts - 1));
+            ml[u] = __hip_atomic_load(reinterpret_cast<uint64_t*>(p.part_ml + 2 * part_row(p, slot, kvh, tid)),
+                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const float mu = __uint_as_float((uint32_t)ml[u]), lu = __uint_as_float((uint32_t)(ml[u] >> 32));
+            const float top = fmaxf(m, mu);
+            if (u0 + u < ft.parts) l = l * __builtin_amdgcn_exp2f(m - top) + lu * __builtin_amdgcn_exp2f(mu - top);
+            m = top;   // (a part that is repeated has no greater maximum)
+        }
     }
     const int qj = (int)p.gqa.div((uint32_t)rj);
     store(((long)ft.row0 + qj) * p.n_heads + kvh * G + (rj - qj * G), m, l);
@@ -250,35 +280,23 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
 template <bool BF, int D, bool EXACT>
 __global__ __launch_bounds__(kPwThreads, 3) void paged_row_stats_kernel(PromptWeightsParams pw) {
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPwTile * 2 * D], s_k1[kPwTile * 2 * D];
+    __shared__ __attribute__((aligned(16))) uint8_t s_k2[kPwTile * 2 * D];
     __shared__ uint32_t s_last;
-    row_stats<BF, D, EXACT>(pw, s_k0, s_k1, s_last);
+    row_stats<BF, D, EXACT>(pw, s_k0, s_k1, s_k2, s_last);
 }
 
-namespace {
-
-// The sums' shares: fixed are key tiles of kPwKeys, cut the row tiles of kPwTile.
-template <Cuts OF>
-__device__ __forceinline__ bool find_key_part(const PromptWeightsParams& pw, uint32_t item, CutItem& t,
-                                              uint32_t& total) {
-    PagedFlashParams p = pw.f;
-    p.target = pw.sum_target;
-    p.least = pw.sum_least;
-    return find_cut<OF>(p, item, [&](int b, CutItem& s) {
-        cut_sequence(p, b, s);
-        s.fixed = s.rows > 0 ? (s.end - s.begin + kPwKeys - 1) / kPwKeys : 0;
-        s.tiles = (int)((uint32_t)(s.rows * (int)p.gqa.d + kPwTile - 1) / kPwTile);
-    }, t, total);
-}
-
-}  // namespace
-
-// The shares are taken by the workgroups in turn: the host does not know the lengths.
+// The shares: fixed are key tiles of kPwKeys, cut the row tiles of kPwTile. The host does not
+// know how many there are, and they differ (a key's rows begin at its own position): the
+// workgroups take one each turn, the last rows' first, every other turn in the reverse order,
+// so that who has many rows has few next. (From a queue in memory: 0.015 us for each of all
+// shares.)
 template <bool BF, int D, bool EXACT>
-__global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWeightsParams pw) {
+__global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWeightsParams pw) {
     using Hf = Half16<BF>;
     constexpr int KS = D / 16, CPR = D / 8, kRowBytes = 2 * D;
     constexpr int kCopies = 16 * CPR / 64, kRowsPerCopy = 64 / CPR;
     __shared__ __attribute__((aligned(16))) uint8_t s_q0[kPwTile * kRowBytes], s_q1[kPwTile * kRowBytes];
+    __shared__ uint32_t s_last;
     __shared__ __attribute__((aligned(16))) float s_by[2][kPwTile], s_inv[2][kPwTile], s_slope[2][kPwTile];
     __shared__ __attribute__((aligned(16))) int s_pos[2][kPwTile];
     const PagedFlashParams& p = pw.f;
@@ -289,12 +307,20 @@ __global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWei
     const ScoreForm<EXACT> form(p.s);
     const uint32_t q_at = (uint32_t)(n * kRowBytes);
     const uint32_t q_sw = (uint32_t)((h ^ swizzle<D>(n)) * 16);
-    uint32_t total = 1;
-    for (uint32_t wg = blockIdx.x;; wg += gridDim.x) {
+    auto sequence = [&](int b, CutItem& s) {
+        cut_sequence(p, b, s);
+        s.fixed = s.rows > 0 ? (s.end - s.begin + kPwKeys - 1) / kPwKeys : 0;
+        s.tiles = (int)((uint32_t)(s.rows * G + kPwTile - 1) / kPwTile);
+    };
+    const Cutter<decltype(sequence)> cutter(p, pw.sum_target, pw.sum_least, pw.sum_few, sequence);
+    for (uint32_t turn_no = 0;; ++turn_no) {
+        const uint32_t wg = turn_no * gridDim.x + (turn_no & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         const int kvh = (int)(wg % (uint32_t)p.c.n_kv_heads);
         CutItem t{};
-        if (!find_key_part<Cuts::kParts>(pw, wg / (uint32_t)p.c.n_kv_heads, t, total)) return;
-        if (t.parts > 1 && part_slot(t, t.part) >= pw.sum_slots) continue;   // (offsets that decrease)
+        const bool found = cutter.find(wg / (uint32_t)p.c.n_kv_heads, t);
+        if (!found) return;
+        // (not: offsets that decrease)
+        const bool fits = t.parts == 1 || (part_slot(t, t.parts - 1) < pw.sum_slots && t.cut < pw.sum_slots / 2);
         const int n_rows = t.rows * G;
         const int key0 = t.begin + kPwKeys * t.tile, key_end = min(t.end, key0 + kPwKeys);
         // The part's rows that see one of the keys: positions key0 .. key_end - 1 + window - 1.
@@ -303,7 +329,7 @@ __global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWei
         const int part0 = t.part * t.part_tiles * kPwTile;
         const int r_lo = max((int)min((long)qi_lo * G, (long)n_rows) / kPwTile * kPwTile, part0);
         const int r_hi = min(max(qi_hi, 0) * G, part0 + t.part_tiles * kPwTile);
-        const int tiles = r_hi > r_lo ? (r_hi - r_lo + kPwTile - 1) / kPwTile : 0;
+        const int tiles = fits && r_hi > r_lo ? (r_hi - r_lo + kPwTile - 1) / kPwTile : 0;
 
         // ---- the wave's keys ----
         const int key_w = key0 + 32 * wave, key = key_w + n;
@@ -315,6 +341,14 @@ __global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWei
             const uint16_t* from = p.c.k + (off < 0 ? 0L : off + (key & 7) * D) + 8 * h;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) kb[ks] = load16(from + 16 * ks);
+        }
+
+        // Its weight so far (read by all of a key tile's parts: the last one adds).
+        float* to = nullptr;
+        float before = 0.0f;
+        if (h == 0 && key_ok && key < pw.w.max_len) {
+            to = weights_of(pw.w, t.b, kvh);
+            if (to != nullptr) before = *(to += key);
         }
 
         // ---- rows of a tile: wave w brings 16 w .. + 15; threads 0 .. 63 their numbers ----
@@ -420,44 +454,50 @@ __global__ __launch_bounds__(kPwThreads, 2) void paged_key_sums_kernel(PromptWei
             if (i + 1 < tiles) turn(s_q1, s_q0, i + 1);
         }
         const float all = xor32_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        if (h == 0) {
-            if (t.parts > 1) {
-                pw.part_sum[((long)part_slot(t, t.part) * p.c.n_kv_heads + kvh) * kPwKeys + 32 * wave + n] = all;
-            } else if (key_ok && key < pw.w.max_len && tiles > 0) {
-                float* const w = weights_of(pw.w, t.b, kvh);
-                if (w != nullptr) w[key] += all;
+        if (t.parts == 1) {
+            if (to != nullptr && tiles > 0) *to = before + all;
+        } else if (fits) {
+            // The last of the key tile's workgroups to arrive adds its parts, in order.
+            auto part_at = [&](int part, int i) {
+                return pw.part_sum + ((long)part_slot(t, part) * p.c.n_kv_heads + kvh) * kPwKeys + i;
+            };
+            if (h == 0) publish_store(part_at(t.part, 32 * wave + n), all);
+            publish_wait();
+            __syncthreads();
+            uint32_t* const counter = pw.sum_counters + (long)t.cut * p.c.n_kv_heads + kvh;
+            if (tid == 0) s_last = arrive_last(counter, (uint32_t)t.parts) ? 1u : 0u;
+            __syncthreads();
+            if (s_last != 0) {
+                if (tid == 0) *counter = 0u;   // for the next call
+                float sum = 0.0f;
+                constexpr int kBatch = 8;   // requested at a time
+                for (int u0 = 0; u0 < t.parts; u0 += kBatch) {
+                    float x[kBatch];
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) x[u] = publish_load(part_at(min(u0 + u, t.parts - 1), 32 * wave + n));
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) sum += u0 + u < t.parts ? x[u] : 0.0f;
+                }
+                if (to != nullptr) *to = before + sum;
             }
         }
-        __builtin_amdgcn_s_waitcnt(0);
+        __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup, and
         __syncthreads();   // the tiles are read before the next share's are copied
     }
-}
-
-// The parts of the key tiles whose rows were cut, added in order.
-__global__ __launch_bounds__(kPwKeys) void paged_key_sums_join_kernel(PromptWeightsParams pw) {
-    const PagedFlashParams& p = pw.f;
-    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads);
-    CutItem t{};
-    uint32_t total;
-    if (!find_key_part<Cuts::kCutTiles>(pw, blockIdx.x / (uint32_t)p.c.n_kv_heads, t, total)) return;
-    if (part_slot(t, t.parts - 1) >= pw.sum_slots) return;
-    const int key = t.begin + kPwKeys * t.tile + (int)threadIdx.x;
-    float* const w = weights_of(pw.w, t.b, kvh);
-    if (w == nullptr || key >= min(t.end, pw.w.max_len)) return;
-    const uint32_t pi = p.c.page.div((uint32_t)key);
-    if ((uint32_t)p.c.table[(long)t.b * p.c.max_pages + pi] >= (uint32_t)p.c.n_pages) return;   // no key
-    float sum = 0.0f;
-    for (int u = 0; u < t.parts; ++u)
-        sum += pw.part_sum[((long)part_slot(t, u) * p.c.n_kv_heads + kvh) * kPwKeys + threadIdx.x];
-    w[key] += sum;
 }
 
 // ---------------------------------------------------------------- host
 
 namespace {
 
-constexpr int kStatsLeast = 4;   // key tiles of a part at least
-constexpr int kSumsLeast = 8;    // row tiles of a part at least
+// The statistics' key tiles are cut for three workgroups per CU, in parts of four tiles or more: us, 32 rows of
+// 8192 tokens with 2, 4, 8 tiles or more 31.1, 27.1, 27.5; 16 rows of 2000 17.7, 18.1, 21.
+constexpr int kStatsPerCu = 3, kStatsLeast = 4;
+// The sums' row tiles into four times as many as three per CU where that leaves eight tiles or more, so that the
+// shares even out; us, a prompt of 4000 tokens with 4, 8, 12, 16, 24 per CU 388, 312, 291, 296, 299; into as many
+// as run at once where they are few, of two or more: 600 tokens in parts of 8, 4, 2 33.2, 29.1, 27.0, two prompts of
+// 1500 tokens of 8, 6 94, 108.
+constexpr int kSumsPerCu = 3, kSumsParts = 12, kSumsLeast = 8;
 
 struct PromptWeightsPlan {
     long row_tiles, sum_grid;
@@ -471,11 +511,14 @@ PromptWeightsPlan plan_prompt_weights(int batch, int rows, int n_heads, int n_kv
     const long seen = observe > 0 ? std::min((long)rows, (long)batch * observe) : rows;
     const long all = seen * (n_heads / n_kv_heads);
     pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min((long)batch, seen));
-    pl.target = std::max(3 * cus / n_kv_heads, 1);
+    pl.target = std::max(kStatsPerCu * cus / n_kv_heads, 1);
     pl.slots = 2u * (uint32_t)pl.target;
-    pl.sum_target = std::max(4 * cus / n_kv_heads, 1);
-    pl.sum_slots = all > (long)kSumsLeast * kPwTile ? 2u * (uint32_t)pl.sum_target : 0u;
-    pl.sum_grid = 2L * cus;
+    pl.sum_target = std::max(kSumsParts * cus / n_kv_heads, 1);
+    const long most = (observe > 0 ? std::min(rows, observe) : rows) * (long)(n_heads / n_kv_heads);   // of a sequence
+    pl.sum_slots = most > 2L * kPwTile ? 2u * (uint32_t)pl.sum_target : 0u;
+    // A counter for each cut tile: where they do not suffice (thousands of KV heads), nothing is cut.
+    if ((long)(pl.target + pl.sum_target) * n_kv_heads > kMaxCounters) pl.slots = pl.sum_slots = 0;
+    pl.sum_grid = (long)kSumsPerCu * cus;
     pl.off_ml = kCounterBytes;
     pl.off_stats = pl.off_ml + align_up((size_t)pl.slots * n_kv_heads * kPfRows * 2 * sizeof(float), 256);
     pl.off_sum = pl.off_stats + align_up((size_t)rows * n_heads * 2 * sizeof(float), 256);
@@ -489,8 +532,6 @@ void launch_prompt(const PromptWeightsParams& pw, const PromptWeightsPlan& pl, h
     paged_row_stats_kernel<BF, D, EXACT>
         <<<(unsigned)((pl.row_tiles + pl.target) * hkv), kPwThreads, 0, stream>>>(pw);
     paged_key_sums_kernel<BF, D, EXACT><<<(unsigned)pl.sum_grid, kPwThreads, 0, stream>>>(pw);
-    if (pl.sum_slots > 0)   // (a tile that is cut has two parts at least)
-        paged_key_sums_join_kernel<<<(unsigned)(pl.sum_target * hkv), kPwKeys, 0, stream>>>(pw);
 }
 
 }  // namespace
@@ -504,23 +545,23 @@ int launch_paged_prefill_weights(const PagedLaunch& a, const PagedWeights& w, in
         plan_prompt_weights(a.batch, a.rows, a.n_heads, a.n_kv_heads, observe, device_cu_count());
     if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
         return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_prefill_weights_workspace_size)");
-    if ((long)pl.slots * a.n_kv_heads > kMaxCounters)
-        return set_error(LLMIK_ERR_UNSUPPORTED, "too many KV heads or compute units for the workspace's counters");
     PromptWeightsParams pw{};
     pw.f = flash_params(a);
     pw.f.splits = 1;
     pw.f.observe = observe > 0 ? observe : INT_MAX;
     pw.f.target = pl.target;
-    pw.f.least = kStatsLeast;
+    pw.f.least = pl.slots > 0 ? kStatsLeast : kUncut;
     pw.f.slots = pl.slots;
     char* ws = static_cast<char*>(a.workspace);
     pw.counters = reinterpret_cast<uint32_t*>(ws);
+    pw.sum_counters = pw.counters + (long)(pl.slots / 2) * a.n_kv_heads;
     pw.f.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
     pw.stats = reinterpret_cast<f32x2*>(ws + pl.off_stats);
     pw.part_sum = reinterpret_cast<float*>(ws + pl.off_sum);
     pw.w = weights_view(w, a.n_kv_heads);
     pw.sum_target = pl.sum_target;
-    pw.sum_least = pl.sum_slots > 0 ? kSumsLeast : INT_MAX;
+    pw.sum_least = pl.sum_slots > 0 ? kSumsLeast : kUncut;
+    pw.sum_few = pl.sum_slots > 0 ? std::max(kSumsPerCu * device_cu_count() / a.n_kv_heads, 1) : 0;
     pw.sum_slots = pl.sum_slots;
     auto go = [&](auto bf, auto exact) {
         constexpr bool BF = decltype(bf)::value, EXACT = decltype(exact)::value;

@@ -4,7 +4,7 @@
 //
 // All drafted tokens and query heads that read a KV head's keys share one pass over
 // them, 128 rows at a time, so the cache's bytes bound it while they are few. The key
-// tiles of the batch are cut into parts of about one length (find_cut): a row
+// tiles of the batch are cut into parts of about one length (Cutter): a row
 // tile's parts are joined by a second kernel.
 #include "paged_flash.hpp"
 
@@ -28,13 +28,12 @@ constexpr int join_rows(int head_dim) { return 256 * 4 / head_dim; }   // of a w
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p) {
     using Hf = Half16<BF>;
-    const int kvh = (int)blockIdx.x % p.c.n_kv_heads;
-    CutItem t{};
-    if (!find_row_part<Cuts::kCutTiles>(p, blockIdx.x / (uint32_t)p.c.n_kv_heads, t)) return;
-    if (part_slot(t, t.parts - 1) >= p.slots) return;
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), cut = (int)(blockIdx.x / (uint32_t)p.c.n_kv_heads);
+    if (cut >= p.records[0].count) return;
+    const CutRecord t = p.records[cut];
     const int row = join_rows(D) * (int)blockIdx.y + (int)threadIdx.x / (D / 4);   // of the tile
     const int r = t.tile * kPfRows + row;
-    if (r >= t.rows * (int)p.gqa.d) return;
+    if (r >= t.rows * (int)p.gqa.d || t.parts == 0) return;
     const int c4 = 4 * ((int)threadIdx.x % (D / 4));
     float top = kNoMax, sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -43,7 +42,7 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
         f32x4 v[kJoinBatch];
 #pragma unroll
         for (int u = 0; u < kJoinBatch; ++u) {
-            const long at = part_row(p, t, min(u0 + u, t.parts - 1), kvh, row);
+            const long at = part_row(p, t.slot + (uint32_t)(min(u0 + u, t.parts - 1) * t.fixed), kvh, row);
             ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * at);
             v[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + c4);
         }
@@ -75,26 +74,30 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
 
 namespace {
 
-constexpr int kTreeLeast = 4;   // key tiles of a part at least
+// The key tiles are cut for two workgroups per CU, into single tiles where there are few. us, a draft of 8 over 700
+// tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0; 30 drafts of 4 .. 24 over 200 .. 8000 tokens for 256, 384, 512,
+// 768 workgroups 88.6, 70.2, 62.0, 76.3; one of 64 over 8192 28.8, 29.6, 30.4, 38.1.
+constexpr int kTreePerCu = 2, kTreeLeast = 1;
 
 struct PagedTreePlan {
     long row_tiles;      // of the call at most
     int target;
     uint32_t slots;      // 0: nothing is cut
-    size_t off_o, bytes;
+    size_t off_o, off_records, bytes;
 };
 
 PagedTreePlan plan_tree(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity, int cus) {
     PagedTreePlan pl{};
     const long all = (long)rows * (n_heads / n_kv_heads);
     pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min(batch, rows));
-    pl.target = std::max(2 * cus / n_kv_heads, 1);
+    pl.target = std::max(kTreePerCu * cus / n_kv_heads, 1);
     if (capacity > (long)kTreeLeast * kPfTile) {
         // A row tile that is cut has more than one length's tiles: less than twice the target's parts.
         pl.slots = 2u * (uint32_t)pl.target;
         const size_t parts = (size_t)pl.slots * n_kv_heads * kPfRows;
         pl.off_o = align_up(parts * 2 * sizeof(float), 256);
-        pl.bytes = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
+        pl.off_records = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
+        pl.bytes = pl.off_records + pl.slots / 2 * sizeof(CutRecord);
     }
     return pl;
 }
@@ -127,6 +130,7 @@ int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, con
         char* ws = static_cast<char*>(a.workspace) + kCounterBytes;
         p.part_ml = reinterpret_cast<float*>(ws);
         p.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+        p.records = reinterpret_cast<CutRecord*>(ws + pl.off_records);
     }
     p.splits = 1;
     p.observe = INT_MAX;
@@ -134,7 +138,7 @@ int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, con
     p.words = words;
     p.positions = positions;
     p.target = pl.target;
-    p.least = pl.slots > 0 ? kTreeLeast : INT_MAX;
+    p.least = pl.slots > 0 ? kTreeLeast : kUncut;
     p.slots = pl.slots;
     const long items = pl.row_tiles + (pl.slots > 0 ? pl.target : 0);
     const long cut = std::min(pl.row_tiles, (long)pl.target);   // (a tile that is cut has two parts at least)
