@@ -20,7 +20,9 @@ bit-identical to the reference cache's view after the same appends:
   integration/prealloc_cache.py:42-79, in INT8).
 
 PagedKVCache keeps fp16 or bf16 tokens of many sequences, each of its own
-length, in one pool of pages (the reference has no counterpart).
+length, in one pool of pages; it drafts and accepts token trees, and, where it
+records the tokens' attention weights, cuts sequences down to those that have
+had the most (the reference has no counterpart).
 """
 from __future__ import annotations
 
@@ -28,7 +30,8 @@ from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
-from . import (_C, paged_decode_attention, paged_prefill_attention, paged_shared_prefix_attention,
+from . import (_C, paged_compact, paged_decode_attention, paged_decode_attention_weights, paged_prefill_attention,
+               paged_prefill_weights, paged_select_tokens, paged_shared_prefix_attention, paged_tree_attention,
                quantize_k_per_channel_groupwise_int4_into, quantize_per_token_into, quantize_v_per_token_int4_into,
                rope_paged_append)
 # One-token steps at small batch are bound by the host: these three come from the
@@ -216,6 +219,10 @@ class PagedBatch(NamedTuple):
     prefix_len: int
     shortest: int = 0                   # the shortest length, the mean length: how much of the
     mean: int = 0                       # prefix a window leaves
+    positions: Optional[torch.Tensor] = None     # [rows] int32; None: the tokens' slots
+    tree_mask: Optional[torch.Tensor] = None     # [rows, words] int64: a drafted tree (PagedKVCache.draft)
+    weight_rows: Optional[torch.Tensor] = None   # [batch] int32: the sequences' rows of the weights
+    shortened: bool = False                      # some sequence has lost tokens: slots are no positions
 
 
 class PagedKVCache:
@@ -244,7 +251,28 @@ class PagedKVCache:
     bits once where decode attention keeps a second part: a sequence's results
     then change (within the output type's rounding, fp16 2^-11, bf16 2^-8 of the
     values' weighted spread) with the sequences beside it. shared_prefix=False
-    keeps decode attention for all batches."""
+    keeps decode attention for all batches.
+
+    Drafted trees: `draft` reserves a tree of tokens behind each sequence,
+    `append` and `attention` take its step like any other, and `accept` keeps one
+    path of it:
+
+        step = cache.draft([a, b], [parents_a, parents_b])
+        ...                                           # every layer: append, attention
+        cache.accept([a, b], [path_a, path_b])        # the tokens that the model agrees with
+
+    A bounded cache: with track_rows > 0 up to so many sequences have a row of
+    `weights` [n_layers, track_rows, n_kv_heads, track_tokens], to which
+    `attention` adds what each token is given (of a prompt's chunk by its last
+    `observe` rows, 0: by all; a drafted tree adds nothing), and `evict` cuts
+    sequences down to the tokens of the largest weight, for every layer and KV
+    head its own:
+
+        cache.evict([a, b], keep=4096, first=4, recent=256)
+
+    The tokens that stay keep their rotation, and new ones go on at the text's
+    positions. A window or slopes are refused for a sequence that has lost
+    tokens: distances would go by slots."""
 
     # A batch's shared prefix is read once for all sequences where that saves so many
     # token rows (of one KV head) and has so many tokens; a shorter one where it saves
@@ -254,11 +282,14 @@ class PagedKVCache:
 
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, head_dim: int = 128,
                  dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None,
-                 n_layers: int = 1, shared_prefix: bool = True) -> None:
+                 n_layers: int = 1, shared_prefix: bool = True, track_rows: int = 0, track_tokens: int = 0,
+                 observe: int = 0) -> None:
         _require(n_pages > 0 and n_kv_heads > 0 and n_layers > 0, "n_pages, n_kv_heads and n_layers must be positive")
         _require(page_size > 0 and page_size % 8 == 0, "page_size must be a positive multiple of 8")
         _require(head_dim in (64, 128), "only head_dim=64 and 128 supported")
         _require(dtype in (torch.float16, torch.bfloat16), "dtype must be fp16 or bf16")
+        _require(track_rows >= 0 and observe >= 0, "track_rows and observe must be >= 0")
+        _require(track_rows == 0 or track_tokens > 0, "track_tokens must be positive where weights are recorded")
         self.device = torch.device("cuda") if device is None else torch.device(device)
         self.shared_prefix = bool(shared_prefix)
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, n_kv_heads, page_size, head_dim
@@ -271,17 +302,30 @@ class PagedKVCache:
         self._pages: dict[int, List[int]] = {}  # sequence -> its pages
         self._length: dict[int, int] = {}
         self._next = 0
+        self._lost: dict[int, int] = {}               # sequence -> tokens that it has lost (its text is longer)
+        self._drafts: dict[int, Tuple[int, int]] = {}   # sequence -> its length without the draft, drafted tokens
+        self.observe = int(observe)
+        self.weights: Optional[torch.Tensor] = None
+        self._rows: dict[int, int] = {}               # sequence -> its row of the weights
+        self._free_rows = list(range(track_rows - 1, -1, -1))
+        if track_rows > 0:
+            self.weights = torch.zeros(n_layers, track_rows, n_kv_heads, track_tokens, device=self.device)
 
     # ---- sequences ----
 
     def add(self, share: Optional[int] = None, tokens: int = 0) -> int:
         """A new sequence, empty or behind the first `tokens` tokens of the
         sequence `share`: whole pages are shared, the rest of the last one is
-        copied. Returns its number."""
+        copied. Returns its number. Recorded weights are copied; a sequence that
+        has lost tokens is shared whole (of its first tokens it has not all)."""
         pages: List[int] = []
+        _require(self.weights is None or len(self._free_rows) > 0, "the cache has no free row of weights")
         if share is not None:
             _require(share in self._pages, "no such sequence")
+            _require(share not in self._drafts, "the shared sequence has a draft that is not accepted")
             _require(0 <= tokens <= self._length[share], "the shared sequence has fewer tokens")
+            _require(self._lost[share] == 0 or tokens in (0, self._length[share]),
+                     "a sequence that has lost tokens is shared whole")
             whole, rest = divmod(tokens, self.page_size)
             pages = self._pages[share][:whole]
             if rest:
@@ -298,19 +342,43 @@ class PagedKVCache:
             _require(tokens == 0, "tokens are shared with a sequence")
         seq, self._next = self._next, self._next + 1
         self._pages[seq], self._length[seq] = list(pages), tokens
+        self._lost[seq] = self._lost[share] if share is not None and tokens else 0
+        if self.weights is not None:
+            self._rows[seq] = row = self._free_rows.pop()
+            self.weights[:, row].zero_()
+            if share is not None:
+                n = min(tokens, self.weights.shape[3])
+                self.weights[:, row, :, :n] = self.weights[:, self._rows[share], :, :n]
         return seq
 
     def remove(self, seq: int) -> None:
         """Ends a sequence; pages that no other one shares become free."""
         _require(seq in self._pages, "no such sequence")
-        for p in self._pages.pop(seq):
+        self._release(self._pages.pop(seq))
+        del self._length[seq], self._lost[seq]
+        self._drafts.pop(seq, None)
+        if self.weights is not None:
+            self._free_rows.append(self._rows.pop(seq))
+
+    def _release(self, pages: Sequence[int]) -> None:
+        for p in pages:
             self._users[p] -= 1
             if self._users[p] == 0:
                 self._free.append(p)
-        del self._length[seq]
+
+    def _shorten(self, seq: int, tokens: int) -> None:
+        """The sequence's first `tokens` slots stay; pages behind them are released."""
+        keep = -(-tokens // self.page_size)
+        self._release(self._pages[seq][keep:])
+        del self._pages[seq][keep:]
+        self._length[seq] = tokens
 
     def length(self, seq: int) -> int:
         return self._length[seq]
+
+    def position(self, seq: int) -> int:
+        """The text position of the sequence's next token: its length and what it has lost."""
+        return self._length[seq] + self._lost[seq]
 
     def free_pages(self) -> int:
         return len(self._free)
@@ -322,11 +390,117 @@ class PagedKVCache:
         the call's tables. The tokens count as live from here on: `append` them
         before anything reads them. Nothing is reserved if the pages do not
         suffice."""
-        counts = [1] * len(seqs) if new is None else [int(n) for n in new]
+        return self._reserve(seqs, [1] * len(seqs) if new is None else [int(n) for n in new], None)
+
+    def draft(self, seqs: Sequence[int], parents: Sequence[Sequence[int]]) -> PagedBatch:
+        """`batch` for a drafted tree behind each sequence: parents[i][j] is the
+        drafted token of seqs[i] that token j follows, an earlier one, or -1: the
+        sequence's last token. The step's attention shows every drafted token the
+        sequence and its own path, at the path's positions; `accept` ends the
+        draft, and until then the sequence is in no other batch."""
+        trees = [[int(p) for p in tree] for tree in parents]
+        _require(len(trees) == len(seqs), "one tree per sequence")
+        _require(all(-1 <= p < j for tree in trees for j, p in enumerate(tree)),
+                 "a drafted token follows an earlier one or -1")
+        return self._reserve(seqs, [len(tree) for tree in trees], trees)
+
+    def accept(self, seqs: Sequence[int], paths: Sequence[Sequence[int]]) -> None:
+        """Ends the drafts of `seqs`: of seqs[i] the drafted tokens paths[i] (numbers in
+        the draft, ascending; none: all are dropped) become its next tokens, in
+        every layer. The draft's step must have been appended to all layers that
+        are read again."""
+        paths = [[int(j) for j in path] for path in paths]
+        _require(len(paths) == len(seqs), "one path per sequence")
+        _require(len(set(seqs)) == len(seqs), "a sequence occurs twice")
+        _require(all(s in self._drafts for s in seqs), "a sequence has no draft")
+        for s, path in zip(seqs, paths):
+            _require(all(a < b for a, b in zip(path, path[1:])) and
+                     all(0 <= j < self._drafts[s][1] for j in path), "a path's tokens are ascending numbers of the draft")
+        moved = [(s, path) for s, path in zip(seqs, paths) if path != list(range(len(path)))]
+        if moved:
+            ctx = [self._drafts[s][0] for s, _ in moved]
+            longest = max(len(path) for _, path in moved)
+            kept = [[c + j for j in path] + [-1] * (longest - len(path)) for c, (_, path) in zip(ctx, moved)]
+            self._compact([s for s, _ in moved], kept, ctx)
+        for s, path in zip(seqs, paths):
+            self._shorten(s, self._drafts.pop(s)[0] + len(path))
+
+    def evict(self, seqs: Sequence[int], keep: int, first: int = 0, recent: int = 0) -> None:
+        """Cuts the sequences down to `keep` tokens for every layer and KV head: the
+        first `first`, the last `recent` and, of the others, those of the largest
+        recorded weight (paged_select_tokens). Shorter ones stay as they are. Pages
+        that other sequences share are copied first: nothing is changed if the free
+        pages do not suffice."""
+        _require(self.weights is not None, "the cache records no weights (track_rows)")
+        _require(len(set(seqs)) == len(seqs), "a sequence occurs twice")
+        _require(all(s in self._pages for s in seqs), "no such sequence")
+        _require(keep > 0 and first >= 0 and recent >= 0 and first + recent <= keep,
+                 "first and recent must be >= 0, together at most keep")
+        _require(all(s not in self._drafts for s in seqs), "a sequence has a draft that is not accepted")
+        long = [s for s in seqs if self._length[s] > keep]
+        _require(all(self._length[s] <= self.weights.shape[3] for s in long),
+                 "a sequence has more tokens than weights (track_tokens)")
+        if not long:
+            return
+        whole = -(-keep // self.page_size)
+        shared = [(s, i) for s in long for i, p in enumerate(self._pages[s][:whole]) if self._users[p] > 1]
+        # (a page that only these sequences share: the last of them keeps it)
+        left = dict((p, self._users[p]) for s in long for p in self._pages[s])
+        copies = []
+        for s, i in shared:
+            p = self._pages[s][i]
+            if left[p] > 1:
+                left[p] -= 1
+                copies.append((s, i))
+        _require(len(copies) <= len(self._free), "the cache has no free page")
+        if copies:
+            src = [self._pages[s][i] for s, i in copies]
+            dst = [self._free.pop() for _ in copies]
+            self.k[:, dst] = self.k[:, src]
+            self.v[:, dst] = self.v[:, src]
+            for (s, i), old, page in zip(copies, src, dst):
+                self._users[page], self._pages[s][i] = 1, page
+                self._release([old])
+        self._compact(long, None, None, keep, first, recent)
+        for s in long:
+            self._lost[s] += self._length[s] - keep
+            self._shorten(s, keep)
+
+    def _compact(self, seqs: Sequence[int], kept: Optional[List[List[int]]], starts: Optional[List[int]],
+                 keep: int = 0, first: int = 0, recent: int = 0) -> None:
+        """Selection (where no lists are given) and moves of all layers in one launch each:
+        the layers' pools are one, whose pages and weight rows are numbered on."""
+        layers, b = self.k.shape[0], len(seqs)
+        width = max(len(self._pages[s]) for s in seqs)
+        flat = [self._length[s] for s in seqs] + (starts or [0] * b)
+        flat += [self._rows.get(s, 0) for s in seqs] + [n for row in kept or [] for n in row]
+        flat += [p for s in seqs for p in self._pages[s] + [-1] * (width - len(self._pages[s]))]
+        dev = self._to_device(flat)
+        lens, first_slots, rows = (dev[i * b:(i + 1) * b].repeat(layers) for i in range(3))
+        pages = dev[len(flat) - b * width:].view(b, width)
+        layer = torch.arange(layers, dtype=torch.int32, device=self.device)[:, None, None]
+        table = torch.where(pages >= 0, pages + layer * self.n_pages, -1).view(-1, width)
+        k, v = self.k.flatten(0, 1), self.v.flatten(0, 1)
+        if kept is not None:
+            lists = dev[3 * b:3 * b + b * len(kept[0])].view(b, -1).repeat(layers, 1)
+            paged_compact(k, v, table, lens, lists, first_slots)
+            return
+        weights = self.weights.flatten(0, 1)
+        rows = rows + (layer.view(-1, 1) * self.weights.shape[1]).expand(-1, b).reshape(-1)
+        lists, _ = paged_select_tokens(weights, lens, keep, first, recent, rows)
+        paged_compact(k, v, table, lens, lists, None, weights, rows)
+
+    def _to_device(self, flat: List[int]) -> torch.Tensor:
+        host = torch.tensor(flat, dtype=torch.int32)
+        return host.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else host
+
+    def _reserve(self, seqs: Sequence[int], counts: List[int], trees: Optional[List[List[int]]]) -> PagedBatch:
         _require(len(counts) == len(seqs), "one count per sequence")
         _require(len(set(seqs)) == len(seqs), "a sequence occurs twice in the batch")
         _require(all(s in self._pages for s in seqs), "no such sequence")
         _require(all(n >= 0 for n in counts), "counts must be >= 0")
+        _require(all(s not in self._drafts for s in seqs), "a sequence has a draft that is not accepted")
+        before = [self._length[s] for s in seqs]
         need = [-(-(self._length[s] + n) // self.page_size) - len(self._pages[s]) for s, n in zip(seqs, counts)]
         _require(sum(need) <= len(self._free), "the cache has no free page")
         for s, n, m in zip(seqs, counts, need):
@@ -337,24 +511,46 @@ class PagedKVCache:
             self._length[s] += n
         pages = [self._pages[s] for s in seqs]
         lens = [self._length[s] for s in seqs]
-        ragged = any(n != 1 for n in counts)
+        ragged = trees is not None or any(n != 1 for n in counts)
+        lost = any(self._lost[s] for s in seqs)
+        positions: List[int] = []
+        words, masks = 0, []
+        if trees is not None:
+            words = max(1, -(-max([len(t) for t in trees] + [0]) // 64))
+            for s, n, tree in zip(seqs, before, trees):
+                self._drafts[s] = (n, len(tree))
+                seen: List[int] = []
+                deep: List[int] = []
+                for j, parent in enumerate(tree):
+                    seen.append((seen[parent] if parent >= 0 else 0) | 1 << j)
+                    deep.append(deep[parent] + 1 if parent >= 0 else n + self._lost[s])
+                masks += [(m >> 32 * w) & 0xFFFFFFFF for m in seen for w in range(2 * words)]
+                positions += deep
+        elif lost:
+            positions = [n + self._lost[s] + j for s, n, c in zip(seqs, before, counts) for j in range(c)]
         cu = [0]
         for n in counts:
             cu.append(cu[-1] + n)
-        shared = 0 if ragged or not self.shared_prefix else self._shared_prefix(pages, lens)
+        shared = 0 if ragged or not self.shared_prefix or self.weights is not None else self._shared_prefix(pages, lens)
         width = max([len(p) for p in pages] + [1])
-        # One copy to the device: lengths, row offsets, then the table.
+        # One copy to the device: lengths, row offsets, then the table, and what else there is.
         flat = lens + cu + [p for row in pages for p in row + [-1] * (width - len(row))]
-        host = torch.tensor(flat, dtype=torch.int32)
-        if self.device.type == "cuda":
-            dev = host.pin_memory().to(self.device, non_blocking=True)
-        else:
-            dev = host
+        ends = [len(flat)]
+        for more in (positions, [self._rows[s] for s in seqs] if self.weights is not None else []):
+            flat += more
+            ends.append(len(flat))
+        flat += [0] * (len(flat) % 2) + [m - (1 << 32) if m >> 31 else m for m in masks]   # (64-bit words)
+        dev = self._to_device(flat)
         b = len(seqs)
-        table = dev[2 * b + 1:].view(b, width) if b else torch.zeros((0, width), dtype=torch.int32, device=self.device)
+        table = dev[2 * b + 1:ends[0]].view(b, width) if b else torch.zeros((0, width), dtype=torch.int32, device=self.device)
+        tree_mask = None
+        if trees is not None:
+            tree_mask = dev[len(flat) - len(masks):].view(torch.int64).view(cu[-1], words)
         return PagedBatch(table, dev[:b], dev[b:2 * b + 1] if ragged else None, cu[-1],
                           table[0, :shared] if shared else None, shared * self.page_size,
-                          min(lens, default=0), sum(lens) // max(b, 1))
+                          min(lens, default=0), sum(lens) // max(b, 1),
+                          dev[ends[0]:ends[1]] if lost or trees is not None else None, tree_mask,
+                          dev[ends[1]:ends[2]] if self.weights is not None else None, lost)
 
     def _shared_prefix(self, pages: List[List[int]], lens: List[int]) -> int:
         """Whole pages that all sequences share from the start on, or 0 where reading
@@ -394,16 +590,29 @@ class PagedKVCache:
         """rope_paged_append of the batch's new tokens to a layer; returns the
         rotated q [rows, n_heads, head_dim]."""
         return rope_paged_append(qkv, cos, sin, self.k[layer], self.v[layer], step.page_table, step.seq_lens,
-                                 step.cu_tokens)
+                                 step.cu_tokens, step.positions)
 
     def attention(self, step: PagedBatch, q: torch.Tensor, softmax_scale: float, softcap: float = 0.0,
                   slopes: Optional[torch.Tensor] = None, window: int = 0, layer: int = 0) -> torch.Tensor:
         """Attention of the batch's new tokens in a layer: decode, decode behind a
-        shared prefix, or prompts, by the batch (and what a window leaves of the prefix)."""
+        shared prefix, prompts, or a drafted tree, by the batch (and what a window leaves
+        of the prefix). Where the cache records weights, those of decode steps and prompts
+        are added: once for every call."""
         k, v = self.k[layer], self.v[layer]
+        _require(not step.shortened or (slopes is None and window <= 0),
+                 "window and slopes need sequences that have lost no tokens")
+        if step.tree_mask is not None:
+            return paged_tree_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, step.tree_mask,
+                                        softmax_scale, softcap, slopes, window, step.positions)
         if step.cu_tokens is not None:
+            if self.weights is not None:
+                paged_prefill_weights(q, k, step.page_table, step.seq_lens, step.cu_tokens, self.weights[layer],
+                                      softmax_scale, softcap, slopes, window, self.observe, step.weight_rows)
             return paged_prefill_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, softmax_scale,
                                            softcap, slopes, window)
+        if self.weights is not None:
+            return paged_decode_attention_weights(q, k, v, step.page_table, step.seq_lens, self.weights[layer],
+                                                  softmax_scale, softcap, slopes, window, step.weight_rows)
         if step.prefix_pages is not None and (window <= 0 or self._window_pays(step, window)):
             return paged_shared_prefix_attention(q, k, v, step.page_table, step.seq_lens, step.prefix_pages,
                                                  step.prefix_len, softmax_scale, softcap, slopes, window)
