@@ -58,10 +58,13 @@ struct PagedDecodeParams {
     float* part_ml;       // [2 * workgroups, chunk_heads, 2]
     uint32_t* counters;   // [workgroups], zero between calls
     int few_steps;        // workgroups that few tiles are spread over, one tile per wave
-    float* scores;        // with SCORES: [batch, n_heads, score_tokens], every key's score (log2), and
-    float* row_ml;        //   [batch, n_heads] (maximum, 1 / sum of 2^(score - maximum))
+    float* scores;        // with SCORES: [batch, n_kv_heads, score_tokens / 32, gqa, 32], every key's score
+    float* row_ml;        //   (log2), and [batch, n_heads] (maximum, 1 / sum of 2^(score - maximum))
     int score_tokens;     // a multiple of 32
 };
+__device__ __forceinline__ long score_tile(const PagedDecodeParams& p, int b, int kvh, int t0) {   // t0 % 32 == 0
+    return ((long)b * p.c.n_kv_heads + kvh) * p.gqa * p.score_tokens + (long)t0 * p.gqa;
+}
 
 // kPieceUnits (llmik_internal.hpp) is a piece's overhead in units of a tile's time: see the shares.
 constexpr int kUncutTiles = 12;   // a slab of so few tiles is not cut: three per wave cost less than a hand-off
@@ -359,7 +362,7 @@ __device__ __forceinline__ void paged_decode(const PagedDecodeParams& p, uint32_
                 }
                 if constexpr (SCORES) {
                     if (c < nh && t0 < p.score_tokens) {
-                        float* dst = p.scores + ((long)b * p.n_heads + head) * p.score_tokens + tk;
+                        float* dst = p.scores + score_tile(p, b, kvh, t0) + 32 * (chunk * p.chunk_heads + c) + 4 * g;
                         *reinterpret_cast<f32x4*>(dst) = f32x4{sc[0], sc[1], sc[2], sc[3]};
                         *reinterpret_cast<f32x4*>(dst + 16) = f32x4{sc[4], sc[5], sc[6], sc[7]};
                     }

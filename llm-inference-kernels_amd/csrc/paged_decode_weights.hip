@@ -3,6 +3,14 @@
 // 4 D per KV head) and each head's maximum and sum, and a second launch adds
 //   weights[row(b), kvh, t] += sum over the KV head's G query heads of 2^(s - m) / l
 // Every weight has one writer, so the sums do not depend on timing.
+//
+// Bound: the cache's bytes, and the scores' (G / D of the keys' and values') twice. GPU us,
+// plain decode against this: 48 sequences of 1500 .. 8192 tokens, 8 KV heads, bf16 136, 171;
+// 64 of 4096 166, 212; one of 900 10.1, 14.5, one of 30000 30.7, 36.6. Of the difference
+// the second launch has 10 (4 for one sequence), the writes among the reads 19, whatever
+// their order, place or part of a line (into the caches alone 5). Adding the weights in
+// the first launch, by the last of a sequence's workgroups: 900 tokens 13.7, 2000 17.5
+// instead of 15.7, 4 x 4000 33.6 instead of 26.9.
 #include "paged_decode.hpp"
 
 namespace llmik {
@@ -19,68 +27,75 @@ __global__ __launch_bounds__(kPdThreads, kPdPerCu) void paged_decode_scores_kern
 
 namespace {
 
-constexpr int kRecordThreads = 256, kRecordTokens = 1024;   // of a workgroup's turn
-
-struct RecordParams {
-    const float* scores;
-    const float* row_ml;
-    const int* lens;
-    WeightsView w;
-    int batch, n_heads, n_kv_heads, gqa, capacity, window, score_tokens;
-};
+constexpr int kRecordThreads = 256, kRecordTokens = 1024;   // of a workgroup's turn: four for each thread
 
 }  // namespace
 
 // The turns (a sequence's KV head and 1024 of its tokens) are numbered over the whole
 // batch and taken by the workgroups in turn: the host does not know the lengths.
-__global__ __launch_bounds__(kRecordThreads) void paged_record_kernel(RecordParams p) {
+// ALIGNED: the weights' rows are aligned to 16 bytes.
+template <bool ALIGNED>
+__global__ __launch_bounds__(kRecordThreads) void paged_record_kernel(PagedDecodeParams p, WeightsView w) {
     const int tid = threadIdx.x, lane = tid & 63;
-    const int per = (p.batch + 63) / 64;
-    const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
-    // A sequence's recorded keys [begin, end) and its turns for one KV head.
-    auto keys_of = [&](int b, int& begin, int& end) {
-        const int len = max(p.lens[b], 0);
-        end = min(min(len, p.capacity), p.score_tokens);
-        begin = min(max(len - p.window, 0), end);
-        end = min(end, p.w.max_len);
-        return end > begin ? (uint32_t)(end - begin + kRecordTokens - 1) / kRecordTokens : 0u;
+    const int per = (p.c.batch + 63) / 64;
+    const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+    // A sequence's recorded keys [begin, end) and its turns for one KV head, from a multiple of 32 on.
+    auto turns_of = [&](int b, int& begin, int& end) {
+        const Keys k = keys_of(p, p.c.lens[b]);
+        begin = k.begin;
+        end = min(min(k.end, p.score_tokens), w.max_len);
+        return end > begin ? (uint32_t)(end - begin / 32 * 32 + kRecordTokens - 1) / kRecordTokens : 0u;
     };
     uint32_t mine = 0;
-    int begin, end;
-    for (int b = b0; b < b1; ++b) mine += keys_of(b, begin, end) * (uint32_t)p.n_kv_heads;
+    int begin = 0, end = 0;   // (the lane's only sequence's, where per is 1)
+    for (int b = b0; b < b1; ++b) mine += turns_of(b, begin, end) * (uint32_t)p.c.n_kv_heads;
     const uint32_t incl = wave_scan(mine), total = lane_u32(incl, 63);
+    const int own_begin = begin, own_end = end;
     for (uint32_t x = blockIdx.x; x < total; x += gridDim.x) {
-        const int at_lane = __ffsll((unsigned long long)__ballot(incl > x)) - 1;
-        uint32_t first = lane_u32(incl - mine, at_lane), turns = 0;
-        int b = at_lane * per;
-        for (;; ++b) {   // ends: the lane's sequences hold turn x
-            turns = keys_of(b, begin, end);
-            if (x - first < turns * (uint32_t)p.n_kv_heads) break;
-            first += turns * (uint32_t)p.n_kv_heads;
-        }
-        const int kvh = (int)((x - first) / turns);
-        const int t0 = begin + kRecordTokens * (int)((x - first) - (uint32_t)kvh * turns);
-        float* const w = weights_of(p.w, b, kvh);
-        if (w == nullptr) continue;
-        const long row = (long)b * p.n_heads + kvh * p.gqa;
-        constexpr int kEach = kRecordTokens / kRecordThreads;
-        float sum[kEach];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) sum[e] = 0.0f;
-        for (int g = 0; g < p.gqa; ++g) {
-            const float m = p.row_ml[2 * (row + g)], inv = p.row_ml[2 * (row + g) + 1];
-            const float* s = p.scores + (row + g) * p.score_tokens;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int t = t0 + e * kRecordThreads + tid;
-                const float x = t < end ? s[t] : -INFINITY;   // (-inf: no key)
-                if (x > -INFINITY || x != x) sum[e] = fmaf(__builtin_amdgcn_exp2f(x - m), inv, sum[e]);
+        const int at = __ffsll((unsigned long long)__ballot(incl > x)) - 1;
+        uint32_t first = lane_u32(incl - mine, at), turns = lane_u32(mine, at) / (uint32_t)p.c.n_kv_heads;
+        int b = at;
+        if (per == 1) {
+            begin = __builtin_amdgcn_readlane(own_begin, at);
+            end = __builtin_amdgcn_readlane(own_end, at);
+        } else {
+            for (b = at * per;; ++b) {   // ends: the lane's sequences hold turn x
+                turns = turns_of(b, begin, end);
+                if (x - first < turns * (uint32_t)p.c.n_kv_heads) break;
+                first += turns * (uint32_t)p.c.n_kv_heads;
             }
         }
+        const int kvh = (int)((x - first) / turns);
+        const int t = begin / 32 * 32 + kRecordTokens * (int)((x - first) - (uint32_t)kvh * turns) + 4 * tid;
+        float* const to = weights_of(w, b, kvh);
+        if (to == nullptr || t >= end) continue;
+        const bool whole = t >= begin && t + 4 <= end;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f}, old = sum;
+        if (whole && ALIGNED) old = *reinterpret_cast<const f32x4*>(to + t);
+        const float* const ml = p.row_ml + 2 * ((long)b * p.n_heads + kvh * p.gqa);
+        const float* const s = p.scores + score_tile(p, b, kvh, t / 32 * 32) + t % 32;
+        for (int g0 = 0; g0 < p.gqa; g0 += 4) {   // four heads' scores requested at a time
+            f32x4 v[4];
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int t = t0 + e * kRecordThreads + tid;
-            if (t < end) w[t] += sum[e];
+            for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4*>(s + 32 * min(g0 + u, p.gqa - 1));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (g0 + u >= p.gqa) break;
+                const float m = ml[2 * (g0 + u)], inv = ml[2 * (g0 + u) + 1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float score = v[u][e];   // (-inf: no key)
+                    if (score > -INFINITY || score != score)
+                        sum[e] = fmaf(__builtin_amdgcn_exp2f(score - m), inv, sum[e]);
+                }
+            }
+        }
+        if (whole && ALIGNED) {
+            *reinterpret_cast<f32x4*>(to + t) = old + sum;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e >= begin && t + e < end) to[t + e] += sum[e];
         }
     }
 }
@@ -148,10 +163,13 @@ int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, hip
                           : launch_scores<false, 64>(p, pl.decode.workgroups, uniform, stream);
     const int st = check_launch();
     if (st != LLMIK_OK) return st;
-    RecordParams r{p.scores, p.row_ml, a.lens, weights_view(w, a.n_kv_heads), a.batch, a.n_heads, a.n_kv_heads,
-                   p.gqa, p.c.capacity, p.s.window, pl.score_tokens};
-    const long turns = (long)a.batch * a.n_kv_heads * ((pl.score_tokens + kRecordTokens - 1) / kRecordTokens);
-    paged_record_kernel<<<(unsigned)std::min(turns, 8L * cus), kRecordThreads, 0, stream>>>(r);
+    const long turns = (long)a.batch * a.n_kv_heads * (pl.score_tokens / kRecordTokens + 2);
+    const unsigned grid = (unsigned)std::min(turns, 8L * cus);
+    const WeightsView view = weights_view(w, a.n_kv_heads);
+    if (w.max_len % 4 == 0 && reinterpret_cast<uintptr_t>(w.weights) % 16 == 0)
+        paged_record_kernel<true><<<grid, kRecordThreads, 0, stream>>>(p, view);
+    else
+        paged_record_kernel<false><<<grid, kRecordThreads, 0, stream>>>(p, view);
     return check_launch();
 }
 

@@ -73,7 +73,8 @@ struct PagedFlashParams {
     int observe;              // rows of a sequence that count: its last ones
     int target, least;
     uint32_t slots;           // parts that the workspace holds: [slots, n_kv_heads, kPfRows, D] and (m, l)
-    CutRecord* records;       // [slots / 2]
+    CutRecord* records;
+    int n_records;
 };
 enum class Flash { kRagged, kPrefix, kTree };
 
@@ -206,12 +207,15 @@ struct CutItem {
     int tile, part;       // this share: which of the fixed, which part
     uint32_t slot;        // of the tile's first part among all parts of tiles that are cut; part i: fixed i further
     uint32_t cut;         // the tile's number among those that are cut
+    uint32_t cut_seq, group;   // the sequence's among those with cut tiles; row groups of those before it
 };
-// What a kernel that joins parts knows of a tile that is cut, and of the call how many there are.
+// What the kernel that joins the parts knows of a sequence whose tiles are cut: its rows
+// are groups `group` .. of kJoinRows rows; and in the first place how many records there are.
+constexpr int kJoinRows = 4;
 struct CutRecord {
-    int b, row0, rows, tile, fixed, parts;
+    int group, row0, rows, fixed, parts;
     uint32_t slot;
-    int count;
+    int count, unused;
 };
 constexpr int kUncut = 1 << 29;         // a part's tiles at least, where nothing is to be cut
 constexpr int kMaxPosition = 1 << 30;   // positions that are given count as at most this
@@ -252,8 +256,9 @@ struct Cutter {
     F sequence;              // (b, CutItem&): its rows, keys, fixed and tiles
     CutItem own{};           // the lane's last sequence: its only one where per is 1
     int per;
-    uint32_t length, items = 0, slots = 0, some = 0, incl, upto, numbered;   // of the lane; running totals
-    uint32_t shares, cuts;   // of the call; cuts: fixed tiles that are cut
+    uint32_t length, items = 0, slots = 0, some = 0, seqs = 0, groups = 0;   // of the lane, and running totals:
+    uint32_t incl, upto, numbered, seqs_upto, groups_upto;
+    uint32_t shares;         // of the call
 
     __device__ __forceinline__ uint32_t parts_of_length(int tiles) const {
         return max(quick_ceil((uint32_t)tiles, length), 1u);
@@ -266,6 +271,10 @@ struct Cutter {
     __device__ __forceinline__ static uint32_t items_of(const CutItem& s) {
         return (uint32_t)s.fixed * (uint32_t)s.parts;
     }
+    __device__ __forceinline__ uint32_t groups_of(const CutItem& s) const {
+        return ((uint32_t)s.rows * p.gqa.d + kJoinRows - 1) / kJoinRows;
+    }
+    __device__ __forceinline__ int cut_sequences() const { return (int)lane_u32(seqs_upto, 63); }
     // About `target` parts, of `least` tiles or more; with `few`, of two or more where they are not more than that.
     __device__ __forceinline__ Cutter(const PagedFlashParams& p_, int target_, int least, int few, F f)
         : p(p_), sequence(f) {
@@ -298,12 +307,15 @@ struct Cutter {
             items += items_of(own);
             slots += own.parts > 1 ? items_of(own) : 0u;
             some += own.parts > 1 ? (uint32_t)own.fixed : 0u;
+            seqs += own.parts > 1 ? 1u : 0u;
+            groups += own.parts > 1 ? groups_of(own) : 0u;
         }
         incl = wave_scan(items);
         upto = wave_scan(slots);
         numbered = wave_scan(some);
+        seqs_upto = wave_scan(seqs);
+        groups_upto = wave_scan(groups);
         shares = lane_u32(incl, 63);
-        cuts = lane_u32(numbered, 63);
     }
     // Share number `item`, false past the last. The last ones come first: a prompt's last rows see the most keys.
     __device__ __forceinline__ bool find(uint32_t item, CutItem& t) const {
@@ -311,7 +323,8 @@ struct Cutter {
         item = shares - 1 - item;
         const int at = __ffsll((unsigned long long)__ballot(incl > item)) - 1;
         uint32_t first = lane_u32(incl - items, at), slot = lane_u32(upto - slots, at);
-        uint32_t cut_at = lane_u32(numbered - some, at);
+        uint32_t cut_at = lane_u32(numbered - some, at), seq_at = lane_u32(seqs_upto - seqs, at);
+        uint32_t group = lane_u32(groups_upto - groups, at);
         t = own;
         t.b = at;
         if (per > 1) {
@@ -323,6 +336,8 @@ struct Cutter {
                 first += n;
                 slot += t.parts > 1 ? n : 0u;
                 cut_at += t.parts > 1 ? (uint32_t)t.fixed : 0u;
+                seq_at += t.parts > 1 ? 1u : 0u;
+                group += t.parts > 1 ? groups_of(t) : 0u;
             }
         }
         const int from = per == 1 ? at : 0;   // (every lane has the same where per > 1)
@@ -341,21 +356,23 @@ struct Cutter {
         t.tile = __builtin_amdgcn_readfirstlane((int)r - t.part * t.fixed);
         t.slot = (uint32_t)__builtin_amdgcn_readfirstlane((int)slot + t.tile);
         t.cut = (uint32_t)__builtin_amdgcn_readfirstlane((int)cut_at + t.tile);
+        t.cut_seq = (uint32_t)__builtin_amdgcn_readfirstlane((int)seq_at);
+        t.group = (uint32_t)__builtin_amdgcn_readfirstlane((int)group);
         return true;
     }
 };
-// Written by the call's first workgroup, and by each cut tile's first part: for the kernel that joins them.
-__device__ __forceinline__ void write_records(CutRecord* to, uint32_t slots, bool first, uint32_t cuts, bool found,
-                                              const CutItem& t) {
-    if (first) to[0].count = (int)min(cuts, slots / 2);   // (a tile that is cut has two parts at least)
-    if (!found || t.parts == 1 || t.part != 0 || t.cut >= slots / 2) return;
-    to[t.cut].b = t.b;
-    to[t.cut].row0 = t.row0;
-    to[t.cut].rows = t.rows;
-    to[t.cut].tile = t.tile;
-    to[t.cut].fixed = t.fixed;
-    to[t.cut].parts = t.slot + (uint32_t)((t.parts - 1) * t.fixed) < slots ? t.parts : 0;   // (0: offsets that decrease)
-    to[t.cut].slot = t.slot;
+// Written by the call's first workgroup, and by each cut sequence's first part.
+__device__ __forceinline__ void write_record(CutRecord* to, int n_records, uint32_t slots, bool first, int count,
+                                             bool found, const CutItem& t) {
+    if (first) to[0].count = min(count, n_records);
+    if (!found || t.parts == 1 || t.part != 0 || t.tile != 0 || t.cut_seq >= (uint32_t)n_records) return;
+    CutRecord& r = to[t.cut_seq];
+    r.group = (int)t.group;
+    r.row0 = t.row0;
+    r.rows = t.slot + (uint32_t)(t.fixed * t.parts) <= slots ? t.rows : 0;   // (none: offsets that decrease)
+    r.fixed = t.fixed;
+    r.parts = t.parts;
+    r.slot = t.slot;
 }
 __device__ __forceinline__ uint32_t part_slot(const CutItem& t, int part) {
     return t.slot + (uint32_t)(part * t.fixed);
@@ -415,7 +432,8 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
             const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
             found = cutter.find(item, ft);
-            if (p.slots != 0 && kvh == 0 && tid == 0) write_records(p.records, p.slots, wg == 0, cutter.cuts, found, ft);
+            if (p.slots != 0 && kvh == 0 && tid == 0)
+                write_record(p.records, p.n_records, p.slots, wg == 0, cutter.cut_sequences(), found, ft);
         }
         else found = find_tile(p, item, ft);
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.

@@ -20,54 +20,107 @@ __global__ __launch_bounds__(kPfThreads, 2) void paged_tree_kernel(PagedFlashPar
     paged_flash<BF, D, Flash::kTree, EXACT>(p, blockIdx.x, gridDim.x, {s_k0, s_k1, s_v0, s_v1, s_lo, s_hi, &s_bad});
 }
 
-namespace {
-constexpr int kJoinBatch = 8;   // parts that a thread requests at a time
-constexpr int join_rows(int head_dim) { return 256 * 4 / head_dim; }   // of a workgroup: a thread has four channels
-}  // namespace
-
+// The parts of the cut sequences' rows, joined. A workgroup has kJoinRows rows, a wave
+// every fourth part of them (eight requested at a time), a lane four channels of
+// kRows rows one after the other; the waves are joined through LDS.
 template <bool BF, int D>
 __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p) {
     using Hf = Half16<BF>;
-    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), cut = (int)(blockIdx.x / (uint32_t)p.c.n_kv_heads);
-    if (cut >= p.records[0].count) return;
-    const CutRecord t = p.records[cut];
-    const int row = join_rows(D) * (int)blockIdx.y + (int)threadIdx.x / (D / 4);   // of the tile
-    const int r = t.tile * kPfRows + row;
-    if (r >= t.rows * (int)p.gqa.d || t.parts == 0) return;
-    const int c4 = 4 * ((int)threadIdx.x % (D / 4));
-    float top = kNoMax, sum = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int u0 = 0; u0 < t.parts; u0 += kJoinBatch) {
-        f32x2 ml[kJoinBatch];
-        f32x4 v[kJoinBatch];
+    constexpr int kWaves = 4, kAtOnce = 64 / (D / 4), kTurns = kJoinRows / kAtOnce, kBatch = 8 / kTurns;
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves][kTurns][64 * 4];
+    __shared__ float s_m[kWaves][kTurns][64], s_l[kWaves][kTurns][64];
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), group = (int)(blockIdx.x / (uint32_t)p.c.n_kv_heads);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // The group's sequence: the last record that begins at or before it.
+    const int count = p.records[0].count;
+    int at = -1;
+    for (int i = 0; i < count; i += 64)
+        at += __popcll(__ballot(i + lane < count && p.records[min(i + lane, count - 1)].group <= group));
+    if (at < 0) return;
+    at = __builtin_amdgcn_readfirstlane(at);
+    const CutRecord t = p.records[at];
+    const int n_rows = t.rows * (int)p.gqa.d, r0 = kJoinRows * (group - t.group);
+    if (r0 >= n_rows) return;
+    const int c4 = 4 * (lane % (D / 4));
+    auto row_of = [&](int turn) { return min(r0 + turn * kAtOnce + lane / (D / 4), n_rows - 1); };
+    auto part_at = [&](int turn, int part) {
+        const int r = row_of(turn), tile = r / kPfRows;
+        return part_row(p, t.slot + (uint32_t)(part * t.fixed + tile), kvh, r - tile * kPfRows);
+    };
+    float top[kTurns], sum[kTurns];
+    f32x4 o[kTurns];
 #pragma unroll
-        for (int u = 0; u < kJoinBatch; ++u) {
-            const long at = part_row(p, t.slot + (uint32_t)(min(u0 + u, t.parts - 1) * t.fixed), kvh, row);
-            ml[u] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * at);
-            v[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + c4);
-        }
-        float m = top;
-#pragma unroll
-        for (int u = 0; u < kJoinBatch; ++u) m = fmaxf(m, ml[u][0]);
-        const float a = join_weight(top - m);
-        top = m;
-        sum *= a;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= a;
-#pragma unroll
-        for (int u = 0; u < kJoinBatch; ++u) {
-            const bool in = u0 + u < t.parts;
-            const float w = join_weight(ml[u][0] - m);
-            sum = in ? fmaf(ml[u][1], w, sum) : sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = in ? fmaf(v[u][e], w, o[e]) : o[e];
-        }
+    for (int k = 0; k < kTurns; ++k) {
+        top[k] = kNoMax;
+        sum[k] = 0.0f;
+        o[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;   // a row without keys is zero
+    // N parts, of which those that `counts` says, into one.
+    auto join = [&](int k, auto n, auto counts, const float* m, const float* l, const f32x4* v) {
+        constexpr int N = decltype(n)::value;
+        float most = top[k];
+#pragma unroll
+        for (int u = 0; u < N; ++u) most = fmaxf(most, counts(u) ? m[u] : kNoMax);
+        const float a = join_weight(top[k] - most);
+        top[k] = most;
+        sum[k] *= a;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][e] *= a;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const float w = join_weight(m[u] - most);
+            sum[k] = counts(u) ? fmaf(l[u], w, sum[k]) : sum[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][e] = counts(u) ? fmaf(v[u][e], w, o[k][e]) : o[k][e];
+        }
+    };
+    for (int u0 = wave; u0 < t.parts; u0 += kWaves * kBatch) {
+        float m[kTurns][kBatch], l[kTurns][kBatch];
+        f32x4 v[kTurns][kBatch];
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k)
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const long from = part_at(k, min(u0 + kWaves * u, t.parts - 1));
+                const f32x2 ml = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * from);
+                m[k][u] = ml[0];
+                l[k][u] = ml[1];
+                v[k][u] = *reinterpret_cast<const f32x4*>(p.part_o + from * D + c4);
+            }
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k)
+            join(k, std::integral_constant<int, kBatch>{}, [&](int u) { return u0 + kWaves * u < t.parts; }, m[k], l[k],
+                 v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+        s_m[wave][k][lane] = top[k];
+        s_l[wave][k][lane] = sum[k];
+        *reinterpret_cast<f32x4*>(&s_o[wave][k][4 * lane]) = o[k];
+    }
+    __syncthreads();
+    if (wave >= kTurns) return;   // wave k: the rows of turn k
+    const int k0 = wave;
+    float m[kWaves], l[kWaves];
+    f32x4 v[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        m[w] = s_m[w][k0][lane];
+        l[w] = s_l[w][k0][lane];
+        v[w] = *reinterpret_cast<const f32x4*>(&s_o[w][k0][4 * lane]);
+    }
+    top[0] = kNoMax;
+    sum[0] = 0.0f;
+    o[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    join(0, std::integral_constant<int, kWaves>{}, [](int) { return true; }, m, l, v);
+    const int r = r0 + k0 * kAtOnce + lane / (D / 4);
+    if (r >= n_rows) return;
+    const float inv = sum[0] > 0.0f || sum[0] != sum[0] ? 1.0f / sum[0] : 0.0f;   // a row without keys is zero
     const int qi = (int)p.gqa.div((uint32_t)r);
     const long q_row = ((long)t.row0 + qi) * p.n_heads + kvh * (int)p.gqa.d + (r - qi * (int)p.gqa.d);
     *reinterpret_cast<u32x2*>(p.out + q_row * D + c4) =
-        u32x2{Hf::pack(o[0] * inv, o[1] * inv), Hf::pack(o[2] * inv, o[3] * inv)};
+        u32x2{Hf::pack(o[0][0] * inv, o[0][1] * inv), Hf::pack(o[0][2] * inv, o[0][3] * inv)};
 }
 
 // ---------------------------------------------------------------- host
@@ -83,6 +136,8 @@ struct PagedTreePlan {
     long row_tiles;      // of the call at most
     int target;
     uint32_t slots;      // 0: nothing is cut
+    int records;         // sequences whose tiles are cut, at most
+    long groups;         // of rows that are joined, at most
     size_t off_o, off_records, bytes;
 };
 
@@ -97,19 +152,20 @@ PagedTreePlan plan_tree(int batch, int rows, int n_heads, int n_kv_heads, int he
         const size_t parts = (size_t)pl.slots * n_kv_heads * kPfRows;
         pl.off_o = align_up(parts * 2 * sizeof(float), 256);
         pl.off_records = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
-        pl.bytes = pl.off_records + pl.slots / 2 * sizeof(CutRecord);
+        pl.records = std::max(std::min({batch, rows, pl.target}), 1);   // (a tile that is cut has two parts at least)
+        pl.groups = all / kJoinRows + pl.records;
+        pl.bytes = pl.off_records + pl.records * sizeof(CutRecord);
     }
     return pl;
 }
 
 template <bool BF, int D>
-void launch_tree(const PagedFlashParams& p, long items, long cut_tiles, hipStream_t stream) {
+void launch_tree(const PagedFlashParams& p, long items, long groups, hipStream_t stream) {
     const unsigned grid = (unsigned)(items * p.c.n_kv_heads);
     if (p.s.cap_x != 0.0f) paged_tree_kernel<BF, D, true><<<grid, kPfThreads, 0, stream>>>(p);
     else paged_tree_kernel<BF, D, false><<<grid, kPfThreads, 0, stream>>>(p);
     if (p.slots == 0) return;
-    const dim3 join((unsigned)(cut_tiles * p.c.n_kv_heads), (unsigned)(kPfRows / join_rows(D)));
-    paged_tree_join_kernel<BF, D><<<join, 256, 0, stream>>>(p);
+    paged_tree_join_kernel<BF, D><<<(unsigned)(groups * p.c.n_kv_heads), 256, 0, stream>>>(p);
 }
 
 }  // namespace
@@ -131,6 +187,7 @@ int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, con
         p.part_ml = reinterpret_cast<float*>(ws);
         p.part_o = reinterpret_cast<float*>(ws + pl.off_o);
         p.records = reinterpret_cast<CutRecord*>(ws + pl.off_records);
+        p.n_records = pl.records;
     }
     p.splits = 1;
     p.observe = INT_MAX;
@@ -141,13 +198,12 @@ int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, con
     p.least = pl.slots > 0 ? kTreeLeast : kUncut;
     p.slots = pl.slots;
     const long items = pl.row_tiles + (pl.slots > 0 ? pl.target : 0);
-    const long cut = std::min(pl.row_tiles, (long)pl.target);   // (a tile that is cut has two parts at least)
     if (a.bf16)
-        a.head_dim == 128 ? launch_tree<true, 128>(p, items, cut, stream)
-                          : launch_tree<true, 64>(p, items, cut, stream);
+        a.head_dim == 128 ? launch_tree<true, 128>(p, items, pl.groups, stream)
+                          : launch_tree<true, 64>(p, items, pl.groups, stream);
     else
-        a.head_dim == 128 ? launch_tree<false, 128>(p, items, cut, stream)
-                          : launch_tree<false, 64>(p, items, cut, stream);
+        a.head_dim == 128 ? launch_tree<false, 128>(p, items, pl.groups, stream)
+                          : launch_tree<false, 64>(p, items, pl.groups, stream);
     return check_launch();
 }
 
