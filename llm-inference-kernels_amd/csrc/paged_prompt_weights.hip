@@ -72,9 +72,21 @@ __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : r
 
 }  // namespace
 
-template <bool BF, int D, bool EXACT>
-__device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t* s_k0, uint8_t* s_k1, uint8_t* s_k2,
-                                          uint32_t& s_last) {
+// What a pass of 128 rows over their keys is for: their statistics, with the parts joined or
+// (where the sums join them) left, or the sums.
+enum class Pass { kStats, kStatParts, kSums };
+
+// What a workgroup keeps in LDS beside three tiles of K; the sums' only but for `last`.
+struct PassLds {
+    float by[kPfRows], inv[kPfRows], slope[kPfRows];   // of the rows
+    int pos[kPfRows];
+    float sum[2][4][kPwTile];                          // a tile's keys', of each wave
+    uint32_t last;
+};
+
+template <bool BF, int D, bool EXACT, Pass PASS>
+__device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t* s_k0, uint8_t* s_k1, uint8_t* s_k2,
+                                         PassLds& s) {
     using Hf = Half16<BF>;
     constexpr int KS = D / 16, CPR = D / 8, kRowBytes = 2 * D;
     constexpr int kCopies = 16 * CPR / 64, kRowsPerCopy = 64 / CPR;
@@ -118,6 +130,8 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
     const int full_hi = (min(end, pos_lo + 1) - begin) >> 6;
     const int seen_lo = (oldest(pos_lo) - begin) >> 6;
     const int seen_hi = live ? ((pos_hi - begin) >> 6) + 1 : INT_MIN;
+    [[maybe_unused]] float* const weights = PASS == Pass::kSums ? weights_of(pw.w, ft.b, kvh) : nullptr;
+    if (PASS == Pass::kSums && (weights == nullptr || tiles == 0)) return;
 
     // ---- copies, as paged_flash's: wave w brings tokens 16 w .. + 15 of every tile ----
     const int* const table_row = p.c.table + (long)ft.b * p.c.max_pages;
@@ -168,9 +182,60 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
 
     const ScoreForm<EXACT> form(p.s);
     float m_run = kNoMax, l_run = 0.0f;   // of row n, this lane's tokens
+    if (tiles > 0) {   // (requested before the rows' statistics are)
+        copy_tile(s_k0, 0);
+        gone_now = gone_next;
+        copy_tile(s_k1, 1);
+    }
+    [[maybe_unused]] float by_row[16], inv_row[16];   // the sums: of rows 8 (e / 4) + 4 h + e % 4 of the wave
+    if constexpr (PASS == Pass::kSums) {
+        // Two threads a row join its parts (every other one each, eight requested at a time).
+        const int row = tid >> 1, rj = r0 + row, rc = min(rj, n_rows - 1), qj = (int)p.gqa.div((uint32_t)rc);
+        const long q_at = ((long)ft.row0 + qj) * p.n_heads + kvh * G + (rc - qj * G);
+        float m = kNoMax, inv = 0.0f;
+        if (ft.parts == 1) {
+            const f32x2 st = pw.stats[q_at];
+            m = st[0];
+            inv = st[1];
+        } else {
+            float l = 0.0f;
+            constexpr int kBatch = 8;
+            for (int u0 = tid & 1; u0 < ft.parts; u0 += 2 * kBatch) {
+                f32x2 ml[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u)
+                    ml[u] = *reinterpret_cast<const f32x2*>(
+                        p.part_ml + 2 * part_row(p, part_slot(ft, min(u0 + 2 * u, ft.parts - 1)), kvh, row));
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (u0 + 2 * u < ft.parts) {
+                        const float top = fmaxf(m, ml[u][0]);
+                        l = l * __builtin_amdgcn_exp2f(m - top) + ml[u][1] * __builtin_amdgcn_exp2f(ml[u][0] - top);
+                        m = top;
+                    }
+                }
+            }
+            const float m2 = dpp_f32<kDppQuadXor1>(m), l2 = dpp_f32<kDppQuadXor1>(l), top = fmaxf(m, m2);
+            l = l * __builtin_amdgcn_exp2f(m - top) + l2 * __builtin_amdgcn_exp2f(m2 - top);
+            m = top;
+            inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        }
+        if ((tid & 1) == 0) {
+            s.by[row] = form.add - m;
+            s.inv[row] = rj < n_rows ? inv : 0.0f;
+            s.pos[row] = rj < n_rows ? ft.ctx + qj : INT_MIN;   // (sees no key)
+            if (p.s.slopes) s.slope[row] = p.s.slopes[kvh * G + (rc - qj * G)] * kLog2eF;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            by_row[e] = s.by[32 * wave + 8 * (e >> 2) + 4 * h + (e & 3)];
+            inv_row[e] = s.inv[32 * wave + 8 * (e >> 2) + 4 * h + (e & 3)];
+        }
+    }
     const uint32_t k_row = (uint32_t)(n * kRowBytes);
     const uint32_t k_sw = (uint32_t)((h ^ swizzle<D>(n)) * 16);
-    auto compute = [&](const uint8_t* sk, int i, uint32_t gone) {
+    auto statistics = [&](const uint8_t* sk, int i, uint32_t gone) {
         const int t0 = begin + kPwTile * i, tk = t0 + 4 * h;
         float sc[32];
 #pragma unroll
@@ -206,30 +271,87 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
         for (int e = 0; e < 32; ++e) sum[e & 3] += __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by));
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     };
+    // The sums: S = Q K^T, a lane has key n of each block and 16 of the wave's rows.
+    auto sums = [&](const uint8_t* sk, int i, uint32_t gone) {
+        const int t0 = begin + kPwTile * i;
+        const bool masked = gone || i < full_lo || i >= full_hi || r_wave + 32 > n_rows;   // wave-uniform
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                acc = Hf::mfma32(qb[ks],
+                                 *reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks))),
+                                 acc);
+            float sc[16], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int key = t0 + 32 * blk + n;
+            auto row_of = [&](int e) { return 32 * wave + 8 * (e >> 2) + 4 * h + (e & 3); };
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = acc[e];
+            form.apply(p.s, sc, [&](int e) { return s.slope[row_of(e)] * (float)(s.pos[row_of(e)] - key); });
+            if (!masked) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sum[e & 3] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by_row[e])), inv_row[e], sum[e & 3]);
+            } else {
+                const bool key_ok = key < end && !((gone >> (4 * blk + (n >> 3))) & 1u);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int at = s.pos[row_of(e)];
+                    const float x = __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by_row[e]));
+                    if (key_ok && at >= key && at - key < p.s.window) sum[e & 3] = fmaf(x, inv_row[e], sum[e & 3]);
+                }
+            }
+            const float all = xor32_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (h == 0) s.sum[i & 1][wave][32 * blk + n] = all;
+        }
+    };
+    // The waves' sums of tile i, added to the weights by the first wave.
+    float weight = 0.0f;   // of the tile before the one computed
+    auto record = [&](int i) {
+        const int key = begin + kPwTile * i + lane;
+        const float all = (s.sum[i & 1][0][lane] + s.sum[i & 1][1][lane]) + (s.sum[i & 1][2][lane] + s.sum[i & 1][3][lane]);
+        if (key < min(end, pw.w.max_len)) weights[key] = weight + all;
+    };
     // Two tiles ahead: a tile's copies are complete once at most the next one's are outstanding (loads
     // complete in order), and for the whole workgroup behind the barrier, where the buffer of the tile
     // before is free.
     auto turn = [&](uint8_t* cur, uint8_t* free, int i) {
         if constexpr (kCopies == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+        if constexpr (PASS == Pass::kSums) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
         const uint32_t gone = gone_now;
         gone_now = gone_next;
+        if constexpr (PASS == Pass::kSums) {
+            if (wave == 0) {   // (before the copies, which the next wait counts)
+                if (i > 0) record(i - 1);
+                weight = weights[min(begin + kPwTile * i + lane, min(end, pw.w.max_len) - 1)];
+            }
+        }
         copy_tile(free, i + 2);
-        if (i >= seen_lo && i < seen_hi) compute(cur, i, gone);
+        const bool sees = i >= seen_lo && i < seen_hi;
+        if constexpr (PASS != Pass::kSums) {
+            if (sees) statistics(cur, i, gone);
+        } else {
+            if (sees) sums(cur, i, gone);
+            else s.sum[i & 1][wave][lane] = 0.0f;
+        }
     };
     static_assert(kCopies == 4 || kCopies == 2, "the wait counts a tile's copies");
-    if (tiles > 0) {
-        copy_tile(s_k0, 0);
-        gone_now = gone_next;
-        copy_tile(s_k1, 1);
-    }
     for (int i = 0; i < tiles; i += 3) {
         turn(s_k0, s_k2, i);
         if (i + 1 < tiles) turn(s_k1, s_k0, i + 1);
         if (i + 2 < tiles) turn(s_k2, s_k1, i + 2);
     }
     __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup
+    if constexpr (PASS == Pass::kSums) {
+        __syncthreads();
+        if (wave == 0) record(tiles - 1);
+        return;
+    }
 
     const float m_row = xor32_max(m_run);
     const float l_row = xor32_sum(l_run * __builtin_amdgcn_exp2f(m_run - m_row));
@@ -241,17 +363,21 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
         if (mine) store(q_row, m_row, l_row);
         return;
     }
+    float* const to = p.part_ml + 2 * part_row(p, part_slot(ft, ft.part), kvh, 32 * wave + n);
+    if constexpr (PASS == Pass::kStatParts) {
+        if (mine) *reinterpret_cast<f32x2*>(to) = f32x2{m_row, l_row};
+        return;
+    }
     if (mine) {
-        float* to = p.part_ml + 2 * part_row(p, part_slot(ft, ft.part), kvh, 32 * wave + n);
         const uint64_t ml = (uint64_t)__float_as_uint(l_row) << 32 | __float_as_uint(m_row);
         __hip_atomic_store(reinterpret_cast<uint64_t*>(to), ml, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     publish_wait();
     __syncthreads();
     uint32_t* const counter = pw.counters + (long)ft.cut * p.c.n_kv_heads + kvh;
-    if (tid == 0) s_last = arrive_last(counter, (uint32_t)ft.parts) ? 1u : 0u;
+    if (tid == 0) s.last = arrive_last(counter, (uint32_t)ft.parts) ? 1u : 0u;
     __syncthreads();
-    if (s_last == 0) return;
+    if (s.last == 0) return;
     if (tid == 0) *counter = 0u;   // for the next call
     const int rj = r0 + tid;
     if (tid >= kPfRows || rj >= n_rows) return;
@@ -277,12 +403,12 @@ __device__ __forceinline__ void row_stats(const PromptWeightsParams& pw, uint8_t
     store(((long)ft.row0 + qj) * p.n_heads + kvh * G + (rj - qj * G), m, l);
 }
 
-template <bool BF, int D, bool EXACT>
-__global__ __launch_bounds__(kPwThreads, 3) void paged_row_stats_kernel(PromptWeightsParams pw) {
+template <bool BF, int D, bool EXACT, Pass PASS>
+__global__ __launch_bounds__(kPwThreads, 3) void paged_row_pass_kernel(PromptWeightsParams pw) {
     __shared__ __attribute__((aligned(16))) uint8_t s_k0[kPwTile * 2 * D], s_k1[kPwTile * 2 * D];
     __shared__ __attribute__((aligned(16))) uint8_t s_k2[kPwTile * 2 * D];
-    __shared__ uint32_t s_last;
-    row_stats<BF, D, EXACT>(pw, s_k0, s_k1, s_k2, s_last);
+    __shared__ __attribute__((aligned(16))) PassLds s;
+    row_pass<BF, D, EXACT, PASS>(pw, s_k0, s_k1, s_k2, s);
 }
 
 // The shares: fixed are key tiles of kPwKeys, cut the row tiles of kPwTile. The host does not
@@ -490,9 +616,10 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
 
 namespace {
 
-// The statistics' key tiles are cut for three workgroups per CU, in parts of four tiles or more: us, 32 rows of
-// 8192 tokens with 2, 4, 8 tiles or more 31.1, 27.1, 27.5; 16 rows of 2000 17.7, 18.1, 21.
-constexpr int kStatsPerCu = 3, kStatsLeast = 4;
+// Key tiles are cut for two workgroups per CU, into single tiles where there are few. us, the last 32 rows of four
+// prompts of 4000 .. 8192 tokens for 1, 2, 3 workgroups 43, 36, 38, the last 16 of 2000 tokens with 1, 2, 4 tiles or
+// more 15.0, 16.0, 19.6, the last 16 of 16 x 4000 for 1, 2, 3 85, 65, 62.
+constexpr int kStatsPerCu = 2, kStatsLeast = 1;
 // The sums' row tiles into four times as many as three per CU where that leaves eight tiles or more, so that the
 // shares even out; us, a prompt of 4000 tokens with 4, 8, 12, 16, 24 per CU 388, 312, 291, 296, 299; into as many
 // as run at once where they are few, of two or more: 600 tokens in parts of 8, 4, 2 33.2, 29.1, 27.0, two prompts of
@@ -502,6 +629,7 @@ constexpr int kSumsPerCu = 3, kSumsParts = 12, kSumsLeast = 8;
 struct PromptWeightsPlan {
     long row_tiles, sum_grid;
     int target, sum_target;
+    bool one_tile;        // a sequence's recorded rows of a KV head are one row tile: its pass sums up whole columns
     uint32_t slots, sum_slots;
     size_t off_ml, off_stats, off_sum, bytes;
 };
@@ -515,6 +643,7 @@ PromptWeightsPlan plan_prompt_weights(int batch, int rows, int n_heads, int n_kv
     pl.slots = 2u * (uint32_t)pl.target;
     pl.sum_target = std::max(kSumsParts * cus / n_kv_heads, 1);
     const long most = (observe > 0 ? std::min(rows, observe) : rows) * (long)(n_heads / n_kv_heads);   // of a sequence
+    pl.one_tile = most <= kPfRows;
     pl.sum_slots = most > 2L * kPwTile ? 2u * (uint32_t)pl.sum_target : 0u;
     // A counter for each cut tile: where they do not suffice (thousands of KV heads), nothing is cut.
     if ((long)(pl.target + pl.sum_target) * n_kv_heads > kMaxCounters) pl.slots = pl.sum_slots = 0;
@@ -529,8 +658,13 @@ PromptWeightsPlan plan_prompt_weights(int batch, int rows, int n_heads, int n_kv
 template <bool BF, int D, bool EXACT>
 void launch_prompt(const PromptWeightsParams& pw, const PromptWeightsPlan& pl, hipStream_t stream) {
     const int hkv = pw.f.c.n_kv_heads;
-    paged_row_stats_kernel<BF, D, EXACT>
-        <<<(unsigned)((pl.row_tiles + pl.target) * hkv), kPwThreads, 0, stream>>>(pw);
+    const unsigned grid = (unsigned)((pl.row_tiles + pl.target) * hkv);
+    if (pl.one_tile) {
+        paged_row_pass_kernel<BF, D, EXACT, Pass::kStatParts><<<grid, kPwThreads, 0, stream>>>(pw);
+        paged_row_pass_kernel<BF, D, EXACT, Pass::kSums><<<grid, kPwThreads, 0, stream>>>(pw);
+        return;
+    }
+    paged_row_pass_kernel<BF, D, EXACT, Pass::kStats><<<grid, kPwThreads, 0, stream>>>(pw);
     paged_key_sums_kernel<BF, D, EXACT><<<(unsigned)pl.sum_grid, kPwThreads, 0, stream>>>(pw);
 }
 

@@ -127,10 +127,12 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
 
 namespace {
 
-// The key tiles are cut for two workgroups per CU, into single tiles where there are few. us, a draft of 8 over 700
-// tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0; 30 drafts of 4 .. 24 over 200 .. 8000 tokens for 256, 384, 512,
-// 768 workgroups 88.6, 70.2, 62.0, 76.3; one of 64 over 8192 28.8, 29.6, 30.4, 38.1.
-constexpr int kTreePerCu = 2, kTreeLeast = 1;
+// Key tiles are cut for two workgroups per CU, or, where there are row tiles for at most a quarter of the CUs, for one:
+// the sums of every part are written and read again, but of many sequences the ends are ragged. us, for 1 and 2
+// workgroups: one draft of 64 over 8192 tokens 28.8, 30.4, of 8 over 30000 37.7, 39.8, four of 16 over 3000 22.5, 24.2,
+// 16 of 32 over 4000 78.7, 73.3, 30 of 4 .. 24 over 200 .. 8000 88.6, 62.0 (for 3 76). Into single tiles where there
+// are few: 8 over 700 tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0.
+constexpr int kTreeLeast = 1;
 
 struct PagedTreePlan {
     long row_tiles;      // of the call at most
@@ -145,7 +147,8 @@ PagedTreePlan plan_tree(int batch, int rows, int n_heads, int n_kv_heads, int he
     PagedTreePlan pl{};
     const long all = (long)rows * (n_heads / n_kv_heads);
     pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min(batch, rows));
-    pl.target = std::max(kTreePerCu * cus / n_kv_heads, 1);
+    const int per_cu = 4 * pl.row_tiles * n_kv_heads <= cus ? 1 : 2;
+    pl.target = std::max(per_cu * cus / n_kv_heads, 1);
     if (capacity > (long)kTreeLeast * kPfTile) {
         // A row tile that is cut has more than one length's tiles: less than twice the target's parts.
         pl.slots = 2u * (uint32_t)pl.target;
