@@ -208,6 +208,7 @@ struct CutItem {
     uint32_t slot;        // of the tile's first part among all parts of tiles that are cut; part i: fixed i further
     uint32_t cut;         // the tile's number among those that are cut
     uint32_t cut_seq, group;   // the sequence's among those with cut tiles; row groups of those before it
+    bool bad;             // its rows' offsets decrease
 };
 // What the kernel that joins the parts knows of a sequence whose tiles are cut: its rows
 // are groups `group` .. of kJoinRows rows; and in the first place how many records there are.
@@ -225,6 +226,7 @@ __device__ __forceinline__ void cut_sequence(const PagedFlashParams& p, int b, C
     const int stop = p.cu[b + 1], len = max(p.c.lens[b], 0);
     s.b = b;
     s.row0 = max(p.cu[b], 0);
+    s.bad = stop < p.cu[b];
     const int all = max(min(stop, p.rows) - s.row0, 0);
     s.rows = min(all, p.observe);
     s.row0 += all - s.rows;
@@ -283,8 +285,10 @@ struct Cutter {
         const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
         const uint32_t target = (uint32_t)target_;
         uint32_t mine = 0, fixed = 0;
+        bool bad = false;
         for (int b = b0; b < b1; ++b) {
             sequence(b, own);
+            bad = bad || own.bad;
             mine += (uint32_t)own.tiles * (uint32_t)own.fixed;
             fixed += (uint32_t)own.fixed;
         }
@@ -292,9 +296,12 @@ struct Cutter {
         length = (uint32_t)least;
         if (few != 0) length = min(length, max(quick_ceil(units, (uint32_t)few), 2u));
         length = max(length, quick_ceil(units, target));
+        // Offsets that decrease give rows to several sequences, more shares than there are workgroups: their
+        // parts would wait for each other in vain.
+        if (__any(bad)) length = kUncut;
         // Every sequence's last part is short, so there are more than the target: where it can be met, twice
         // a greater length for as many as there were.
-        if (per == 1 && lane_u32(wave_scan(fixed), 63) <= target) {
+        if (per == 1 && length < kUncut && lane_u32(wave_scan(fixed), 63) <= target) {
 #pragma unroll
             for (int turn = 0; turn < 2; ++turn) {
                 const uint32_t n = lane_u32(wave_scan((uint32_t)own.fixed * parts_of_length(own.tiles)), 63);
@@ -369,7 +376,7 @@ __device__ __forceinline__ void write_record(CutRecord* to, int n_records, uint3
     CutRecord& r = to[t.cut_seq];
     r.group = (int)t.group;
     r.row0 = t.row0;
-    r.rows = t.slot + (uint32_t)(t.fixed * t.parts) <= slots ? t.rows : 0;   // (none: offsets that decrease)
+    r.rows = t.slot + (uint32_t)(t.fixed * t.parts) <= slots ? t.rows : 0;
     r.fixed = t.fixed;
     r.parts = t.parts;
     r.slot = t.slot;
@@ -513,7 +520,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
         }
         parts = ft.parts;
-        if (parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (offsets that decrease)
+        if (parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (the workspace's end)
         begin = ft.begin + ft.part * ft.part_tiles * kPfTile;
         end = min(ft.end, begin + ft.part_tiles * kPfTile);
         tiles = min(ft.part_tiles, ft.tiles - ft.part * ft.part_tiles);

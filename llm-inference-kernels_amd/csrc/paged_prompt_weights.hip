@@ -105,7 +105,7 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
     const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
     if (!cutter.find(item, ft)) return;
-    if (ft.parts > 1 && (part_slot(ft, ft.parts - 1) >= p.slots || ft.cut >= p.slots / 2)) return;   // (offsets that decrease)
+    if (ft.parts > 1 && (part_slot(ft, ft.parts - 1) >= p.slots || ft.cut >= p.slots / 2)) return;   // (the workspace's end)
 
     const int n_rows = ft.rows * G;
     const int r0 = ft.tile * kPfRows, r_wave = r0 + 32 * wave;
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
         CutItem t{};
         const bool found = cutter.find(wg / (uint32_t)p.c.n_kv_heads, t);
         if (!found) return;
-        // (not: offsets that decrease)
+        // (the workspace's end)
         const bool fits = t.parts == 1 || (part_slot(t, t.parts - 1) < pw.sum_slots && t.cut < pw.sum_slots / 2);
         const int n_rows = t.rows * G;
         const int key0 = t.begin + kPwKeys * t.tile, key_end = min(t.end, key0 + kPwKeys);

@@ -82,11 +82,15 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
         for (int k = 0; k < kTurns; ++k)
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const long from = part_at(k, min(u0 + kWaves * u, t.parts - 1));
-                const f32x2 ml = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * from);
+                f32x2 ml = {kNoMax, 0.0f};
+                v[k][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (u0 + kWaves * u < t.parts) {   // (of the wave)
+                    const long from = part_at(k, u0 + kWaves * u);
+                    ml = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * from);
+                    v[k][u] = *reinterpret_cast<const f32x4*>(p.part_o + from * D + c4);
+                }
                 m[k][u] = ml[0];
                 l[k][u] = ml[1];
-                v[k][u] = *reinterpret_cast<const f32x4*>(p.part_o + from * D + c4);
             }
 #pragma unroll
         for (int k = 0; k < kTurns; ++k)
@@ -149,14 +153,15 @@ PagedTreePlan plan_tree(int batch, int rows, int n_heads, int n_kv_heads, int he
     pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min(batch, rows));
     const int per_cu = 4 * pl.row_tiles * n_kv_heads <= cus ? 1 : 2;
     pl.target = std::max(per_cu * cus / n_kv_heads, 1);
-    if (capacity > (long)kTreeLeast * kPfTile) {
+    pl.records = std::max(std::min({batch, rows, pl.target}), 1);   // (a tile that is cut has two parts at least)
+    pl.groups = all / kJoinRows + pl.records;
+    // (As many rows as no launch of the join holds fill the card uncut.)
+    if (capacity > (long)kTreeLeast * kPfTile && pl.groups * n_kv_heads * 256 < 1L << 32) {
         // A row tile that is cut has more than one length's tiles: less than twice the target's parts.
         pl.slots = 2u * (uint32_t)pl.target;
         const size_t parts = (size_t)pl.slots * n_kv_heads * kPfRows;
         pl.off_o = align_up(parts * 2 * sizeof(float), 256);
         pl.off_records = pl.off_o + align_up(parts * head_dim * sizeof(float), 256);
-        pl.records = std::max(std::min({batch, rows, pl.target}), 1);   // (a tile that is cut has two parts at least)
-        pl.groups = all / kJoinRows + pl.records;
         pl.bytes = pl.off_records + pl.records * sizeof(CutRecord);
     }
     return pl;
