@@ -616,15 +616,19 @@ typedef struct llmik_token_weights {
 } llmik_token_weights;
 
 /*
- * llmik_paged_decode_attention that also adds, for every live key t, the sum of its
- * probabilities over the KV head's query heads to weights[row][kv_head][t]. out has
- * the same bits as llmik_paged_decode_attention's.
+ * llmik_paged_decode_attention (and its workspace, llmik_paged_workspace_size with
+ * prefix_len 0) that also adds, for every live key t, the sum of its probabilities
+ * over the KV head's query heads to weights[row][kv_head][t]. out has the same bits
+ * as llmik_paged_decode_attention's. scratch holds the scores between two launches, 4
+ * bytes per query head and token of the longest sequence that the table and max_len
+ * allow; what it held before or holds afterwards does not matter.
  */
-LLMIK_API size_t llmik_paged_decode_weights_workspace_size(const llmik_paged_cache* cache, int n_heads,
-                                                           const llmik_token_weights* weights);
+LLMIK_API size_t llmik_paged_decode_weights_scratch_size(const llmik_paged_cache* cache, int n_heads,
+                                                         const llmik_token_weights* weights);
 LLMIK_API llmik_status llmik_paged_decode_attention_weights(const llmik_paged_cache* cache, const void* q, void* out,
                                                             int n_heads, const llmik_score_options* options,
-                                                            const llmik_token_weights* weights, void* workspace,
+                                                            const llmik_token_weights* weights, void* scratch,
+                                                            size_t scratch_bytes, void* workspace,
                                                             size_t workspace_bytes, void* stream);
 
 /*

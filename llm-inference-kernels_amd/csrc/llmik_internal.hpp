@@ -186,14 +186,14 @@ size_t paged_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_d
 size_t paged_prefill_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
 size_t paged_prefix_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity, int prefix_len);
 size_t paged_tree_workspace(int batch, int rows, int n_heads, int n_kv_heads, int head_dim, long capacity);
-size_t paged_decode_weights_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity,
-                                      int max_len);
+size_t paged_decode_weights_scratch(int batch, int n_heads, long capacity, int max_len);
 size_t paged_prefill_weights_workspace(int batch, int rows, int n_heads, int n_kv_heads, int observe);
 int launch_paged_append(const PagedAppend& a, hipStream_t stream);
 int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, const int* positions,
                       hipStream_t stream);
 int launch_paged_prefill_weights(const PagedLaunch& a, const PagedWeights& w, int observe, hipStream_t stream);
-int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, hipStream_t stream);
+int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, void* scratch, size_t scratch_bytes,
+                                hipStream_t stream);
 int launch_paged_select(const PagedWeights& w, const int* lens, int batch, int n_kv_heads, int keep, int first,
                         int recent, int* kept, int* new_lens, hipStream_t stream);
 int launch_paged_compact(const PagedLaunch& a, const PagedWeights& w, const int* kept, int kept_heads, int n,

@@ -309,27 +309,28 @@ LLMIK_API llmik_status llmik_paged_tree_attention(const llmik_paged_cache* cache
     return launch_paged_tree(a, tree_mask, words, positions, as_stream(stream));
 }
 
-LLMIK_API size_t llmik_paged_decode_weights_workspace_size(const llmik_paged_cache* cache, int n_heads,
+LLMIK_API size_t llmik_paged_decode_weights_scratch_size(const llmik_paged_cache* cache, int n_heads,
                                                            const llmik_token_weights* weights) {
     if (check_shapes(cache, n_heads) != LLMIK_OK || cache->batch == 0) return 0;
     if (check_weights(weights, cache->batch) != LLMIK_OK) return 0;
-    return paged_decode_weights_workspace(cache->batch, n_heads, cache->n_kv_heads, cache->head_dim,
-                                          capacity_of(*cache), weights->max_len);
+    return paged_decode_weights_scratch(cache->batch, n_heads, capacity_of(*cache), weights->max_len);
 }
 
 LLMIK_API llmik_status llmik_paged_decode_attention_weights(const llmik_paged_cache* cache, const void* q, void* out,
                                                             int n_heads, const llmik_score_options* options,
-                                                            const llmik_token_weights* weights, void* workspace,
+                                                            const llmik_token_weights* weights, void* scratch,
+                                                            size_t scratch_bytes, void* workspace,
                                                             size_t workspace_bytes, void* stream) {
     int st = check_cache(cache, n_heads);
     if (st == LLMIK_OK) st = check_options(options);
     if (st == LLMIK_OK) st = check_weights(weights, cache->batch);
     if (st != LLMIK_OK || cache->batch == 0) return st;
     if ((st = check_q(q, out)) != LLMIK_OK) return st;
+    if (!aligned(scratch, 16)) return misaligned("scratch must be 16-byte aligned");
     PagedLaunch a = launch_of(*cache, q, out, n_heads, *options);
     a.workspace = workspace;
     a.workspace_bytes = workspace_bytes;
-    return launch_paged_decode_weights(a, weights_of(*weights), as_stream(stream));
+    return launch_paged_decode_weights(a, weights_of(*weights), scratch, scratch_bytes, as_stream(stream));
 }
 
 LLMIK_API size_t llmik_paged_prefill_weights_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows,

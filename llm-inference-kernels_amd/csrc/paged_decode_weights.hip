@@ -104,20 +104,16 @@ __global__ __launch_bounds__(kRecordThreads) void paged_record_kernel(PagedDecod
 
 namespace {
 
-struct DecodeWeightsPlan {
-    PagedDecodePlan decode;
-    int score_tokens;
-    size_t off_ml, off_scores, bytes;
+struct ScoresPlan {
+    int tokens;   // of a sequence
+    size_t off_scores, bytes;
 };
 
-DecodeWeightsPlan plan_decode_weights(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity,
-                                      int max_len, int cus) {
-    DecodeWeightsPlan pl{};
-    pl.decode = plan_paged_decode(batch, n_heads, n_kv_heads, head_dim, capacity, cus);
-    pl.score_tokens = (int)align_up((size_t)std::min(capacity, (long)max_len), 64);
-    pl.off_ml = align_up(pl.decode.bytes, 256);
-    pl.off_scores = pl.off_ml + align_up((size_t)batch * n_heads * 2 * sizeof(float), 256);
-    pl.bytes = pl.off_scores + (size_t)batch * n_heads * pl.score_tokens * sizeof(float);
+ScoresPlan plan_scores(int batch, int n_heads, long capacity, int max_len) {
+    ScoresPlan pl{};
+    pl.tokens = (int)align_up((size_t)std::min(capacity, (long)max_len), 64);
+    pl.off_scores = align_up((size_t)batch * n_heads * 2 * sizeof(float), 256);
+    pl.bytes = pl.off_scores + (size_t)batch * n_heads * pl.tokens * sizeof(float);
     return pl;
 }
 
@@ -135,35 +131,36 @@ void launch_scores(const PagedDecodeParams& p, int workgroups, bool uniform, hip
 
 }  // namespace
 
-size_t paged_decode_weights_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, long capacity,
-                                      int max_len) {
-    return plan_decode_weights(batch, n_heads, n_kv_heads, head_dim, capacity, max_len, device_cu_count()).bytes;
+size_t paged_decode_weights_scratch(int batch, int n_heads, long capacity, int max_len) {
+    return plan_scores(batch, n_heads, capacity, max_len).bytes;
 }
 
-int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, hipStream_t stream) {
+int launch_paged_decode_weights(const PagedLaunch& a, const PagedWeights& w, void* scratch, size_t scratch_bytes,
+                                hipStream_t stream) {
     const int cus = device_cu_count();
     const long capacity = std::min((long)a.max_pages * a.page_size, kMaxPagedTokens);
-    const DecodeWeightsPlan pl =
-        plan_decode_weights(a.batch, a.n_heads, a.n_kv_heads, a.head_dim, capacity, w.max_len, cus);
+    const PagedDecodePlan pl = plan_paged_decode(a.batch, a.n_heads, a.n_kv_heads, a.head_dim, capacity, cus);
+    const ScoresPlan sc = plan_scores(a.batch, a.n_heads, capacity, w.max_len);
     if (a.workspace == nullptr || a.workspace_bytes < pl.bytes)
-        return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_decode_weights_workspace_size)");
-    if ((long)pl.decode.workgroups > kMaxCounters)
+        return set_error(LLMIK_ERR_WORKSPACE, "workspace too small (llmik_paged_workspace_size)");
+    if (scratch == nullptr || scratch_bytes < sc.bytes)
+        return set_error(LLMIK_ERR_WORKSPACE, "scratch too small (llmik_paged_decode_weights_scratch_size)");
+    if ((long)pl.workgroups > kMaxCounters)
         return set_error(LLMIK_ERR_UNSUPPORTED, "too many compute units for the workspace's counters");
-    PagedDecodeParams p = paged_decode_params(a, pl.decode);
-    char* ws = static_cast<char*>(a.workspace);
-    p.row_ml = reinterpret_cast<float*>(ws + pl.off_ml);
-    p.scores = reinterpret_cast<float*>(ws + pl.off_scores);
-    p.score_tokens = pl.score_tokens;
+    PagedDecodeParams p = paged_decode_params(a, pl);
+    p.row_ml = static_cast<float*>(scratch);
+    p.scores = reinterpret_cast<float*>(static_cast<char*>(scratch) + sc.off_scores);
+    p.score_tokens = sc.tokens;
     const bool uniform = a.page_size % 32 == 0;
     if (a.bf16)
-        a.head_dim == 128 ? launch_scores<true, 128>(p, pl.decode.workgroups, uniform, stream)
-                          : launch_scores<true, 64>(p, pl.decode.workgroups, uniform, stream);
+        a.head_dim == 128 ? launch_scores<true, 128>(p, pl.workgroups, uniform, stream)
+                          : launch_scores<true, 64>(p, pl.workgroups, uniform, stream);
     else
-        a.head_dim == 128 ? launch_scores<false, 128>(p, pl.decode.workgroups, uniform, stream)
-                          : launch_scores<false, 64>(p, pl.decode.workgroups, uniform, stream);
+        a.head_dim == 128 ? launch_scores<false, 128>(p, pl.workgroups, uniform, stream)
+                          : launch_scores<false, 64>(p, pl.workgroups, uniform, stream);
     const int st = check_launch();
     if (st != LLMIK_OK) return st;
-    const long turns = (long)a.batch * a.n_kv_heads * (pl.score_tokens / kRecordTokens + 2);
+    const long turns = (long)a.batch * a.n_kv_heads * (sc.tokens / kRecordTokens + 2);
     const unsigned grid = (unsigned)std::min(turns, 8L * cus);
     const WeightsView view = weights_view(w, a.n_kv_heads);
     if (w.max_len % 4 == 0 && reinterpret_cast<uintptr_t>(w.weights) % 16 == 0)

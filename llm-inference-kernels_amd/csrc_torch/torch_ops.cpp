@@ -921,8 +921,12 @@ Tensor paged_decode_attention_weights(const Tensor& q, const Tensor& k_cache, co
     Tensor out = at::empty_like(q);
     if (c.batch == 0) return out;
     const hipStream_t st = stream_of(q);
-    const CallWorkspace ws = call_workspace(q, st, llmik_paged_decode_weights_workspace_size(&c, H, &w));
-    check(llmik_paged_decode_attention_weights(&c, ptr(q), ptr(out), H, &o, &w, ws.ptr, ws.bytes, st));
+    const CallWorkspace ws = call_workspace(q, st, llmik_paged_workspace_size(&c, H, 0));
+    // (As long as the table and the weights are: the allocator's, not the stream's workspace.)
+    const size_t scores = llmik_paged_decode_weights_scratch_size(&c, H, &w);
+    const Tensor scratch = at::empty({(int64_t)scores}, q.options().dtype(at::kByte));
+    check(llmik_paged_decode_attention_weights(&c, ptr(q), ptr(out), H, &o, &w, ptr(scratch), scores, ws.ptr, ws.bytes,
+                                               st));
     return out;
 }
 

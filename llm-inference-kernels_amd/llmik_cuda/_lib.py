@@ -97,8 +97,8 @@ _SIGNATURES = {
     "llmik_rope_paged_append_at": (_i, [_p, _p, _p, _p, _i, _i, _p, _p, _p, _i, _i, _p]),
     "llmik_paged_tree_workspace_size": (_sz, [_p, _i, _i]),
     "llmik_paged_tree_attention": (_i, [_p, _p, _p, _p, _i, _p, _p, _i, _i, _p, _p, _sz, _p]),
-    "llmik_paged_decode_weights_workspace_size": (_sz, [_p, _i, _p]),
-    "llmik_paged_decode_attention_weights": (_i, [_p, _p, _p, _i, _p, _p, _p, _sz, _p]),
+    "llmik_paged_decode_weights_scratch_size": (_sz, [_p, _i, _p]),
+    "llmik_paged_decode_attention_weights": (_i, [_p, _p, _p, _i, _p, _p, _p, _sz, _p, _sz, _p]),
     "llmik_paged_prefill_weights_workspace_size": (_sz, [_p, _i, _i, _i]),
     "llmik_paged_prefill_weights": (_i, [_p, _p, _p, _i, _i, _p, _i, _p, _p, _sz, _p]),
     "llmik_paged_select_tokens": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p]),

@@ -20,7 +20,7 @@ def _weights(**more):
 
 def _c_calls(lib, c, o, w, ws=16, n=1 << 60):
     return [lambda: lib.llmik_paged_tree_attention(_at(c), 16, 16, 16, 1, 16, 16, 2, 4, _at(o), ws, n, None),
-            lambda: lib.llmik_paged_decode_attention_weights(_at(c), 16, 16, 4, _at(o), _at(w), ws, n, None),
+            lambda: lib.llmik_paged_decode_attention_weights(_at(c), 16, 16, 4, _at(o), _at(w), 16, n, ws, n, None),
             lambda: lib.llmik_paged_prefill_weights(_at(c), 16, 16, 2, 4, _at(o), 0, _at(w), ws, n, None)]
 
 
@@ -57,7 +57,7 @@ def test_c_layer_refuses_options_and_weights(lib):   # noqa: F811
                      lambda: lib.llmik_paged_select_tokens(_at(bad), 16, 2, 2, 8, 0, 0, 16, 16, None),
                      lambda: lib.llmik_paged_compact(_at(c), 16, 1, 3, 16, _at(bad), None)]:
             assert call() == code and msg in err(), more
-        assert lib.llmik_paged_decode_weights_workspace_size(_at(c), 4, _at(bad)) == 0
+        assert lib.llmik_paged_decode_weights_scratch_size(_at(c), 4, _at(bad)) == 0
 
 
 def test_c_layer_refuses_arguments(lib):   # noqa: F811
@@ -88,13 +88,14 @@ def test_c_layer_refuses_arguments(lib):   # noqa: F811
     assert tree(c=_at(many), rows=1 << 14) == UNSUPPORTED and "capacity" in err()
     assert lib.llmik_paged_tree_workspace_size(_at(many), 4, 1 << 14) == 0
 
-    need = lib.llmik_paged_decode_weights_workspace_size(_at(c), 4, _at(w))
-    assert need > lib.llmik_paged_workspace_size(_at(c), 4, 0)
-    decode = lambda q=16, out=16, ws=16, n=need: lib.llmik_paged_decode_attention_weights(   # noqa: E731
-        _at(c), q, out, 4, _at(o), _at(w), ws, n, None)
+    scratch, need = lib.llmik_paged_decode_weights_scratch_size(_at(c), 4, _at(w)), lib.llmik_paged_workspace_size(_at(c), 4, 0)
+    assert scratch == 2 * 4 * 64 * 4 + 256        # 32 tokens in two pages, in 64s; two numbers a head
+    decode = lambda q=16, out=16, sc=16, m=scratch, ws=16, n=need: lib.llmik_paged_decode_attention_weights(   # noqa: E731
+        _at(c), q, out, 4, _at(o), _at(w), sc, m, ws, n, None)
     assert decode(n=need - 1) == WORKSPACE and decode(ws=None) == WORKSPACE
-    assert decode(q=None) == INVALID and decode(out=24) == ALIGNMENT
-    assert lib.llmik_paged_decode_attention_weights(_at(c), 16, 16, 4, _at(o), None, 16, need, None) == INVALID
+    assert decode(m=scratch - 1) == WORKSPACE and decode(sc=None) == WORKSPACE and "scratch too small" in err()
+    assert decode(q=None) == INVALID and decode(out=24) == ALIGNMENT and decode(sc=24) == ALIGNMENT
+    assert lib.llmik_paged_decode_attention_weights(_at(c), 16, 16, 4, _at(o), None, 16, scratch, 16, need, None) == INVALID
 
     def prompt(**a):
         return lib.llmik_paged_prefill_weights(*{**dict(c=_at(c), q=16, cu=16, rows=2, heads=4, o=_at(o), observe=0,
