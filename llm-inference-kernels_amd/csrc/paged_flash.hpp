@@ -277,28 +277,28 @@ struct Cutter {
         return ((uint32_t)s.rows * p.gqa.d + kJoinRows - 1) / kJoinRows;
     }
     __device__ __forceinline__ int cut_sequences() const { return (int)lane_u32(seqs_upto, 63); }
-    // About `target` parts, of `least` tiles or more; with `few`, of two or more where they are not more than that.
-    __device__ __forceinline__ Cutter(const PagedFlashParams& p_, int target_, int least, int few, F f)
+    // About `target` parts, of `least` tiles or more.
+    __device__ __forceinline__ Cutter(const PagedFlashParams& p_, int target_, int least, F f)
         : p(p_), sequence(f) {
         const int lane = threadIdx.x & 63;
         per = (p.c.batch + 63) / 64;
         const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
         const uint32_t target = (uint32_t)target_;
-        uint32_t mine = 0, fixed = 0;
+        uint64_t mine = 0;
+        uint32_t fixed = 0;
         bool bad = false;
         for (int b = b0; b < b1; ++b) {
             sequence(b, own);
             bad = bad || own.bad;
-            mine += (uint32_t)own.tiles * (uint32_t)own.fixed;
+            mine += (uint64_t)(uint32_t)own.tiles * (uint32_t)own.fixed;
             fixed += (uint32_t)own.fixed;
         }
-        const uint32_t units = lane_u32(wave_scan(mine), 63);
-        length = (uint32_t)least;
-        if (few != 0) length = min(length, max(quick_ceil(units, (uint32_t)few), 2u));
-        length = max(length, quick_ceil(units, target));
+        const bool many = mine >= 1u << 24;
+        const uint32_t units = lane_u32(wave_scan(many ? 0u : (uint32_t)mine), 63);
+        length = max((uint32_t)least, quick_ceil(units, target));
         // Offsets that decrease give rows to several sequences, more shares than there are workgroups: their
-        // parts would wait for each other in vain.
-        if (__any(bad)) length = kUncut;
+        // parts would wait for each other in vain. And so many tiles fill the card.
+        if (__any(bad || many)) length = kUncut;
         // Every sequence's last part is short, so there are more than the target: where it can be met, twice
         // a greater length for as many as there were.
         if (per == 1 && length < kUncut && lane_u32(wave_scan(fixed), 63) <= target) {
@@ -437,7 +437,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         bool found;
         if constexpr (TREE) {
             auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
-            const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
+            const Cutter<decltype(sequence)> cutter(p, p.target, p.least, sequence);
             found = cutter.find(item, ft);
             if (p.slots != 0 && kvh == 0 && tid == 0)
                 write_record(p.records, p.n_records, p.slots, wg == 0, cutter.cut_sequences(), found, ft);

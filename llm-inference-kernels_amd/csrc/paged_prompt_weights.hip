@@ -6,8 +6,10 @@
 // other through LDS:
 //   statistics: 128 rows (32 per wave) over the keys in tiles of 64. S^T = K Q^T gives
 //     a lane one row's scores, so its maximum and sum stay in the lane.
-//   sums: 128 keys (32 per wave) over the rows in tiles of 64. S = Q K^T gives a lane
-//     one key's scores, so its sum of 2^(s - m) / l stays in the lane.
+//   sums: 128 keys (32 per wave) over the rows in tiles of 64. S^T = K Q^T again: a lane
+//     has one row's m and 1 / l in registers and sums 2^(s - m) / l of its 16 keys; the
+//     lanes are added once, behind the last tile. (S = Q K^T leaves a key's sum in one lane,
+//     but reads 16 rows' m and 1 / l from LDS for 16 scores.)
 // Both cut their streamed axis where there are few tiles of the other (Cutter). The parts
 // of a cut row or key tile are joined, in order, by the last of its workgroups to arrive:
 // nothing depends on timing.
@@ -18,16 +20,17 @@ namespace llmik {
 constexpr int kPwThreads = 256;
 constexpr int kPwKeys = 128;     // of a workgroup of the sums
 constexpr int kPwTile = 64;      // rows or keys of a streamed tile
+constexpr int kSumsLeast = 2;    // pairs of a workgroup of the sums at least
 
 struct PromptWeightsParams {
     PagedFlashParams f;          // target, least and slots: the statistics' cuts
-    f32x2* stats;                // [rows, n_heads]: (maximum, 1 / sum)
+    f32x2* stats;                // [n_kv_heads, rows, G]: (maximum, 1 / sum); where that is no number, (that, 1)
     uint32_t* counters;          // of the cut tiles [slots / 2, n_kv_heads], zero between calls
-    uint32_t* sum_counters;      // [sum_slots / 2, n_kv_heads]
+    uint32_t* sum_counters;      // [sum_items, n_kv_heads]
     WeightsView w;
-    float* part_sum;             // [sum_slots, n_kv_heads, kPwKeys]
-    int sum_target, sum_least, sum_few;
-    uint32_t sum_slots;
+    float* part_sum;             // [2 sum_items, n_kv_heads, kPwKeys]
+    int sum_items;               // workgroups of the sums for a KV head
+    double sum_rate;             // 1 / sum_items
 };
 
 namespace {
@@ -103,7 +106,7 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
         item = (2 * turn_no + 1) * turn_items - 1 - item;
     CutItem ft{};
     auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
-    const Cutter<decltype(sequence)> cutter(p, p.target, p.least, 0, sequence);
+    const Cutter<decltype(sequence)> cutter(p, p.target, p.least, sequence);
     if (!cutter.find(item, ft)) return;
     if (ft.parts > 1 && (part_slot(ft, ft.parts - 1) >= p.slots || ft.cut >= p.slots / 2)) return;   // (the workspace's end)
 
@@ -114,6 +117,7 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     const int qi = (int)p.gqa.div((uint32_t)r);
     const int head = kvh * G + (r - qi * G);
     const long q_row = ((long)ft.row0 + qi) * p.n_heads + head;
+    const long st_row = ((long)kvh * p.rows + ft.row0) * G;   // of the sequence's first row
     const int pos = ft.ctx + qi;
     auto pos_of = [&](int row) { return ft.ctx + (int)p.gqa.div((uint32_t)min(row, n_rows - 1)); };
     const int pos_lo = __builtin_amdgcn_readfirstlane(pos_of(r_wave));
@@ -191,10 +195,9 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     if constexpr (PASS == Pass::kSums) {
         // Two threads a row join its parts (every other one each, eight requested at a time).
         const int row = tid >> 1, rj = r0 + row, rc = min(rj, n_rows - 1), qj = (int)p.gqa.div((uint32_t)rc);
-        const long q_at = ((long)ft.row0 + qj) * p.n_heads + kvh * G + (rc - qj * G);
         float m = kNoMax, inv = 0.0f;
         if (ft.parts == 1) {
-            const f32x2 st = pw.stats[q_at];
+            const f32x2 st = pw.stats[st_row + rc];
             m = st[0];
             inv = st[1];
         } else {
@@ -356,11 +359,11 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     const float m_row = xor32_max(m_run);
     const float l_row = xor32_sum(l_run * __builtin_amdgcn_exp2f(m_run - m_row));
     auto store = [&](long at, float m, float l) {
-        pw.stats[at] = f32x2{m, l > 0.0f || l != l ? 1.0f / l : 0.0f};
+        pw.stats[at] = l != l ? f32x2{l, 1.0f} : f32x2{m, l > 0.0f ? 1.0f / l : 0.0f};
     };
     const bool mine = h == 0 && r_wave + n < n_rows;
     if (ft.parts == 1) {
-        if (mine) store(q_row, m_row, l_row);
+        if (mine) store(st_row + r, m_row, l_row);
         return;
     }
     float* const to = p.part_ml + 2 * part_row(p, part_slot(ft, ft.part), kvh, 32 * wave + n);
@@ -399,8 +402,7 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
             m = top;   // (a part that is repeated has no greater maximum)
         }
     }
-    const int qj = (int)p.gqa.div((uint32_t)rj);
-    store(((long)ft.row0 + qj) * p.n_heads + kvh * G + (rj - qj * G), m, l);
+    store(st_row + rj, m, l);
 }
 
 template <bool BF, int D, bool EXACT, Pass PASS>
@@ -411,11 +413,50 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_row_pass_kernel(PromptWei
     row_pass<BF, D, EXACT, PASS>(pw, s_k0, s_k1, s_k2, s);
 }
 
-// The shares: fixed are key tiles of kPwKeys, cut the row tiles of kPwTile. The host does not
-// know how many there are, and they differ (a key's rows begin at its own position): the
-// workgroups take one each turn, the last rows' first, every other turn in the reverse order,
-// so that who has many rows has few next. (From a queue in memory: 0.015 us for each of all
-// shares.)
+// The work of the sums is a list of (key tile of kPwKeys, row tile of kPwTile) pairs, key tile by
+// key tile, of which every workgroup of a KV head takes the same number, one after the other: where
+// that ends inside a key tile the next workgroup goes on. Key tile i of a sequence is seen by row
+// tiles first(i) .. last(i) - 1, which move by 2 G from one to the next until they reach the rows'
+// end, so that a sequence's pairs up to any key tile are a closed sum.
+struct KeySeq {
+    int b, row0, rows, ctx;   // as CutItem's
+    int begin, end;           // the keys that are recorded
+    int keys, row_tiles;      // key tiles, row tiles
+    long lo, hi;              // first(0) and last(0), which may lie outside the rows
+    int at_lo, at_hi;         // key tiles from which on lo + 2 G i >= 0, hi + 2 G i >= row_tiles (or `keys`)
+
+    __device__ __forceinline__ int first(int i, int G) const { return (int)max(lo + 2L * G * i, 0L); }
+    __device__ __forceinline__ int last(int i, int G) const { return (int)min(hi + 2L * G * i, (long)row_tiles); }
+    // The pairs of the first n key tiles.
+    __device__ __forceinline__ long pairs(int n, int G) const {
+        const long below = max(n - at_lo, 0), moving = min(n, at_hi);
+        return moving * (hi + G * (moving - 1)) + (n - moving) * row_tiles - below * (lo + G * (at_lo + n - 1L));
+    }
+};
+
+__device__ __forceinline__ void key_sequence(const PromptWeightsParams& pw, int b, KeySeq& s) {
+    const PagedFlashParams& p = pw.f;
+    const int G = (int)p.gqa.d;
+    CutItem t;
+    cut_sequence(p, b, t);
+    s.b = b;
+    s.row0 = t.row0;
+    s.rows = t.rows;
+    s.ctx = t.ctx;
+    s.begin = t.begin;
+    s.end = min(min(t.end, pw.w.max_len), t.ctx + t.rows);
+    s.row_tiles = (int)((uint32_t)(t.rows * G + kPwTile - 1) / kPwTile);
+    // The first key lies d tokens behind the first row, and `reach` in front of the first that sees none of its tile.
+    const long d = (long)s.begin - s.ctx, reach = d + kPwKeys - 1 + p.s.window;
+    s.lo = (d * G) >> 6;
+    s.hi = min((reach * G + kPwTile - 1) >> 6, (long)s.row_tiles);
+    const bool recorded = t.rows > 0 && s.end > s.begin && s.hi > 0 && weights_of(pw.w, b, 0) != nullptr;
+    s.keys = recorded ? (s.end - s.begin + kPwKeys - 1) / kPwKeys : 0;
+    auto tiles_to = [&](long keys) { return (int)min(max(keys + kPwKeys - 1, 0L) / kPwKeys, (long)s.keys); };
+    s.at_lo = tiles_to(-d);
+    s.at_hi = tiles_to(t.rows - reach);
+}
+
 template <bool BF, int D, bool EXACT>
 __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWeightsParams pw) {
     using Hf = Half16<BF>;
@@ -423,6 +464,8 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
     constexpr int kCopies = 16 * CPR / 64, kRowsPerCopy = 64 / CPR;
     __shared__ __attribute__((aligned(16))) uint8_t s_q0[kPwTile * kRowBytes], s_q1[kPwTile * kRowBytes];
     __shared__ uint32_t s_last;
+    __shared__ KeySeq s_seq[64];   // the last of sequences per * l .. per * l + per - 1
+    __shared__ long s_upto[64];    // the pairs up to its end
     __shared__ __attribute__((aligned(16))) float s_by[2][kPwTile], s_inv[2][kPwTile], s_slope[2][kPwTile];
     __shared__ __attribute__((aligned(16))) int s_pos[2][kPwTile];
     const PagedFlashParams& p = pw.f;
@@ -433,29 +476,80 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
     const ScoreForm<EXACT> form(p.s);
     const uint32_t q_at = (uint32_t)(n * kRowBytes);
     const uint32_t q_sw = (uint32_t)((h ^ swizzle<D>(n)) * 16);
-    auto sequence = [&](int b, CutItem& s) {
-        cut_sequence(p, b, s);
-        s.fixed = s.rows > 0 ? (s.end - s.begin + kPwKeys - 1) / kPwKeys : 0;
-        s.tiles = (int)((uint32_t)(s.rows * G + kPwTile - 1) / kPwTile);
-    };
-    const Cutter<decltype(sequence)> cutter(p, pw.sum_target, pw.sum_least, pw.sum_few, sequence);
-    for (uint32_t turn_no = 0;; ++turn_no) {
-        const uint32_t wg = turn_no * gridDim.x + (turn_no & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        const int kvh = (int)(wg % (uint32_t)p.c.n_kv_heads);
-        CutItem t{};
-        const bool found = cutter.find(wg / (uint32_t)p.c.n_kv_heads, t);
-        if (!found) return;
-        // (the workspace's end)
-        const bool fits = t.parts == 1 || (part_slot(t, t.parts - 1) < pw.sum_slots && t.cut < pw.sum_slots / 2);
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.c.n_kv_heads), item = (int)(blockIdx.x / (uint32_t)p.c.n_kv_heads);
+    const int per = (p.c.batch + 63) / 64;
+    if (wave == 0) {
+        long upto = 0;
+        KeySeq s{};
+        for (int b = min(lane * per, p.c.batch); b < min(lane * per + per, p.c.batch); ++b) {
+            key_sequence(pw, b, s);
+            upto += s.pairs(s.keys, G);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long other = __shfl_up(upto, d);
+            if (lane >= d) upto += other;
+        }
+        s_seq[lane] = s;
+        s_upto[lane] = upto;
+    }
+    __syncthreads();
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    auto uniform64 = [&](long x) { return (long)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x); };
+    const long pairs = uniform64(s_upto[63]);
+    long chunk = (long)((double)pairs * pw.sum_rate);
+    if (chunk * pw.sum_items < pairs) ++chunk;
+    chunk = max(chunk, (long)kSumsLeast);
+    chunk = uniform64(chunk);
+    const long stop = min(pairs, (item + 1) * chunk);
+    for (long at = item * chunk; at < stop;) {
+        // ---- the pair `at`: its sequence, its key tile, its row tile ----
+        const int lane_at = __popcll(__ballot(s_upto[lane] <= at));
+        KeySeq t = s_seq[lane_at];
+        long into = at;   // the pair's number among its sequence's
+        if (per == 1) into -= s_upto[lane_at] - t.pairs(t.keys, G);
+        else {
+            into -= lane_at > 0 ? s_upto[lane_at - 1] : 0L;
+            for (int b = lane_at * per;; ++b) {   // ends: the lane's sequences hold the pair
+                key_sequence(pw, b, t);
+                const long n = t.pairs(t.keys, G);
+                if (into < n || b + 1 >= min(lane_at * per + per, p.c.batch)) break;
+                into -= n;
+            }
+        }
+        into = uniform64(into);
+        t.b = uniform(t.b);
+        t.row0 = uniform(t.row0);
+        t.rows = uniform(t.rows);
+        t.ctx = uniform(t.ctx);
+        t.begin = uniform(t.begin);
+        t.end = uniform(t.end);
+        t.keys = uniform(t.keys);
+        t.row_tiles = uniform(t.row_tiles);
+        t.lo = uniform64(t.lo);
+        t.hi = uniform64(t.hi);
+        t.at_lo = uniform(t.at_lo);
+        t.at_hi = uniform(t.at_hi);
+        int tile = 0;
+        for (int n = t.keys; n > 1;) {   // the last with pairs(tile) <= into, among n: 64 of them at once
+            const int step = (n + 63) / 64, probe = min((lane + 1) * step, n);
+            const int more = __popcll(__ballot(probe < n && t.pairs(tile + probe, G) <= into)) * step;
+            tile += more;
+            n = min(n - more, step);
+        }
+        const int rt0 = t.first(tile, G), of_tile = t.last(tile, G) - rt0;
+        const int before = (int)(into - t.pairs(tile, G));
+        const int tiles = (int)min((long)(of_tile - before), stop - at), after = of_tile - before - tiles;
+        at += tiles;
+        // Its parts: this one, and those of the workgroups before and behind (all but the last take `chunk`).
+        const uint32_t length = (uint32_t)min(chunk, 1L << 30);
+        const int part = (int)quick_ceil((uint32_t)before, length);
+        const int parts = part + 1 + (int)quick_ceil((uint32_t)after, length);
+        const int item0 = item - part;   // that of the first
         const int n_rows = t.rows * G;
-        const int key0 = t.begin + kPwKeys * t.tile, key_end = min(t.end, key0 + kPwKeys);
-        // The part's rows that see one of the keys: positions key0 .. key_end - 1 + window - 1.
-        const int qi_lo = max(key0 - t.ctx, 0);
-        const int qi_hi = (int)min((long)t.rows, (long)key_end - 1 + p.s.window - t.ctx);
-        const int part0 = t.part * t.part_tiles * kPwTile;
-        const int r_lo = max((int)min((long)qi_lo * G, (long)n_rows) / kPwTile * kPwTile, part0);
-        const int r_hi = min(max(qi_hi, 0) * G, part0 + t.part_tiles * kPwTile);
-        const int tiles = fits && r_hi > r_lo ? (r_hi - r_lo + kPwTile - 1) / kPwTile : 0;
+        const int key0 = t.begin + kPwKeys * tile, key_end = min(t.end, key0 + kPwKeys);
+        const int r_lo = kPwTile * (rt0 + before);
+        const int r_hi = min((int)min((long)t.rows, (long)key_end - 1 + p.s.window - t.ctx) * G, r_lo + kPwTile * tiles);
 
         // ---- the wave's keys ----
         const int key_w = key0 + 32 * wave, key = key_w + n;
@@ -469,40 +563,55 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
             for (int ks = 0; ks < KS; ++ks) kb[ks] = load16(from + 16 * ks);
         }
 
-        // Its weight so far (read by all of a key tile's parts: the last one adds).
+        // Lane (h, n < 16) adds key `own` of the wave's in the end. Its weight so far (read by all of a key tile's
+        // parts: the last one adds).
+        const int own = 8 * ((n & 15) >> 2) + 4 * h + (n & 3);
+        const uint32_t keys_ok = (uint32_t)__ballot(key_ok);
         float* to = nullptr;
-        float before = 0.0f;
-        if (h == 0 && key_ok && key < pw.w.max_len) {
+        float weight = 0.0f;
+        if (n < 16 && keys_ok >> own & 1u && key_w + own < pw.w.max_len) {
             to = weights_of(pw.w, t.b, kvh);
-            if (to != nullptr) before = *(to += key);
+            if (to != nullptr) weight = *(to += key_w + own);
         }
 
         // ---- rows of a tile: wave w brings 16 w .. + 15; threads 0 .. 63 their numbers ----
         const uint16_t* const q_seq = p.q + ((long)t.row0 * p.n_heads + kvh * G) * D;
+        const f32x2* const st_seq = pw.stats + ((long)kvh * p.rows + t.row0) * G;
         const int crow = lane / CPR, cslot = lane % CPR;
+        // The next tile's first row: its query token, its head. Where G divides a tile the rows lie alike in all
+        // tiles (and the look-up of their places was a fifth of the vector work).
+        const int step_q = (int)p.gqa.div((uint32_t)kPwTile), step_head = kPwTile - step_q * G;
+        int next_q = __builtin_amdgcn_readfirstlane((int)p.gqa.div((uint32_t)r_lo)), next_head = r_lo - next_q * G;
+        uint32_t place[kCopies];
         auto copy_tile = [&](uint8_t* dst, int i) {
             if (i >= tiles) return;
-            const int r0 = r_lo + kPwTile * i;
-            const int q0 = __builtin_amdgcn_readfirstlane((int)p.gqa.div((uint32_t)r0));
-            const __amdgpu_buffer_rsrc_t rq = make_buffer_rsrc(q_seq + (long)q0 * p.n_heads * D, 0xFFFFFFFFu);
+            if (i == 0 || step_head != 0) {
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-                const int trow = 16 * wave + kRowsPerCopy * c + crow;
-                const int r = min(r0 + trow, n_rows - 1);   // rows past the end repeat the last
-                const int qi = (int)p.gqa.div((uint32_t)r);
-                const uint32_t at = (uint32_t)((qi - q0) * p.n_heads + (r - qi * G)) * kRowBytes;
+                for (int c = 0; c < kCopies; ++c) {
+                    const int trow = 16 * wave + kRowsPerCopy * c + crow, r = next_head + trow;
+                    const int qi = (int)p.gqa.div((uint32_t)r);
+                    place[c] = (uint32_t)(qi * p.n_heads + (r - qi * G)) * kRowBytes + 16u * (uint32_t)(cslot ^ swizzle<D>(trow));
+                }
+            }
+            // (Rows behind the sequence's last token lie outside the buffer's range: zeros.)
+            const long left = (long)(t.rows - next_q) * p.n_heads * kRowBytes;
+            const __amdgpu_buffer_rsrc_t rq = make_buffer_rsrc(q_seq + (long)next_q * p.n_heads * D,
+                                                               (uint32_t)min(left, 0xFFFFFFFFl));
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     rq, (__attribute__((address_space(3))) void*)(dst + (16 * wave + kRowsPerCopy * c) * kRowBytes), 16,
-                    (int)(at + 16 * (cslot ^ swizzle<D>(trow))), 0, 0, 0);
+                    (int)place[c], 0, 0, 0);
+            next_q += step_q;
+            next_head += step_head;
+            if (next_head >= G) {
+                next_head -= G;
+                ++next_q;
             }
         };
         f32x2 st = {0.0f, 0.0f};
         auto load_stats = [&](int i) {
-            const int r = r_lo + kPwTile * i + tid;
-            if (tid < kPwTile && i < tiles) {
-                const int rc = min(r, n_rows - 1), qi = (int)p.gqa.div((uint32_t)rc);
-                st = pw.stats[((long)t.row0 + qi) * p.n_heads + kvh * G + (rc - qi * G)];
-            }
+            if (tid < kPwTile && i < tiles) st = st_seq[min(r_lo + kPwTile * i + tid, n_rows - 1)];
         };
         auto put_stats = [&](int i) {
             if (tid < kPwTile && i < tiles) {
@@ -515,52 +624,52 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
             }
         };
 
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // of key n, this lane's rows
+        float sum[16] = {};   // of keys 8 (e / 4) + 4 h + e % 4, rows n of the blocks
         auto compute = [&](const uint8_t* sq, int i) {
             const int r0 = r_lo + kPwTile * i, at = i & 1;
             const int pos_lo = t.ctx + (int)p.gqa.div((uint32_t)r0);
             const int pos_hi = t.ctx + (int)p.gqa.div((uint32_t)min(r0 + kPwTile, r_hi) - 1u);
             if (pos_hi < key_w || key_w >= key_end) return;   // wave-uniform
             const bool full = r0 + kPwTile <= r_hi && pos_lo >= key_w + 31 && pos_hi - key_w < p.s.window;
+            // The rows' operands, eight products ahead.
+            u32x4 qa[2][KS];
+            auto load_q = [&](int blk, int ks) {
+                qa[blk][ks] = *reinterpret_cast<const u32x4*>(sq + q_at + 32 * blk * kRowBytes + (q_sw ^ (32u * ks)));
+            };
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) load_q(0, ks);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
                 f32x16 acc;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    acc = Hf::mfma32(
-                        *reinterpret_cast<const u32x4*>(sq + q_at + 32 * blk * kRowBytes + (q_sw ^ (32u * ks))), kb[ks],
-                        acc);
-                float sc[16], by[16], inv[16];
-                auto row_of = [&](int e) { return 32 * blk + 8 * (e >> 2) + 4 * h + (e & 3); };
+                for (int ks = 0; ks < KS; ++ks) {
+                    acc = Hf::mfma32(kb[ks], qa[blk][ks], acc);
+                    if (blk == 0) load_q(1, ks);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int row = 32 * blk + n, key0 = key_w + 4 * h;
+                const float by = s_by[at][row], inv = s_inv[at][row];
+                float sc[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[e] = acc[e];
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const f32x4 b4 = *reinterpret_cast<const f32x4*>(&s_by[at][row_of(e)]);
-                    const f32x4 i4 = *reinterpret_cast<const f32x4*>(&s_inv[at][row_of(e)]);
-#pragma unroll
-                    for (int e2 = 0; e2 < 4; ++e2) {
-                        by[e + e2] = b4[e2];
-                        inv[e + e2] = i4[e2];
-                    }
-                }
                 form.apply(p.s, sc, [&](int e) {
-                    return s_slope[at][row_of(e)] * (float)(s_pos[at][row_of(e)] - key);
+                    return s_slope[at][row] * (float)(s_pos[at][row] - (key0 + 8 * (e >> 2) + (e & 3)));
                 });
-                if (full) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        sum[e & 3] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by[e])), inv[e], sum[e & 3]);
-                } else {
+                for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by));
+                if (!full) {
+                    const int pos = s_pos[at][row];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int pos = s_pos[at][row_of(e)];
-                        const float x = __builtin_amdgcn_exp2f(fmaf(sc[e], form.mult, by[e]));
-                        if (pos >= key && pos - key < p.s.window) sum[e & 3] = fmaf(x, inv[e], sum[e & 3]);
+                        const int k = key0 + 8 * (e >> 2) + (e & 3);
+                        if (pos < k || pos - k >= p.s.window) sc[e] = 0.0f;
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum[e] = fmaf(sc[e], inv, sum[e]);
             }
         };
         auto turn = [&](uint8_t* cur, uint8_t* far, int i) {
@@ -579,36 +688,46 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
             turn(s_q0, s_q1, i);
             if (i + 1 < tiles) turn(s_q1, s_q0, i + 1);
         }
-        const float all = xor32_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        if (t.parts == 1) {
-            if (to != nullptr && tiles > 0) *to = before + all;
-        } else if (fits) {
+        // The rows' 32 classes together: a lane passes on the half of its keys that the other's bit of n names.
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+            for (int e = 0; e < w; ++e) {
+                const float keep = n & w ? sum[e + w] : sum[e], give = n & w ? sum[e] : sum[e + w];
+                sum[e] = keep + __shfl_xor(give, w);
+            }
+        const float all = sum[0] + __shfl_xor(sum[0], 16);
+        if (parts == 1) {
+            if (to != nullptr) *to = weight + all;
+        } else {
             // The last of the key tile's workgroups to arrive adds its parts, in order.
+            // A workgroup's last key tile, which the next one continues, has its odd slot, its first the even one.
             auto part_at = [&](int part, int i) {
-                return pw.part_sum + ((long)part_slot(t, part) * p.c.n_kv_heads + kvh) * kPwKeys + i;
+                const long slot = 2L * (item0 + part) + (part == 0 ? 1 : 0);
+                return pw.part_sum + (slot * p.c.n_kv_heads + kvh) * kPwKeys + i;
             };
-            if (h == 0) publish_store(part_at(t.part, 32 * wave + n), all);
+            if (n < 16) publish_store(part_at(part, 32 * wave + own), all);
             publish_wait();
             __syncthreads();
-            uint32_t* const counter = pw.sum_counters + (long)t.cut * p.c.n_kv_heads + kvh;
-            if (tid == 0) s_last = arrive_last(counter, (uint32_t)t.parts) ? 1u : 0u;
+            uint32_t* const counter = pw.sum_counters + (long)item0 * p.c.n_kv_heads + kvh;
+            if (tid == 0) s_last = arrive_last(counter, (uint32_t)parts) ? 1u : 0u;
             __syncthreads();
             if (s_last != 0) {
                 if (tid == 0) *counter = 0u;   // for the next call
                 float sum = 0.0f;
                 constexpr int kBatch = 8;   // requested at a time
-                for (int u0 = 0; u0 < t.parts; u0 += kBatch) {
+                for (int u0 = 0; u0 < parts; u0 += kBatch) {
                     float x[kBatch];
 #pragma unroll
-                    for (int u = 0; u < kBatch; ++u) x[u] = publish_load(part_at(min(u0 + u, t.parts - 1), 32 * wave + n));
+                    for (int u = 0; u < kBatch; ++u) x[u] = publish_load(part_at(min(u0 + u, parts - 1), 32 * wave + own));
 #pragma unroll
-                    for (int u = 0; u < kBatch; ++u) sum += u0 + u < t.parts ? x[u] : 0.0f;
+                    for (int u = 0; u < kBatch; ++u) sum += u0 + u < parts ? x[u] : 0.0f;
                 }
-                if (to != nullptr) *to = before + sum;
+                if (to != nullptr) *to = weight + sum;
             }
         }
         __builtin_amdgcn_s_waitcnt(0);   // no copy into LDS outlives the workgroup, and
-        __syncthreads();   // the tiles are read before the next share's are copied
+        __syncthreads();   // the tiles are read before the next ones are copied
     }
 }
 
@@ -620,17 +739,14 @@ namespace {
 // prompts of 4000 .. 8192 tokens for 1, 2, 3 workgroups 43, 36, 38, the last 16 of 2000 tokens with 1, 2, 4 tiles or
 // more 15.0, 16.0, 19.6, the last 16 of 16 x 4000 for 1, 2, 3 85, 65, 62.
 constexpr int kStatsPerCu = 2, kStatsLeast = 1;
-// The sums' row tiles into four times as many as three per CU where that leaves eight tiles or more, so that the
-// shares even out; us, a prompt of 4000 tokens with 4, 8, 12, 16, 24 per CU 388, 312, 291, 296, 299; into as many
-// as run at once where they are few, of two or more: 600 tokens in parts of 8, 4, 2 33.2, 29.1, 27.0, two prompts of
-// 1500 tokens of 8, 6 94, 108.
-constexpr int kSumsPerCu = 3, kSumsParts = 12, kSumsLeast = 8;
+// Three workgroups of the sums run on a CU at once.
+constexpr int kSumsPerCu = 3;
 
 struct PromptWeightsPlan {
-    long row_tiles, sum_grid;
-    int target, sum_target;
+    long row_tiles;
+    int target, sum_items;
     bool one_tile;        // a sequence's recorded rows of a KV head are one row tile: its pass sums up whole columns
-    uint32_t slots, sum_slots;
+    uint32_t slots;
     size_t off_ml, off_stats, off_sum, bytes;
 };
 
@@ -641,17 +757,18 @@ PromptWeightsPlan plan_prompt_weights(int batch, int rows, int n_heads, int n_kv
     pl.row_tiles = std::min((all + (long)batch * (kPfRows - 1)) / kPfRows, all / kPfRows + std::min((long)batch, seen));
     pl.target = std::max(kStatsPerCu * cus / n_kv_heads, 1);
     pl.slots = 2u * (uint32_t)pl.target;
-    pl.sum_target = std::max(kSumsParts * cus / n_kv_heads, 1);
+    pl.sum_items = std::max(kSumsPerCu * cus / n_kv_heads, 1);
     const long most = (observe > 0 ? std::min(rows, observe) : rows) * (long)(n_heads / n_kv_heads);   // of a sequence
     pl.one_tile = most <= kPfRows;
-    pl.sum_slots = most > 2L * kPwTile ? 2u * (uint32_t)pl.sum_target : 0u;
     // A counter for each cut tile: where they do not suffice (thousands of KV heads), nothing is cut.
-    if ((long)(pl.target + pl.sum_target) * n_kv_heads > kMaxCounters) pl.slots = pl.sum_slots = 0;
-    pl.sum_grid = (long)kSumsPerCu * cus;
+    if ((long)(pl.target + pl.sum_items) * n_kv_heads > kMaxCounters) {
+        pl.slots = 0;
+        pl.sum_items = 1;
+    }
     pl.off_ml = kCounterBytes;
     pl.off_stats = pl.off_ml + align_up((size_t)pl.slots * n_kv_heads * kPfRows * 2 * sizeof(float), 256);
     pl.off_sum = pl.off_stats + align_up((size_t)rows * n_heads * 2 * sizeof(float), 256);
-    pl.bytes = pl.off_sum + (size_t)pl.sum_slots * n_kv_heads * kPwKeys * sizeof(float);
+    pl.bytes = pl.off_sum + 2 * (size_t)pl.sum_items * n_kv_heads * kPwKeys * sizeof(float);
     return pl;
 }
 
@@ -665,7 +782,7 @@ void launch_prompt(const PromptWeightsParams& pw, const PromptWeightsPlan& pl, h
         return;
     }
     paged_row_pass_kernel<BF, D, EXACT, Pass::kStats><<<grid, kPwThreads, 0, stream>>>(pw);
-    paged_key_sums_kernel<BF, D, EXACT><<<(unsigned)pl.sum_grid, kPwThreads, 0, stream>>>(pw);
+    paged_key_sums_kernel<BF, D, EXACT><<<(unsigned)(pl.sum_items * hkv), kPwThreads, 0, stream>>>(pw);
 }
 
 }  // namespace
@@ -693,10 +810,8 @@ int launch_paged_prefill_weights(const PagedLaunch& a, const PagedWeights& w, in
     pw.stats = reinterpret_cast<f32x2*>(ws + pl.off_stats);
     pw.part_sum = reinterpret_cast<float*>(ws + pl.off_sum);
     pw.w = weights_view(w, a.n_kv_heads);
-    pw.sum_target = pl.sum_target;
-    pw.sum_least = pl.sum_slots > 0 ? kSumsLeast : kUncut;
-    pw.sum_few = pl.sum_slots > 0 ? std::max(kSumsPerCu * device_cu_count() / a.n_kv_heads, 1) : 0;
-    pw.sum_slots = pl.sum_slots;
+    pw.sum_items = pl.sum_items;
+    pw.sum_rate = 1.0 / pl.sum_items;
     auto go = [&](auto bf, auto exact) {
         constexpr bool BF = decltype(bf)::value, EXACT = decltype(exact)::value;
         if (a.head_dim == 128) launch_prompt<BF, 128, EXACT>(pw, pl, stream);
