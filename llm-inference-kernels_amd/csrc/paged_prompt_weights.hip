@@ -241,15 +241,24 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     auto statistics = [&](const uint8_t* sk, int i, uint32_t gone) {
         const int t0 = begin + kPwTile * i, tk = t0 + 4 * h;
         float sc[32];
+        u32x4 ka[2][KS];   // the keys' operands, eight products ahead
+        auto load_k = [&](int blk, int ks) {
+            ka[blk][ks] = *reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks)));
+        };
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) load_k(0, ks);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             f32x16 acc;
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                acc = Hf::mfma32(*reinterpret_cast<const u32x4*>(sk + k_row + 32 * blk * kRowBytes + (k_sw ^ (32u * ks))),
-                                 qb[ks], acc);
+            for (int ks = 0; ks < KS; ++ks) {
+                acc = Hf::mfma32(ka[blk][ks], qb[ks], acc);
+                if (blk == 0) load_k(1, ks);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[16 * blk + e] = acc[e];
         }
