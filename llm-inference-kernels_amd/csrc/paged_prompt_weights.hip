@@ -101,7 +101,7 @@ __device__ __forceinline__ void row_pass(const PromptWeightsParams& pw, uint8_t*
     // Of the workgroups that run at once, one per CU and turn, every other turn's order is reversed: a CU's
     // then have about the same work together as another's.
     uint32_t item = blockIdx.x / (uint32_t)p.c.n_kv_heads;
-    const uint32_t turn_items = p.per_round / (uint32_t)p.c.n_kv_heads, turn_no = item / max(turn_items, 1u);
+    const uint32_t turn_items = max(p.per_round / (uint32_t)p.c.n_kv_heads, 1u), turn_no = item / turn_items;
     if (turn_no & 1u && (turn_no + 1) * turn_items <= gridDim.x / (uint32_t)p.c.n_kv_heads)
         item = (2 * turn_no + 1) * turn_items - 1 - item;
     CutItem ft{};
