@@ -97,7 +97,7 @@ __device__ __forceinline__ bool find_tile(const PagedFlashParams& p, uint32_t it
     const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
     auto tokens_of = [&](int b, int& row0) {   // query tokens of sequence b, kept inside q
         row0 = max(p.cu[b], 0);
-        return max(min(p.cu[b + 1], p.rows) - row0, 0);
+        return max(min(max(p.cu[b + 1], 0), p.rows) - row0, 0);
     };
     auto tiles_of = [&](int b) {
         int row0;
@@ -227,7 +227,7 @@ __device__ __forceinline__ void cut_sequence(const PagedFlashParams& p, int b, C
     s.b = b;
     s.row0 = max(p.cu[b], 0);
     s.bad = stop < p.cu[b];
-    const int all = max(min(stop, p.rows) - s.row0, 0);
+    const int all = max(min(max(stop, 0), p.rows) - s.row0, 0);   // (whatever the offsets: inside q)
     s.rows = min(all, p.observe);
     s.row0 += all - s.rows;
     s.ctx = len - (stop - s.row0);
@@ -460,7 +460,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     // The tree form: where drafted token j of the sequence stands (row qi is token qi).
     [[maybe_unused]] auto tree_pos = [&](int j) {
         if constexpr (TREE) {
-            j = min(j, ft.rows - 1);
+            j = (int)min((uint32_t)j, (uint32_t)(ft.rows - 1));
             const int at = p.positions != nullptr ? p.positions[ft.row0 + j] : ft.ctx + j;
             return min(max(at, max(ft.ctx, 0)), kMaxPosition);
         }
