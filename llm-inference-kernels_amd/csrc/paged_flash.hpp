@@ -284,21 +284,19 @@ struct Cutter {
         per = (p.c.batch + 63) / 64;
         const int b0 = min(lane * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
         const uint32_t target = (uint32_t)target_;
-        uint64_t mine = 0;
-        uint32_t fixed = 0;
+        uint32_t mine = 0, fixed = 0;
         bool bad = false;
         for (int b = b0; b < b1; ++b) {
             sequence(b, own);
             bad = bad || own.bad;
-            mine += (uint64_t)(uint32_t)own.tiles * (uint32_t)own.fixed;
+            mine += (uint32_t)own.tiles * (uint32_t)own.fixed;   // (the host refuses calls with 2^31 or more)
             fixed += (uint32_t)own.fixed;
         }
-        const bool many = mine >= 1u << 24;
-        const uint32_t units = lane_u32(wave_scan(many ? 0u : (uint32_t)mine), 63);
+        const uint32_t units = lane_u32(wave_scan(mine), 63);
         length = max((uint32_t)least, quick_ceil(units, target));
         // Offsets that decrease give rows to several sequences, more shares than there are workgroups: their
-        // parts would wait for each other in vain. And so many tiles fill the card.
-        if (__any(bad || many)) length = kUncut;
+        // parts would wait for each other in vain.
+        if (__any(bad)) length = kUncut;
         // Every sequence's last part is short, so there are more than the target: where it can be met, twice
         // a greater length for as many as there were.
         if (per == 1 && length < kUncut && lane_u32(wave_scan(fixed), 63) <= target) {

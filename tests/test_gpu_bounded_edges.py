@@ -199,3 +199,122 @@ def test_a_query_that_is_no_number_reaches_only_the_keys_that_it_sees(llmik, cud
     assert bool(w[0, 1, sees].isnan().all())
     ref.check(w[0, 0], want[0, 0], bound[0, 0])
     ref.check(w[0, 1, ~sees], want[0, 1, ~sees], bound[0, 1, ~sees])
+
+
+@pytest.mark.parametrize("opts", [{"softcap": 5.0}, {}, {"window": 60}], ids=str)
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales_that_are_not_positive(llmik, cuda, scale, opts):
+    ctx, new, H, Hkv, D = [300, 20], [40, 130], 8, 2, 128
+    lens = [a + b for a, b in zip(ctx, new)]
+    k, v, table, seq = ref.make_cache(lens, Hkv, D, 16, BF16, cuda, 20)
+    q, cu = _q(sum(new), H, D, BF16, cuda, 21), ref.offsets(new, cuda)
+    mask, pos = bref.trees(random.Random(22), new, ctx)
+    at = torch.tensor(pos, dtype=torch.int32, device=cuda)
+    got = llmik.paged_tree_attention(q, k, v, table, seq, cu, bref.words_of(mask, 3, cuda), scale, positions=at, **opts)
+    ref.check(got, *bref.tree(q, k, v, table, lens, new, mask, pos, scale, 16, **opts))
+    for observe in (0, 7):
+        w = torch.zeros(2, Hkv, 340, device=cuda)
+        want, bound = bref.weights(w, None, q, k, table, lens, new, scale, 16, observe, **opts)
+        llmik.paged_prefill_weights(q, k, table, seq, cu, w, scale, observe=observe, **opts)
+        ref.check(w, want, bound)
+    w = torch.zeros(2, Hkv, 340, device=cuda)
+    want, bound = bref.weights(w, None, q[:2], k, table, lens, [1, 1], scale, 16, **opts)
+    llmik.paged_decode_attention_weights(q[:2], k, v, table, seq, w, scale, **opts)
+    ref.check(w, want, bound)
+
+
+def test_a_drafted_key_that_is_no_number_is_its_descendants_own(llmik, cuda):
+    """K of a drafted token is NaN: the rows that see it are NaN, the others are right."""
+    ctx, new, H, Hkv, D = 200, 40, 8, 2, 64
+    mask, pos = bref.trees(random.Random(8), [new], [ctx])
+    k, v, table, seq = ref.make_cache([ctx + new], Hkv, D, 16, F16, cuda, 23)
+    q, cu = _q(new, H, D, F16, cuda, 24), ref.offsets([new], cuda)
+    place = int(table[0, (ctx + 5) // 16]), slice(None), (ctx + 5) % 16
+    sees = torch.tensor([bool(m >> 5 & 1) for m in mask], device=cuda)
+    assert 0 < int(sees.sum()) < new
+    k[place] = 0.0
+    want, bound = bref.tree(q, k, v, table, [ctx + new], [new], mask, pos, 0.05, 16)
+    k[place] = float("nan")
+    got = llmik.paged_tree_attention(q, k, v, table, seq, cu, bref.words_of(mask, 1, cuda), 0.05,
+                                     positions=torch.tensor(pos, dtype=torch.int32, device=cuda))
+    assert bool(got[sees].isnan().all())
+    ref.check(got[~sees], want[~sees], bound[~sees])
+
+
+def test_pools_of_more_than_2_to_the_31_elements(llmik, cuda):
+    """The same tokens on a large pool's last pages: the same bits."""
+    lens, new, H, Hkv, D, page = [500, 90], [40, 9], 8, 2, 128, 64
+    small_k, small_v, table, seq = ref.make_cache(lens, Hkv, D, page, F16, cuda, 25)
+    n = small_k.shape[0]
+    more = 2 ** 31 // (Hkv * page * D) + 3
+    k = torch.zeros(more + n, Hkv, page, D, dtype=F16, device=cuda)
+    v = torch.zeros_like(k)
+    k[more:], v[more:] = small_k, small_v
+    far = torch.where((table >= 0) & (table < n), table + more, -1).to(torch.int32)
+    q, cu = _q(sum(new), H, D, F16, cuda, 26), ref.offsets(new, cuda)
+    words = torch.full((sum(new), 1), 1023, dtype=torch.int64, device=cuda)
+    kept = torch.tensor([list(range(30, 490, 2)) + [-1] * 5, list(range(5, 90)) + [-1] * 150], dtype=torch.int32, device=cuda)
+
+    def all_of(k, v, table):
+        out = [llmik.paged_tree_attention(q, k, v, table, seq, cu, words, 0.1)]
+        for observe in (0, 9):
+            out.append(llmik.paged_prefill_weights(q, k, table, seq, cu, torch.zeros(2, Hkv, 500, device=cuda), 0.1,
+                                                   observe=observe))
+        w = torch.zeros(2, Hkv, 500, device=cuda)
+        out += [llmik.paged_decode_attention_weights(q[:2], k, v, table, seq, w, 0.1), w]
+        llmik.paged_compact(k, v, table, seq, kept, torch.tensor([0, 4], dtype=torch.int32, device=cuda))
+        return out
+    for a, b in zip(all_of(k, v, far), all_of(small_k, small_v, table)):
+        assert torch.equal(a, b)
+    assert torch.equal(k[more:], small_k) and torch.equal(v[more:], small_v)
+    assert int(k[:more].count_nonzero()) == 0 and int(v[:more].count_nonzero()) == 0
+
+
+REFUSED = [
+    ("tree", {"mask": lambda m: m.to(torch.int32)}, "int64"), ("tree", {"mask": lambda m: m[:4]}, "int64"),
+    ("tree", {"mask": lambda m: m[:, :0]}, "at least one word"), ("tree", {"mask": lambda m: m[:, 0]}, "int64"),
+    ("tree", {"mask": lambda m: m.expand(-1, 2)}, "contiguous"), ("tree", {"mask": lambda m: m.cpu()}, "CUDA"),
+    ("tree", {"at": lambda t: t[:3]}, "positions"), ("tree", {"at": lambda t: t.long()}, "positions"),
+    ("tree", {"at": lambda t: t.cpu()}, "CUDA"), ("append", {"at": lambda t: t[:3]}, "positions"),
+    ("tree", {"q": lambda t: t.transpose(0, 1)}, "contiguous"),
+    ("decode", {"w": lambda t: t.half()}, "fp32"), ("decode", {"w": lambda t: t[:, :1]}, "n_kv_heads"),
+    ("decode", {"w": lambda t: t[:1]}, "row per sequence"), ("prompt", {"w": lambda t: t[..., ::2]}, "contiguous"),
+    ("prompt", {"w": lambda t: t[..., :0].contiguous()}, "tokens per row"), ("prompt", {"w": lambda t: t.cpu()}, "CUDA"),
+    ("prompt", {"rows": lambda t: t[:1]}, "weight_rows"), ("decode", {"rows": lambda t: t.long()}, "weight_rows"),
+    ("select", {"rows": lambda t: t.cpu()}, "CUDA"), ("select", {"w": lambda t: t[0]}, "weights"),
+    ("select", {"keep": lambda n: 0}, "keep"), ("select", {"first": lambda n: -1}, "first and recent"),
+    ("select", {"recent": lambda n: 8}, "first and recent"), ("select", {"lens": lambda t: t.long()}, "seq_lens"),
+    ("compact", {"kept": lambda t: t.long()}, "kept"), ("compact", {"kept": lambda t: t[:1]}, "kept"),
+    ("compact", {"kept": lambda t: t[:, :1]}, "kept"), ("compact", {"kept": lambda t: t.transpose(0, 1)}, "kept"),
+    ("compact", {"starts": lambda t: t[:1]}, "starts"), ("compact", {"starts": lambda t: t.long()}, "starts"),
+    ("compact", {"w": lambda t: None}, "weight_rows come with weights"),
+]
+
+
+@pytest.mark.parametrize("name,change,msg", REFUSED, ids=["%s-%s-%d" % (n, *c, i) for i, (n, c, _) in enumerate(REFUSED)])
+def test_refusals(llmik, cuda, name, change, msg):
+    """Nothing is launched: k, v and weights keep their bits."""
+    H, Hkv, D = 8, 2, 64
+    k, v, table, seq = ref.make_cache([40, 20], Hkv, D, 16, F16, cuda, 18)
+    a = dict(q=_q(5, H, D, F16, cuda, 19), cu=ref.offsets([3, 2], cuda), mask=torch.ones(5, 1, dtype=torch.int64, device=cuda),
+             at=torch.full((5,), 40, dtype=torch.int32, device=cuda), w=torch.rand(2, Hkv, 40, device=cuda),
+             rows=torch.tensor([0, 1], dtype=torch.int32, device=cuda), keep=8, first=1, recent=1, lens=seq,
+             kept=torch.zeros(2, Hkv, 5, dtype=torch.int32, device=cuda), starts=torch.zeros(2, dtype=torch.int32, device=cuda))
+    weights, kept = a["w"], [t.clone() for t in (k, v, a["w"])]
+    for key, f in change.items():
+        a[key] = f(a[key])
+    if name == "decode" and change.keys() == {"w"}:
+        a["rows"] = None
+    calls = {
+        "tree": lambda: llmik.paged_tree_attention(a["q"], k, v, table, seq, a["cu"], a["mask"], 0.1, positions=a["at"]),
+        "append": lambda: llmik.rope_paged_append(torch.zeros(5, (H + 2 * Hkv) * D, dtype=F16, device=cuda), None, None, k, v,
+                                                  table, seq, a["cu"], a["at"]),
+        "decode": lambda: llmik.paged_decode_attention_weights(a["q"][:2], k, v, table, seq, a["w"], 0.1,
+                                                               weight_rows=a["rows"]),
+        "prompt": lambda: llmik.paged_prefill_weights(a["q"], k, table, seq, a["cu"], a["w"], 0.1, weight_rows=a["rows"]),
+        "select": lambda: llmik.paged_select_tokens(a["w"], a["lens"], a["keep"], a["first"], a["recent"], a["rows"]),
+        "compact": lambda: llmik.paged_compact(k, v, table, seq, a["kept"], a["starts"], a["w"], a["rows"]),
+    }
+    with pytest.raises(RuntimeError, match=msg):
+        calls[name]()
+    assert all(torch.equal(x, y) for x, y in zip((k, v, weights), kept))
