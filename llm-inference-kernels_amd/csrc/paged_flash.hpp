@@ -71,6 +71,7 @@ struct PagedFlashParams {
     const int* positions;     // [rows], or null: a row's slot
     // Work that is cut by length (Cutter).
     int observe;              // rows of a sequence that count: its last ones
+    float part_cost;          // tiles of a part at least: the root of all pairs of tiles times this
     int target, least;
     uint32_t slots;           // parts that the workspace holds: [slots, n_kv_heads, kPfRows, D] and (m, l)
     CutRecord* records;
@@ -277,7 +278,7 @@ struct Cutter {
         return ((uint32_t)s.rows * p.gqa.d + kJoinRows - 1) / kJoinRows;
     }
     __device__ __forceinline__ int cut_sequences() const { return (int)lane_u32(seqs_upto, 63); }
-    // About `target` parts, of `least` tiles or more.
+    // About `target` parts, of `least` tiles or more, and (part_cost) not so many that their sums cost more.
     __device__ __forceinline__ Cutter(const PagedFlashParams& p_, int target_, int least, F f)
         : p(p_), sequence(f) {
         const int lane = threadIdx.x & 63;
@@ -294,6 +295,7 @@ struct Cutter {
         }
         const uint32_t units = lane_u32(wave_scan(mine), 63);
         length = max((uint32_t)least, quick_ceil(units, target));
+        length = max(length, (uint32_t)__builtin_sqrtf((float)units * p.part_cost));
         // Offsets that decrease give rows to several sequences, more shares than there are workgroups: their
         // parts would wait for each other in vain.
         if (__any(bad)) length = kUncut;

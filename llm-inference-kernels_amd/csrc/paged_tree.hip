@@ -137,6 +137,12 @@ namespace {
 // 16 of 32 over 4000 78.7, 73.3, 30 of 4 .. 24 over 200 .. 8000 88.6, 62.0 (for 3 76). Into single tiles where there
 // are few: 8 over 700 tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0.
 constexpr int kTreeLeast = 1;
+// A part's sums, 64 KiB, are written and read again, which takes 0.026 us of the card's time, a tile 1.3 us of its
+// workgroup's: of N pairs of tiles in parts of t the sum of 1.3 t and 0.026 N / t is least at t^2 = N / 50, and a row
+// tile whose keys are less than twice that is better whole (t^2 = N / 25). us without this rule, with N / 50, with
+// N / 25: 32 drafts of 16 over 200 tokens 27.2, 18.1, 18.1, over 600 33.7, 33.7, 27.0, 8 of 16 over 600 19.7, 18.0,
+// 19.4, 16 of 32 over 500 30.0, 29.9, 27.6.
+constexpr float kTreePartCost = 25.0f;
 
 struct PagedTreePlan {
     long row_tiles;      // of the call at most
@@ -205,6 +211,7 @@ int launch_paged_tree(const PagedLaunch& a, const uint64_t* mask, int words, con
     p.target = pl.target;
     p.least = pl.slots > 0 ? kTreeLeast : kUncut;
     p.slots = pl.slots;
+    p.part_cost = a.n_kv_heads / kTreePartCost;
     const long items = pl.row_tiles + (pl.slots > 0 ? pl.target : 0);
     if (a.bf16)
         a.head_dim == 128 ? launch_tree<true, 128>(p, items, pl.groups, stream)
