@@ -5,14 +5,24 @@
 // computed twice, by two kernels that keep one operand in registers and stream the
 // other through LDS:
 //   statistics: 128 rows (32 per wave) over the keys in tiles of 64. S^T = K Q^T gives
-//     a lane one row's scores, so its maximum and sum stay in the lane.
+//     a lane one row's scores, so its maximum and sum stay in the lane. Where there are few
+//     row tiles, their keys are cut into parts (Cutter).
 //   sums: 128 keys (32 per wave) over the rows in tiles of 64. S^T = K Q^T again: a lane
 //     has one row's m and 1 / l in registers and sums 2^(s - m) / l of its 16 keys; the
 //     lanes are added once, behind the last tile. (S = Q K^T leaves a key's sum in one lane,
 //     but reads 16 rows' m and 1 / l from LDS for 16 scores.)
-// Both cut their streamed axis where there are few tiles of the other (Cutter). The parts
-// of a cut row or key tile are joined, in order, by the last of its workgroups to arrive:
-// nothing depends on timing.
+// The parts of a cut row or key tile are joined, in order, by the last of its workgroups to
+// arrive: nothing depends on timing. Where a sequence's recorded rows are one row tile (the
+// last 32 tokens of four heads, say), its pass over the keys is the sums' too: whole columns,
+// no joins, the statistics' parts joined by those who need them.
+//
+// Measured (32 heads over 8 KV heads of 128, bf16): all rows of 4000 tokens 185 .. 193 us, with a cap
+// 255 .. 265, of 8192 tokens 635 .. 655; the products alone, twice, are 104 us at a large matrix
+// product's rate. The statistics' vector units work 86 % of the cycles (9.5 instructions a score
+// with a cap, three of them transcendental at half rate), the sums' 70 %. The last 32 rows of
+// four prompts of 4000 .. 8192 tokens 31 .. 36 us, K's 48 MB read twice: 3 TB/s with two launches,
+// their look-ups and the hand-off of the statistics. Three prompts of 17 .. 150 tokens 14: the two
+// chains of launch, lengths, pages, keys.
 #include "paged_flash.hpp"
 
 namespace llmik {
@@ -20,7 +30,6 @@ namespace llmik {
 constexpr int kPwThreads = 256;
 constexpr int kPwKeys = 128;     // of a workgroup of the sums
 constexpr int kPwTile = 64;      // rows or keys of a streamed tile
-constexpr int kSumsLeast = 2;    // pairs of a workgroup of the sums at least
 
 struct PromptWeightsParams {
     PagedFlashParams f;          // target, least and slots: the statistics' cuts
@@ -426,7 +435,10 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_row_pass_kernel(PromptWei
 // key tile, of which every workgroup of a KV head takes the same number, one after the other: where
 // that ends inside a key tile the next workgroup goes on. Key tile i of a sequence is seen by row
 // tiles first(i) .. last(i) - 1, which move by 2 G from one to the next until they reach the rows'
-// end, so that a sequence's pairs up to any key tile are a closed sum.
+// end, so that a sequence's pairs up to any key tile are a closed sum. (Equal cuts of all row tiles,
+// of which a causal prompt's key tiles see half: us, 4000 tokens 208 against 189, two of 1500
+// 91, 77. Short ones with 1, 2, 4 pairs for a workgroup at least: 100 tokens 18.4, 19.6, 22.2, 200
+// 19.4, 23.7, 26.5, 600 27.1, 27.1, 30.9, 8 of 150 25.1, 24.3, 26.9.)
 struct KeySeq {
     int b, row0, rows, ctx;   // as CutItem's
     int begin, end;           // the keys that are recorded
@@ -508,7 +520,6 @@ __global__ __launch_bounds__(kPwThreads, 3) void paged_key_sums_kernel(PromptWei
     const long pairs = uniform64(s_upto[63]);
     long chunk = (long)((double)pairs * pw.sum_rate);
     if (chunk * pw.sum_items < pairs) ++chunk;
-    chunk = max(chunk, (long)kSumsLeast);
     chunk = uniform64(chunk);
     const long stop = min(pairs, (item + 1) * chunk);
     for (long at = item * chunk; at < stop;) {
