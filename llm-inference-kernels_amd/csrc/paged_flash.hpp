@@ -24,7 +24,7 @@
 // reads of eight rows fall into different banks; the copies place them so.
 //
 // Where there are fewer row tiles than two workgroups per CU, their keys are cut into
-// parts, whose sums a second kernel joins (paged_flash.hip, paged_prefix.hip).
+// parts, whose sums a second kernel joins (paged_flash.hip, paged_prefix.hip, paged_tree.hip).
 //
 // Measured: a prompt of 8192 tokens, 32 heads over 8 KV heads of 128, bf16: 518 .. 570
 // us, 0.96 .. 1.06 PFLOP/s (a large matrix product reaches 1.42): the matrix units work 57 % of

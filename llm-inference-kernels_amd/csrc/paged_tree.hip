@@ -5,7 +5,15 @@
 // All drafted tokens and query heads that read a KV head's keys share one pass over
 // them, 128 rows at a time, so the cache's bytes bound it while they are few. The key
 // tiles of the batch are cut into parts of about one length (Cutter): a row
-// tile's parts are joined by a second kernel.
+// tile's parts are joined by a second kernel. A row's mask is one 64-bit word for a tile
+// of 64 keys, shifted to the tile's beginning; tiles of cached tokens need none.
+//
+// Measured (GPU us, kernel and join): 8 drafted tokens over 700 8.8 + 3.9, 64 over 8192 22 + 5.2, 32
+// sequences of 4 .. 24 over 200 .. 8000 54 + 5.4, all with 32 heads over 8 KV heads of 128. The last
+// reads 235 MB at 4.3 TB/s (8 drafted tokens over each of 32 x 8000: 1.05 GB in 197 us, 5.3 TB/s); of
+// the second a workgroup's 8 tiles take 2.2 us each, one wave per SIMD, whose products, exponentials
+// and copies follow one another, and 17 MB of parts are written and read; the first is launches and
+// look-ups.
 #include "paged_flash.hpp"
 
 namespace llmik {
