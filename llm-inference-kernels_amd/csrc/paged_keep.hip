@@ -7,9 +7,9 @@
 // the 8 bits below what is settled gives the digit of the need-th largest, four times.
 // Then every wave counts, in a segment of its own, the weights above that value and
 // those equal to it, and after a sum over the waves writes its slots in order.
-// Bound: a chain of barriers, the weights are read once (8192 tokens of 8 KV heads 10.0 us with
-// the launch's 5 of host time, 64 x 8 x 3500 .. 6000 15.0; with one histogram and the weights
-// read anew for every digit 26, 29).
+// Bound: a chain of reads and barriers, the waves wait 62 % of the time (8192 tokens of 8 KV
+// heads 10.0 us, 64 x 8 x 3500 .. 6000 15.0; with one histogram and the weights read anew for
+// every digit 26, 29).
 //
 // Compaction. Token kept[i] goes to slot start + i. No entry lies before its new slot
 // (kept[i] >= start + i; others are not moved), so a workgroup that takes the entries

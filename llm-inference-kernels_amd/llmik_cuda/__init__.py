@@ -27,7 +27,12 @@ the reference):
     (integration/w4a16_patch.py:78-84);
   * `rope_paged_append`, `paged_decode_attention`, `paged_prefill_attention`,
     `paged_shared_prefix_attention`: a cache of pages for sequences of
-    different lengths (`llmik_cuda.kv_cache.PagedKVCache` manages one).
+    different lengths (`llmik_cuda.kv_cache.PagedKVCache` manages one);
+  * `paged_tree_attention`: drafted token trees over that cache, and
+    `paged_compact`, which brings the accepted tokens together;
+    `paged_decode_attention_weights`, `paged_prefill_weights` and
+    `paged_select_tokens`: the attention weight that each cached token has had,
+    and the tokens that a cache of a bounded length keeps by it.
 """
 from __future__ import annotations
 
@@ -465,9 +470,10 @@ def rope_paged_append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optio
     token of sequence b. cos, sin [positions, head_dim], fp32 or of qkv's
     dtype, are indexed by position, which is the token's slot or, with positions
     [rows] int32, what that says (a drafted token's depth, a sequence that has
-    lost tokens); None, None: no rotation. Rows from cu_tokens[-1] on, and rows of empty sequences, give a zero q and are
-    written nowhere; so are positions past the tables. Two rows that name one
-    slot (a page mapped twice) write it in no particular order."""
+    lost tokens); None, None: no rotation. Rows from cu_tokens[-1] on, and rows
+    of empty sequences, give a zero q and are written nowhere; so are positions
+    past the tables. Two rows that name one slot (a page mapped twice) write it
+    in no particular order."""
     _require(_is_device(qkv) and _is_device(k_cache) and _is_device(v_cache) and
              _is_device(page_table) and _is_device(seq_lens), "all inputs must be CUDA tensors")
     return _C.rope_paged_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_tokens, positions)
