@@ -11,9 +11,9 @@
 // Measured (GPU us, kernel and join): 8 drafted tokens over 700 8.8 + 3.9, 64 over 8192 22 + 5.2, 32
 // sequences of 4 .. 24 over 200 .. 8000 54 + 5.4, all with 32 heads over 8 KV heads of 128. The last
 // reads 235 MB at 4.3 TB/s (8 drafted tokens over each of 32 x 8000: 1.05 GB in 197 us, 5.3 TB/s); of
-// the second a workgroup's 8 tiles take 2.2 us each, one wave per SIMD, whose products, exponentials
-// and copies follow one another, and 17 MB of parts are written and read; the first is launches and
-// look-ups.
+// the second launch and look-ups take 8 us, a workgroup's 8 or 9 tiles follow one another, and 17 MB
+// of parts are written and read (eight waves in two teams, each with half of a part's keys, gain 1 us
+// there and lose 1 at 700 tokens); the first is launches and look-ups.
 #include "paged_flash.hpp"
 
 namespace llmik {
