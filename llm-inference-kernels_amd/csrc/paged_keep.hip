@@ -56,7 +56,7 @@ struct SelectLds {
     uint32_t hist[kSelCopies * kSelCopy];
     uint32_t count[256];
     uint32_t above[kSelWaves], equal[kSelWaves];
-    uint32_t digit, rest;
+    uint32_t digit, rest, all;   // all: the value's digits so far leave no more than stay
 };
 
 // The candidates' `need` largest, of n: their slots, in order, to `out`. CACHED: in LDS,
@@ -91,8 +91,9 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
 
     // ---- the need-th largest value ----
     uint32_t found = 0, rest = (uint32_t)need;   // of the top digits; its rank among those with these
+    int shift = 24;
 #pragma unroll 1
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    for (;; shift -= 8) {   // until all with these digits stay
         for (int i0 = 0; i0 < n && !(CACHED && shift == 24); i0 += 4 * kSelThreads) {
             uint32_t x[4];
 #pragma unroll
@@ -120,21 +121,24 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
             const uint32_t upto = wave_scan(mine);
             const int at = __ffsll((unsigned long long)__ballot(upto >= rest)) - 1;   // (all are >= rest together)
             if (lane == at) {
-                uint32_t r = rest - (upto - mine), digit = 255u - 4u * lane;
+                uint32_t r = rest - (upto - mine), digit = 255u - 4u * lane, here = c[0];
                 bool more = true;
 #pragma unroll
                 for (int e = 0; e < 3; ++e) {
                     more = more && r > c[e];
                     r -= more ? c[e] : 0u;
                     digit -= more ? 1u : 0u;
+                    here = more ? c[e + 1] : here;
                 }
                 s.digit = digit;
                 s.rest = r;
+                s.all = r == here ? 1u : 0u;
             }
         }
         __syncthreads();
         found = found << 8 | s.digit;
         rest = s.rest;
+        if (shift == 0 || s.all != 0) break;
     }
     // ---- every wave's segment: what lies above the value, and what equals it (the first `rest` stay) ----
     const int seg = ((n + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
@@ -147,8 +151,8 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const bool in = i0 + 64 * u + lane < i_end;
-            above += in && x[u] > found;
-            equal += in && x[u] == found;
+            above += in && x[u] >> shift > found;
+            equal += in && x[u] >> shift == found;
         }
     }
     above = wave_sum(above);
@@ -172,8 +176,8 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = i0 + 64 * u + lane;
-            const bool is_equal = i < i_end && x[u] == found;
-            const uint64_t eq = __ballot(is_equal), ab = __ballot(i < i_end && x[u] > found);
+            const bool is_equal = i < i_end && x[u] >> shift == found;
+            const uint64_t eq = __ballot(is_equal), ab = __ballot(i < i_end && x[u] >> shift > found);
             const uint32_t eq_before = at_equal + before(eq);
             if ((ab >> lane & 1u) || (is_equal && eq_before < rest))
                 out[first + at_above + before(ab) + min(eq_before, rest)] = first + i;
