@@ -4,11 +4,12 @@
 // Selection. Of a sequence's n tokens the first f and the last r stay, and of those
 // between them the `need` of the largest weight, ties to the lowest slot. The weights,
 // as integers of the same order, are searched by digits from the top: a histogram of
-// the 8 bits below what is settled gives the digit of the need-th largest, four times.
+// the 8 bits below what is settled gives the digit of the need-th largest, until all that share
+// its digits stay (four times at most).
 // Then every wave counts, in a segment of its own, the weights above that value and
 // those equal to it, and after a sum over the waves writes its slots in order.
 // Bound: a chain of reads and barriers, the waves wait 62 % of the time (8192 tokens of 8 KV
-// heads 10.0 us, 64 x 8 x 3500 .. 6000 15.0; with one histogram and the weights read anew for
+// heads 9.5 us, 64 x 8 x 3500 .. 6000 14.4; with one histogram and the weights read anew for
 // every digit 26, 29).
 //
 // Compaction. Token kept[i] goes to slot start + i. No entry lies before its new slot
@@ -26,7 +27,7 @@ namespace {
 
 // ---------------------------------------------------------------- selection
 
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave;
+constexpr int kSelWaves = 16;   // of a workgroup at most
 constexpr int kSelCached = 36864;   // of 160 KiB of LDS, 16 for the rest
 // Copies of the histogram, a lane's by its number: the weights' exponents are few, and additions to one place
 // wait for each other. (Their bins lie in different banks.)
@@ -61,7 +62,7 @@ struct SelectLds {
 
 // The candidates' `need` largest, of n: their slots, in order, to `out`. CACHED: in LDS,
 // read once; else every pass reads them again.
-template <bool CACHED>
+template <bool CACHED, int THREADS>
 __device__ __forceinline__ void select_largest(const float* w, int n, int need, int first, int* out, uint32_t* s_value,
                                                SelectLds& s) {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -72,18 +73,18 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
         if constexpr (CACHED) return s_value[i];
         else return read(i);
     };
-    for (int i = tid; i < kSelCopies * kSelCopy; i += kSelThreads) s.hist[i] = 0u;
+    for (int i = tid; i < kSelCopies * kSelCopy; i += THREADS) s.hist[i] = 0u;
     __syncthreads();
     uint32_t* const hist = s.hist + (lane & (kSelCopies - 1)) * kSelCopy;
     if constexpr (CACHED) {   // with the first digit's histogram
-        for (int i0 = 0; i0 < n; i0 += 4 * kSelThreads) {
+        for (int i0 = 0; i0 < n; i0 += 4 * THREADS) {
             uint32_t x[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = read(min(i0 + u * kSelThreads + tid, n - 1));
+            for (int u = 0; u < 4; ++u) x[u] = read(min(i0 + u * THREADS + tid, n - 1));
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (i0 + u * kSelThreads + tid < n) {
-                    s_value[i0 + u * kSelThreads + tid] = x[u];
+                if (i0 + u * THREADS + tid < n) {
+                    s_value[i0 + u * THREADS + tid] = x[u];
                     atomicAdd(&hist[x[u] >> 24], 1u);
                 }
         }
@@ -94,13 +95,13 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
     int shift = 24;
 #pragma unroll 1
     for (;; shift -= 8) {   // until all with these digits stay
-        for (int i0 = 0; i0 < n && !(CACHED && shift == 24); i0 += 4 * kSelThreads) {
+        for (int i0 = 0; i0 < n && !(CACHED && shift == 24); i0 += 4 * THREADS) {
             uint32_t x[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = value(min(i0 + u * kSelThreads + tid, n - 1));
+            for (int u = 0; u < 4; ++u) x[u] = value(min(i0 + u * THREADS + tid, n - 1));
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (i0 + u * kSelThreads + tid < n && (shift == 24 || x[u] >> (shift + 8) == found))
+                if (i0 + u * THREADS + tid < n && (shift == 24 || x[u] >> (shift + 8) == found))
                     atomicAdd(&hist[x[u] >> shift & 255u], 1u);
         }
         __syncthreads();
@@ -141,7 +142,8 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
         if (shift == 0 || s.all != 0) break;
     }
     // ---- every wave's segment: what lies above the value, and what equals it (the first `rest` stay) ----
-    const int seg = ((n + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
+    constexpr int kWaves = THREADS / kWave;
+    const int seg = ((n + kWaves - 1) / kWaves + 63) / 64 * 64;
     const int i_begin = min(wave * seg, n), i_end = min((wave + 1) * seg, n);
     uint32_t above = 0, equal = 0;
     for (int i0 = i_begin; i0 < i_end; i0 += 256) {
@@ -188,7 +190,8 @@ __device__ __forceinline__ void select_largest(const float* w, int n, int need, 
 }
 
 // One workgroup per (sequence, KV head).
-__global__ __launch_bounds__(kSelThreads) void paged_select_kernel(SelectParams p) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
     extern __shared__ uint32_t s_value[];
     __shared__ SelectLds s_all;
     const int tid = threadIdx.x;
@@ -197,25 +200,30 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(SelectParams 
     int* const out = p.kept + (long)blockIdx.x * p.keep;
     if (kvh == 0 && tid == 0) p.new_lens[b] = min(len, p.keep);
     if (len <= p.keep) {
-        for (int i = tid; i < p.keep; i += kSelThreads) out[i] = i < len ? i : -1;
+        for (int i = tid; i < p.keep; i += THREADS) out[i] = i < len ? i : -1;
         return;
     }
     const float* const w = weights_of(p.w, b, kvh);
     const int n = len - p.first - p.recent;   // the candidates: > need, as first + recent <= keep < len
     const int need = p.keep - p.first - p.recent;
-    for (int i = tid; i < p.first; i += kSelThreads) out[i] = i;
-    for (int i = tid; i < p.recent; i += kSelThreads) out[p.first + need + i] = len - p.recent + i;
+    for (int i = tid; i < p.first; i += THREADS) out[i] = i;
+    for (int i = tid; i < p.recent; i += THREADS) out[p.first + need + i] = len - p.recent + i;
     if (need == 0) return;
     const float* const from = w != nullptr ? w + p.first : nullptr;
-    if (n <= p.cached) select_largest<true>(from, n, need, p.first, out, s_value, s_all);
-    else select_largest<false>(from, n, need, p.first, out, s_value, s_all);
+    if (n <= p.cached) select_largest<true, THREADS>(from, n, need, p.first, out, s_value, s_all);
+    else select_largest<false, THREADS>(from, n, need, p.first, out, s_value, s_all);
 }
 
 int launch_paged_select(const PagedWeights& w, const int* lens, int batch, int n_kv_heads, int keep, int first,
                         int recent, int* kept, int* new_lens, hipStream_t stream) {
     const int cached = std::min(w.max_len, kSelCached);
     const SelectParams p{weights_view(w, n_kv_heads), lens, kept, new_lens, keep, first, recent, cached};
-    paged_select_kernel<<<(unsigned)(batch * n_kv_heads), kSelThreads, (size_t)cached * 4, stream>>>(p);
+    // Eight waves where they read a row in one turn of four weights a thread, else sixteen. us, 16, 8, 4 waves, sequences of
+    // 8 KV heads x tokens: 1 x 2000 6.6, 5.9, 7.4, 256 x 2000 31.1, 18.5, 16.4, 1 x 4000 7.1, 7.8, 64 x 4000 10.7, 11.1,
+    // 64 x 3500 .. 6000 14.4, 13.6, 64 x 7000 15.7, 18.2, 1 x 8192 9.5, 11.5, 17.4.
+    const unsigned grid = (unsigned)(batch * n_kv_heads);
+    if (cached <= 4 * 512) paged_select_kernel<512><<<grid, 512, (size_t)cached * 4, stream>>>(p);
+    else paged_select_kernel<1024><<<grid, 1024, (size_t)cached * 4, stream>>>(p);
     return check_launch();
 }
 
