@@ -310,7 +310,7 @@ LLMIK_API llmik_status llmik_paged_tree_attention(const llmik_paged_cache* cache
 }
 
 LLMIK_API size_t llmik_paged_decode_weights_scratch_size(const llmik_paged_cache* cache, int n_heads,
-                                                           const llmik_token_weights* weights) {
+                                                         const llmik_token_weights* weights) {
     if (check_shapes(cache, n_heads) != LLMIK_OK || cache->batch == 0) return 0;
     if (check_weights(weights, cache->batch) != LLMIK_OK) return 0;
     return paged_decode_weights_scratch(cache->batch, n_heads, capacity_of(*cache), weights->max_len);
