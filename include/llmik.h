@@ -480,8 +480,8 @@ LLMIK_API llmik_status llmik_silu_mul_halves(const void* gate_up, void* out, lon
  *
  * Scores, sums and softmax statistics are fp32, and outputs are rounded once. A
  * probability enters the product with V as 22 (fp16) or 16 (bf16) bits in decode
- * attention and for a sequence's own tokens behind a shared prefix, rounded once to
- * the type, 11 or 8 bits, in prompts and for the shared prefix: an error of at most
+ * attention, for drafted trees and for a sequence's own tokens behind a shared prefix,
+ * rounded once to the type, 11 or 8 bits, in prompts and for the shared prefix: an error of at most
  * 2^-11 (2^-8) of sum_j p_j |v_j - out|, the size of the output's own rounding.
  */
 #define LLMIK_F16 0
@@ -592,8 +592,8 @@ LLMIK_API llmik_status llmik_rope_paged_append_at(const llmik_paged_cache* cache
  *   positions [rows]: of the drafted tokens, for slopes and window; one below the
  *     sequence's cached tokens counts as their number, one above 2^30 as that. NULL:
  *     their slots. A cached token's position is its slot.
- * Probabilities are rounded as llmik_paged_prefill_attention's. A row that sees no
- * token gives zeros.
+ * Probabilities enter the products with V as a pair of 16-bit values, as in
+ * llmik_paged_decode_attention. A row that sees no token gives zeros.
  */
 LLMIK_API size_t llmik_paged_tree_workspace_size(const llmik_paged_cache* cache, int n_heads, int rows);
 LLMIK_API llmik_status llmik_paged_tree_attention(const llmik_paged_cache* cache, const void* q,

@@ -17,7 +17,8 @@
 //     from LDS by the transposing 64-bit read (16 lanes give four tokens' 16
 //     channels and get one channel's four tokens each).
 // P is rounded once to 16 bits, as 2^8 p (fp16 keeps its full precision down to
-// 2^-22); sums and statistics are fp32.
+// 2^-22); sums and statistics are fp32. A tree's rows stand in for decode steps, whose P
+// enters as a pair of 16-bit values: theirs does too (two products; the loads bound them).
 //
 // K and V tiles are copied to LDS asynchronously, one tile ahead. The 16-byte
 // chunks of a row are permuted (xor with the row number) so that the operand
@@ -397,7 +398,7 @@ struct FlashLds {
     static constexpr int kTileBytes = kPfTile * D * 2;
     uint8_t *k0, *k1, *v0, *v1;
     int *lo, *hi;              // [4]
-    uint32_t* bad;             // some V is no number (see the end of paged_flash)
+    uint32_t* bad;             // some V is no number (see the end of paged_flash; not the tree form's)
 };
 
 // Workgroup wg of n_wg. EXACT: for a cap above kPlainCap (capped_tanh; a kernel of its
@@ -515,9 +516,6 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                 pos_lo = min(pos_lo, __shfl_xor(pos_lo, d));
                 pos_hi = max(pos_hi, __shfl_xor(pos_hi, d));
             }
-            if (lane == 0) s_hi[wave] = live ? pos_hi : 0;
-            __syncthreads();
-            wg_hi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
         }
         parts = ft.parts;
         if (parts > 1 && part_slot(ft, ft.part) >= p.slots) return;   // (the workspace's end)
@@ -560,9 +558,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
     const int full_hi = (min(end, first_own) - begin) >> kPfTileLog;
     const int seen_hi = live ? ((last_seen - begin) >> kPfTileLog) + 1 : INT_MIN;
     const int wg_full_lo = (oldest(wg_hi) - begin + kPfTile - 1) >> kPfTileLog;
-    int wg_full_hi;
-    if constexpr (TREE) wg_full_hi = (ft.ctx - begin) >> kPfTileLog;
-    else wg_full_hi = (wg_lo + 1 - begin) >> kPfTileLog;
+    const int wg_full_hi = (wg_lo + 1 - begin) >> kPfTileLog;
 
     // ---- copies: wave w brings tokens 16 w .. + 15 of every tile ----
     // Every wave looks up all octets, eight tiles at a time: lane l octet l % 8 of tile
@@ -781,15 +777,26 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) t[e] = __builtin_amdgcn_exp2f(t[e]);
+        if constexpr (TREE) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sum[e & 3] += t[e];
+            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
             u32x4 pb;
+            [[maybe_unused]] u32x4 rest;   // the tree form: what pb leaves of each
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t p2 = Hf::pack(t[8 * kk + 2 * e], t[8 * kk + 2 * e + 1]);
+                const float p0 = t[8 * kk + 2 * e], p1 = t[8 * kk + 2 * e + 1];
+                const uint32_t p2 = Hf::pack(p0, p1);
                 pb[e] = p2;
-                l_run = Hf::add_pair(p2, l_run);   // the sum of what the products use
+                if constexpr (TREE)
+                    rest[e] = Hf::pack(p0 - Hf::to_f32((uint16_t)p2), p1 - Hf::to_f32((uint16_t)(p2 >> 16)));
+                else l_run = Hf::add_pair(p2, l_run);   // the sum of what the products use
             }
+            u32x4 av[CB];
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 const uint8_t* a = sv + v_at + 16 * kk * kRowBytes + 16 * ((v_chunk + 4 * cb) ^ v_sw);
@@ -798,7 +805,12 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
                 const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 8 * kRowBytes));
                 const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-                o[cb] = Hf::mfma32(make_u32x4(l2[0], l2[1], h2[0], h2[1]), pb, o[cb]);
+                av[cb] = make_u32x4(l2[0], l2[1], h2[0], h2[1]);
+                o[cb] = Hf::mfma32(av[cb], pb, o[cb]);
+            }
+            if constexpr (TREE) {
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) o[cb] = Hf::mfma32(av[cb], rest, o[cb]);
             }
         }
     };
@@ -814,8 +826,9 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
         auto copies = [&](int v, int c) { copy(v ? v_far : k_far, v, c); };
         // Where some row does not see some token, every wave looks through its 16 rows of V
         // for infinities and NaN (bits of |x| from the type's infinity on): a probability
-        // of 0 would make NaN of them. Such a tile's rows are done again, below.
-        if (i < wg_full_lo || i >= wg_full_hi) {   // workgroup-uniform
+        // of 0 would make NaN of them. Such a tile's rows are done again, below. (Trees look at their
+        // sums instead: the second part of a probability makes NaN of an infinity that all rows see, too.)
+        if (!TREE && (i < wg_full_lo || i >= wg_full_hi)) {   // workgroup-uniform
             u32x4 w[kCopies];
 #pragma unroll
             for (int c = 0; c < kCopies; ++c)
@@ -839,7 +852,7 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             for (int c = 0; c < 2 * kCopies; ++c) copies(c / kCopies, c % kCopies);
         }
     };
-    if (tid == 0) s_bad = 0u;   // (the first turn's barrier follows)
+    if (!TREE && tid == 0) s_bad = 0u;   // (the first turn's barrier follows)
     if (tiles > 0) {
         prepare(0);
 #pragma unroll
@@ -915,9 +928,20 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             if (row < n_live) *reinterpret_cast<u32x4*>(p.out + to * D + 8 * c) = v;
         }
     }
-    if (tiles == 0 || __builtin_amdgcn_readfirstlane((int)s_bad) == 0) return;
+    bool again;
+    if constexpr (TREE) {
+        float all = 0.0f;   // NaN if any sum is (or where infinities of both signs are, which does no harm)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) all += o[cb][e];
+        again = __any(all != all && l_run == l_run);
+    } else {
+        again = s_bad != 0;
+    }
+    if (tiles == 0 || __builtin_amdgcn_readfirstlane((int)again) == 0) return;
 
-    // ---- some V is no number, and not all rows see it: the wave's rows one by one,
+    // ---- some V is no number, and not all rows see it, or a tree's do: the wave's rows one by one,
     // 64 keys at a time (a lane its key's score, then two channels of every key's
     // value that the row sees) ----
     __builtin_amdgcn_s_waitcnt(0);   // the stores above come first

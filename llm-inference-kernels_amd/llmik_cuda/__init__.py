@@ -547,8 +547,8 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ancestors'). Score options as in paged_decode_attention; distances go by
     positions [rows] int32 (a drafted token's depth; at least the number of cached
     tokens, the slot by default) and, of cached tokens, by slots. A row that sees
-    no token, and rows of no sequence, give zeros. Probabilities are rounded as
-    paged_prefill_attention's."""
+    no token, and rows of no sequence, give zeros. Probabilities are as exact as
+    paged_decode_attention's."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and
              _is_device(seq_lens) and _is_device(cu_tokens) and _is_device(tree_mask), "all inputs must be CUDA tensors")
     return _C.paged_tree_attention(q, k_cache, v_cache, page_table, seq_lens, cu_tokens, tree_mask,
