@@ -440,8 +440,9 @@ __device__ __forceinline__ void paged_flash(const PagedFlashParams& p, uint32_t 
             auto sequence = [&](int b, CutItem& s) { cut_sequence(p, b, s); };
             const Cutter<decltype(sequence)> cutter(p, p.target, p.least, sequence);
             found = cutter.find(item, ft);
+            const int cut_sequences = cutter.cut_sequences();   // (read from the last lane: not in the branch)
             if (p.slots != 0 && kvh == 0 && tid == 0)
-                write_record(p.records, p.n_records, p.slots, wg == 0, cutter.cut_sequences(), found, ft);
+                write_record(p.records, p.n_records, p.slots, wg == 0, cut_sequences, found, ft);
         }
         else found = find_tile(p, item, ft);
         // Rows that belong to no sequence (a padded batch) are zeroed, by all workgroups together.
