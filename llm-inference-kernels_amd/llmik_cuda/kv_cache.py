@@ -26,6 +26,7 @@ had the most (the reference has no counterpart).
 """
 from __future__ import annotations
 
+import warnings
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -225,6 +226,12 @@ class PagedBatch(NamedTuple):
     shortened: bool = False                      # some sequence has lost tokens: slots are no positions
 
 
+class _Draft(NamedTuple):
+    length: int            # of the sequence without the draft
+    tokens: int            # drafted ones
+    parents: List[int]
+
+
 class PagedKVCache:
     """Sequences of different lengths over a pool of `n_pages` pages of `page_size`
     tokens per layer: k, v [n_layers, n_pages, n_kv_heads, page_size, head_dim]. A
@@ -303,7 +310,7 @@ class PagedKVCache:
         self._length: dict[int, int] = {}
         self._next = 0
         self._lost: dict[int, int] = {}               # sequence -> tokens that it has lost (its text is longer)
-        self._drafts: dict[int, Tuple[int, int]] = {}   # sequence -> its length without the draft, drafted tokens
+        self._drafts: dict[int, _Draft] = {}          # sequence -> its draft that is not accepted
         self.observe = int(observe)
         self.weights: Optional[torch.Tensor] = None
         self._rows: dict[int, int] = {}               # sequence -> its row of the weights
@@ -408,22 +415,28 @@ class PagedKVCache:
         """Ends the drafts of `seqs`: of seqs[i] the drafted tokens paths[i] (numbers in
         the draft, ascending; none: all are dropped) become its next tokens, in
         every layer. The draft's step must have been appended to all layers that
-        are read again."""
+        are read again. A path begins at a token that follows the sequence and goes
+        on from each token to one that follows it; other lists give a warning, as
+        their tokens were rotated, and shown others, as what they then are not."""
         paths = [[int(j) for j in path] for path in paths]
         _require(len(paths) == len(seqs), "one path per sequence")
         _require(len(set(seqs)) == len(seqs), "a sequence occurs twice")
         _require(all(s in self._drafts for s in seqs), "a sequence has no draft")
         for s, path in zip(seqs, paths):
             _require(all(a < b for a, b in zip(path, path[1:])) and
-                     all(0 <= j < self._drafts[s][1] for j in path), "a path's tokens are ascending numbers of the draft")
+                     all(0 <= j < self._drafts[s].tokens for j in path), "a path's tokens are ascending numbers of the draft")
+        strays = [s for s, path in zip(seqs, paths) if [self._drafts[s].parents[j] for j in path] != [-1, *path][:len(path)]]
+        if strays:
+            warnings.warn(f"PagedKVCache.accept: what is accepted of the sequences {strays} is no path of their drafts: "
+                          "its keys and values belong to other positions and other tokens before them", stacklevel=2)
         moved = [(s, path) for s, path in zip(seqs, paths) if path != list(range(len(path)))]
         if moved:
-            ctx = [self._drafts[s][0] for s, _ in moved]
+            ctx = [self._drafts[s].length for s, _ in moved]
             longest = max(len(path) for _, path in moved)
             kept = [[c + j for j in path] + [-1] * (longest - len(path)) for c, (_, path) in zip(ctx, moved)]
             self._compact([s for s, _ in moved], kept, ctx)
         for s, path in zip(seqs, paths):
-            self._shorten(s, self._drafts.pop(s)[0] + len(path))
+            self._shorten(s, self._drafts.pop(s).length + len(path))
 
     def evict(self, seqs: Sequence[int], keep: int, first: int = 0, recent: int = 0) -> None:
         """Cuts the sequences down to `keep` tokens for every layer and KV head: the
@@ -518,7 +531,7 @@ class PagedKVCache:
         if trees is not None:
             words = max(1, -(-max([len(t) for t in trees] + [0]) // 64))
             for s, n, tree in zip(seqs, before, trees):
-                self._drafts[s] = (n, len(tree))
+                self._drafts[s] = _Draft(n, len(tree), tree)
                 seen: List[int] = []
                 deep: List[int] = []
                 for j, parent in enumerate(tree):
