@@ -224,12 +224,15 @@ class PagedBatch(NamedTuple):
     tree_mask: Optional[torch.Tensor] = None     # [rows, words] int64: a drafted tree (PagedKVCache.draft)
     weight_rows: Optional[torch.Tensor] = None   # [batch] int32: the sequences' rows of the weights
     shortened: bool = False                      # some sequence has lost tokens: slots are no positions
+    queries: Optional[dict] = None               # layer -> a draft's q and score options, kept until it is accepted
 
 
 class _Draft(NamedTuple):
     length: int            # of the sequence without the draft
     tokens: int            # drafted ones
     parents: List[int]
+    row: int               # of its first token in the step's q
+    queries: Optional[dict]   # of the step
 
 
 class PagedKVCache:
@@ -271,11 +274,17 @@ class PagedKVCache:
     A bounded cache: with track_rows > 0 up to so many sequences have a row of
     `weights` [n_layers, track_rows, n_kv_heads, track_tokens], to which
     `attention` adds what each token is given (of a prompt's chunk by its last
-    `observe` rows, 0: by all; a drafted tree adds nothing), and `evict` cuts
-    sequences down to the tokens of the largest weight, for every layer and KV
-    head its own:
+    `observe` rows, 0: by all), and `evict` cuts sequences down to the tokens of the
+    largest weight, for every layer and KV head its own:
 
         cache.evict([a, b], keep=4096, first=4, recent=256)
+
+    A drafted tree's attention adds nothing, as most of its tokens are dropped.
+    With track_drafts=True the cache keeps a copy of the tree's q of every layer,
+    and `accept` adds what the accepted tokens give, as decode steps of the same
+    tokens would have (paged_prefill_weights of their rows). Without it the
+    weights know nothing of drafted steps: accepted tokens count as ones that
+    nothing has attended to, and an `evict` that meets them gives a warning.
 
     The tokens that stay keep their rotation, and new ones go on at the text's
     positions. A window or slopes are refused for a sequence that has lost
@@ -290,13 +299,14 @@ class PagedKVCache:
     def __init__(self, n_pages: int, n_kv_heads: int, page_size: int = 64, head_dim: int = 128,
                  dtype: torch.dtype = torch.float16, device: Optional[torch.device] = None,
                  n_layers: int = 1, shared_prefix: bool = True, track_rows: int = 0, track_tokens: int = 0,
-                 observe: int = 0) -> None:
+                 observe: int = 0, track_drafts: bool = False) -> None:
         _require(n_pages > 0 and n_kv_heads > 0 and n_layers > 0, "n_pages, n_kv_heads and n_layers must be positive")
         _require(page_size > 0 and page_size % 8 == 0, "page_size must be a positive multiple of 8")
         _require(head_dim in (64, 128), "only head_dim=64 and 128 supported")
         _require(dtype in (torch.float16, torch.bfloat16), "dtype must be fp16 or bf16")
         _require(track_rows >= 0 and observe >= 0, "track_rows and observe must be >= 0")
         _require(track_rows == 0 or track_tokens > 0, "track_tokens must be positive where weights are recorded")
+        _require(track_rows > 0 or not track_drafts, "track_drafts needs track_rows")
         self.device = torch.device("cuda") if device is None else torch.device(device)
         self.shared_prefix = bool(shared_prefix)
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, n_kv_heads, page_size, head_dim
@@ -311,7 +321,8 @@ class PagedKVCache:
         self._next = 0
         self._lost: dict[int, int] = {}               # sequence -> tokens that it has lost (its text is longer)
         self._drafts: dict[int, _Draft] = {}          # sequence -> its draft that is not accepted
-        self.observe = int(observe)
+        self.observe, self.track_drafts = int(observe), bool(track_drafts)
+        self._unrecorded: set[int] = set()            # sequences with accepted tokens that no weights were recorded of
         self.weights: Optional[torch.Tensor] = None
         self._rows: dict[int, int] = {}               # sequence -> its row of the weights
         self._free_rows = list(range(track_rows - 1, -1, -1))
@@ -354,6 +365,8 @@ class PagedKVCache:
             self._rows[seq] = row = self._free_rows.pop()
             self.weights[:, row].zero_()
             if share is not None:
+                if share in self._unrecorded and tokens:
+                    self._unrecorded.add(seq)
                 n = min(tokens, self.weights.shape[3])
                 self.weights[:, row, :, :n] = self.weights[:, self._rows[share], :, :n]
         return seq
@@ -364,6 +377,7 @@ class PagedKVCache:
         self._release(self._pages.pop(seq))
         del self._length[seq], self._lost[seq]
         self._drafts.pop(seq, None)
+        self._unrecorded.discard(seq)
         if self.weights is not None:
             self._free_rows.append(self._rows.pop(seq))
 
@@ -415,7 +429,8 @@ class PagedKVCache:
         """Ends the drafts of `seqs`: of seqs[i] the drafted tokens paths[i] (numbers in
         the draft, ascending; none: all are dropped) become its next tokens, in
         every layer. The draft's step must have been appended to all layers that
-        are read again. A path begins at a token that follows the sequence and goes
+        are read again. With track_drafts the weights that the accepted tokens give are
+        recorded, in the layers that the step's `attention` was called for. A path begins at a token that follows the sequence and goes
         on from each token to one that follows it; other lists give a warning, as
         their tokens were rotated, and shown others, as what they then are not."""
         paths = [[int(j) for j in path] for path in paths]
@@ -435,15 +450,42 @@ class PagedKVCache:
             longest = max(len(path) for _, path in moved)
             kept = [[c + j for j in path] + [-1] * (longest - len(path)) for c, (_, path) in zip(ctx, moved)]
             self._compact([s for s, _ in moved], kept, ctx)
-        for s, path in zip(seqs, paths):
-            self._shorten(s, self._drafts.pop(s).length + len(path))
+        drafts = [self._drafts.pop(s) for s in seqs]
+        for s, path, draft in zip(seqs, paths, drafts):
+            self._shorten(s, draft.length + len(path))
+            if self.weights is not None and path and len(draft.queries or ()) < self.k.shape[0]:
+                self._unrecorded.add(s)
+        if self.track_drafts:
+            self._record_accepted(seqs, paths, drafts)
+
+    def _record_accepted(self, seqs: Sequence[int], paths: List[List[int]], drafts: List[_Draft]) -> None:
+        """The weights that accepted tokens give: they are the sequences' last ones now, in order, as
+        a prompt's are."""
+        steps: dict[int, list] = {}
+        for s, path, draft in zip(seqs, paths, drafts):
+            if path and draft.queries:
+                steps.setdefault(id(draft.queries), []).append((s, path, draft))
+        for items in steps.values():
+            b, width = len(items), max(len(self._pages[s]) for s, _, _ in items)
+            cu = [0]
+            for _, path, _ in items:
+                cu.append(cu[-1] + len(path))
+            flat = [self._length[s] for s, _, _ in items] + [self._rows[s] for s, _, _ in items] + cu
+            flat += [p for s, _, _ in items for p in self._pages[s] + [-1] * (width - len(self._pages[s]))]
+            flat += [draft.row + j for _, path, draft in items for j in path]
+            dev = self._to_device(flat)
+            table, rows = dev[3 * b + 1:3 * b + 1 + b * width].view(b, width), dev[len(flat) - cu[-1]:]
+            for layer, (q, *options) in items[0][2].queries.items():
+                paged_prefill_weights(q.index_select(0, rows), self.k[layer], table, dev[:b], dev[2 * b:3 * b + 1],
+                                      self.weights[layer], *options, 0, dev[b:2 * b])
 
     def evict(self, seqs: Sequence[int], keep: int, first: int = 0, recent: int = 0) -> None:
         """Cuts the sequences down to `keep` tokens for every layer and KV head: the
         first `first`, the last `recent` and, of the others, those of the largest
         recorded weight (paged_select_tokens). Shorter ones stay as they are. Pages
         that other sequences share are copied first: nothing is changed if the free
-        pages do not suffice."""
+        pages do not suffice. A sequence that accepted drafted tokens without their
+        weights (track_drafts) gives a warning."""
         _require(self.weights is not None, "the cache records no weights (track_rows)")
         _require(len(set(seqs)) == len(seqs), "a sequence occurs twice")
         _require(all(s in self._pages for s in seqs), "no such sequence")
@@ -466,6 +508,11 @@ class PagedKVCache:
                 left[p] -= 1
                 copies.append((s, i))
         _require(len(copies) <= len(self._free), "the cache has no free page")
+        blind = [s for s in long if s in self._unrecorded]
+        if blind:
+            warnings.warn(f"PagedKVCache.evict: the weights of the sequences {blind} hold nothing of drafted tokens that "
+                          "were accepted, which go first (track_drafts=True records them)", stacklevel=2)
+            self._unrecorded.difference_update(blind)
         if copies:
             src = [self._pages[s][i] for s, i in copies]
             dst = [self._free.pop() for _ in copies]
@@ -528,10 +575,11 @@ class PagedKVCache:
         lost = any(self._lost[s] for s in seqs)
         positions: List[int] = []
         words, masks = 0, []
+        queries: Optional[dict] = {} if trees is not None and self.track_drafts else None
         if trees is not None:
             words = max(1, -(-max([len(t) for t in trees] + [0]) // 64))
             for s, n, tree in zip(seqs, before, trees):
-                self._drafts[s] = _Draft(n, len(tree), tree)
+                self._drafts[s] = _Draft(n, len(tree), tree, len(positions), queries)
                 seen: List[int] = []
                 deep: List[int] = []
                 for j, parent in enumerate(tree):
@@ -563,7 +611,7 @@ class PagedKVCache:
                           table[0, :shared] if shared else None, shared * self.page_size,
                           min(lens, default=0), sum(lens) // max(b, 1),
                           dev[ends[0]:ends[1]] if lost or trees is not None else None, tree_mask,
-                          dev[ends[1]:ends[2]] if self.weights is not None else None, lost)
+                          dev[ends[1]:ends[2]] if self.weights is not None else None, lost, queries)
 
     def _shared_prefix(self, pages: List[List[int]], lens: List[int]) -> int:
         """Whole pages that all sequences share from the start on, or 0 where reading
@@ -610,13 +658,16 @@ class PagedKVCache:
         """Attention of the batch's new tokens in a layer: decode, decode behind a
         shared prefix, prompts, or a drafted tree, by the batch (and what a window leaves
         of the prefix). Where the cache records weights, those of decode steps and prompts
-        are added: once for every call."""
+        are added: once for every call (a tree's by `accept`, of the layer's last call)."""
         k, v = self.k[layer], self.v[layer]
         _require(not step.shortened or (slopes is None and window <= 0),
                  "window and slopes need sequences that have lost no tokens")
         if step.tree_mask is not None:
-            return paged_tree_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, step.tree_mask,
-                                        softmax_scale, softcap, slopes, window, step.positions)
+            out = paged_tree_attention(q, k, v, step.page_table, step.seq_lens, step.cu_tokens, step.tree_mask,
+                                       softmax_scale, softcap, slopes, window, step.positions)
+            if step.queries is not None:
+                step.queries[layer] = (q.clone(), softmax_scale, softcap, slopes, window)
+            return out
         if step.cu_tokens is not None:
             if self.weights is not None:
                 paged_prefill_weights(q, k, step.page_table, step.seq_lens, step.cu_tokens, self.weights[layer],
