@@ -660,9 +660,12 @@ LLMIK_API llmik_status llmik_paged_select_tokens(const llmik_token_weights* weig
  * starts[b] + i (NULL: i), for i < n.
  *   kept [batch, kept_heads, n]: kept_heads n_kv_heads, or 1 for one list for all heads.
  *     An entry that is negative, at or behind the sequence's length, or in front of its
- *     new slot moves nothing, nor do unmapped pages. The entries may have any order.
- *   weights (NULL: none) are moved alike, and those from the first negative entry's new
- *     slot on become 0.
+ *     new slot moves nothing. A token moves where both slots' pages are mapped. The entries
+ *     may have any order.
+ *   weights (NULL: none) are moved by the same entries, but by slots alone: a weight's place
+ *     does not depend on the page table, so it moves where an unmapped page keeps its token from
+ *     moving. Those from the first negative entry's new slot on become 0, also where entries
+ *     behind that one move tokens: a list that is meant whole has its negative entries last.
  * Slots behind the moved tokens keep what they hold. seq_lens are the lengths before;
  * they are not changed. Sequences that share a page that is written, or that map one
  * twice, get no particular order.

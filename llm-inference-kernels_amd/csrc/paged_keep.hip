@@ -266,7 +266,7 @@ __global__ __launch_bounds__(1024) void paged_compact_kernel(CompactParams p) {
         return t < len && t > start + i ? t : -1;   // (start + i <= t: no overflow where it counts; n <= 2^30)
     };
 
-    if (part == 2 * p.slices) {   // the weights: moved alike, those behind the kept ones become 0
+    if (part == 2 * p.slices) {   // the weights: moved by slots (no pages), those behind the kept ones become 0
         float* const w = weights_of(p.w, b, kvh);
         if (w == nullptr) return;
         const int stop = min(len, p.w.max_len);

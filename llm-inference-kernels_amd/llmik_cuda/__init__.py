@@ -603,9 +603,10 @@ def paged_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torc
     (kept [batch, n_kv_heads, n] or, for all heads alike, [batch, n] int32) goes to
     slot starts[b] + i (starts [batch] int32; default 0). seq_lens are the lengths
     before. Entries that are negative, at or behind the length, or in front of their
-    new slot move nothing; otherwise the order is free. With `weights` each token's
-    weight moves along, and the weights from the first negative entry's new slot on
-    become 0. Slots behind the moved tokens keep what they hold. A page that is
+    new slot move nothing; otherwise the order is free. Tokens move where both pages are
+    mapped. With `weights` the entries' weights move too, by slots alone, whatever the page
+    table has there, and the weights from the first negative entry's new slot on become 0,
+    whatever entries follow it. Slots behind the moved tokens keep what they hold. A page that is
     written must be one sequence's own."""
     _require(_is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and _is_device(seq_lens) and
              _is_device(kept), "all inputs must be CUDA tensors")
