@@ -4,13 +4,13 @@
 //   weights[row(b), kvh, t] += sum over the KV head's G query heads of 2^(s - m) / l
 // Every weight has one writer, so the sums do not depend on timing.
 //
-// Bound: the cache's bytes, and the scores' (G / D of the keys' and values') twice. GPU us,
-// plain decode against this: 48 sequences of 1500 .. 8192 tokens, 8 KV heads, bf16 136, 171;
-// 64 of 4096 166, 212; one of 900 10.1, 14.5, one of 30000 30.7, 36.6. Of the difference
-// the second launch has 10 (4 for one sequence), the writes among the reads 19, whatever
-// their order, place or part of a line (into the caches alone 5). Adding the weights in
-// the first launch, by the last of a sequence's workgroups: 900 tokens 13.7, 2000 17.5
-// instead of 15.7, 4 x 4000 33.6 instead of 26.9.
+// Bound: the cache's bytes, and the scores' (G / D of the keys' and values') twice. us, a call
+// among others, plain decode against this: 48 sequences of 1500 .. 8192 tokens, 8 KV heads, bf16
+// 134, 170; 64 of 4096 164, 210; one of 900 9.2, 13.8, one of 30000 28.3, 34.2. Under the tracer the
+// first of these is 133.4 against 160.4 and 9.5: the writes among the reads cost 27, whatever their
+// order, place or part of a line, and the second launch the rest (64 of 4096 35 and 11.3, one of 900
+// 1.4 and 3.9). Adding the weights in the first launch, by the last of a sequence's workgroups:
+// 900 tokens 13.7, 2000 17.5 instead of 15.7, 4 x 4000 33.6 instead of 26.9.
 #include "paged_decode.hpp"
 
 namespace llmik {

@@ -18,7 +18,7 @@
 //     channels and get one channel's four tokens each).
 // P is rounded once to 16 bits, as 2^8 p (fp16 keeps its full precision down to
 // 2^-22); sums and statistics are fp32. A tree's rows stand in for decode steps, whose P
-// enters as a pair of 16-bit values: theirs does too (two products; the loads bound them).
+// enters as a pair of 16-bit values: theirs does too (two products).
 //
 // K and V tiles are copied to LDS asynchronously, one tile ahead. The 16-byte
 // chunks of a row are permuted (xor with the row number) so that the operand
@@ -239,7 +239,7 @@ __device__ __forceinline__ void cut_sequence(const PagedFlashParams& p, int b, C
     s.fixed = (int)((uint32_t)(s.rows * (int)p.gqa.d + kPfRows - 1) / kPfRows);
 }
 
-// n / d, rounded up, for n + d < 2^31 and d > 0. The quotient of floats is off by at most n 2^-21 / d + 1, so
+// n / d, rounded up, for n + d < 2^32 and d > 0. The quotient of floats is off by at most n 2^-21 / d + 1, so
 // its remainder is below 2^11 + 2 d, and that one's quotient off by one at most.
 __device__ __forceinline__ uint32_t quick_ceil(uint32_t n, uint32_t d) {
     const uint32_t x = n + d - 1;

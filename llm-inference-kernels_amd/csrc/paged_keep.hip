@@ -10,7 +10,9 @@
 // those equal to it, and after a sum over the waves writes its slots in order.
 // Bound: a chain of reads and barriers, the waves wait 62 % of the time (8192 tokens of 8 KV
 // heads 9.5 us, 64 x 8 x 3500 .. 6000 14.4; with one histogram and the weights read anew for
-// every digit 26, 29).
+// every digit 26, 29). Where a sequence has more candidates than LDS holds they are read again for every
+// digit and count, by one workgroup: of 8 KV heads 36000 tokens 26 us, 40000 48, 100000 110, 32 x 40000 87,
+// 16 x 100000 220.
 //
 // Compaction. Token kept[i] goes to slot start + i. No entry lies before its new slot
 // (kept[i] >= start + i; others are not moved), so a workgroup that takes the entries
@@ -218,9 +220,12 @@ int launch_paged_select(const PagedWeights& w, const int* lens, int batch, int n
                         int recent, int* kept, int* new_lens, hipStream_t stream) {
     const int cached = std::min(w.max_len, kSelCached);
     const SelectParams p{weights_view(w, n_kv_heads), lens, kept, new_lens, keep, first, recent, cached};
-    // Eight waves where they read a row in one turn of four weights a thread, else sixteen. us, 16, 8, 4 waves, sequences of
-    // 8 KV heads x tokens: 1 x 2000 6.6, 5.9, 7.4, 256 x 2000 31.1, 18.5, 16.4, 1 x 4000 7.1, 7.8, 64 x 4000 10.7, 11.1,
-    // 64 x 3500 .. 6000 14.4, 13.6, 64 x 7000 15.7, 18.2, 1 x 8192 9.5, 11.5, 17.4.
+    // Waves and LDS go by the rows' width, which bounds the lengths; the lengths themselves are on the device. Eight
+    // waves where they read a whole row in one turn of four weights a thread, else sixteen. us, 16, 8, 4 waves, sequences
+    // of 8 KV heads x tokens in rows that end with them: 1 x 2000 6.6, 5.9, 7.4, 256 x 2000 31.1, 18.5, 16.4, 1 x 4000 7.1,
+    // 7.8, 64 x 4000 10.7, 11.1, 64 x 3500 .. 6000 14.4, 13.6, 64 x 7000 15.7, 18.2, 1 x 8192 9.5, 11.5, 17.4. Short
+    // sequences in wide rows pay for the width: 256 x 2000 in rows of 2000, 8192, 32768 17.7, 30.5, 46.8 (sixteen waves,
+    // then one workgroup per CU), 64 x 3500 .. 6000 in rows of 6016, 20480 and more 14.3, 19.
     const unsigned grid = (unsigned)(batch * n_kv_heads);
     if (cached <= 4 * 512) paged_select_kernel<512><<<grid, 512, (size_t)cached * 4, stream>>>(p);
     else paged_select_kernel<1024><<<grid, 1024, (size_t)cached * 4, stream>>>(p);

@@ -8,12 +8,13 @@
 // tile's parts are joined by a second kernel. A row's mask is one 64-bit word for a tile
 // of 64 keys, shifted to the tile's beginning; tiles of cached tokens need none.
 //
-// Measured (GPU us, kernel and join): 8 drafted tokens over 700 8.8 + 3.9, 64 over 8192 22 + 5.2, 32
-// sequences of 4 .. 24 over 200 .. 8000 54 + 5.4, all with 32 heads over 8 KV heads of 128. The last
-// reads 235 MB at 4.3 TB/s (8 drafted tokens over each of 32 x 8000: 1.05 GB in 197 us, 5.3 TB/s); of
-// the second launch and look-ups take 8 us, a workgroup's 8 or 9 tiles follow one another, and 17 MB
-// of parts are written and read (eight waves in two teams, each with half of a part's keys, gain 1 us
-// there and lose 1 at 700 tokens); the first is launches and look-ups.
+// Measured (us under the tracer, kernel and join): 8 drafted tokens over 700 8.5 + 3.6, 64 over 8192
+// 26 + 5.2, 32 sequences of 4 .. 24 over 200 .. 8000 60 + 5.4, all with 32 heads over 8 KV heads of 128
+// (a call among others 11.2, 28.8, 64). The last reads 235 MB at 3.9 TB/s (8 drafted tokens over each of
+// 32 x 8000: 1.05 GB in 196 us, 5.4 TB/s); of the second launch and look-ups take 8 us, a workgroup's 8 or 9
+// tiles follow one another (the second product of a probability's pair is 3.5 us of them), and 17 MB of
+// parts are written and read (eight waves in two teams, each with half of a part's keys, gain 1 us there and
+// lose 1 at 700 tokens); the first is launches and look-ups.
 #include "paged_flash.hpp"
 
 namespace llmik {
@@ -140,16 +141,16 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
 namespace {
 
 // Key tiles are cut for two workgroups per CU, or, where there are row tiles for at most a quarter of the CUs, for one:
-// the sums of every part are written and read again, but of many sequences the ends are ragged. us, for 1 and 2
-// workgroups: one draft of 64 over 8192 tokens 28.8, 30.4, of 8 over 30000 37.7, 39.8, four of 16 over 3000 22.5, 24.2,
+// the sums of every part are written and read again, but of many sequences the ends are ragged. us (these and below
+// replayed from a graph, probabilities of one part), for 1 and 2 workgroups: one draft of 64 over 8192 tokens 28.8, 30.4, of 8 over 30000 37.7, 39.8, four of 16 over 3000 22.5, 24.2,
 // 16 of 32 over 4000 78.7, 73.3, 30 of 4 .. 24 over 200 .. 8000 88.6, 62.0 (for 3 76). Into single tiles where there
 // are few: 8 over 700 tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0.
 constexpr int kTreeLeast = 1;
 // A part's sums, 64 KiB, are written and read again, which takes 0.026 us of the card's time, a tile 1.3 us of its
-// workgroup's: of N pairs of tiles in parts of t the sum of 1.3 t and 0.026 N / t is least at t^2 = N / 50, and a row
-// tile whose keys are less than twice that is better whole (t^2 = N / 25). us without this rule, with N / 50, with
-// N / 25: 32 drafts of 16 over 200 tokens 27.2, 18.1, 18.1, over 600 33.7, 33.7, 27.0, 8 of 16 over 600 19.7, 18.0,
-// 19.4, 16 of 32 over 500 30.0, 29.9, 27.6.
+// workgroup's (1.6 with probabilities of two parts, a tenth of the root): of N pairs of tiles in parts of t the sum
+// of 1.3 t and 0.026 N / t is least at t^2 = N / 50, and a row tile whose keys are less than twice that is better whole
+// (t^2 = N / 25). us without this rule, with N / 50, with N / 25: 32 drafts of 16 over 200 tokens 27.2, 18.1, 18.1, over
+// 600 33.7, 33.7, 27.0, 8 of 16 over 600 19.7, 18.0, 19.4, 16 of 32 over 500 30.0, 29.9, 27.6.
 constexpr float kTreePartCost = 25.0f;
 
 struct PagedTreePlan {

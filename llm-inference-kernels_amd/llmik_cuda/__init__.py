@@ -563,7 +563,9 @@ def paged_decode_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     """paged_decode_attention (the same bits) that adds each live key's
     probabilities, summed over the query heads of its KV head, to `weights` in
     place. Deterministic; the weights' last bits depend on the lengths of the
-    whole batch, as the output's do."""
+    whole batch, as the output's do. The scores lie in memory of the call, 4 bytes
+    per sequence, query head and token of the longest sequence that page_table and
+    weights allow, whatever the lengths are."""
     _require(_is_device(q) and _is_device(k_cache) and _is_device(v_cache) and _is_device(page_table) and
              _is_device(seq_lens) and _is_device(weights), "all inputs must be CUDA tensors")
     return _C.paged_decode_attention_weights(q, k_cache, v_cache, page_table, seq_lens, weights,
