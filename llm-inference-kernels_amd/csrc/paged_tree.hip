@@ -141,10 +141,12 @@ __global__ __launch_bounds__(256) void paged_tree_join_kernel(PagedFlashParams p
 namespace {
 
 // Key tiles are cut for two workgroups per CU, or, where there are row tiles for at most a quarter of the CUs, for one:
-// the sums of every part are written and read again, but of many sequences the ends are ragged. us (these and below
-// replayed from a graph, probabilities of one part), for 1 and 2 workgroups: one draft of 64 over 8192 tokens 28.8, 30.4, of 8 over 30000 37.7, 39.8, four of 16 over 3000 22.5, 24.2,
-// 16 of 32 over 4000 78.7, 73.3, 30 of 4 .. 24 over 200 .. 8000 88.6, 62.0 (for 3 76). Into single tiles where there
-// are few: 8 over 700 tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0.
+// the sums of every part are written and read again, but of many sequences the ends are ragged. us, a call among others,
+// for 1, 2, 3 workgroups: one draft of 64 over 8192 tokens 31.4, 31.2, 31.0, over 16000 41.2, 46.4, 46.4, over 30000
+// 65.6, 66.4, 66.4, of 32 over 30000 43.0, 49.5, 49.4, two of 64 over 8192 41.9, 45.9, 46.5; eight of 64 over 2000 (128 row
+// tiles) 45.6, 48.8, 48.5, 16 of 32 over 4000 80.1, 80.1, 80.2, 30 of 4 .. 24 over 200 .. 8000 96.1, 65.8, 74.2. Into
+// single tiles where there are few: 8 over 700 tokens with 1, 2, 4 tiles or more 12.3, 13.1, 14.0 (this and below
+// replayed from a graph, with probabilities of one part).
 constexpr int kTreeLeast = 1;
 // A part's sums, 64 KiB, are written and read again, which takes 0.026 us of the card's time, a tile 1.3 us of its
 // workgroup's (1.6 with probabilities of two parts, a tenth of the root): of N pairs of tiles in parts of t the sum
